@@ -727,6 +727,112 @@ int hier_lse_gather_merge_peers(const void* const* o_bases, const float* const* 
                                 const int32_t* local_owner, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Per-head prologue (no reference counterpart: the reference norms whole rows)
+ * ------------------------------------------------------------------------- */
+
+/* RMSNorm of every head of q (hq heads) and k (hk heads) with the position
+ * rotation in the same pass: y = R(p) (x * rsqrt(mean(x^2) + eps) * w), fp32
+ * with one bf16 rounding.  q, k bf16 [rows][heads*D] (D 64, 128 or 256; rows
+ * 16-byte aligned, strides in elements); wq, wk [D] bf16 (w_f32 = 0) or float;
+ * freqs float [freqs_rows][D/2][2] (cos, sin) rotating pairs (2i, 2i+1).
+ * positions int32 [rows] picks the table row; a negative one skips the row
+ * (zeros are written when zero_skipped), one past the table skips it and sets
+ * *dev_err; NULL: row r % freqs_rows, freqs_rows dividing rows.
+ * q_out_rows / k_out_rows int32 [rows] or NULL: the output row of each row, of
+ * q_out_total / k_out_total rows (negative: not written; past the end: not
+ * written, *dev_err set). */
+int hier_head_norm_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                        int64_t rows, int32_t hq, int32_t hk, int32_t D, const void* wq,
+                        const void* wk, int32_t w_f32, const float* freqs, int64_t freqs_rows,
+                        const int32_t* positions, float eps, void* q_out, int64_t qo_stride,
+                        const int32_t* q_out_rows, int64_t q_out_total, void* k_out,
+                        int64_t ko_stride, const int32_t* k_out_rows, int64_t k_out_total,
+                        int32_t zero_skipped, int32_t* dev_err, void* stream);
+
+/* Backward of hier_head_norm_rope without row maps: dq, dk from the gradients
+ * gq, gk of its outputs (all bf16), dwq, dwk [D] in the weights' type.
+ * partials float [blocks][2][D], blocks from ..._bwd_partials: the sums are
+ * added in a fixed order.  Skipped rows get zero gradients. */
+int hier_head_norm_rope_bwd_partials(int64_t rows, int32_t hq, int32_t hk, int32_t D,
+                                     int32_t* blocks);
+int hier_head_norm_rope_bwd(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                            int64_t rows, int32_t hq, int32_t hk, int32_t D, const void* wq,
+                            const void* wk, int32_t w_f32, const float* freqs, int64_t freqs_rows,
+                            const int32_t* positions, float eps, const void* gq, int64_t gq_stride,
+                            const void* gk, int64_t gk_stride, void* dq, int64_t dq_stride,
+                            void* dk, int64_t dk_stride, float* partials, int32_t blocks,
+                            void* dwq, void* dwk, int32_t* dev_err, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit paged key/value cache (no reference counterpart: the reference's page
+ * table, kernels/hier_paged_attention.py:232-249, lists bf16 rows)
+ *
+ * A page holds 64 tokens of every key head.  codes of one (page, head):
+ *   keys   [2][64][64]  dimension half, token, 64 dimensions
+ *   values [128][64]    dimension, token
+ * int8 (format 0, -127..127) or e4m3 (format 1), one float scale per page and
+ * head for keys and one for values, a power of two; value = code * scale.
+ * Requests are ragged: request b owns rows q_start[b] .. q_start[b+1] - 1 and
+ * holds lengths[b] tokens, the last of them those rows'; token t is in page
+ * table[b][t / 64].  All tables are int32 on the device; nothing syncs.
+ * status (device int32) collects bits: 1 row starts outside the rows, 2 a
+ * length outside the table, 4 a page outside the pool, 8 a NaN or an infinity
+ * given to the cache (held as 0 and as the block's largest value).  What such
+ * an entry addresses is skipped.
+ * ------------------------------------------------------------------------- */
+
+/* Block tables and slot maps of one step, from request lengths: request b goes
+ * from lengths[b] to lengths[b] + add[b] tokens (negative add drops its last
+ * tokens).  Pages given up go to the end of free_pages [capacity] (*free_count
+ * listed) in request order, pages needed come off its end in request order
+ * into the table rows ([n][table_stride], width used).  Writes lengths_out [n]
+ * and *free_count_out (may be the inputs), q_start [n + 1] over the
+ * max(add, 0) new tokens, and per row its slot (page * 64 + token of the page)
+ * and position, -1 behind the last request.  status: 1 too few free pages, 2
+ * too few rows, 4 a length outside the table, 8 add below -length or above
+ * max_add (max_add < 0: no limit), 16 a count outside the list; with any of
+ * them the step changes nothing, q_start is 0 and no row is mapped. */
+int hier_page_step(const int32_t* lengths, const int32_t* add, int32_t n, int32_t* table,
+                   int64_t table_stride, int32_t width, int32_t* free_pages, int32_t capacity,
+                   const int32_t* free_count, int32_t rows, int32_t max_add, int32_t* lengths_out,
+                   int32_t* free_count_out, int32_t* q_start, int32_t* slots, int32_t* positions,
+                   int32_t* status, void* stream);
+
+/* Write the new rows k, v (bf16 [rows][heads*128], 8-byte aligned) into their
+ * pages (lengths count them in).  Scale of a (page, head): the least power of
+ * two that holds the page's new values, never below that of the tokens the
+ * page held before, whose codes are re-encoded when it grows.  A page must
+ * belong to one request of the call. */
+int hier_paged8_append(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                       int32_t rows, int32_t heads, int32_t format, void* k_codes, void* v_codes,
+                       float* k_scale, float* v_scale, int32_t n_pages, const int32_t* table,
+                       int64_t table_stride, int32_t width, const int32_t* lengths,
+                       const int32_t* q_start, int32_t n, int32_t* status, void* stream);
+
+/* Attention of q (bf16 [rows][heads*128], 16-byte aligned) over the cache:
+ * query head h reads key head h / (heads / kv_heads).  Row i of request b is
+ * at position p = lengths[b] - (its rows) + i and sees token j when
+ *   block == 0, or j / frame / block <= p / frame / block, and
+ *   window < 0, or p / frame - j / frame < window
+ * (frames of `frame` tokens, causal blocks of `block` frames, window in
+ * frames).  out bf16 [rows][heads*128] is 0 for rows that see nothing; rows
+ * behind the last request are left, or zeroed with zero_tail.  lse (or NULL):
+ * float [rows][heads], log2-sum-exp of the scaled scores.  max_rows: the most
+ * rows a request has, as far as the caller knows (it chooses kernels, not
+ * results); <= 0: unknown.  workspace: floats of ..._workspace for the same
+ * sizes. */
+int hier_paged8_attn_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t n,
+                               int32_t width, int32_t max_rows, int64_t* floats);
+int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, int32_t heads,
+                     int32_t kv_heads, int32_t D, int32_t format, const void* k_codes,
+                     const void* v_codes, const float* k_scale, const float* v_scale,
+                     int32_t n_pages, const int32_t* table, int64_t table_stride, int32_t width,
+                     const int32_t* lengths, const int32_t* q_start, int32_t n, int32_t frame,
+                     int32_t block, int32_t window, float softmax_scale, int32_t max_rows,
+                     void* out, int64_t out_stride, float* lse, int32_t zero_tail,
+                     float* workspace, int32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Self-test of the tensor-core operand encodings (no reference counterpart):
  * with A, B bf16 [128,128] row-major,
  *   c_ss = A @ B^T   (both operands K-major in shared memory)

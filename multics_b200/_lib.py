@@ -198,6 +198,24 @@ _SIGS = {
                                             _P, _P]),
     "hier_plan_check": (c_int, [_P, c_int32, _P, c_int64, c_int64, _P, c_int64, _P, c_int32, _P,
                                 _P]),
+    "hier_head_norm_rope": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int32, c_int32, c_int32, _P,
+                                    _P, c_int32, _P, c_int64, _P, c_float, _P, c_int64, _P, c_int64,
+                                    _P, c_int64, _P, c_int64, c_int32, _P, _P]),
+    "hier_head_norm_rope_bwd_partials": (c_int, [c_int64, c_int32, c_int32, c_int32, _P]),
+    "hier_head_norm_rope_bwd": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int32, c_int32, c_int32,
+                                        _P, _P, c_int32, _P, c_int64, _P, c_float, _P, c_int64, _P,
+                                        c_int64, _P, c_int64, _P, c_int64, _P, c_int32, _P, _P, _P,
+                                        _P]),
+    "hier_page_step": (c_int, [_P, _P, c_int32, _P, c_int64, c_int32, _P, c_int32, _P, c_int32,
+                               c_int32, _P, _P, _P, _P, _P, _P, _P]),
+    "hier_paged8_append": (c_int, [_P, c_int64, _P, c_int64, c_int32, c_int32, c_int32, _P, _P, _P,
+                                   _P, c_int32, _P, c_int64, c_int32, _P, _P, c_int32, _P, _P]),
+    "hier_paged8_attn_workspace": (c_int, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                           _P]),
+    "hier_paged8_attn": (c_int, [_P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P,
+                                 _P, _P, c_int32, _P, c_int64, c_int32, _P, _P, c_int32, c_int32,
+                                 c_int32, c_int32, c_float, c_int32, _P, c_int64, _P, c_int32, _P,
+                                 _P, _P]),
     "hier_selftest_umma": (c_int, [_P, _P, _P, _P, _P, _P, _P]),
     "hier_selftest_wait_timeout": (c_int, [c_int64, _P, _P, _P]),
 }
@@ -205,7 +223,7 @@ _SIGS = {
 _LIB = None
 
 # hier_abi_version() of the library these signatures describe
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 
 def lib():

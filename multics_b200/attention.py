@@ -31,7 +31,7 @@ from .hier_masks import HierBlockMask, block_mask_for_spec, build_dense_block_pl
 
 __all__ = ["hier_prep_qk", "hier_block_attention", "freqs_table", "RMSNorm", "SelfAttention",
            "AttentionPlan", "attention_from_plan", "HierSequencePlan", "sequence_plan",
-           "hier_attention_layer", "attention_mask_plan", "CrossAttention"]
+           "hier_attention_layer", "attention_mask_plan", "CrossAttention", "hier_head_norm_rope"]
 
 # Work plan of the full-sequence layer entry points: "segments" (the
 # HierSequencePlan wherever the grouping allows it) or "blocks" (always the
@@ -43,6 +43,8 @@ _DEV_ERR = {}
 
 def _dev_err(device):
     key = torch.device(device).index
+    if key is None:  # "cuda" is the current device, whose tensors carry its index
+        key = torch.cuda.current_device()
     t = _DEV_ERR.get(key)
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=device)
@@ -130,6 +132,98 @@ def hier_prep_qk(qx, kx, freqs, num_heads, *, norm_q_weight, norm_k_weight, cam_
         ptr(q2), ptr(k2), q2.stride(0), ptr(cam), cam_dim, ptr(cam_q_weight), ptr(cam_k_weight),
         ptr(nqw), ptr(nkw), ptr(ft), ft.shape[0], S, num_heads, D, float(eps), ptr(q_out), ptr(k_out),
         q_out.stride(0), ptr(out_rows), ptr(k_out_rows), stream_ptr(q2.device)))
+    return q_out, k_out
+
+
+def head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight, k_weight, positions):
+    """The checked arguments of the per-head prologue: q and k as aligned rows,
+    the head size, contiguous weights of one type, the rotation table and the
+    positions."""
+    from .paged8 import token_rows
+
+    if num_heads < 1 or num_kv_heads < 1 or q.shape[-1] % num_heads:
+        raise ValueError(f"q {tuple(q.shape)} does not split into {num_heads} heads")
+    D = q.shape[-1] // num_heads
+    if D not in (64, 128, 256):
+        raise NotImplementedError(f"the per-head norm supports head_dim 64, 128 and 256; got {D}")
+    q, k = token_rows("q", q, num_heads * D), token_rows("k", k, num_kv_heads * D)
+    T = q.shape[0]
+    if k.shape[0] != T:
+        raise ValueError(f"q has {T} rows, k {k.shape[0]}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if tuple(w.shape) != (D,):
+            raise ValueError(f"{name} must be [{D}], got {tuple(w.shape)}")
+    if q_weight.dtype == k_weight.dtype == torch.bfloat16:
+        wq, wk = q_weight.contiguous(), k_weight.contiguous()
+    else:
+        wq, wk = q_weight.float().contiguous(), k_weight.float().contiguous()
+    ft = freqs if (freqs.dtype == torch.float32 and freqs.dim() == 3
+                   and freqs.shape[-1] == 2) else freqs_table(freqs)
+    if ft.shape[0] < 1 or ft.shape[1] * 2 != D:
+        raise ValueError(f"freqs must be [F, {D // 2}, 2] (or complex [F, 1, {D // 2}]), got "
+                         f"{tuple(freqs.shape)}")
+    if positions is None:
+        if T % ft.shape[0]:
+            raise ValueError(f"without positions the {ft.shape[0]} table rows must divide the "
+                             f"{T} rows")
+    elif positions.dtype != torch.int32 or tuple(positions.shape) != (T,):
+        raise ValueError(f"positions must be int32 [{T}], got {positions.dtype} "
+                         f"{tuple(positions.shape)}")
+    if not q.is_cuda:
+        raise NotImplementedError("the per-head norm requires CUDA tensors")
+    ft = ft.to(q.device).contiguous()
+    if ft.data_ptr() % 16:
+        ft = ft.clone()
+    for name, t in (("k", k), ("q_weight", wq), ("k_weight", wk), ("positions", positions)):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, expected {q.device}")
+    return q, k, D, wq, wk, ft, None if positions is None else positions.contiguous()
+
+
+def hier_head_norm_rope(q, k, freqs, num_heads, num_kv_heads, *, q_weight, k_weight,
+                        positions=None, eps=1e-6, out=None, out_rows=None, k_out_rows=None):
+    """``rope(rmsnorm over each head of q * q_weight)`` and the same for k, bf16,
+    in one pass: the per-head counterpart of :func:`hier_prep_qk`.
+
+    ``q`` bf16 ``[T, num_heads * D]``, ``k`` ``[T, num_kv_heads * D]`` (D 64, 128
+    or 256; weights ``[D]`` shared by the heads).  ``freqs`` as in
+    :func:`hier_prep_qk`; row ``r`` is rotated by table row ``positions[r]``
+    (int32 on the device; ``r % F`` without them).  Rows with a negative
+    position are zeros, or left as they were in a given ``out``; a position past
+    the table counts as negative and sets :func:`device_error`.  ``out``:
+    ``(q_out, k_out)`` to write to (16-byte aligned rows), ``out_rows`` / ``k_out_rows`` (int32 ``[T]``)
+    the row of each token in them (``k_out_rows`` for k alone, e.g. the slots of
+    a paged pool; negative: not written)."""
+    from .paged8 import on_device
+
+    q2, k2, D, wq, wk, ft, pos = head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight,
+                                                k_weight, positions)
+    T, dev = q2.shape[0], q2.device
+    k_rows = out_rows if k_out_rows is None else k_out_rows
+    for name, m in (("out_rows", out_rows), ("k_out_rows", k_out_rows)):
+        if m is not None and (m.dtype != torch.int32 or tuple(m.shape) != (T,) or m.device != dev
+                              or not m.is_contiguous()):
+            raise ValueError(f"{name} must be int32 [{T}] on {dev}")
+    if out is None and k_out_rows is not None:
+        raise ValueError("k_out_rows needs out=(q_out, k_out)")
+    with on_device(dev):
+        if out is None:
+            q_out = torch.empty((T, num_heads * D), dtype=torch.bfloat16, device=dev)
+            k_out = torch.empty((T, num_kv_heads * D), dtype=torch.bfloat16, device=dev)
+        else:
+            q_out, k_out = out
+            for name, t, w, m in (("q_out", q_out, num_heads * D, out_rows),
+                                  ("k_out", k_out, num_kv_heads * D, k_rows)):
+                if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != w or t.device != dev \
+                        or t.stride(1) != 1 or (m is None and t.shape[0] < T):
+                    raise ValueError(f"{name} must be bf16 [{T}, {w}] rows on {dev}, got {t.dtype} "
+                                     f"{tuple(t.shape)}")
+        check(_lib.lib().hier_head_norm_rope(
+            ptr(q2), q2.stride(0), ptr(k2), k2.stride(0), T, num_heads, num_kv_heads, D, ptr(wq),
+            ptr(wk), int(wq.dtype == torch.float32), ptr(ft), ft.shape[0], ptr(pos), float(eps),
+            ptr(q_out), q_out.stride(0), ptr(out_rows), q_out.shape[0], ptr(k_out),
+            k_out.stride(0), ptr(k_rows), k_out.shape[0], int(out is None), ptr(_dev_err(dev)),
+            stream_ptr(dev)))
     return q_out, k_out
 
 
@@ -446,19 +540,22 @@ class SelfAttention(nn.Module):
     bool mask (``build_stage2_hier_self_attn_mask`` or any other) or None, as
     the reference's Flex and sdpa call sites pass.  The q/k/v/o
     projections run as cuBLAS GEMMs; the camera add, both RMSNorms and RoPE
-    run in one prologue kernel and the attention in the tcgen05 kernel."""
+    run in one prologue kernel and the attention in the tcgen05 kernel.
+    ``head_norm`` norms every head of q and k by itself (weights ``[head_dim]``)
+    instead of the whole rows, the camera projection added before it."""
 
-    def __init__(self, dim: int, num_heads: int, eps: float = 1e-6):
+    def __init__(self, dim: int, num_heads: int, eps: float = 1e-6, head_norm: bool = False):
         super().__init__()
         self.dim = dim
         self.num_heads = num_heads
         self.head_dim = dim // num_heads
+        self.head_norm = bool(head_norm)
         self.q = nn.Linear(dim, dim)
         self.k = nn.Linear(dim, dim)
         self.v = nn.Linear(dim, dim)
         self.o = nn.Linear(dim, dim)
-        self.norm_q = RMSNorm(dim, eps=eps)
-        self.norm_k = RMSNorm(dim, eps=eps)
+        self.norm_q = RMSNorm(self.head_dim if head_norm else dim, eps=eps)
+        self.norm_k = RMSNorm(self.head_dim if head_norm else dim, eps=eps)
         self.sink_size = 0
         self.local_attn_size = 6
         self.num_frame_per_block = 7
@@ -498,13 +595,30 @@ class SelfAttention(nn.Module):
         qx = self.q(x)
         kx = self.k(x)
         v = self.v(x)
-        q, k = hier_prep_qk(
+        q, k = self._prologue(qx, kx, freqs, cam_tokens, out_rows=out_rows)
+        return q, k, _rows(v)
+
+    def _prologue(self, qx, kx, freqs, cam_tokens, *, out_rows=None, train=False):
+        """Camera add, RMSNorm (of whole rows, or of every head) and RoPE of the
+        projections: ``(q, k)`` ``[S, dim]`` rows, differentiable with ``train``."""
+        from .train import head_norm_rope_grad, prologue_grad
+
+        if self.head_norm:
+            if cam_tokens is not None:
+                qx, kx = qx + self.cam_q(cam_tokens.to(qx)), kx + self.cam_k(cam_tokens.to(kx))
+            prep, kw = (head_norm_rope_grad, {}) if train else (hier_head_norm_rope, {})
+            if out_rows is not None:
+                kw = dict(out=(torch.empty_like(_rows(qx)), torch.empty_like(_rows(kx))),
+                          out_rows=out_rows)
+            return prep(qx, kx, freqs, self.num_heads, self.num_heads, q_weight=self.norm_q.weight,
+                        k_weight=self.norm_k.weight, eps=self.norm_q.eps, **kw)
+        kw = {} if out_rows is None else dict(out_rows=out_rows)
+        return (prologue_grad if train else hier_prep_qk)(
             qx, kx, freqs, self.num_heads, norm_q_weight=self.norm_q.weight,
             norm_k_weight=self.norm_k.weight, cam_tokens=cam_tokens,
             cam_q_weight=None if self.cam_q is None else self.cam_q.weight,
             cam_k_weight=None if self.cam_k is None else self.cam_k.weight, eps=self.norm_q.eps,
-            out_rows=out_rows)
-        return q, k, _rows(v)
+            **kw)
 
     def forward(self, x, freqs, mask=None, cam_tokens=None):
         """``attention.py:436-442``.  ``mask`` is what the reference's call
@@ -544,7 +658,7 @@ class SelfAttention(nn.Module):
         (:func:`multics_b200.train.prologue_grad`), the attention on the block
         plan through :func:`multics_b200.train.hier_block_attention_grad`
         (tcgen05 forward and backward kernels)."""
-        from .train import hier_block_attention_grad, prologue_grad
+        from .train import hier_block_attention_grad
 
         if cam_tokens is not None and (self.cam_q is None or self.cam_k is None):
             raise RuntimeError("camera_pose was provided but enable_camera_pose_qk() was not called")
@@ -554,11 +668,7 @@ class SelfAttention(nn.Module):
         if cam_tokens is not None and self.training and self.cam_dropout_p > 0:
             cam_tokens = torch.nn.functional.dropout(cam_tokens, p=self.cam_dropout_p, training=True)
         qx, kx, v = self.q(x), self.k(x), self.v(x)
-        q, k = prologue_grad(qx, kx, freqs, self.num_heads, norm_q_weight=self.norm_q.weight,
-                             norm_k_weight=self.norm_k.weight, cam_tokens=cam_tokens,
-                             cam_q_weight=None if self.cam_q is None else self.cam_q.weight,
-                             cam_k_weight=None if self.cam_k is None else self.cam_k.weight,
-                             eps=self.norm_q.eps)
+        q, k = self._prologue(qx, kx, freqs, cam_tokens, train=True)
         bm = attention_mask_plan(mask, x.shape[1], x.device)
         out = hier_block_attention_grad(q, k, _rows(v), bm, self.num_heads)
         return self.o(out.view(x.shape))
@@ -582,19 +692,56 @@ class SelfAttention(nn.Module):
             if self.training and self.cam_dropout_p > 0:
                 cam_tokens = torch.nn.functional.dropout(cam_tokens, p=self.cam_dropout_p,
                                                          training=True)
-        if train:
-            from .train import prologue_grad
-            prep = prologue_grad
-        else:
-            prep = hier_prep_qk
-        q, k = prep(
-            self.q(x).reshape(B * L, dim), self.k(x).reshape(B * L, dim), freqs, self.num_heads,
-            norm_q_weight=self.norm_q.weight, norm_k_weight=self.norm_k.weight,
-            cam_tokens=cam_tokens, cam_q_weight=None if self.cam_q is None else self.cam_q.weight,
-            cam_k_weight=None if self.cam_k is None else self.cam_k.weight, eps=self.norm_q.eps)
+        q, k = self._prologue(self.q(x).reshape(B * L, dim), self.k(x).reshape(B * L, dim), freqs,
+                              cam_tokens, train=train)
         out = shared_mask_attention(q.view(B, L, dim), k.view(B, L, dim), self.v(x),
                                     self.num_heads, mask)
         return self.o(out)
+
+
+    @torch.no_grad()
+    def paged_forward(self, x, freqs, cache, table, step, *, tokens_per_frame=1, block_frames=1,
+                      window=-1, cam_tokens=None, max_rows=None):
+        """Self-attention of the new tokens of several requests against an 8-bit
+        paged cache (:mod:`multics_b200.paged8`), which takes their keys and
+        values first.  ``x`` ``[T, dim]`` (or ``[1, T, dim]``) holds the tokens
+        request by request, ``step`` is the :func:`~multics_b200.paged8.page_step`
+        that placed them, ``table`` its block table; ``freqs`` is indexed by a
+        token's position in its request.  Rows behind the last request give the
+        output projection's bias.  Masks as in
+        :func:`~multics_b200.paged8.paged8_attention`."""
+        from .paged8 import paged8_append, paged8_attention
+
+        if cam_tokens is not None and (self.cam_q is None or self.cam_k is None):
+            raise RuntimeError("camera_pose was provided but enable_camera_pose_qk() was not called")
+        T = x.shape[-2]
+        if x.dim() not in (2, 3) or x.numel() != T * self.dim or step.positions.shape[0] != T:
+            raise ValueError(f"x {tuple(x.shape)} does not hold the step's "
+                             f"{step.positions.shape[0]} rows of {self.dim}")
+        if cam_tokens is not None and cam_tokens.shape[-2] != T:
+            raise ValueError(f"camera tokens {tuple(cam_tokens.shape)} must match the {T} rows")
+        x2 = x.reshape(T, self.dim)
+        cam = None if cam_tokens is None else cam_tokens.reshape(T, -1)
+        qx, kx, v = self.q(x2), self.k(x2), self.v(x2)
+        ft = freqs if (freqs.dtype == torch.float32 and freqs.dim() == 3
+                       and freqs.shape[-1] == 2) else freqs_table(freqs)
+        if self.head_norm:
+            if cam is not None:
+                qx, kx = qx + self.cam_q(cam.to(qx)), kx + self.cam_k(cam.to(kx))
+            q, k = hier_head_norm_rope(qx, kx, ft, self.num_heads, self.num_heads,
+                                       q_weight=self.norm_q.weight, k_weight=self.norm_k.weight,
+                                       positions=step.positions, eps=self.norm_q.eps)
+        else:
+            ft, pos = ft.to(x.device), step.positions
+            # a position past the table reads NaN, which the cache reports
+            rows = ft[pos.clamp(0, ft.shape[0] - 1).long()].masked_fill(
+                (pos >= ft.shape[0])[:, None, None], float("nan"))
+            q, k = self._prologue(qx, kx, rows, cam) if T else (qx, kx)
+        paged8_append(cache, k, v, table, step.lengths, step.q_start)
+        out = paged8_attention(q, cache, table, step.lengths, step.q_start, self.num_heads,
+                               tokens_per_frame=tokens_per_frame, block_frames=block_frames,
+                               window=window, max_rows=max_rows)
+        return self.o(out).view(x.shape)
 
 
 class CrossAttention(nn.Module):

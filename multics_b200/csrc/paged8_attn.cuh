@@ -1,0 +1,147 @@
+// What the attention kernels over an 8-bit paged cache share: their arguments,
+// the tiles of rows a call is cut into, and the exponents of its rows.
+//
+// out[r, h] = sum_j softmax_j(scale q[r, h] . (sk K8[j])) sv V8[j] over the keys
+// that row r sees.  A tile is `kRows` consecutive (row, head of the key head's
+// group) pairs of one request, row-major: rho = row * G + g.  Tile t of request
+// b is number q_start[b] * G / kRows + b + t, so a launch needs no count from
+// the device; numbers between the requests' tiles are empty.  The rows behind
+// the last request are tiles of the "request" n.
+//
+// The page scales never touch the codes: a page's key scale multiplies its
+// scores, and its value scale 2^ve is added to their exponents, so that with
+//   x_j = scale log2(e) sk q.k_j + ve,   m = max x_j,   p_j = 2^(x_j - m)
+// the product sum p_j V8[j] is the output times 2^-m, p_j is at most 1 (fp16
+// keeps 11 bits of it whatever the pages' scales are), and the softmax's
+// denominator is sum p_j 2^-ve.
+#pragma once
+
+#include "paged8.cuh"
+
+namespace hier {
+
+struct Paged8Args {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  int rows, heads, kv_heads, group;
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* k_scale;
+  const float* v_scale;
+  int n_pages;
+  const int32_t* table;
+  int64_t table_stride;
+  int width;
+  const int32_t* lengths;
+  const int32_t* q_start;
+  int n;
+  Paged8Mask mask;
+  float scale_log2;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  float* lse;       // [rows][heads] log2-sum-exp, or NULL
+  int zero_tail;    // write zeros to the rows behind the last request
+  int splits;       // most parts a tile's keys are cut into
+  float* part_o;    // [tile][kv head][split][kRows][128]
+  float* part_ml;   // [tile][kv head][split][kRows][2]
+  int row_limit;    // small kernel: requests of more row-head pairs are left to the large one
+  int32_t* status;
+};
+
+template <int kRows>
+__host__ __device__ inline int64_t paged8_tiles(int64_t rows, int group, int n) {
+  return rows * group / kRows + n + 1;
+}
+
+struct Paged8Tile {
+  int b;
+  Paged8Request rq;
+  int rho0, pairs;  // first pair of the tile, pairs of the request
+  int lo, hi;       // keys the tile's rows see between them
+  int p0, np;       // their pages
+  bool live;
+};
+
+// position of row i of a request; negative rows see nothing
+__device__ __forceinline__ int row_pos(const Paged8Request& r, int i) { return r.held - r.n + i; }
+
+__device__ __forceinline__ void row_keys(const Paged8Args& a, const Paged8Request& r, int i, int& lo,
+                                         int& hi) {
+  const int pos = row_pos(r, i);
+  if (pos >= 0) {
+    lo = a.mask.first(pos);
+    hi = a.mask.end(pos, r.held);
+  } else {  // rows beyond the held tokens see keys only where positions do not matter
+    lo = 0;
+    hi = a.mask.block == 0 && a.mask.window < 0 ? r.held : 0;
+  }
+}
+
+template <int kRows>
+__device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t tile, bool report) {
+  Paged8Tile t;
+  const int32_t* qs = a.q_start;
+  const int64_t G = a.group;
+  t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
+  t.live = false;
+  t.rho0 = t.pairs = t.lo = t.hi = t.p0 = t.np = 0;
+  const int64_t first = qs[t.b] * G / kRows + t.b;
+  if (tile < first) return t;
+  const int64_t rho0 = (tile - first) * kRows;
+  if (t.b == a.n) {  // rows behind the last request
+    t.rq.row0 = qs[a.n];
+    t.rq.n = a.rows - t.rq.row0;
+    t.rq.held = 0;
+    t.rq.ok = t.rq.row0 >= 0 && t.rq.n > 0;
+    if (!t.rq.ok || rho0 >= t.rq.n * G) return t;
+  } else {
+    t.rq = paged8_request(a.q_start, a.lengths, t.b, a.rows, a.width, false,
+                          report ? a.status : nullptr);
+    if (t.rq.row0 < 0 || t.rq.n <= 0 || t.rq.row0 + (int64_t)t.rq.n > a.rows ||
+        rho0 >= t.rq.n * G)
+      return t;
+    if (!t.rq.ok) t.rq.held = 0;  // a length outside the table: the rows see nothing
+  }
+  t.live = true;
+  t.rho0 = (int)rho0;
+  t.pairs = (int)(t.rq.n * G);
+  if (t.b == a.n) return t;
+  const int last = min(t.pairs, t.rho0 + kRows) - 1;
+  int unused;
+  row_keys(a, t.rq, t.rho0 / a.group, t.lo, unused);
+  row_keys(a, t.rq, last / a.group, unused, t.hi);
+  if (t.hi > t.lo) {
+    t.p0 = t.lo / kPage;
+    t.np = (t.hi + kPage - 1) / kPage - t.p0;
+  }
+  return t;
+}
+
+// parts that np pages are really cut into: at least kMin pages each
+template <int kMin>
+__device__ __forceinline__ int parts_of(int np, int splits) {
+  return max(1, min(splits, np / kMin));
+}
+
+// power of two that brings a row's largest magnitude into [2^14, 2^15) in
+// fp16: bf16 values keep all their bits there down to 2^-28 of the largest
+__device__ __forceinline__ int fp16_shift(float amax) {
+  if (!(amax > 0.f) || !(amax < INFINITY)) return 0;
+  return min(120, 14 - ilogbf(amax));
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// exponent of a power-of-two scale
+__device__ __forceinline__ int scale_log2_of(float s) {
+  return (int)((__float_as_uint(s) >> 23) & 0xffu) - 127;
+}
+
+int paged8_launch_small(const Paged8Args& a, int format, int warps, int64_t units, cudaStream_t st);
+int paged8_launch_large(const Paged8Args& a, int format, int64_t tiles, cudaStream_t st);
+
+}  // namespace hier

@@ -1,0 +1,330 @@
+"""Key/value caches held in 8 bits, in pages: several sessions served at once
+from one pool.
+
+The reference keeps bf16 rolling caches per session and lists their rows in a
+page table (``multics/models/kernels/hier_paged_attention.py:232-249``).  Here
+a pool of 64-token pages holds int8 or e4m3 codes with one power-of-two scale
+per page and head (:class:`Paged8Cache`), half the bytes of bf16, and the
+tables are built on the GPU:
+
+* :func:`page_step` - block tables, slots and positions of one step from the
+  requests' lengths (tokens appended, dropped, requests ended);
+* :func:`paged8_append` - the new keys and values into their pages;
+* :func:`paged8_attention` - attention of the new rows over the pages, causal
+  by blocks of latent frames and windowed like the action branch's masks
+  (``multics/models/blocks.py:300-305,366-371``).
+
+None of them reads back from the device, so a step can be captured into a CUDA
+graph.  What a kernel finds wrong in device tables (a page outside the pool, a
+length outside the table) it skips and records in the cache's status word
+(:meth:`Paged8Cache.check`).
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from ._lib import check, ptr, stream_ptr
+
+__all__ = ["PAGE_TOKENS", "Paged8Cache", "PageStep", "page_step", "paged8_append",
+           "paged8_attention"]
+
+PAGE_TOKENS = 64
+HEAD_DIM = 128
+_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_STATUS = {}
+
+_CACHE_BITS = ((1, "row starts leave the rows or descend"),
+               (2, "a length leaves the block table"),
+               (4, "a block table entry leaves the page pool"),
+               (8, "a NaN or an infinity was given to the cache"))
+_STEP_BITS = ((1, "too few free pages"), (2, "more new tokens than rows"),
+              (4, "a length leaves the block table"),
+              (8, "an addition is below -length or above the step's most"),
+              (16, "the free count leaves the free list"))
+
+
+def on_device(dev):
+    """A context in which ``dev`` is the current device (none when it is)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _need(name, t, dtype, dev, dim):
+    if t.dtype != dtype or t.dim() != dim:
+        raise ValueError(f"{name} must be {dtype} with {dim} dimension(s), got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+
+
+def _vector(name, t, n, dev):
+    _need(name, t, torch.int32, dev, 1)
+    if t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{n}], got {tuple(t.shape)}")
+
+
+def _cuda(what, dev):
+    if dev.type != "cuda":
+        raise NotImplementedError(f"{what} requires CUDA tensors")
+
+
+def _raise_bits(what, bits, table):
+    if bits:
+        raise ValueError(f"{what}: " + "; ".join(msg for bit, msg in table if bits & bit))
+
+
+def token_rows(name, x, width):
+    """``x`` ``[T, width]`` or ``[1, T, width]`` bf16 as 16-byte aligned rows."""
+    if x.dim() == 3 and x.shape[0] == 1:
+        x = x[0]
+    if x.dim() != 2 or x.shape[1] != width:
+        raise ValueError(f"{name} must be [T, {width}], got {tuple(x.shape)}")
+    if x.dtype != torch.bfloat16:
+        raise NotImplementedError(f"{name} must be bf16; got {x.dtype}")
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < width or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+class Paged8Cache:
+    """A pool of ``num_pages`` pages of 64 tokens of ``num_heads`` key heads.
+
+    ``k`` ``[pages, heads, 2, 64, 64]`` (dimension half, token, dimension) and
+    ``v`` ``[pages, heads, 128, 64]`` (dimension, token) hold the codes (int8 or
+    float8_e4m3fn), ``k_scale`` / ``v_scale`` float32 ``[pages, heads]`` their
+    power-of-two scales.  int8 has the finer steps for values of like size,
+    e4m3 for values spread over many magnitudes.  The cache holds finite
+    numbers: a NaN is held as 0 and an infinity as the largest value of its
+    block, and :meth:`check` reports it."""
+
+    def __init__(self, num_pages: int, num_heads: int, *, dtype=torch.int8, device="cuda",
+                 head_dim: int = HEAD_DIM):
+        if head_dim != HEAD_DIM:
+            raise NotImplementedError(f"the 8-bit cache needs head_dim {HEAD_DIM}; got {head_dim}")
+        if dtype not in _FORMATS:
+            raise ValueError(f"dtype must be torch.int8 or torch.float8_e4m3fn, got {dtype}")
+        if num_pages < 1 or num_heads < 1:
+            raise ValueError(f"invalid num_pages={num_pages} or num_heads={num_heads}")
+        dev = torch.device(device)
+        shape = (num_pages, num_heads)
+        self._set(torch.zeros(*shape, 2, PAGE_TOKENS, 64, dtype=torch.int8, device=dev).view(dtype),
+                  torch.zeros(*shape, HEAD_DIM, PAGE_TOKENS, dtype=torch.int8, device=dev).view(dtype),
+                  torch.ones(shape, device=dev), torch.ones(shape, device=dev),
+                  torch.zeros(1, dtype=torch.int32, device=dev))
+
+    def _set(self, k, v, k_scale, v_scale, status):
+        self.k, self.v, self.k_scale, self.v_scale, self.status = k, v, k_scale, v_scale, status
+        self.num_pages, self.num_heads = k.shape[0], k.shape[1]
+        self.dtype, self.device = k.dtype, k.device
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale, v_scale, status=None) -> "Paged8Cache":
+        """A cache over tensors in the layout above (finite codes, power-of-two
+        scales).  Without ``status`` (int32 ``[1]``, zero) the caches made this
+        way share one word per device."""
+        if k.dtype not in _FORMATS or v.dtype != k.dtype:
+            raise ValueError(f"codes must both be int8 or float8_e4m3fn, got {k.dtype}, {v.dtype}")
+        if k.dim() != 5 or tuple(k.shape[2:]) != (2, PAGE_TOKENS, 64):
+            raise ValueError(f"k must be [pages, heads, 2, 64, 64], got {tuple(k.shape)}")
+        if tuple(v.shape) != (*k.shape[:2], HEAD_DIM, PAGE_TOKENS):
+            raise ValueError(f"v must be [pages, heads, 128, 64] like k {tuple(k.shape)}, got "
+                             f"{tuple(v.shape)}")
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if s.dtype != torch.float32 or s.shape != k.shape[:2]:
+                raise ValueError(f"{name} must be float32 {tuple(k.shape[:2])}, got {s.dtype} "
+                                 f"{tuple(s.shape)}")
+        for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
+            if not t.is_contiguous() or t.device != k.device:
+                raise ValueError(f"{name} must be contiguous on {k.device}")
+        if status is None:
+            status = _STATUS.get(k.device)
+            if status is None:
+                status = _STATUS[k.device] = torch.zeros(1, dtype=torch.int32, device=k.device)
+        else:
+            _vector("status", status, 1, k.device)
+        self = cls.__new__(cls)
+        self._set(k, v, k_scale, v_scale, status)
+        return self
+
+    def check(self):
+        """Raise ValueError for what the kernels recorded since the last check
+        (one host read)."""
+        bits = int(self.status.item())
+        self.status.zero_()
+        _raise_bits("8-bit cache", bits, _CACHE_BITS)
+
+    def dequantized(self):
+        """The pool's keys and values as bf16 ``[pages, heads, 64, 128]`` (exact)."""
+        k = self.k.float() * self.k_scale[..., None, None, None]
+        v = self.v.float() * self.v_scale[..., None, None]
+        return (k.permute(0, 1, 3, 2, 4).flatten(3).bfloat16(), v.transpose(2, 3).bfloat16())
+
+
+class PageStep(NamedTuple):
+    """What :func:`page_step` built: the requests' new ``lengths``, the
+    ``free_count`` left, ``q_start`` ``[n + 1]`` of their rows, and per row its
+    ``slots`` entry (page * 64 + token of the page: the row of a 64-token paged
+    pool) and ``positions`` entry, -1 behind the last request.  int32 on the
+    device."""
+
+    lengths: torch.Tensor
+    free_count: torch.Tensor
+    q_start: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    status: torch.Tensor
+
+    def check(self):
+        """Raise ValueError when the step could not be taken (one host read)."""
+        _raise_bits("page step refused", int(self.status.item()), _STEP_BITS)
+
+
+def page_step(lengths, add, table, free_pages, free_count, rows: int, *,
+              most_new: Optional[int] = None, in_place: bool = False) -> PageStep:
+    """One step of a paged cache's bookkeeping, on the GPU: request ``b`` goes
+    from ``lengths[b]`` to ``lengths[b] + add[b]`` tokens (``add < 0`` drops its
+    last tokens, ``-lengths[b]`` ends it).
+
+    ``table`` int32 ``[n, width]`` (row-major, updated) lists each request's
+    pages; ``free_pages`` int32 (updated) is a stack of ``free_count`` (int32
+    ``[1]``) free pages: pages given up are put on its end, pages needed are
+    taken from there, both in request order.  ``rows`` is the number of rows of
+    the step's token tensors; the new tokens fill them request by request.  A
+    step that cannot be taken whole (too few pages or rows, a length outside the
+    table, an addition above ``most_new``) changes nothing and maps no row;
+    :meth:`PageStep.check` reports it.  ``in_place`` writes the new lengths and
+    count over the old ones (a captured step)."""
+    dev = table.device
+    _need("table", table, torch.int32, dev, 2)
+    n, width = table.shape
+    if n and width and (table.stride(1) != 1 or table.stride(0) < width):
+        raise ValueError("table must be row-major")
+    _vector("lengths", lengths, n, dev)
+    _vector("add", add, n, dev)
+    _vector("free_pages", free_pages, free_pages.shape[0], dev)
+    _vector("free_count", free_count, 1, dev)
+    rows = int(rows)
+    if rows < 0 or rows >= 1 << 31:
+        raise ValueError(f"rows must be in [0, 2^31), got {rows}")
+    if most_new is not None and most_new < 0:
+        raise ValueError(f"most_new must not be negative, got {most_new}")
+    _cuda("page_step", dev)
+    held, count = (0, 0) if in_place else (n, 1)
+    with on_device(dev):
+        out = torch.empty(held + count + n + 2 + 2 * rows, dtype=torch.int32, device=dev)
+        new_len, new_count, q_start, status, slots, positions = out.split(
+            (held, count, n + 1, 1, rows, rows))
+        if in_place:
+            new_len, new_count = lengths, free_count
+        check(_lib.lib().hier_page_step(
+            ptr(lengths), ptr(add), n, ptr(table), max(table.stride(0), width), width,
+            ptr(free_pages), free_pages.shape[0], ptr(free_count), rows,
+            -1 if most_new is None else int(most_new), ptr(new_len), ptr(new_count), ptr(q_start),
+            ptr(slots), ptr(positions), ptr(status), stream_ptr(dev)))
+    return PageStep(new_len, new_count, q_start, slots, positions, status)
+
+
+def _requests(cache, table, lengths, q_start):
+    _need("table", table, torch.int32, cache.device, 2)
+    n, width = table.shape
+    if n and width and (table.stride(1) != 1 or table.stride(0) < width):
+        raise ValueError("table must be row-major")
+    _vector("lengths", lengths, n, cache.device)
+    _vector("q_start", q_start, n + 1, cache.device)
+    return n, width
+
+
+def paged8_append(cache: Paged8Cache, k, v, table, lengths, q_start):
+    """Write the new rows ``k``, ``v`` (bf16 ``[T, heads * 128]``) of every
+    request into its pages: rows ``q_start[b] .. q_start[b + 1] - 1`` are the
+    last of request ``b``'s ``lengths[b]`` tokens.  A page written to must
+    belong to one request (pages that several requests list are for reading).
+    When a page's scale grows, the codes it held are re-encoded."""
+    width_k = cache.num_heads * HEAD_DIM
+    k, v = token_rows("k", k, width_k), token_rows("v", v, width_k)
+    if k.shape != v.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} disagree")
+    n, width = _requests(cache, table, lengths, q_start)
+    _cuda("paged8_append", cache.device)
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError(f"k, v must be on {cache.device}")
+    with on_device(cache.device):
+        check(_lib.lib().hier_paged8_append(
+            ptr(k), k.stride(0), ptr(v), v.stride(0), k.shape[0], cache.num_heads,
+            _FORMATS[cache.dtype], ptr(cache.k), ptr(cache.v), ptr(cache.k_scale),
+            ptr(cache.v_scale), cache.num_pages, ptr(table), max(table.stride(0), width), width,
+            ptr(lengths), ptr(q_start), n, ptr(cache.status), stream_ptr(cache.device)))
+
+
+def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: int, *,
+                     tokens_per_frame: int = 1, block_frames: int = 1, window: int = -1,
+                     softmax_scale: Optional[float] = None, max_rows: Optional[int] = None,
+                     out=None, return_lse: bool = False):
+    """Attention of the rows ``q`` (bf16 ``[T, num_heads * 128]``) over an
+    8-bit cache; ``num_heads`` is a multiple of the cache's heads, consecutive
+    query heads sharing a key head.
+
+    Row ``i`` of request ``b`` is at position ``p = lengths[b] - rows + i`` (the
+    rows are the last tokens held; append first).  In frames of
+    ``tokens_per_frame`` tokens, token ``j`` is seen when its block of
+    ``block_frames`` frames is not after ``p``'s (``block_frames=0``: always, as
+    in a cross-attention) and, with a ``window``, when it is less than
+    ``window`` frames back: ``cached_frame_mask`` over token positions.
+    Rows that see nothing are 0.  Rows behind the last request are zeros, or
+    left as they were in a given ``out``.  ``max_rows``: the most rows any
+    request has, where the caller knows it; it chooses kernels, not results.
+    Returns ``[T, num_heads * 128]`` bf16, with ``return_lse`` also the float32
+    ``[T, num_heads]`` log2-sum-exp of the scaled scores."""
+    if num_heads < 1 or num_heads % cache.num_heads:
+        raise ValueError(f"{num_heads} query heads are not a multiple of the cache's "
+                         f"{cache.num_heads}")
+    if tokens_per_frame < 1 or block_frames < 0 or window == 0 or window < -1:
+        raise ValueError(f"invalid tokens_per_frame={tokens_per_frame}, "
+                         f"block_frames={block_frames} or window={window}")
+    if max(tokens_per_frame, block_frames, window) > 1 << 30:
+        raise ValueError("tokens_per_frame, block_frames and window must be below 2^30")
+    if max_rows is not None and max_rows < 0:
+        raise ValueError(f"max_rows must not be negative, got {max_rows}")
+    dim = num_heads * HEAD_DIM
+    q = token_rows("q", q, dim)
+    n, width = _requests(cache, table, lengths, q_start)
+    dev, T = cache.device, q.shape[0]
+    if out is not None and (out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != dev
+                            or out.stride(1) != 1 or (T > 1 and out.stride(0) < dim)):
+        raise ValueError(f"out must be bf16 {tuple(q.shape)} rows on {dev}")
+    _cuda("paged8_attention", dev)
+    if q.device != dev:
+        raise ValueError(f"q must be on {dev}")
+    scale = 1.0 / math.sqrt(HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    zero_tail = out is None
+    most = 0 if max_rows is None else int(max_rows)
+    L = _lib.lib()
+    with on_device(dev):
+        given = out
+        if out is None:
+            out = torch.empty((T, dim), dtype=torch.bfloat16, device=dev)
+        elif out.data_ptr() % 16 or out.stride(0) % 8:  # rows the kernels cannot store to
+            out = out.clone(memory_format=torch.contiguous_format)
+        lse = torch.empty((T, num_heads), dtype=torch.float32, device=dev) if return_lse else None
+        floats = ctypes.c_int64()
+        check(L.hier_paged8_attn_workspace(T, num_heads, cache.num_heads, n, width, most,
+                                           ctypes.byref(floats)))
+        ws = (torch.empty(floats.value, dtype=torch.float32, device=dev) if floats.value else None)
+        check(L.hier_paged8_attn(
+            ptr(q), q.stride(0), T, num_heads, cache.num_heads, HEAD_DIM, _FORMATS[cache.dtype],
+            ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), cache.num_pages,
+            ptr(table), max(table.stride(0), width), width, ptr(lengths), ptr(q_start), n,
+            int(tokens_per_frame), int(block_frames), int(window), scale, most, ptr(out),
+            out.stride(0), ptr(lse), int(zero_tail), ptr(ws), ptr(cache.status),
+            stream_ptr(dev)))
+        if given is not None and out is not given:
+            out = given.copy_(out)
+    return (out, lse) if return_lse else out

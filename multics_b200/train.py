@@ -29,7 +29,7 @@ from .attention import _dev_err, _rows
 from .hier_masks import HierBlockMask
 
 __all__ = ["BlockPlanGrad", "block_plan_grad", "hier_block_attention_grad", "plan_attention_grad",
-           "prologue_grad"]
+           "prologue_grad", "head_norm_rope_grad"]
 
 
 def _plan_extent(plan):
@@ -230,6 +230,62 @@ def prologue_grad(qx, kx, freqs, num_heads, *, norm_q_weight, norm_k_weight, cam
     ft = ft.to(qx.device).contiguous()
     return _PrologueFn.apply(qx, kx, norm_q_weight, norm_k_weight, cam_q_weight, cam_k_weight,
                              cam_tokens, ft, num_heads, eps)
+
+
+class _HeadNormFn(torch.autograd.Function):
+    """Per-head RMSNorm + RoPE of q and k with the fused kernels both ways
+    (``hier_head_norm_rope`` / ``hier_head_norm_rope_bwd``)."""
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, ft, positions, num_heads, num_kv_heads, eps):
+        from .attention import hier_head_norm_rope
+
+        ctx.save_for_backward(q, k, wq, wk, ft, positions)
+        ctx.sizes = num_heads, num_kv_heads, eps
+        return hier_head_norm_rope(q, k, ft, num_heads, num_kv_heads, q_weight=wq, k_weight=wk,
+                                   positions=positions, eps=eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        from .attention import head_norm_args
+        from .paged8 import on_device, token_rows
+
+        q, k, wq0, wk0, ft, positions = ctx.saved_tensors
+        H, Hk, eps = ctx.sizes
+        q2, k2, D, wq, wk, ft, pos = head_norm_args(q, k, ft, H, Hk, wq0, wk0, positions)
+        T, dev = q2.shape[0], q2.device
+        L = _lib.lib()
+        with on_device(dev):
+            gq = (torch.zeros((T, H * D), dtype=torch.bfloat16, device=dev) if gq is None
+                  else token_rows("gradient of q", gq.to(torch.bfloat16), H * D))
+            gk = (torch.zeros((T, Hk * D), dtype=torch.bfloat16, device=dev) if gk is None
+                  else token_rows("gradient of k", gk.to(torch.bfloat16), Hk * D))
+            dq = torch.empty((T, H * D), dtype=torch.bfloat16, device=dev)
+            dk = torch.empty((T, Hk * D), dtype=torch.bfloat16, device=dev)
+            dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+            n = ctypes.c_int32()
+            check(L.hier_head_norm_rope_bwd_partials(T, H, Hk, D, ctypes.byref(n)))
+            part = torch.empty((n.value, 2, D), dtype=torch.float32, device=dev)
+            check(L.hier_head_norm_rope_bwd(
+                ptr(q2), q2.stride(0), ptr(k2), k2.stride(0), T, H, Hk, D, ptr(wq), ptr(wk),
+                int(wq.dtype == torch.float32), ptr(ft), ft.shape[0], ptr(pos), float(eps), ptr(gq),
+                gq.stride(0), ptr(gk), gk.stride(0), ptr(dq), dq.stride(0), ptr(dk), dk.stride(0),
+                ptr(part), n.value, ptr(dwq), ptr(dwk), ptr(_dev_err(dev)), stream_ptr(dev)))
+            return (dq.view(q.shape), dk.view(k.shape), dwq.to(wq0.dtype), dwk.to(wk0.dtype), None,
+                    None, None, None, None)
+
+
+def head_norm_rope_grad(q, k, freqs, num_heads: int, num_kv_heads: int, *, q_weight, k_weight,
+                        positions=None, eps=1e-6):
+    """Differentiable :func:`~multics_b200.attention.hier_head_norm_rope`: roped
+    ``(q, k)`` with gradients for q, k and the norm weights (the weights'
+    gradients are sums over all rows and heads in a fixed order)."""
+    from .attention import freqs_table
+
+    ft = freqs if (freqs.dtype == torch.float32 and freqs.dim() == 3
+                   and freqs.shape[-1] == 2) else freqs_table(freqs)
+    return _HeadNormFn.apply(q, k, q_weight, k_weight, ft, positions, num_heads, num_kv_heads, eps)
 
 
 def hier_block_attention_grad(q, k, v, mask, num_heads: int, *, softmax_scale=None):
