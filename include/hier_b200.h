@@ -819,8 +819,9 @@ int hier_paged8_append(const void* k, int64_t k_stride, const void* v, int64_t v
  * behind the last request are left, or zeroed with zero_tail.  lse (or NULL):
  * float [rows][heads], log2-sum-exp of the scaled scores.  max_rows: the most
  * rows a request has, as far as the caller knows (it chooses kernels, not
- * results); <= 0: unknown.  workspace: floats of ..._workspace for the same
- * sizes. */
+ * results); <= 0: unknown.  softmax_scale is positive and finite.  workspace:
+ * floats of ..._workspace for the same sizes.  dev_err: the kernels' sticky
+ * timeout word. */
 int hier_paged8_attn_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t n,
                                int32_t width, int32_t max_rows, int64_t* floats);
 int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, int32_t heads,
@@ -830,7 +831,7 @@ int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, int32_t head
                      const int32_t* lengths, const int32_t* q_start, int32_t n, int32_t frame,
                      int32_t block, int32_t window, float softmax_scale, int32_t max_rows,
                      void* out, int64_t out_stride, float* lse, int32_t zero_tail,
-                     float* workspace, int32_t* status, void* stream);
+                     float* workspace, int32_t* status, int32_t* dev_err, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Self-test of the tensor-core operand encodings (no reference counterpart):

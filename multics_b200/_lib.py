@@ -215,7 +215,7 @@ _SIGS = {
     "hier_paged8_attn": (c_int, [_P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P,
                                  _P, _P, c_int32, _P, c_int64, c_int32, _P, _P, c_int32, c_int32,
                                  c_int32, c_int32, c_float, c_int32, _P, c_int64, _P, c_int32, _P,
-                                 _P, _P]),
+                                 _P, _P, _P]),
     "hier_selftest_umma": (c_int, [_P, _P, _P, _P, _P, _P, _P]),
     "hier_selftest_wait_timeout": (c_int, [c_int64, _P, _P, _P]),
 }

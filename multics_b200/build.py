@@ -19,7 +19,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libhier_b200.so"
 SOURCES = ["hier_capi.cu", "hier_meta.cu", "hier_prep.cu", "hier_attn.cu", "hier_selftest.cu",
            "hier_cached.cu", "hier_tiled.cu", "hier_shard.cu", "hier_bwd.cu", "hier_head_norm.cu",
-           "hier_paged8.cu", "hier_paged8_attn.cu"]
+           "hier_paged8.cu", "hier_paged8_attn.cu", "hier_paged8_mma.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

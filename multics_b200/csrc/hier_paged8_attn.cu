@@ -18,12 +18,14 @@
 // fp32 with their maximum and sum, merged in split order by a second kernel)
 // and over the four warps of a block (merged in shared memory).
 
+#include <math.h>
+
 #include "paged8_attn.cuh"
 
 namespace hier {
 namespace {
 
-constexpr int kRows = 8;
+constexpr int kRows = kPaged8SmallRows;
 constexpr int kWarps = 4;
 constexpr int kPitch = 132;  // floats: 8 x 4 lanes of one store fall into 32 banks
 
@@ -314,26 +316,34 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged8_small_kernel(Paged8Args
   }
 }
 
-// The parts of a tile's keys joined in split order; one warp per (row, head) pair.
-template <int WPU>
-__global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a) {
-  const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int kvh = blockIdx.x % a.kv_heads;
-  const int64_t tile_id = blockIdx.x / a.kv_heads;
-  const Paged8Tile tl = paged8_tile<kRows>(a, tile_id, false);
-  if (!tl.live || tl.b == a.n || tl.pairs > a.row_limit) return;
-  const int parts = parts_of<kMinPages<WPU>>(tl.np, a.splits);
+// The parts of a tile's keys joined in split order; one warp per (row, head)
+// pair.  The large kernel numbers its tiles from the last and counts its parts
+// in 128-key tiles.
+template <int kTileRows>
+__global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t tiles) {
+  constexpr bool kLarge = kTileRows == kPaged8LargeRows;
+  constexpr int kGroups = kTileRows / 8;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = blockIdx.x / kGroups;  // (tile, key head) as its kernel numbers them
+  const int r = (int)(blockIdx.x % kGroups) * 8 + (threadIdx.x >> 5);
+  const int kvh = (int)(unit % a.kv_heads);
+  const int64_t tile = kLarge ? tiles - 1 - unit / a.kv_heads : unit / a.kv_heads;
+  const Paged8Tile tl = paged8_tile<kTileRows>(a, tile, false);
+  if (!tl.live || tl.b == a.n || (tl.pairs <= a.row_limit) == kLarge) return;
+  const int parts = kLarge ? parts_of<kPaged8LargeMin>((tl.np + 1) / 2, a.splits)
+                           : parts_of<kMinPages<4>>(tl.np, a.splits);
   const int pr = tl.rho0 + r;
   if (parts == 1 || pr >= tl.pairs) return;
-  const int64_t at = (int64_t)blockIdx.x * a.splits * kRows + r;
+  const int64_t at = unit * a.splits * kTileRows + r;
   float M = -INFINITY;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[(at + s * kRows) * 2]);
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[(at + (int64_t)s * kTileRows) * 2]);
   const float ref = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[4] = {};
 #pragma unroll 4
   for (int s = 0; s < parts; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at + s * kRows) * 2);
-    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (at + s * kRows) * 128 + 4 * lane);
+    const int64_t ps = at + (int64_t)s * kTileRows;
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + ps * 2);
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + ps * 128 + 4 * lane);
     const float f = ex2_approx(ml.x - ref);
     L = fmaf(ml.y, f, L);
     acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
@@ -347,55 +357,83 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a) {
   if (a.lse && lane == 0) a.lse[orow * a.heads + oh] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
-// How a call of the small kernel is cut: warps per tile and parts of its keys.
-struct SmallShape {
-  int warps, splits;
-  int64_t units;
+// How a call is cut, from the sizes the host knows (the same for every content
+// of the device tables).  Requests of up to kSmallPairs (row, head) pairs per
+// key head run on the small kernel, longer ones on the large one; a call that
+// may hold both runs both, each leaving the other's requests.
+constexpr int kSmallPairs = 16;
+
+struct Shape {
+  bool small, large;
+  int direct, warps, small_splits, large_splits;
+  int64_t small_tiles, large_tiles;
+  int64_t floats;  // workspace: the small kernel's parts, then the large one's
+  int64_t small_floats;
 };
 
-// Enough warps to keep the memory busy (about 8 per SM), from the sizes the
-// host knows: the tiles that can be there and the pages a table row can list.
-SmallShape small_shape(int64_t tiles, int kv_heads, int pages) {
-  SmallShape s = {1, 1, 0};
-  const int64_t work = tiles * kv_heads;
-  if (pages > 4) {
-    s.warps = 4;
-    const int64_t want = (148 * 2 + work - 1) / work;
-    s.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
-    const int most = pages / 8 < 1 ? 1 : pages / 8;
-    if (s.splits > most) s.splits = most;
+int clamp_int(int64_t v, int64_t lo, int64_t hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
+
+Shape shape_of(int64_t rows, int group, int kv_heads, int n, int width, int max_rows) {
+  Shape s = {};
+  const int64_t most = max_rows > 0 && max_rows < rows ? max_rows : rows;
+  const int64_t some = n < rows ? n : rows;  // requests that can have rows
+  s.small = most * group <= kSmallPairs || n > 1;
+  s.large = most * group > kSmallPairs;
+  if (s.small) {
+    s.direct = s.large ? (kSmallPairs + kRows - 1) / kRows : 0;
+    s.small_tiles = s.large ? (int64_t)n * s.direct : paged8_tiles<kRows>(rows, group, n);
+    // tiles that are likely there, to size the splits by
+    int64_t real = s.large ? some : (rows * group + kRows - 1) / kRows;
+    if (real < some) real = some;
+    s.warps = width > 4 ? 4 : 1;
+    s.small_splits = 1;
+    if (s.warps == 4) {
+      const int64_t want = (148 * 2 + real * kv_heads - 1) / (real * kv_heads);
+      s.small_splits = clamp_int(want, 1, clamp_int(width / kMinPages<4>, 1, 64));
+    }
+    if (s.small_splits > 1) s.small_floats = s.small_tiles * kv_heads * s.small_splits * kRows * 130;
   }
-  s.units = work * s.splits;
+  if (s.large) {
+    s.large_tiles = paged8_tiles<kPaged8LargeRows>(rows, group, n);
+    const int64_t real = (rows * group + kPaged8LargeRows - 1) / kPaged8LargeRows;
+    const int64_t work = real * kv_heads;
+    s.large_splits = clamp_int(148 / work, 1, clamp_int(width / (2 * kPaged8LargeMin), 1, 16));
+  }
+  s.floats = s.small_floats;
+  if (s.large_splits > 1)
+    s.floats += s.large_tiles * kv_heads * s.large_splits * kPaged8LargeRows * 130;
   return s;
 }
 
-}  // namespace
+template <int kTileRows>
+int launch_merge(const Paged8Args& a, int64_t tiles, cudaStream_t st) {
+  const int64_t blocks = tiles * a.kv_heads * (kTileRows / 8);
+  if (blocks > INT32_MAX) {
+    set_error(HIER_EVALUE, "too many rows, requests and heads");
+    return HIER_EVALUE;
+  }
+  paged8_merge_kernel<kTileRows><<<(unsigned)blocks, 256, 0, st>>>(a, tiles);
+  HIER_CHECK_CUDA(cudaGetLastError(), "paged8_merge_kernel launch");
+  return HIER_OK;
+}
 
-int paged8_launch_small(const Paged8Args& a, int format, int warps, int64_t units,
-                        cudaStream_t st) {
+int launch_small(const Paged8Args& a, int format, int warps, int64_t tiles, cudaStream_t st) {
+  const int64_t units = tiles * a.kv_heads * a.splits;
   const int64_t blocks = warps == 1 ? (units + kWarps - 1) / kWarps : units;
   if (blocks > INT32_MAX) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
   }
-  if (warps == 1) {
-    if (format == P8_INT8)
-      paged8_small_kernel<P8_INT8, 1><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, units);
-    else
-      paged8_small_kernel<P8_E4M3, 1><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, units);
-  } else {
-    if (format == P8_INT8)
-      paged8_small_kernel<P8_INT8, 4><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, units);
-    else
-      paged8_small_kernel<P8_E4M3, 4><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, units);
-  }
+  auto* kernel = warps == 1 ? (format == P8_INT8 ? paged8_small_kernel<P8_INT8, 1>
+                                                 : paged8_small_kernel<P8_E4M3, 1>)
+                            : (format == P8_INT8 ? paged8_small_kernel<P8_INT8, 4>
+                                                 : paged8_small_kernel<P8_E4M3, 4>);
+  kernel<<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, units);
   HIER_CHECK_CUDA(cudaGetLastError(), "paged8_small_kernel launch");
-  if (a.splits > 1) {
-    paged8_merge_kernel<4><<<(unsigned)(units / a.splits), 256, 0, st>>>(a);
-    HIER_CHECK_CUDA(cudaGetLastError(), "paged8_merge_kernel launch");
-  }
-  return HIER_OK;
+  return a.splits > 1 ? launch_merge<kPaged8SmallRows>(a, tiles, st) : HIER_OK;
 }
+
+}  // namespace
 
 }  // namespace hier
 
@@ -427,11 +465,7 @@ extern "C" int hier_paged8_attn_workspace(int32_t rows, int32_t heads, int32_t k
   clear_error();
   int rc = check_paged8(rows, heads, kv_heads, n, width);
   if (rc) return rc;
-  *floats = 0;
-  if (rows == 0) return HIER_OK;
-  const int64_t tiles = paged8_tiles<kRows>(rows, heads / kv_heads, n);
-  const SmallShape s = small_shape(tiles, kv_heads, width);
-  if (s.splits > 1) *floats = s.units * kRows * 130;
+  *floats = rows ? shape_of(rows, heads / kv_heads, kv_heads, n, width, max_rows).floats : 0;
   return HIER_OK;
 }
 
@@ -443,7 +477,8 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
                                 int32_t n, int32_t frame, int32_t block, int32_t window,
                                 float softmax_scale, int32_t max_rows, void* out,
                                 int64_t out_stride, float* lse, int32_t zero_tail,
-                                float* workspace, int32_t* status, void* stream) {
+                                float* workspace, int32_t* status, int32_t* dev_err,
+                                void* stream) {
   clear_error();
   int rc = check_paged8(rows, heads, kv_heads, n, width);
   if (rc) return rc;
@@ -459,6 +494,10 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
       block > (1 << 30) || window == 0 || window > (1 << 30)) {
     set_error(HIER_EVALUE, "invalid pages=%d, table stride=%lld, frame=%d, block=%d or window=%d",
               n_pages, (long long)table_stride, frame, block, window);
+    return HIER_EVALUE;
+  }
+  if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY)) {
+    set_error(HIER_EVALUE, "softmax_scale must be positive and finite, got %g", softmax_scale);
     return HIER_EVALUE;
   }
   if ((reinterpret_cast<uintptr_t>(q) & 15) || q_stride % 8 || (reinterpret_cast<uintptr_t>(out) & 15) ||
@@ -482,20 +521,33 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.out_stride = out_stride;
   a.lse = lse;
-  a.zero_tail = zero_tail;
   a.status = status;
+  a.err = dev_err;
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t tiles = paged8_tiles<kRows>(rows, a.group, n);
-  const SmallShape s = small_shape(tiles, kv_heads, width);
-  a.splits = s.splits;
-  a.row_limit = INT32_MAX;
-  if (s.splits > 1) {
-    if (!workspace) {
-      set_error(HIER_EVALUE, "this call needs a workspace (hier_paged8_attn_workspace)");
-      return HIER_EVALUE;
-    }
-    a.part_o = workspace;
-    a.part_ml = workspace + s.units * kRows * 128;
+  const Shape s = shape_of(rows, a.group, kv_heads, n, width, max_rows);
+  if (s.floats > 0 && !workspace) {
+    set_error(HIER_EVALUE, "this call needs a workspace (hier_paged8_attn_workspace)");
+    return HIER_EVALUE;
   }
-  return paged8_launch_small(a, format, s.warps, s.units, st);
+  // both kernels: one rule for whose a request is, and the rows behind the last
+  // request are the large one's
+  a.row_limit = !s.large ? INT32_MAX : s.small ? kSmallPairs : 0;
+  if (s.large) {
+    a.zero_tail = zero_tail;
+    a.splits = s.large_splits;
+    a.part_o = workspace + s.small_floats;
+    a.part_ml = a.part_o + (s.floats - s.small_floats) / 130 * 128;
+    rc = paged8_launch_large(a, format, s.large_tiles, st);
+    if (!rc && a.splits > 1) rc = launch_merge<kPaged8LargeRows>(a, s.large_tiles, st);
+    if (rc) return rc;
+  }
+  if (s.small) {
+    a.zero_tail = s.large ? 0 : zero_tail;
+    a.direct = s.direct;
+    a.splits = s.small_splits;
+    a.part_o = workspace;
+    a.part_ml = workspace + s.small_floats / 130 * 128;
+    rc = launch_small(a, format, s.warps, s.small_tiles, st);
+  }
+  return rc;
 }

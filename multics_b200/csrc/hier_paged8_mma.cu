@@ -1,0 +1,590 @@
+// Attention of many rows over an 8-bit paged cache on the tensor cores
+// (sm_100a: tcgen05, TMEM, bulk copies).
+//
+// One CTA per (256 (row, head) pairs of one key head, part of the keys): two
+// 128-pair halves that ping-pong over one list of 128-key tiles (two pages
+// each), as in the bf16 attention kernel:
+//
+//   S0(0) S1(0) | PV0(0) S0(1) PV1(0) S1(1) | PV0(1) S0(2) PV1(1) S1(2) | ...
+//
+// What differs is the operands.  Codes are exact in fp16, so keys and values
+// are turned into fp16 tiles in shared memory by a warpgroup of their own and
+// both products run as kind::f16 on fp16 operands: the queries are brought
+// into fp16's range by a power of two per row when they are loaded (bf16 keeps
+// all its bits), the weights are rounded to fp16 (11 bits), and the page
+// scales enter the exponents only (paged8_attn.cuh).  An fp8 product would
+// have to round the queries and the weights to 4 bits.  Both operands of both
+// products are K-major: the value pages are stored with the tokens along the
+// row.
+//
+// Warp roles (512 threads, four warpgroups):
+//   warp 0       loads pages: bulk copies of 8 KiB (page, head) blocks, one
+//                16 KiB stage for keys and one for values
+//   warp 1       MMA issuer (one lane), TMEM allocator
+//   warps 4-7    codes -> fp16 tiles (two stages of each)
+//   warps 8-11   queries and softmax of half 0, one pair per thread
+//   warps 12-15  the same of half 1
+// Shared memory: Q 2 x 32 KiB, K and V 2 x 32 KiB each, codes 2 x 16 KiB.
+// Tensor memory: S0 | S1 | O0 | O1, P over the first half of its S.
+// Every mbarrier wait is bounded and records a timeout in dev_err.
+
+#include <float.h>
+
+#include "paged8_attn.cuh"
+#include "tile_mma.cuh"
+
+namespace hier {
+namespace {
+
+constexpr int kRows = kPaged8LargeRows;
+constexpr int kStages = 2;
+constexpr int kThreads = 512;
+constexpr int kSmemQ = 0;
+constexpr int kSmemK = 2 * kTile;
+constexpr int kSmemV = kSmemK + kStages * kTile;
+constexpr int kSmemRaw = kSmemV + kStages * kTile;  // codes of a key tile, of a value tile
+constexpr int kRawTile = 2 * kPageHeadBytes;
+constexpr int kSmemBar = kSmemRaw + 2 * kRawTile;
+constexpr int kNumBars = 1 + 4 * kStages + 4 + 8;
+constexpr int kSmemBytes = kSmemBar + 256 + 1024;  // + slack for 1024-byte alignment
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+static_assert(kNumBars * 8 + 8 <= 256, "barriers and the TMEM slot");
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColO = 256;
+
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr uint32_t kRegsControl = 40;
+constexpr uint32_t kRegsConvert = 72;
+constexpr uint32_t kRegsSoftmax = 200;
+static_assert(128 * (kRegsControl + kRegsConvert) + 256 * kRegsSoftmax <= kThreads * 128,
+              "register split exceeds the launch allocation");
+
+struct Bars {
+  uint64_t* q_full;
+  uint64_t* k_full;
+  uint64_t* k_empty;
+  uint64_t* v_full;
+  uint64_t* v_empty;
+  uint64_t* raw_full;   // [keys, values]
+  uint64_t* raw_empty;
+  uint64_t* s_full;     // [half]
+  uint64_t* p_full;
+  uint64_t* p_lo;
+  uint64_t* o_final;
+};
+
+// fp16 operands, fp32 accumulation, both K-major
+constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(128 >> 3) << 17) |
+                            (static_cast<uint32_t>(128 >> 4) << 24);
+
+template <int k>
+__device__ __forceinline__ void s_step(uint32_t d, uint32_t qlo, uint32_t klo) {
+  constexpr uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+  umma_ss_lo<off, off>(d, qlo, klo, kIdesc, k > 0 ? 1u : 0u);
+}
+__device__ __forceinline__ void issue_s_f16(uint32_t d, uint32_t qlo, uint32_t klo) {
+  s_step<0>(d, qlo, klo), s_step<1>(d, qlo, klo), s_step<2>(d, qlo, klo), s_step<3>(d, qlo, klo);
+  s_step<4>(d, qlo, klo), s_step<5>(d, qlo, klo), s_step<6>(d, qlo, klo), s_step<7>(d, qlo, klo);
+}
+template <int k>
+__device__ __forceinline__ void pv_step(uint32_t o, uint32_t p, uint32_t vlo, bool acc) {
+  constexpr uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+  umma_ts_lo<k * 8, off>(o, p, vlo, kIdesc, (acc || k > 0) ? 1u : 0u);
+}
+template <int H>
+__device__ __forceinline__ void issue_pv_f16(uint32_t o, uint32_t p, uint32_t vlo, bool acc) {
+  pv_step<4 * H>(o, p, vlo, acc), pv_step<4 * H + 1>(o, p, vlo, acc);
+  pv_step<4 * H + 2>(o, p, vlo, acc), pv_step<4 * H + 3>(o, p, vlo, acc);
+}
+
+// What every role of a CTA works from.
+struct Job {
+  Paged8Tile tl;
+  int kvh;
+  int page0, n_kv;       // first page, 128-key tiles of this part
+  int page_end;          // pages from here on are not this part's
+  int lo[2], hi[2];      // keys that a half's rows see between them (lo = hi: none)
+  const int32_t* row;    // block table row
+};
+
+// a half has rows that see some key of the tile that starts at page p
+__device__ __forceinline__ bool uses(const Job& J, int h, int p) {
+  return p * kPage < (h ? J.hi[1] : J.hi[0]) && (p + 2) * kPage > (h ? J.lo[1] : J.lo[0]);
+}
+
+__device__ __forceinline__ int page_of(const Paged8Args& a, const Job& J, int p) {
+  if (p >= J.page_end) return -1;
+  const int page = J.row[p];
+  return page >= 0 && page < a.n_pages ? page : -1;
+}
+
+__device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uint8_t* smem,
+                                          const Bars& B) {
+  int pg[2] = {page_of(a, J, J.page0), page_of(a, J, J.page0 + 1)};
+  for (int j = 0; j < J.n_kv; ++j) {
+    const int p = J.page0 + 2 * j;
+    const int now[2] = {pg[0], pg[1]};
+    if (now[0] < 0 || (now[1] < 0 && p + 1 < J.page_end)) atomicOr(a.status, P8_BAD_PAGE);
+    if (j + 1 < J.n_kv) pg[0] = page_of(a, J, p + 2), pg[1] = page_of(a, J, p + 3);
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      if (j > 0 && !mbar_wait(B.raw_empty + kind, (j - 1) & 1, a.err, 40 + kind)) return;
+      const uint32_t bytes = ((now[0] >= 0) + (now[1] >= 0)) * kPageHeadBytes;
+      if (bytes)
+        mbar_arrive_expect_tx(B.raw_full + kind, bytes);
+      else
+        mbar_arrive(B.raw_full + kind);
+      const uint8_t* src = kind ? a.v : a.k;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (now[i] >= 0)
+          bulk_load(smem + kSmemRaw + kind * kRawTile + i * kPageHeadBytes,
+                    src + ((int64_t)now[i] * a.kv_heads + J.kvh) * kPageHeadBytes, kPageHeadBytes,
+                    B.raw_full + kind);
+    }
+  }
+}
+
+__device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint32_t tbase,
+                                         uint8_t* smem, const Bars& B) {
+  const uint32_t q_lo[2] = {sdesc_lo_kmajor(smem_u32(smem + kSmemQ)),
+                            sdesc_lo_kmajor(smem_u32(smem + kSmemQ + kTile))};
+  const uint32_t k_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemK));
+  const uint32_t v_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemV));
+  int cp[2] = {0, 0};  // PVs issued per half
+  if (!mbar_wait(B.q_full, 0, a.err, 42)) return;
+  // every phase of the stage barriers is waited for, used or not
+  if (!mbar_wait(B.k_full, 0, a.err, 43)) return;
+  tc_fence_after();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (!uses(J, h, J.page0)) continue;
+    issue_s_f16(tbase + h * kBN, q_lo[h], k_lo0);
+    umma_commit(B.s_full + h);
+  }
+  umma_commit(B.k_empty);
+  for (int j = 0; j < J.n_kv; ++j) {
+    const bool more = j + 1 < J.n_kv;
+    const int p = J.page0 + 2 * j;
+    const int stv = j % kStages, stk = (j + 1) % kStages;
+    if (!mbar_wait(B.v_full + stv, (j / kStages) & 1, a.err, 44)) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (uses(J, h, p)) {
+        const uint32_t o_t = tbase + kColO + h * kBN, p_t = tbase + h * kBN;
+        const uint32_t v_lo = v_lo0 + ((stv * kTile) >> 4);
+        if (!mbar_wait(B.p_lo + h, cp[h] & 1, a.err, 45)) return;
+        tc_fence_after();
+        issue_pv_f16<0>(o_t, p_t, v_lo, cp[h] > 0);
+        if (!mbar_wait(B.p_full + h, cp[h] & 1, a.err, 46)) return;
+        tc_fence_after();
+        issue_pv_f16<1>(o_t, p_t, v_lo, true);
+        ++cp[h];
+      }
+      if (!more) continue;
+      if (h == 0 && !mbar_wait(B.k_full + stk, ((j + 1) / kStages) & 1, a.err, 43)) return;
+      if (uses(J, h, p + 2)) {
+        tc_fence_after();
+        issue_s_f16(tbase + h * kBN, q_lo[h], k_lo0 + ((stk * kTile) >> 4));
+        umma_commit(B.s_full + h);
+      }
+    }
+    umma_commit(B.v_empty + stv);
+    if (more) umma_commit(B.k_empty + stk);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (cp[h] > 0) umma_commit(B.o_final + h);
+}
+
+// A page's 128 lines of 64 codes (keys: 64 of each dimension half; values: one
+// per dimension) become lines of 128 bytes in the swizzled tile.  Eight lanes
+// read two lines of codes (128 bytes) and write two lines of eight different
+// 16-byte columns: no bank conflicts either way.
+template <int FMT>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, bool values,
+                                             bool have0, bool have1, int tid) {
+  const int t = tid & 3, line0 = tid >> 2;
+#pragma unroll 4
+  for (int i = 0; i < 8; ++i) {
+    const int page = i >> 2, line = line0 + 32 * (i & 3);
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (page ? have1 : have0)
+      v = *reinterpret_cast<const uint4*>(raw + page * kPageHeadBytes + line * 64 + t * 16);
+    uint32_t o[8];
+    decode4<FMT>(v.x, o[0], o[1]);
+    decode4<FMT>(v.y, o[2], o[3]);
+    decode4<FMT>(v.z, o[4], o[5]);
+    decode4<FMT>(v.w, o[6], o[7]);
+    const int r = values ? line : 64 * page + (line & 63);
+    uint8_t* d = dst + (values ? page : line >> 6) * kHalf + r * 128;
+    *reinterpret_cast<uint4*>(d + (((2 * t) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(d + (((2 * t + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+template <int FMT>
+__device__ __forceinline__ void convert_role(const Paged8Args& a, const Job& J, uint8_t* smem,
+                                             const Bars& B, int tid) {
+  for (int j = 0; j < J.n_kv; ++j) {
+    const int st = j % kStages, p = J.page0 + 2 * j;
+    const bool have0 = page_of(a, J, p) >= 0, have1 = page_of(a, J, p + 1) >= 0;
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      uint64_t* empty = (kind ? B.v_empty : B.k_empty) + st;
+      if (j >= kStages && !mbar_wait(empty, ((j / kStages) - 1) & 1, a.err, 47)) return;
+      if (!mbar_wait(B.raw_full + kind, j & 1, a.err, 48)) return;
+      convert_tile<FMT>(smem + kSmemRaw + kind * kRawTile,
+                        smem + (kind ? kSmemV : kSmemK) + st * kTile, kind == 1, have0, have1, tid);
+      fence_proxy_async_smem();
+      mbar_arrive((kind ? B.v_full : B.k_full) + st);
+      mbar_arrive(B.raw_empty + kind);
+    }
+  }
+}
+
+// bits [a, b) of the 32 keys that start at key k
+__device__ __forceinline__ uint32_t key_bits(int lo, int hi, int k) {
+  const int a = min(32, max(0, lo - k)), b = min(32, max(0, hi - k));
+  const uint32_t below_a = a >= 32 ? ~0u : (1u << a) - 1u, below_b = b >= 32 ? ~0u : (1u << b) - 1u;
+  return below_b & ~below_a;
+}
+
+__device__ __forceinline__ void rescale_o(uint32_t o_col, float alpha) {
+#pragma unroll 1
+  for (int q = 0; q < 16; ++q) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7])
+                 : "r"(o_col + q * 8));
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(o_col + q * 8), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                   "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  }
+}
+
+// The pair's query row into the swizzled fp16 tile; returns the factor of its
+// scores: scale * log2(e) over the power of two it was multiplied by.
+__device__ __forceinline__ float stage_query(const Paged8Args& a, const __nv_bfloat16* q, bool in,
+                                             uint8_t* tile, int row) {
+  uint4 v[16];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    v[i] = in ? reinterpret_cast<const uint4*>(q)[i] : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[j] << 16)),
+                               fabsf(__uint_as_float(w[j] & 0xffff0000u))));
+  }
+  const int sh = fp16_shift(amax);
+  const float f = exp2_int(sh);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[i]);
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = pack_f16x2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
+    *reinterpret_cast<uint4*>(tile + (i >> 3) * kHalf + row * 128 + (((i & 7) ^ (row & 7)) << 4)) =
+        make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  return a.scale_log2 * exp2_int(-sh);
+}
+
+struct PageScale {
+  float ks, ve, unscale;  // key scale, log2 of the value scale, 2^-ve
+};
+
+__device__ __forceinline__ PageScale page_scale(const Paged8Args& a, const Job& J, int page) {
+  PageScale s = {0.f, 0.f, 0.f};
+  if (page < 0) return s;
+  const int64_t at = (int64_t)page * a.kv_heads + J.kvh;
+  const int ve = scale_log2_of(a.v_scale[at]);
+  s.ks = a.k_scale[at];
+  s.ve = (float)ve;
+  s.unscale = exp2_int(max(-126, min(126, -ve)));
+  return s;
+}
+
+__device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, int split, int parts,
+                                             uint32_t tbase, int warp, uint8_t* smem,
+                                             const Bars& B) {
+  const int h = (warp >> 2) - 2;
+  const int row = threadIdx.x - 256 - 128 * h;
+  const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+  const uint32_t s_col = tbase + lane_base + h * kBN;
+  const uint32_t o_col = tbase + lane_base + kColO + h * kBN;
+  const int rho = J.tl.rho0 + 128 * h + row;
+  const bool in_row = rho < J.tl.pairs;
+  const int qi = (in_row ? rho : 0) / a.group;
+  const int head = J.kvh * a.group + (in_row ? rho : 0) % a.group;
+  const int64_t grow = J.tl.rq.row0 + (int64_t)qi;
+  float m_run = -INFINITY, l_run = 0.f;
+  int c = 0;
+  if (J.n_kv > 0) {
+    const float sc = stage_query(a, a.q + grow * a.q_stride + head * 128, in_row && J.tl.b < a.n,
+                                 smem + kSmemQ + h * kTile, row);
+    fence_proxy_async_smem();
+    mbar_arrive(B.q_full);
+    int lo = 0, hi = 0;
+    if (in_row && J.tl.b < a.n) row_keys(a, J.tl.rq, qi, lo, hi);
+    // tiles that every row of the half sees whole need no mask
+    int all_lo, all_hi, unused;
+    {
+      const int first = J.tl.rho0 + 128 * h, last = min(first + 128, J.tl.pairs) - 1;
+      all_lo = INT_MAX, all_hi = 0;
+      if (first <= last) {
+        row_keys(a, J.tl.rq, last / a.group, all_lo, unused);
+        row_keys(a, J.tl.rq, first / a.group, unused, all_hi);
+      }
+    }
+    int pg0 = page_of(a, J, J.page0), pg1 = page_of(a, J, J.page0 + 1);
+    PageScale n0 = page_scale(a, J, pg0), n1 = page_scale(a, J, pg1);
+    bool nb0 = pg0 >= 0, nb1 = pg1 >= 0;
+    if (J.n_kv > 1) pg0 = page_of(a, J, J.page0 + 2), pg1 = page_of(a, J, J.page0 + 3);
+    for (int j = 0; j < J.n_kv; ++j) {
+      const int p = J.page0 + 2 * j;
+      // scales one tile ahead, table entries two
+      const PageScale e0 = n0, e1 = n1;
+      const bool b0 = nb0, b1 = nb1;
+      if (j + 1 < J.n_kv) {
+        n0 = page_scale(a, J, pg0), n1 = page_scale(a, J, pg1);
+        nb0 = pg0 >= 0, nb1 = pg1 >= 0;
+        if (j + 2 < J.n_kv) pg0 = page_of(a, J, p + 4), pg1 = page_of(a, J, p + 5);
+      }
+      if (!uses(J, h, p)) continue;
+      const float c0 = fmaxf(sc * e0.ks, FLT_MIN), c1 = fmaxf(sc * e1.ks, FLT_MIN);
+      const int k0 = p * kPage;
+      const bool partial = !(k0 >= all_lo && k0 + 2 * kPage <= all_hi && b0 && b1);
+      // S_h is committed after the half's previous PV, so once it is visible O
+      // holds every earlier product and can be rescaled without another wait
+      if (!mbar_wait(B.s_full + h, c & 1, a.err, 49)) return;
+      tc_fence_after();
+      float sv[kBN];
+      {
+        uint32_t* r = reinterpret_cast<uint32_t*>(sv);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          tmem_ld32(s_col + q * 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * q));
+        tmem_wait_ld();
+      }
+      if (partial) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t w = (q < 2 ? b0 : b1) ? key_bits(lo, hi, k0 + 32 * q) : 0u;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sv[32 * q + i] = ((w >> i) & 1u) ? sv[32 * q + i] : -INFINITY;
+        }
+      }
+      float m8[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m8[i] = sv[i], m8[4 + i] = sv[64 + i];
+#pragma unroll
+      for (int i = 4; i < 64; ++i) {
+        m8[i & 3] = fmaxf(m8[i & 3], sv[i]);
+        m8[4 + (i & 3)] = fmaxf(m8[4 + (i & 3)], sv[64 + i]);
+      }
+      const float mx = fmaxf(fmaf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), c0, e0.ve),
+                             fmaf(fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])), c1, e1.ve));
+      const bool grow_max = mx > m_run + kRescaleThreshold;
+      const bool need_rescale = grow_max && m_run != -INFINITY;
+      if (__any_sync(0xffffffffu, need_rescale)) {
+        const float alpha = need_rescale ? ex2_approx(m_run - mx) : 1.f;
+        rescale_o(o_col, alpha);
+        l_run *= alpha;
+      }
+      if (grow_max) m_run = mx;
+      const float nref = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float ch = half ? c1 : c0, rh = nref + (half ? e1.ve : e0.ve);
+        const uint64_t sc2 = f2_pack(ch, ch), ref2 = f2_pack(rh, rh);
+        uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint64_t arg = f2_fma(f2_pack(sv[64 * half + 2 * i], sv[64 * half + 2 * i + 1]), sc2, ref2);
+          float a0, a1;
+          f2_unpack(arg, a0, a1);
+          const float p0 = ex2_approx(a0), p1 = ex2_approx(a1);
+          acc[i & 3] = f2_add(acc[i & 3], f2_pack(p0, p1));
+          pk[i] = pack_f16x2(p0, p1);
+        }
+        tmem_st32(s_col + 32 * half, pk);
+        if (half == 0) {  // keys 0-63 of P: the first half of PV can start
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(B.p_lo + h);
+        }
+        float s0, s1;
+        f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
+        l_run = fmaf(s0 + s1, half ? e1.unscale : e0.unscale, l_run);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(B.p_full + h);
+      ++c;
+    }
+  }
+  if (c > 0) {
+    if (!mbar_wait(B.o_final + h, 0, a.err, 50)) return;
+    tc_fence_after();
+  }
+  const bool whole = parts == 1;
+  const float inv = whole ? (l_run > 0.f ? 1.f / l_run : l_run == 0.f ? 0.f : l_run) : 1.f;
+  __nv_bfloat16* orow = a.out + grow * a.out_stride + head * 128;
+  const int64_t at = whole ? 0
+                           : ((int64_t)blockIdx.x * kRows + 128 * h + row);
+  if (in_row) {
+    if (whole) {
+      if (a.lse) a.lse[grow * a.heads + head] = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
+    } else {
+      *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_run, l_run);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t r[32];
+    if (c > 0) {
+      tmem_ld32(o_col + q * 32, r);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = 0u;
+    }
+    if (!in_row) continue;
+    if (whole) {
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
+      uint4* dst = reinterpret_cast<uint4*>(orow + q * 32);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    } else {
+      uint4* dst = reinterpret_cast<uint4*>(a.part_o + at * 128 + q * 32);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        dst[k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+    }
+  }
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, int64_t tiles) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = warp_id(), lane = lane_id();
+  // the last tiles of a request see the most keys: they come first
+  const int split = blockIdx.x % a.splits;
+  Job J;
+  J.kvh = blockIdx.x / a.splits % a.kv_heads;
+  const int64_t tile = tiles - 1 - blockIdx.x / ((int64_t)a.splits * a.kv_heads);
+  J.tl = paged8_tile<kRows>(a, tile, threadIdx.x == 0 && split == 0 && J.kvh == 0);
+  if (!J.tl.live) return;
+  const bool tail = J.tl.b == a.n;
+  if (tail ? !a.zero_tail : J.tl.pairs <= a.row_limit) return;
+  const int kv_all = (J.tl.np + 1) / 2;
+  const int parts = parts_of<kPaged8LargeMin>(kv_all, a.splits);
+  if (split >= parts) return;
+  const int t0 = (int)((int64_t)kv_all * split / parts), t1 = (int)((int64_t)kv_all * (split + 1) / parts);
+  J.page0 = J.tl.p0 + 2 * t0;
+  J.n_kv = t1 - t0;
+  J.page_end = min(J.tl.p0 + J.tl.np, J.tl.p0 + 2 * t1);
+  J.row = tail ? a.table : a.table + J.tl.b * a.table_stride;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int first = J.tl.rho0 + 128 * h, last = min(first + 128, J.tl.pairs) - 1;
+    J.lo[h] = J.hi[h] = 0;
+    int unused;
+    if (first <= last && !tail) {
+      row_keys(a, J.tl.rq, first / a.group, J.lo[h], unused);
+      row_keys(a, J.tl.rq, last / a.group, unused, J.hi[h]);
+      if (J.hi[h] <= J.lo[h]) J.lo[h] = J.hi[h] = 0;
+    }
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBar);
+  Bars B;
+  B.q_full = bars;
+  B.k_full = B.q_full + 1;
+  B.k_empty = B.k_full + kStages;
+  B.v_full = B.k_empty + kStages;
+  B.v_empty = B.v_full + kStages;
+  B.raw_full = B.v_empty + kStages;
+  B.raw_empty = B.raw_full + 2;
+  B.s_full = B.raw_empty + 2;
+  B.p_full = B.s_full + 2;
+  B.p_lo = B.p_full + 2;
+  B.o_final = B.p_lo + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
+  if (threadIdx.x == 0) {
+    mbar_init(B.q_full, 256);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(B.k_full + s, 128);
+      mbar_init(B.k_empty + s, 1);
+      mbar_init(B.v_full + s, 128);
+      mbar_init(B.v_empty + s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(B.raw_full + i, 1);
+      mbar_init(B.raw_empty + i, 128);
+      mbar_init(B.s_full + i, 1);
+      mbar_init(B.p_full + i, 128);
+      mbar_init(B.p_lo + i, 128);
+      mbar_init(B.o_final + i, 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    softmax_role(a, J, split, parts, tbase, warp, smem, B);
+  } else if (warp >= 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
+    if (J.n_kv > 0) convert_role<FMT>(a, J, smem, B, threadIdx.x - 128);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    if (J.n_kv > 0 && lane == 0) {
+      if (warp == 0) load_role(a, J, smem, B);
+      if (warp == 1) mma_role(a, J, tbase, smem, B);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, kTmemCols);
+  }
+}
+
+}  // namespace
+
+int paged8_launch_large(const Paged8Args& a, int format, int64_t tiles, cudaStream_t st) {
+  const int64_t blocks = tiles * a.kv_heads * a.splits;
+  if (blocks > INT32_MAX) {
+    set_error(HIER_EVALUE, "too many rows, requests and heads");
+    return HIER_EVALUE;
+  }
+  auto* kernel = format == P8_INT8 ? paged8_mma_kernel<P8_INT8> : paged8_mma_kernel<P8_E4M3>;
+  HIER_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kSmemBytes),
+                  "cudaFuncSetAttribute(paged8_mma_kernel)");
+  kernel<<<(unsigned)blocks, kThreads, kSmemBytes, st>>>(a, tiles);
+  HIER_CHECK_CUDA(cudaGetLastError(), "paged8_mma_kernel launch");
+  return HIER_OK;
+}
+
+}  // namespace hier

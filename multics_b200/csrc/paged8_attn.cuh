@@ -44,9 +44,16 @@ struct Paged8Args {
   int splits;       // most parts a tile's keys are cut into
   float* part_o;    // [tile][kv head][split][kRows][128]
   float* part_ml;   // [tile][kv head][split][kRows][2]
-  int row_limit;    // small kernel: requests of more row-head pairs are left to the large one
+  int row_limit;    // requests of up to row_limit pairs are the small kernel's, the others the
+                    // large one's (INT_MAX: all the small one's, 0: all the large one's)
+  int direct;       // small kernel: > 0: tile t is tile t % direct of request t / direct
   int32_t* status;
+  int* err;         // bounded waits
 };
+
+constexpr int kPaged8SmallRows = 8;
+constexpr int kPaged8LargeRows = 256;
+constexpr int kPaged8LargeMin = 4;  // 128-key tiles of a part at least
 
 template <int kRows>
 __host__ __device__ inline int64_t paged8_tiles(int64_t rows, int group, int n) {
@@ -82,12 +89,18 @@ __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t t
   Paged8Tile t;
   const int32_t* qs = a.q_start;
   const int64_t G = a.group;
-  t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
   t.live = false;
   t.rho0 = t.pairs = t.lo = t.hi = t.p0 = t.np = 0;
-  const int64_t first = qs[t.b] * G / kRows + t.b;
-  if (tile < first) return t;
-  const int64_t rho0 = (tile - first) * kRows;
+  int64_t rho0;
+  if (kRows == kPaged8SmallRows && a.direct) {
+    t.b = (int)(tile / a.direct);
+    rho0 = tile % a.direct * kRows;
+  } else {
+    t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
+    const int64_t first = qs[t.b] * G / kRows + t.b;
+    if (tile < first) return t;
+    rho0 = (tile - first) * kRows;
+  }
   if (t.b == a.n) {  // rows behind the last request
     t.rq.row0 = qs[a.n];
     t.rq.n = a.rows - t.rq.row0;
@@ -141,7 +154,6 @@ __device__ __forceinline__ int scale_log2_of(float s) {
   return (int)((__float_as_uint(s) >> 23) & 0xffu) - 127;
 }
 
-int paged8_launch_small(const Paged8Args& a, int format, int warps, int64_t units, cudaStream_t st);
 int paged8_launch_large(const Paged8Args& a, int format, int64_t tiles, cudaStream_t st);
 
 }  // namespace hier

@@ -293,6 +293,9 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
         raise ValueError("tokens_per_frame, block_frames and window must be below 2^30")
     if max_rows is not None and max_rows < 0:
         raise ValueError(f"max_rows must not be negative, got {max_rows}")
+    scale = 1.0 / math.sqrt(HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
     dim = num_heads * HEAD_DIM
     q = token_rows("q", q, dim)
     n, width = _requests(cache, table, lengths, q_start)
@@ -303,9 +306,10 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
     _cuda("paged8_attention", dev)
     if q.device != dev:
         raise ValueError(f"q must be on {dev}")
-    scale = 1.0 / math.sqrt(HEAD_DIM) if softmax_scale is None else float(softmax_scale)
     zero_tail = out is None
     most = 0 if max_rows is None else int(max_rows)
+    from .attention import _dev_err
+
     L = _lib.lib()
     with on_device(dev):
         given = out
@@ -324,7 +328,7 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
             ptr(table), max(table.stride(0), width), width, ptr(lengths), ptr(q_start), n,
             int(tokens_per_frame), int(block_frames), int(window), scale, most, ptr(out),
             out.stride(0), ptr(lse), int(zero_tail), ptr(ws), ptr(cache.status),
-            stream_ptr(dev)))
+            ptr(_dev_err(dev)), stream_ptr(dev)))
         if given is not None and out is not given:
             out = given.copy_(out)
     return (out, lse) if return_lse else out

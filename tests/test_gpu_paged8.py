@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import paged8_oracle as P
+from multics_b200.attention import device_error
 from multics_b200.paged8 import Paged8Cache, page_step, paged8_append, paged8_attention
 
 pytestmark = pytest.mark.gpu
@@ -343,6 +344,7 @@ def _check(c, table, lengths, counts, heads, g, *, spare=0, q=None, **kw):
     # log2 of a sum whose terms are off by 2^-11 at most, and fp32's own step
     assert ((lse - want_lse)[fin].abs() <= 2.0 ** -10 + want_lse[fin].abs() * 2.0 ** -20).all()
     c.check()
+    assert device_error() == 0
     return out
 
 

@@ -77,7 +77,8 @@ def test_append_and_attention_refusals():
     q = torch.zeros(3, 512, dtype=BF)
     for kw in (dict(num_heads=3), dict(num_heads=0), dict(window=0), dict(window=-2),
                dict(tokens_per_frame=0), dict(block_frames=-1), dict(window=(1 << 30) + 1),
-               dict(max_rows=-1), dict(out=torch.zeros(3, 512)), dict(out=torch.zeros(2, 512, dtype=BF))):
+               dict(max_rows=-1), dict(softmax_scale=0.0),
+               dict(softmax_scale=-0.1), dict(softmax_scale=float("nan")), dict(out=torch.zeros(3, 512)), dict(out=torch.zeros(2, 512, dtype=BF))):
         with pytest.raises(ValueError):
             paged8_attention(q, c, t, n, s, **{"num_heads": 4, **kw})
     with pytest.raises(ValueError, match="q must be"):
@@ -110,7 +111,7 @@ def test_entry_points_refuse_before_any_device_work():
              q=None):
         return L.hier_paged8_attn(q, 256, rows, heads, kv, D, fmt, None, None, None, None, 1, None,
                                   stride, width, None, None, 1, frame, block, window, 0.1, 0, None,
-                                  256, None, 1, None, None, None)
+                                  256, None, 1, None, None, None, None)
 
     for kw, exc in ((dict(D=64), NotImplementedError), (dict(heads=3), ValueError),
                     (dict(fmt=2), ValueError), (dict(stride=0), ValueError),
