@@ -1,24 +1,29 @@
 // Attention of a few rows over an 8-bit paged cache (sm_100a), the merge of
-// split keys, and the entry point of both attention kernels.
+// split keys, and the entry point of all attention kernels.
 //
 // A warp takes 8 (row, head) pairs of one key head and walks pages of 64 keys.
 // Bound by the bytes of the cache: the codes go from global memory straight to
-// registers (16 bytes per lane, every 128-byte line used whole), are turned
-// into fp16 there and fed to m16n8k16 products with the keys (or the value
-// dimensions) as rows and the 8 pairs as columns:
+// registers (16 bytes per lane, every line used whole), are turned into fp16
+// there and fed to m16n8k16 products with the keys (or the value dimensions) as
+// rows and the 8 pairs as columns:
 //   S^T (keys x pairs) = K Q^T,    O^T (dimensions x pairs) += V^T P^T.
-// The page layout gives a lane 16 consecutive codes of the reduction axis; the
+// The page layout gives a lane consecutive codes of the reduction axis; the
 // order of the reduction inside a product is free as long as both operands use
 // the same one, so no code is moved between lanes.  P^T goes from the layout
 // of a result to that of an operand by an 8x8 transpose in the register file.
-// While a page's scores are computed its values are in flight, and while its
-// values are consumed the next page's keys are.
 //
-// With few tiles the keys of each are split over blocks (partial outputs in
-// fp32 with their maximum and sum, merged in split order by a second kernel)
-// and over the four warps of a block (merged in shared memory).
+// Two kernels.  paged8_long_kernel, for block tables of more than kShortPages
+// pages: four warps of a block share a tile's pages (joined in shared memory),
+// and with few tiles the keys are also split over blocks (partial outputs in
+// fp32 with their maximum and sum, joined in split order by a second kernel).
+// While a page's scores are computed its values are in flight, and while its
+// values are consumed the next page's keys are: the loads of one take the
+// registers that the other's products have just used.  paged8_short_kernel: a
+// warp per tile, and products over 16 or 32 keys at a time.
 
 #include <math.h>
+
+#include <algorithm>
 
 #include "paged8_attn.cuh"
 
@@ -44,12 +49,28 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
+// 16 codes, or zeros; volatile, so that the loads stay where they are written
+// between the products and the registers they fill are those just used up
+__device__ __forceinline__ uint4 ld_codes(const uint8_t* p, bool in) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((int)in));
+  return v;
+}
+
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-__device__ __forceinline__ uint4 ld_codes(const uint8_t* p, bool in) {
-  return in ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+__device__ __forceinline__ uint2 ld_shared2(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
 }
 
 // page of the table entry, or -1 (reported) when it leaves the pool
@@ -60,265 +81,455 @@ __device__ __forceinline__ int page_at(const Paged8Args& a, const int32_t* row, 
   return -1;
 }
 
-template <int WPU>
-constexpr int kMinPages = 2 * WPU;
+// row of a request and head of the group of pair rho
+__device__ __forceinline__ void split_pair(const Paged8Args& a, int rho, int& row, int& g) {
+  if (a.group == 1) {
+    row = rho, g = 0;
+  } else {
+    row = rho / a.group;
+    g = rho - row * a.group;
+  }
+}
 
-template <int FMT, int WPU>
-__global__ void __launch_bounds__(kWarps * 32, 2) paged8_small_kernel(Paged8Args a, int64_t units) {
-  __shared__ __align__(16) float so[kWarps][kRows][kPitch];
-  __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The 8 pairs of tile i of request b, from pair rho0.
+__device__ __forceinline__ Paged8Tile small_tile(const Paged8Args& a, int b, int rho0, bool report) {
+  Paged8Tile t;
+  t.b = b;
+  t.rho0 = rho0;
+  t.lo = t.hi = t.p0 = t.np = t.pairs = 0;
+  t.rq = paged8_request(a.q_start, a.lengths, b, a.rows, a.width, false, report ? a.status : nullptr);
+  t.live = t.rq.row0 >= 0 && t.rq.n > 0 && t.rq.row0 + (int64_t)t.rq.n <= a.rows;
+  if (!t.live) return t;
+  t.pairs = t.rq.n * a.group;
+  t.live = rho0 < t.pairs && t.pairs <= a.row_limit;
+  if (!t.rq.ok) t.rq.held = 0;  // a length outside the table: the rows see nothing
+  if (t.live) paged8_span(a, t, kRows);
+  return t;
+}
+
+// What a lane knows of its tile's pairs.  In the products a lane's group g owns
+// column g of the queries, and it holds results of columns 2t and 2t + 1.
+struct Columns {
+  const __nv_bfloat16* q;  // the lane's 32 query values of pair g of key head 0
+  bool in;
+  int lo[2], hi[2];        // keys that columns 2t, 2t + 1 see
+  int all_lo, all_hi;      // keys that every pair sees
+};
+
+__device__ __forceinline__ Columns columns(const Paged8Args& a, const Paged8Tile& tl, int lane) {
   const int g = lane >> 2, t = lane & 3;
-  const int64_t unit = WPU == 1 ? (int64_t)blockIdx.x * kWarps + warp : (int64_t)blockIdx.x;
-  const int w = WPU == 1 ? 0 : warp;
-  if (unit >= units) return;
-  const int split = (int)(unit % a.splits);
-  const int kvh = (int)(unit / a.splits % a.kv_heads);
-  const int64_t tile_id = unit / ((int64_t)a.splits * a.kv_heads);
-  const Paged8Tile tl = paged8_tile<kRows>(a, tile_id, split == 0 && kvh == 0 && lane == 0 && w == 0);
-  if (!tl.live) return;
-  const int parts = parts_of<kMinPages<WPU>>(tl.np, a.splits);
-  if (split >= parts) return;
-  if (tl.b == a.n) {
-    if (!a.zero_tail) return;
-  } else if (tl.pairs > a.row_limit) {
-    return;
-  }
-  // row of this lane's group: a column of the products
+  Columns c;
   const int rho = tl.rho0 + g;
-  const bool in_row = rho < tl.pairs && tl.b < a.n;
-  const int qi = rho / a.group, head = kvh * a.group + rho % a.group;
-  int lo_g = INT_MAX, hi_g = 0;
-  if (in_row) row_keys(a, tl.rq, qi, lo_g, hi_g);
-  const int np0 = tl.np ? (int)((int64_t)tl.np * split / parts) : 0;
-  const int np1 = tl.np ? (int)((int64_t)tl.np * (split + 1) / parts) : 0;
-  float o[8][4] = {};
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-  if (np0 < np1) {
-    uint32_t qf[8][2];
-    float sc_g;
-    {
-      const __nv_bfloat16* qp = a.q + (tl.rq.row0 + (int64_t)qi) * a.q_stride + head * 128 + 16 * t;
-      uint4 raw[4];
+  c.in = rho < tl.pairs;
+  int qi, qg, lo = INT_MAX, hi = 0;
+  split_pair(a, c.in ? rho : tl.rho0, qi, qg);
+  if (c.in) row_keys(a, tl.rq, qi, lo, hi);
+  c.q = a.q + (tl.rq.row0 + (int64_t)qi) * a.q_stride + qg * 128 + 16 * t;
+  c.all_lo = c.in ? lo : 0, c.all_hi = c.in ? hi : INT_MAX;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        raw[i] = in_row ? *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8)
-                        : make_uint4(0u, 0u, 0u, 0u);
-      float amax = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t x = word(raw[i], j);
-          amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x << 16)),
-                                   fabsf(__uint_as_float(x & 0xffff0000u))));
-        }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int sh = fp16_shift(amax);
-      const float f = exp2_int(sh);
-      sc_g = a.scale_log2 * exp2_int(-sh);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t x = word(raw[i], j);
-          // 8 dimensions = words of two products: (i, j) -> product 2i + j/2, register j % 2
-          qf[2 * i + (j >> 1)][j & 1] =
-              pack_f16x2(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
-        }
-    }
-    float sc[2];
-    int lo[2], hi[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      sc[c] = __shfl_sync(0xffffffffu, sc_g, (2 * t + c) * 4);
-      lo[c] = __shfl_sync(0xffffffffu, lo_g, (2 * t + c) * 4);
-      hi[c] = __shfl_sync(0xffffffffu, hi_g, (2 * t + c) * 4);
-    }
-    // keys that every row of the tile sees
-    int all_lo = in_row ? lo_g : 0, all_hi = in_row ? hi_g : INT_MAX;
-#pragma unroll
-    for (int i = 4; i < 32; i <<= 1) {
-      all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, i));
-      all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, i));
-    }
-    const int32_t* row = a.table + tl.b * a.table_stride;
-    const int key0 = 16 * (g >> 1) + (g & 1);  // key of row g (+ 2: row g + 8) of product m: + 4 m
-    uint4 kr[4][2][2];
-    const auto load_k = [&](int p, int page) {
-      const uint8_t* kp = a.k + ((int64_t)page * a.kv_heads + kvh) * kPageHeadBytes + t * 16;
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = key0 + 4 * m + 2 * e;
-          const bool in = page >= 0 && p * kPage + key >= tl.lo && p * kPage + key < tl.hi;
-          kr[m][e][0] = ld_codes(kp + key * 64, in);
-          kr[m][e][1] = ld_codes(kp + kPage * 64 + key * 64, in);
-        }
-    };
-    int p = tl.p0 + np0 + w;
-    const int p_end = tl.p0 + np1;
-    int page = -1, page_next = -1;
-    if (p < p_end) {
-      page = page_at(a, row, p, lane);
-      if (p + WPU < p_end) page_next = page_at(a, row, p + WPU, lane);
-      load_k(p, page);
-    }
-    for (; p < p_end; p += WPU) {
-      const int page_now = page;
-      page = page_next;
-      if (p + 2 * WPU < p_end) page_next = page_at(a, row, p + 2 * WPU, lane);
-      if (page_now < 0) {
-        if (p + WPU < p_end) load_k(p + WPU, page);
-        continue;
-      }
-      const int64_t at = (int64_t)page_now * a.kv_heads + kvh;
-      const float ks = a.k_scale[at], vs = a.v_scale[at];
-      uint4 vr[8][2];
-      {
-        const uint8_t* vp = a.v + at * kPageHeadBytes + t * 16;
-        const bool in = p * kPage + 16 * t + 15 >= tl.lo && p * kPage + 16 * t < tl.hi;
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) vr[d][e] = ld_codes(vp + (16 * d + 8 * e + g) * kPage, in);
-      }
-      float s[4][4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a0, a1, a2, a3;
-            decode4<FMT>(word(kr[m][0][h], i), a0, a2);
-            decode4<FMT>(word(kr[m][1][h], i), a1, a3);
-            mma_f16(s[m], a0, a1, a2, a3, qf[4 * h + i][0], qf[4 * h + i][1]);
-          }
-      }
-      if (p + WPU < p_end) load_k(p + WPU, page);
-      const int ve = scale_log2_of(vs);
-      const float vef = (float)ve;
-      const bool whole = p * kPage >= all_lo && (p + 1) * kPage <= all_hi;
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int c = r & 1;
-          float x = fmaf(s[m][r], sc[c] * ks, vef);
-          if (!whole) {
-            const int key = p * kPage + key0 + 4 * m + (r & 2);
-            x = key >= lo[c] && key < hi[c] ? x : -INFINITY;
-          }
-          s[m][r] = x;
-          mx[c] = fmaxf(mx[c], x);
-        }
-#pragma unroll
-      for (int i = 4; i < 32; i <<= 1) {
-        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], i));
-        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], i));
-      }
-      float ref[2], alpha[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float m_new = fmaxf(m_run[c], mx[c]);
-        ref[c] = m_new == -INFINITY ? 0.f : m_new;
-        alpha[c] = ex2_approx(m_run[c] - ref[c]);
-        m_run[c] = m_new;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[d][r] *= alpha[r & 1];
-        l_run[0] *= alpha[0];
-        l_run[1] *= alpha[1];
-      }
-      const float unscale = exp2_int(max(-126, min(126, -ve)));
-      float sum[2] = {0.f, 0.f};
-      uint32_t pb[4][2];
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p0 = ex2_approx(s[m][2 * e] - ref[0]), p1 = ex2_approx(s[m][2 * e + 1] - ref[1]);
-          sum[0] += p0;
-          sum[1] += p1;
-          pb[m][e] = transpose8x8(pack_f16x2(p0, p1));
-        }
-      l_run[0] = fmaf(sum[0], unscale, l_run[0]);
-      l_run[1] = fmaf(sum[1], unscale, l_run[1]);
-#pragma unroll
-      for (int d = 0; d < 8; ++d)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          uint32_t a0, a1, a2, a3;
-          decode4<FMT>(word(vr[d][0], m), a0, a2);
-          decode4<FMT>(word(vr[d][1], m), a1, a3);
-          mma_f16(o[d], a0, a1, a2, a3, pb[m][0], pb[m][1]);
-        }
-    }
-#pragma unroll
-    for (int i = 4; i < 32; i <<= 1) {
-      l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], i);
-      l_run[1] += __shfl_xor_sync(0xffffffffu, l_run[1], i);
-    }
+  for (int i = 4; i < 32; i <<= 1) {
+    c.all_lo = max(c.all_lo, __shfl_xor_sync(0xffffffffu, c.all_lo, i));
+    c.all_hi = min(c.all_hi, __shfl_xor_sync(0xffffffffu, c.all_hi, i));
   }
-  // results: rows of 128 through shared memory
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    c.lo[k] = __shfl_sync(0xffffffffu, lo, (2 * t + k) * 4);
+    c.hi[k] = __shfl_sync(0xffffffffu, hi, (2 * t + k) * 4);
+  }
+  return c;
+}
+
+// The queries of a key head as fragments of the eight products over the
+// dimensions, fp16 after one power of two per pair; sc: the factors of the
+// scores of columns 2t, 2t + 1.
+__device__ __forceinline__ void load_queries(const Paged8Args& a, const Columns& c, int kvh, int t,
+                                             uint32_t (&qf)[8][2], float (&sc)[2]) {
+  const __nv_bfloat16* q = c.q + (int64_t)kvh * a.group * 128;
+  uint4 raw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    raw[i] = c.in ? *reinterpret_cast<const uint4*>(q + (i >> 1) * 64 + (i & 1) * 8)
+                  : make_uint4(0u, 0u, 0u, 0u);
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = word(raw[i], j);
+      amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x << 16)), fabsf(__uint_as_float(x & 0xffff0000u))));
+    }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const int sh = fp16_shift(amax);
+  const float f = exp2_int(sh), mine = a.scale_log2 * exp2_int(-sh);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = word(raw[i], j);
+      // 8 dimensions = words of two products: (i, j) -> product 2i + j/2, register j % 2
+      qf[2 * i + (j >> 1)][j & 1] =
+          pack_f16x2(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
+    }
+  sc[0] = __shfl_sync(0xffffffffu, mine, 8 * t);
+  sc[1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
+}
+
+// Running softmax of a lane's two columns and their output.
+struct Running {
+  float m[2], l[2], o[8][4];
+};
+
+__device__ __forceinline__ void start(Running& R) {
+#pragma unroll
+  for (int d = 0; d < 8; ++d) R.o[d][0] = R.o[d][1] = R.o[d][2] = R.o[d][3] = 0.f;
+  R.m[0] = R.m[1] = -INFINITY;
+  R.l[0] = R.l[1] = 0.f;
+}
+
+// Scores of 16 * MB keys to weights (operand fragments) and their sums.  key0:
+// key of the lane's result row g of product 0; product m is + 4 m, row g + 8 + 2.
+template <int MB>
+__device__ __forceinline__ void weigh(Running& R, float (&s)[MB][4], const Columns& c,
+                                      const float (&sc)[2], float ks, float vs, bool whole, bool have,
+                                      int key0, uint32_t (&pb)[MB][2]) {
+  const int ve = scale_log2_of(vs);
+  const float vef = (float)ve;
+  float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = r & 1;
+      float x = fmaf(s[m][r], sc[k] * ks, vef);
+      if (!whole) {
+        const int key = key0 + 4 * m + (r & 2);
+        x = have && key >= c.lo[k] && key < c.hi[k] ? x : -INFINITY;
+      }
+      s[m][r] = x;
+      mx[k] = fmaxf(mx[k], x);
+    }
+#pragma unroll
+  for (int i = 4; i < 32; i <<= 1) {
+    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], i));
+    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], i));
+  }
+  float ref[2], alpha[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float m_new = fmaxf(R.m[k], mx[k]);
+    ref[k] = m_new == -INFINITY ? 0.f : m_new;
+    alpha[k] = ex2_approx(R.m[k] - ref[k]);
+    R.m[k] = m_new;
+  }
+  if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) R.o[d][r] *= alpha[r & 1];
+    R.l[0] *= alpha[0];
+    R.l[1] *= alpha[1];
+  }
+  const float unscale = exp2_int(max(-126, min(126, -ve)));
+  float sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float p0 = ex2_approx(s[m][2 * e] - ref[0]), p1 = ex2_approx(s[m][2 * e + 1] - ref[1]);
+      sum[0] += p0;
+      sum[1] += p1;
+      pb[m][e] = transpose8x8(pack_f16x2(p0, p1));
+    }
+  R.l[0] = fmaf(sum[0], unscale, R.l[0]);
+  R.l[1] = fmaf(sum[1], unscale, R.l[1]);
+}
+
+// The lanes' results as rows of 128 floats in shared memory.
+__device__ __forceinline__ void spill(Running& R, float (*so)[kPitch], float* sm, float* sl, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 4; i < 32; i <<= 1) {
+    R.l[0] += __shfl_xor_sync(0xffffffffu, R.l[0], i);
+    R.l[1] += __shfl_xor_sync(0xffffffffu, R.l[1], i);
+  }
 #pragma unroll
   for (int d = 0; d < 8; ++d)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) so[warp][2 * t + (r & 1)][16 * d + 8 * (r >> 1) + g] = o[d][r];
+    for (int r = 0; r < 4; ++r) so[2 * t + (r & 1)][16 * d + 8 * (r >> 1) + g] = R.o[d][r];
   if (g == 0) {
-    sm[warp][2 * t] = m_run[0], sm[warp][2 * t + 1] = m_run[1];
-    sl[warp][2 * t] = l_run[0], sl[warp][2 * t + 1] = l_run[1];
+    sm[2 * t] = R.m[0], sm[2 * t + 1] = R.m[1];
+    sl[2 * t] = R.l[0], sl[2 * t + 1] = R.l[1];
   }
-  if (WPU == 1)
-    __syncwarp();
-  else
+}
+
+// one pair's output row: 4 dimensions per lane, M and L its maximum and sum
+__device__ __forceinline__ void write_pair(const Paged8Args& a, const Paged8Tile& tl, int rho, int kvh,
+                                           int lane, const float (&acc)[4], float M, float L) {
+  int row, g;
+  split_pair(a, rho, row, g);
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const int64_t r = tl.rq.row0 + (int64_t)row;
+  const int h = kvh * a.group + g;
+  *reinterpret_cast<uint2*>(a.out + r * a.out_stride + h * 128 + 4 * lane) = make_uint2(
+      pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  if (a.lse && lane == 0) a.lse[r * a.heads + h] = L > 0.f ? M + log2f(L) : -INFINITY;
+}
+
+// zeros to the rows behind the last request, worker i of n taking every n-th
+__device__ __forceinline__ void zero_tail(const Paged8Args& a, int kvh, int64_t i, int64_t n, int lane) {
+  const int end = a.q_start[a.n];
+  if (end < 0) return;
+  for (int64_t r = end + i; r < a.rows; r += n) {
+    uint4* dst = reinterpret_cast<uint4*>(a.out + r * a.out_stride + kvh * a.group * 128);
+    for (int e = lane; e < a.group * 16; e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
+    if (a.lse)
+      for (int e = lane; e < a.group; e += 32) a.lse[r * a.heads + kvh * a.group + e] = -INFINITY;
+  }
+}
+
+constexpr int kMinPages = 2 * kWarps;  // of a part at least
+
+template <int FMT>
+__global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args a) {
+  __shared__ __align__(16) float so[kWarps][kRows][kPitch];
+  __shared__ __align__(16) uint32_t sq[kWarps][8][32][2];
+  __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int split = (int)(blockIdx.x % a.splits);
+  const int kvh = (int)(blockIdx.x / a.splits % a.kv_heads);
+  const int tile = (int)(blockIdx.x / a.splits / a.kv_heads);
+  const int b = tile / a.direct, first = tile % a.direct * kRows;
+  if (a.zero_tail && split == 0)
+    zero_tail(a, kvh, (int64_t)tile * kWarps + w, (int64_t)a.n * a.direct * kWarps, lane);
+  // Tiles beyond those the launch counted on (a request of more rows than
+  // max_rows said) follow in the same block, their keys in one part.
+  for (int rho0 = first;; rho0 += a.direct * kRows) {
+    const Paged8Tile tl = small_tile(a, b, rho0, split == 0 && kvh == 0 && threadIdx.x == 0);
+    if (!tl.live) return;
+    const int parts = rho0 == first ? parts_of<kMinPages>(tl.np, a.splits) : 1;
+    if (split >= parts) return;
+    const int p_end = tl.p0 + (int)((int64_t)tl.np * (split + 1) / parts);
+    int p = tl.p0 + (int)((int64_t)tl.np * split / parts) + w;
+    Running R;
+    start(R);
+    if (p < p_end) {
+      const int32_t* row = a.table + tl.b * a.table_stride;
+      int page = page_at(a, row, p, lane);
+      int page_next = p + kWarps < p_end ? page_at(a, row, p + kWarps, lane) : -1;
+      const Columns c = columns(a, tl, lane);
+      const int key0 = 16 * (g >> 1) + (g & 1);  // key of row g (+ 2: row g + 8) of product m: + 4 m
+      // codes of product m: [row g, g + 8][dimension half]
+      const auto load_k = [&](uint4 (&kr)[2][2], int m, int pp, int pg) {
+        const uint8_t* kp = a.k + ((int64_t)pg * a.kv_heads + kvh) * kPageHeadBytes + t * 16;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = key0 + 4 * m + 2 * e;
+          const bool in = pg >= 0 && pp * kPage + key >= tl.lo && pp * kPage + key < tl.hi;
+          kr[e][0] = ld_codes(kp + key * 64, in);
+          kr[e][1] = ld_codes(kp + kPage * 64 + key * 64, in);
+        }
+      };
+      uint4 kr[4][2][2];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) load_k(kr[m], m, p, page);
+      float sc[2];
+      {  // the query fragments wait in shared memory: a lane reads back its own
+        uint32_t qf[8][2];
+        load_queries(a, c, kvh, t, qf, sc);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq[w][i][lane][0] = qf[i][0], sq[w][i][lane][1] = qf[i][1];
+      }
+      const uint32_t q_at = smem_u32(&sq[w][0][lane][0]);
+      for (; p < p_end; p += kWarps) {
+        const int page_now = page;
+        page = page_next;
+        page_next = p + 2 * kWarps < p_end ? page_at(a, row, p + 2 * kWarps, lane) : -1;
+        const bool have = page_now >= 0;
+        const int64_t at = have ? (int64_t)page_now * a.kv_heads + kvh : 0;
+        const float ks = a.k_scale[at], vs = a.v_scale[at];
+        const uint8_t* vp = a.v + at * kPageHeadBytes + t * 16 + g * kPage;
+        const bool v_in = have && p * kPage + 16 * t + 15 >= tl.lo && p * kPage + 16 * t < tl.hi;
+        // the values' codes take the registers that the keys' leave
+        uint4 vr[8][2];
+        float s[4][4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a0, a1, a2, a3;
+              decode4<FMT>(word(kr[m][0][h], i), a0, a2);
+              decode4<FMT>(word(kr[m][1][h], i), a1, a3);
+              const uint2 qf = ld_shared2(q_at + (4 * h + i) * 256);
+              mma_f16(s[m], a0, a1, a2, a3, qf.x, qf.y);
+            }
+#pragma unroll
+          for (int d = 2 * m; d < 2 * m + 2; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) vr[d][e] = ld_codes(vp + (16 * d + 8 * e) * kPage, v_in);
+        }
+        const bool whole = have && p * kPage >= c.all_lo && (p + 1) * kPage <= c.all_hi;
+        uint32_t pb[4][2];
+        weigh<4>(R, s, c, sc, ks, vs, whole, have, p * kPage + key0, pb);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            uint32_t a0, a1, a2, a3;
+            decode4<FMT>(word(vr[d][0], m), a0, a2);
+            decode4<FMT>(word(vr[d][1], m), a1, a3);
+            mma_f16(R.o[d], a0, a1, a2, a3, pb[m][0], pb[m][1]);
+          }
+          // the next page's keys (zeros behind the last) take the values' registers
+          if (d & 1) load_k(kr[d >> 1], d >> 1, p + kWarps, page);
+        }
+      }
+    }
+    spill(R, so[w], sm[w], sl[w], lane);
     __syncthreads();
-  // 8 rows x 32 lanes of 4 dimensions over the unit's warps
-  for (int r = w; r < kRows; r += WPU) {
-    const int pr = tl.rho0 + r;
-    if (pr >= tl.pairs) break;
-    float M = -INFINITY;
+    for (int r = w; r < kRows && tl.rho0 + r < tl.pairs; r += kWarps) {
+      float M = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < WPU; ++q) M = fmaxf(M, sm[WPU == 1 ? warp : q][r]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[4] = {};
+      for (int q = 0; q < kWarps; ++q) M = fmaxf(M, sm[q][r]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      float L = 0.f, acc[4] = {};
 #pragma unroll
-    for (int q = 0; q < WPU; ++q) {
-      const int src = WPU == 1 ? warp : q;
-      const float f = ex2_approx(sm[src][r] - ref);
-      L = fmaf(sl[src][r], f, L);
-      const float4 v = *reinterpret_cast<const float4*>(&so[src][r][4 * lane]);
-      acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
-      acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
+      for (int q = 0; q < kWarps; ++q) {
+        const float f = ex2_approx(sm[q][r] - ref);
+        L = fmaf(sl[q][r], f, L);
+        const float4 v = *reinterpret_cast<const float4*>(&so[q][r][4 * lane]);
+        acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
+        acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
+      }
+      if (parts == 1) {
+        write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, M, L);
+      } else {
+        const int64_t at = (int64_t)blockIdx.x * kRows + r;
+        *reinterpret_cast<float4*>(a.part_o + at * 128 + 4 * lane) =
+            make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+      }
     }
-    if (parts == 1) {
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      const int64_t orow = tl.rq.row0 + (int64_t)(pr / a.group);
-      const int oh = kvh * a.group + pr % a.group;
-      const uint2 v = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv),
-                                 pack_bf16x2(acc[2] * inv, acc[3] * inv));
-      *reinterpret_cast<uint2*>(a.out + orow * a.out_stride + oh * 128 + 4 * lane) = v;
-      if (a.lse && lane == 0) a.lse[orow * a.heads + oh] = L > 0.f ? M + log2f(L) : -INFINITY;
-    } else {
-      const int64_t at = unit * kRows + r;
-      *reinterpret_cast<float4*>(a.part_o + at * 128 + 4 * lane) =
-          make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+    __syncthreads();
+  }
+}
+
+template <int MB>
+__device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t (&w)[MB]) {
+  static_assert(MB == 1 || MB == 2, "4 or 8 bytes");
+  if (MB == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x, w[MB - 1] = v.y;
+  } else {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+
+// 16 * MB of a page's keys from token `base` of it.  Keys outside [from, to] of
+// the page read the nearest one inside: they are masked.
+template <int FMT, int MB>
+__device__ __forceinline__ void short_keys(const Paged8Args& a, const Columns& c, Running& R,
+                                           const uint32_t (&qf)[8][2], const float (&sc)[2], int64_t at,
+                                           int page_key, int base, int from, int to, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  const uint8_t* kp = a.k + at * kPageHeadBytes + t * 16;
+  const uint8_t* vp = a.v + at * kPageHeadBytes + g * kPage + base + 4 * MB * t;
+  const float ks = a.k_scale[at], vs = a.v_scale[at];
+  const int key0 = base + 4 * MB * (g >> 1) + (g & 1);
+  uint4 kr[MB][2][2];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int key = min(max(key0 + 4 * m + 2 * e, from), to);
+      kr[m][e][0] = __ldg(reinterpret_cast<const uint4*>(kp + key * 64));
+      kr[m][e][1] = __ldg(reinterpret_cast<const uint4*>(kp + kPage * 64 + key * 64));
     }
+  uint32_t vw[8][2][MB];
+#pragma unroll
+  for (int d = 0; d < 8; ++d)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) ld_words<MB>(vp + (16 * d + 8 * e) * kPage, vw[d][e]);
+  float s[MB][4];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
+  // the products of different keys are independent: they alternate
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        uint32_t a0, a1, a2, a3;
+        decode4<FMT>(word(kr[m][0][h], i), a0, a2);
+        decode4<FMT>(word(kr[m][1][h], i), a1, a3);
+        mma_f16(s[m], a0, a1, a2, a3, qf[4 * h + i][0], qf[4 * h + i][1]);
+      }
+  const bool whole = page_key + base >= c.all_lo && page_key + base + 16 * MB <= c.all_hi;
+  uint32_t pb[MB][2];
+  weigh<MB>(R, s, c, sc, ks, vs, whole, true, page_key + key0, pb);
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      uint32_t a0, a1, a2, a3;
+      decode4<FMT>(vw[d][0][m], a0, a2);
+      decode4<FMT>(vw[d][1][m], a1, a3);
+      mma_f16(R.o[d], a0, a1, a2, a3, pb[m][0], pb[m][1]);
+    }
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args a, int64_t units) {
+  __shared__ __align__(16) float so[kWarps][kRows][kPitch];
+  __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t unit = (int64_t)blockIdx.x * kWarps + w;
+  if (unit >= units) return;
+  const int kvh = (int)(unit % a.kv_heads), tile = (int)(unit / a.kv_heads);
+  const int b = tile / a.direct;
+  if (a.zero_tail) zero_tail(a, kvh, tile, (int64_t)a.n * a.direct, lane);
+  for (int rho0 = tile % a.direct * kRows;; rho0 += a.direct * kRows) {
+    const Paged8Tile tl = small_tile(a, b, rho0, kvh == 0 && lane == 0);
+    if (!tl.live) return;
+    const Columns c = columns(a, tl, lane);
+    const int32_t* row = a.table + tl.b * a.table_stride;
+    Running R;
+    start(R);
+    uint32_t qf[8][2];
+    float sc[2];
+    load_queries(a, c, kvh, lane & 3, qf, sc);
+    for (int p = tl.p0; p < tl.p0 + tl.np; ++p) {
+      const int page = page_at(a, row, p, lane);
+      if (page < 0) continue;
+      const int64_t at = (int64_t)page * a.kv_heads + kvh;
+      const int from = max(tl.lo - p * kPage, 0), to = min(tl.hi - p * kPage, kPage) - 1;
+      for (int base = from & ~15; base <= to; base += 32) {
+        if (to - base < 16)
+          short_keys<FMT, 1>(a, c, R, qf, sc, at, p * kPage, base, from, to, lane);
+        else
+          short_keys<FMT, 2>(a, c, R, qf, sc, at, p * kPage, base, from, to, lane);
+      }
+    }
+    spill(R, so[w], sm[w], sl[w], lane);
+    __syncwarp();
+    for (int r = 0; r < kRows && tl.rho0 + r < tl.pairs; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(&so[w][r][4 * lane]);
+      const float acc[4] = {v.x, v.y, v.z, v.w};
+      write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, sm[w][r], sl[w][r]);
+    }
+    __syncwarp();
   }
 }
 
 // The parts of a tile's keys joined in split order; one warp per (row, head)
 // pair.  The large kernel numbers its tiles from the last and counts its parts
-// in 128-key tiles.
+// in 128-key tiles.  Launched to overlap the end of the attention kernel.
 template <int kTileRows>
 __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t tiles) {
   constexpr bool kLarge = kTileRows == kPaged8LargeRows;
@@ -327,34 +538,36 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
   const int64_t unit = blockIdx.x / kGroups;  // (tile, key head) as its kernel numbers them
   const int r = (int)(blockIdx.x % kGroups) * 8 + (threadIdx.x >> 5);
   const int kvh = (int)(unit % a.kv_heads);
-  const int64_t tile = kLarge ? tiles - 1 - unit / a.kv_heads : unit / a.kv_heads;
-  const Paged8Tile tl = paged8_tile<kTileRows>(a, tile, false);
-  if (!tl.live || tl.b == a.n || (tl.pairs <= a.row_limit) == kLarge) return;
+  const int64_t tile = unit / a.kv_heads;
+  const Paged8Tile tl = kLarge ? paged8_tile<kTileRows>(a, tiles - 1 - tile, false)
+                               : small_tile(a, (int)(tile / a.direct), (int)(tile % a.direct) * kRows, false);
+  // every block waits: what follows this kernel on the stream needs the attention done
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!tl.live || (kLarge && (tl.b == a.n || tl.pairs <= a.row_limit))) return;
   const int parts = kLarge ? parts_of<kPaged8LargeMin>((tl.np + 1) / 2, a.splits)
-                           : parts_of<kMinPages<4>>(tl.np, a.splits);
+                           : parts_of<kMinPages>(tl.np, a.splits);
   const int pr = tl.rho0 + r;
   if (parts == 1 || pr >= tl.pairs) return;
   const int64_t at = unit * a.splits * kTileRows + r;
-  float M = -INFINITY;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[(at + (int64_t)s * kTileRows) * 2]);
-  const float ref = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc[4] = {};
-#pragma unroll 4
+  // lane s holds part s's maximum and sum (at most 32 parts)
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < parts) ml = *reinterpret_cast<const float2*>(a.part_ml + (at + (int64_t)lane * kTileRows) * 2);
+  float M = ml.x;
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
+  const float mine = ex2_approx(ml.x - (M == -INFINITY ? 0.f : M));
+  float L = ml.y * mine;
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) L += __shfl_xor_sync(0xffffffffu, L, i);
+  float acc[4] = {};
+#pragma unroll 8
   for (int s = 0; s < parts; ++s) {
-    const int64_t ps = at + (int64_t)s * kTileRows;
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + ps * 2);
-    const float4 v = *reinterpret_cast<const float4*>(a.part_o + ps * 128 + 4 * lane);
-    const float f = ex2_approx(ml.x - ref);
-    L = fmaf(ml.y, f, L);
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (at + (int64_t)s * kTileRows) * 128 + 4 * lane);
+    const float f = __shfl_sync(0xffffffffu, mine, s);
     acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
     acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-  const int64_t orow = tl.rq.row0 + (int64_t)(pr / a.group);
-  const int oh = kvh * a.group + pr % a.group;
-  *reinterpret_cast<uint2*>(a.out + orow * a.out_stride + oh * 128 + 4 * lane) = make_uint2(
-      pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-  if (a.lse && lane == 0) a.lse[orow * a.heads + oh] = L > 0.f ? M + log2f(L) : -INFINITY;
+  write_pair(a, tl, pr, kvh, lane, acc, M, L);
 }
 
 // How a call is cut, from the sizes the host knows (the same for every content
@@ -362,10 +575,11 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
 // key head run on the small kernel, longer ones on the large one; a call that
 // may hold both runs both, each leaving the other's requests.
 constexpr int kSmallPairs = 16;
+constexpr int kShortPages = 4;
 
 struct Shape {
   bool small, large;
-  int direct, warps, small_splits, large_splits;
+  int direct, small_splits, large_splits;
   int64_t small_tiles, large_tiles;
   int64_t floats;  // workspace: the small kernel's parts, then the large one's
   int64_t small_floats;
@@ -377,19 +591,20 @@ Shape shape_of(int64_t rows, int group, int kv_heads, int n, int width, int max_
   Shape s = {};
   const int64_t most = max_rows > 0 && max_rows < rows ? max_rows : rows;
   const int64_t some = n < rows ? n : rows;  // requests that can have rows
-  s.small = most * group <= kSmallPairs || n > 1;
-  s.large = most * group > kSmallPairs;
+  s.small = n > 0 && (most * group <= kSmallPairs || n > 1);
+  s.large = n == 0 || most * group > kSmallPairs;
   if (s.small) {
-    s.direct = s.large ? (kSmallPairs + kRows - 1) / kRows : 0;
-    s.small_tiles = s.large ? (int64_t)n * s.direct : paged8_tiles<kRows>(rows, group, n);
-    // tiles that are likely there, to size the splits by
-    int64_t real = s.large ? some : (rows * group + kRows - 1) / kRows;
-    if (real < some) real = some;
-    s.warps = width > 4 ? 4 : 1;
+    const int64_t pairs = s.large ? kSmallPairs : most * group;
+    s.direct = (int)((pairs + kRows - 1) / kRows);
+    s.small_tiles = (int64_t)n * s.direct;
     s.small_splits = 1;
-    if (s.warps == 4) {
-      const int64_t want = (148 * 2 + real * kv_heads - 1) / (real * kv_heads);
-      s.small_splits = clamp_int(want, 1, clamp_int(width / kMinPages<4>, 1, 64));
+    if (width > kShortPages) {
+      // one wave of blocks (3 per SM) with 2 pages per warp at least, or four
+      // waves, which even out unequal lengths, with 4
+      const int64_t work = some * s.direct * kv_heads;
+      const int64_t one = std::min<int64_t>(148 * 3 / work, width / kMinPages);
+      const int64_t four = std::min<int64_t>(148 * 12 / work, width / (2 * kMinPages));
+      s.small_splits = clamp_int(std::max(one, four), 1, 32);
     }
     if (s.small_splits > 1) s.small_floats = s.small_tiles * kv_heads * s.small_splits * kRows * 130;
   }
@@ -412,24 +627,35 @@ int launch_merge(const Paged8Args& a, int64_t tiles, cudaStream_t st) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
   }
-  paged8_merge_kernel<kTileRows><<<(unsigned)blocks, 256, 0, st>>>(a, tiles);
-  HIER_CHECK_CUDA(cudaGetLastError(), "paged8_merge_kernel launch");
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged8_merge_kernel<kTileRows>, a, tiles),
+                  "paged8_merge_kernel launch");
   return HIER_OK;
 }
 
-int launch_small(const Paged8Args& a, int format, int warps, int64_t tiles, cudaStream_t st) {
+int launch_small(const Paged8Args& a, int format, int64_t tiles, cudaStream_t st) {
   const int64_t units = tiles * a.kv_heads * a.splits;
-  const int64_t blocks = warps == 1 ? (units + kWarps - 1) / kWarps : units;
-  if (blocks > INT32_MAX) {
+  if (units > INT32_MAX) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
   }
-  auto* kernel = warps == 1 ? (format == P8_INT8 ? paged8_small_kernel<P8_INT8, 1>
-                                                 : paged8_small_kernel<P8_E4M3, 1>)
-                            : (format == P8_INT8 ? paged8_small_kernel<P8_INT8, 4>
-                                                 : paged8_small_kernel<P8_E4M3, 4>);
-  kernel<<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, units);
-  HIER_CHECK_CUDA(cudaGetLastError(), "paged8_small_kernel launch");
+  if (a.width <= kShortPages) {
+    auto* kernel = format == P8_INT8 ? paged8_short_kernel<P8_INT8> : paged8_short_kernel<P8_E4M3>;
+    kernel<<<(unsigned)((units + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(a, units);
+    HIER_CHECK_CUDA(cudaGetLastError(), "paged8_short_kernel launch");
+    return HIER_OK;
+  }
+  auto* kernel = format == P8_INT8 ? paged8_long_kernel<P8_INT8> : paged8_long_kernel<P8_E4M3>;
+  kernel<<<(unsigned)units, kWarps * 32, 0, st>>>(a);
+  HIER_CHECK_CUDA(cudaGetLastError(), "paged8_long_kernel launch");
   return a.splits > 1 ? launch_merge<kPaged8SmallRows>(a, tiles, st) : HIER_OK;
 }
 
@@ -547,7 +773,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
     a.splits = s.small_splits;
     a.part_o = workspace;
     a.part_ml = workspace + s.small_floats / 130 * 128;
-    rc = launch_small(a, format, s.warps, s.small_tiles, st);
+    rc = launch_small(a, format, s.small_tiles, st);
   }
   return rc;
 }

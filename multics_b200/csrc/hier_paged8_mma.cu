@@ -483,6 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  asm volatile("griddepcontrol.launch_dependents;");
   const int warp = warp_id(), lane = lane_id();
   // the last tiles of a request see the most keys: they come first
   const int split = blockIdx.x % a.splits;

@@ -46,7 +46,7 @@ struct Paged8Args {
   float* part_ml;   // [tile][kv head][split][kRows][2]
   int row_limit;    // requests of up to row_limit pairs are the small kernel's, the others the
                     // large one's (INT_MAX: all the small one's, 0: all the large one's)
-  int direct;       // small kernel: > 0: tile t is tile t % direct of request t / direct
+  int direct;       // small kernel: its tile t is tile t % direct of request t / direct
   int32_t* status;
   int* err;         // bounded waits
 };
@@ -84,23 +84,29 @@ __device__ __forceinline__ void row_keys(const Paged8Args& a, const Paged8Reques
   }
 }
 
+// the keys that the tile's rows (up to kRows pairs from rho0) see between them
+__device__ __forceinline__ void paged8_span(const Paged8Args& a, Paged8Tile& t, int rows) {
+  const int last = min(t.pairs, t.rho0 + rows) - 1;
+  int unused;
+  row_keys(a, t.rq, t.rho0 / a.group, t.lo, unused);
+  row_keys(a, t.rq, last / a.group, unused, t.hi);
+  if (t.hi > t.lo) {
+    t.p0 = t.lo / kPage;
+    t.np = (t.hi + kPage - 1) / kPage - t.p0;
+  }
+}
+
 template <int kRows>
 __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t tile, bool report) {
   Paged8Tile t;
   const int32_t* qs = a.q_start;
   const int64_t G = a.group;
+  t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
   t.live = false;
   t.rho0 = t.pairs = t.lo = t.hi = t.p0 = t.np = 0;
-  int64_t rho0;
-  if (kRows == kPaged8SmallRows && a.direct) {
-    t.b = (int)(tile / a.direct);
-    rho0 = tile % a.direct * kRows;
-  } else {
-    t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
-    const int64_t first = qs[t.b] * G / kRows + t.b;
-    if (tile < first) return t;
-    rho0 = (tile - first) * kRows;
-  }
+  const int64_t first = qs[t.b] * G / kRows + t.b;
+  if (tile < first) return t;
+  const int64_t rho0 = (tile - first) * kRows;
   if (t.b == a.n) {  // rows behind the last request
     t.rq.row0 = qs[a.n];
     t.rq.n = a.rows - t.rq.row0;
@@ -118,15 +124,7 @@ __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t t
   t.live = true;
   t.rho0 = (int)rho0;
   t.pairs = (int)(t.rq.n * G);
-  if (t.b == a.n) return t;
-  const int last = min(t.pairs, t.rho0 + kRows) - 1;
-  int unused;
-  row_keys(a, t.rq, t.rho0 / a.group, t.lo, unused);
-  row_keys(a, t.rq, last / a.group, unused, t.hi);
-  if (t.hi > t.lo) {
-    t.p0 = t.lo / kPage;
-    t.np = (t.hi + kPage - 1) / kPage - t.p0;
-  }
+  if (t.b < a.n) paged8_span(a, t, kRows);
   return t;
 }
 

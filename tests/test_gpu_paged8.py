@@ -376,6 +376,15 @@ def test_attention_long_keys_few_heads(dtype, lengths, counts):
     _check(c, table, lengths, counts, 4, g, max_rows=max(counts))
 
 
+@pytest.mark.parametrize("width", [None, 90])
+def test_attention_max_rows_chooses_kernels_not_results(width):
+    """Requests of more rows than the caller said, short and split keys."""
+    lengths, counts = [300, 40, 2000 if width else 200], [30, 17, 9]
+    c, table, g = _filled(lengths, 2, torch.int8, width=width)
+    for most in (1, 8, 9, 20, None):
+        _check(c, table, lengths, counts, 4, g, spare=5, max_rows=most)
+
+
 def test_attention_rows_of_other_sequences_than_the_cache():
     """block_frames=0: the rows need not be tokens of the cache."""
     lengths, counts = [30, 0, 100], [70, 5, 3]
