@@ -269,3 +269,11 @@ def stream_ptr(device=None):
     import torch
 
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(index):
+    """Handle of the current stream of device ``index`` (an int: what
+    ``current_stream(device).cuda_stream`` gives, without the objects)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)

@@ -28,6 +28,7 @@ import torch.nn as nn
 from . import _lib
 from ._lib import check, ptr, stream_ptr
 from .hier_masks import HierBlockMask, block_mask_for_spec, build_dense_block_plan
+from .paged8 import on_device, token_rows
 
 __all__ = ["hier_prep_qk", "hier_block_attention", "freqs_table", "RMSNorm", "SelfAttention",
            "AttentionPlan", "attention_from_plan", "HierSequencePlan", "sequence_plan",
@@ -42,7 +43,7 @@ _DEV_ERR = {}
 
 
 def _dev_err(device):
-    key = torch.device(device).index
+    key = device.index if isinstance(device, torch.device) else torch.device(device).index
     if key is None:  # "cuda" is the current device, whose tensors carry its index
         key = torch.cuda.current_device()
     t = _DEV_ERR.get(key)
@@ -139,25 +140,24 @@ def head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight, k_weight, pos
     """The checked arguments of the per-head prologue: q and k as aligned rows,
     the head size, contiguous weights of one type, the rotation table and the
     positions."""
-    from .paged8 import token_rows
-
-    if num_heads < 1 or num_kv_heads < 1 or q.shape[-1] % num_heads:
+    dim = q.shape[-1]
+    if num_heads < 1 or num_kv_heads < 1 or dim % num_heads:
         raise ValueError(f"q {tuple(q.shape)} does not split into {num_heads} heads")
-    D = q.shape[-1] // num_heads
+    D = dim // num_heads
     if D not in (64, 128, 256):
         raise NotImplementedError(f"the per-head norm supports head_dim 64, 128 and 256; got {D}")
-    q, k = token_rows("q", q, num_heads * D), token_rows("k", k, num_kv_heads * D)
-    T = q.shape[0]
+    q, k = token_rows("q", q, dim), token_rows("k", k, num_kv_heads * D)
+    T, dev = q.shape[0], q.device
     if k.shape[0] != T:
         raise ValueError(f"q has {T} rows, k {k.shape[0]}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if tuple(w.shape) != (D,):
-            raise ValueError(f"{name} must be [{D}], got {tuple(w.shape)}")
-    if q_weight.dtype == k_weight.dtype == torch.bfloat16:
+    if q_weight.shape != (D,) or k_weight.shape != (D,):
+        raise ValueError(f"q_weight and k_weight must be [{D}], got {tuple(q_weight.shape)} and "
+                         f"{tuple(k_weight.shape)}")
+    if q_weight.dtype is k_weight.dtype is torch.bfloat16:
         wq, wk = q_weight.contiguous(), k_weight.contiguous()
     else:
         wq, wk = q_weight.float().contiguous(), k_weight.float().contiguous()
-    ft = freqs if (freqs.dtype == torch.float32 and freqs.dim() == 3
+    ft = freqs if (freqs.dtype is torch.float32 and freqs.dim() == 3
                    and freqs.shape[-1] == 2) else freqs_table(freqs)
     if ft.shape[0] < 1 or ft.shape[1] * 2 != D:
         raise ValueError(f"freqs must be [F, {D // 2}, 2] (or complex [F, 1, {D // 2}]), got "
@@ -166,18 +166,19 @@ def head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight, k_weight, pos
         if T % ft.shape[0]:
             raise ValueError(f"without positions the {ft.shape[0]} table rows must divide the "
                              f"{T} rows")
-    elif positions.dtype != torch.int32 or tuple(positions.shape) != (T,):
+    elif positions.dtype is not torch.int32 or positions.shape != (T,):
         raise ValueError(f"positions must be int32 [{T}], got {positions.dtype} "
                          f"{tuple(positions.shape)}")
-    if not q.is_cuda:
+    else:
+        positions = positions.contiguous()
+    if dev.type != "cuda":
         raise NotImplementedError("the per-head norm requires CUDA tensors")
-    ft = ft.to(q.device).contiguous()
-    if ft.data_ptr() % 16:
-        ft = ft.clone()
-    for name, t in (("k", k), ("q_weight", wq), ("k_weight", wk), ("positions", positions)):
-        if t is not None and t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, expected {q.device}")
-    return q, k, D, wq, wk, ft, None if positions is None else positions.contiguous()
+    if ft.device != dev or not ft.is_contiguous() or ft.data_ptr() % 16:
+        ft = ft.to(dev).clone(memory_format=torch.contiguous_format)
+    if k.device != dev or wq.device != dev or wk.device != dev or (positions is not None and
+                                                                   positions.device != dev):
+        raise ValueError(f"q, k, the weights and positions must be on one device, {dev}")
+    return q, k, D, wq, wk, ft, positions
 
 
 def hier_head_norm_rope(q, k, freqs, num_heads, num_kv_heads, *, q_weight, k_weight,
@@ -194,36 +195,42 @@ def hier_head_norm_rope(q, k, freqs, num_heads, num_kv_heads, *, q_weight, k_wei
     ``(q_out, k_out)`` to write to (16-byte aligned rows), ``out_rows`` / ``k_out_rows`` (int32 ``[T]``)
     the row of each token in them (``k_out_rows`` for k alone, e.g. the slots of
     a paged pool; negative: not written)."""
-    from .paged8 import on_device
-
-    q2, k2, D, wq, wk, ft, pos = head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight,
-                                                k_weight, positions)
-    T, dev = q2.shape[0], q2.device
-    k_rows = out_rows if k_out_rows is None else k_out_rows
-    for name, m in (("out_rows", out_rows), ("k_out_rows", k_out_rows)):
-        if m is not None and (m.dtype != torch.int32 or tuple(m.shape) != (T,) or m.device != dev
-                              or not m.is_contiguous()):
-            raise ValueError(f"{name} must be int32 [{T}] on {dev}")
+    args = head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight, k_weight, positions)
     if out is None and k_out_rows is not None:
         raise ValueError("k_out_rows needs out=(q_out, k_out)")
+    return head_norm_launch(args, num_heads, num_kv_heads, eps, out, out_rows,
+                            out_rows if k_out_rows is None else k_out_rows)
+
+
+def head_norm_launch(args, num_heads, num_kv_heads, eps, out=None, q_rows=None, k_rows=None):
+    """The per-head prologue kernel on checked arguments (:func:`head_norm_args`)."""
+    q2, k2, D, wq, wk, ft, pos = args
+    T, dev = q2.shape[0], q2.device
+    for m in (q_rows, k_rows):
+        if m is not None and (m.dtype != torch.int32 or tuple(m.shape) != (T,) or m.device != dev
+                              or not m.is_contiguous()):
+            raise ValueError(f"out_rows and k_out_rows must be int32 [{T}] on {dev}")
     with on_device(dev):
         if out is None:
             q_out = torch.empty((T, num_heads * D), dtype=torch.bfloat16, device=dev)
             k_out = torch.empty((T, num_kv_heads * D), dtype=torch.bfloat16, device=dev)
         else:
             q_out, k_out = out
-            for name, t, w, m in (("q_out", q_out, num_heads * D, out_rows),
+            for name, t, w, m in (("q_out", q_out, num_heads * D, q_rows),
                                   ("k_out", k_out, num_kv_heads * D, k_rows)):
                 if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != w or t.device != dev \
                         or t.stride(1) != 1 or (m is None and t.shape[0] < T):
                     raise ValueError(f"{name} must be bf16 [{T}, {w}] rows on {dev}, got {t.dtype} "
                                      f"{tuple(t.shape)}")
-        check(_lib.lib().hier_head_norm_rope(
-            ptr(q2), q2.stride(0), ptr(k2), k2.stride(0), T, num_heads, num_kv_heads, D, ptr(wq),
-            ptr(wk), int(wq.dtype == torch.float32), ptr(ft), ft.shape[0], ptr(pos), float(eps),
-            ptr(q_out), q_out.stride(0), ptr(out_rows), q_out.shape[0], ptr(k_out),
-            k_out.stride(0), ptr(k_rows), k_out.shape[0], int(out is None), ptr(_dev_err(dev)),
-            stream_ptr(dev)))
+        rc = _lib.lib().hier_head_norm_rope(
+            q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, num_heads, num_kv_heads,
+            D, wq.data_ptr(), wk.data_ptr(), int(wq.dtype is torch.float32), ft.data_ptr(),
+            ft.shape[0], None if pos is None else pos.data_ptr(), float(eps), q_out.data_ptr(),
+            q_out.stride(0), None if q_rows is None else q_rows.data_ptr(), q_out.shape[0],
+            k_out.data_ptr(), k_out.stride(0), None if k_rows is None else k_rows.data_ptr(),
+            k_out.shape[0], int(out is None), _dev_err(dev).data_ptr(), _lib.raw_stream(dev.index))
+    if rc:
+        check(rc)
     return q_out, k_out
 
 

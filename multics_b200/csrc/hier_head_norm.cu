@@ -369,6 +369,10 @@ extern "C" int hier_head_norm_rope_bwd_partials(int64_t rows, int32_t hq, int32_
   clear_error();
   int rc = check_sizes(rows, hq, hk, D, 1, nullptr, nullptr);
   if (rc) return rc;
+  if (!blocks) {
+    set_error(HIER_EVALUE, "no place for the number of partial rows");
+    return HIER_EVALUE;
+  }
   *blocks = bwd_blocks(rows, hq, hk, D);
   return HIER_OK;
 }

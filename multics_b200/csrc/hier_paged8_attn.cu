@@ -355,21 +355,26 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
         // the values' codes take the registers that the keys' leave
         uint4 vr[8][2];
         float s[4][4];
+        // two products' chains alternate
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
+        for (int m = 0; m < 4; m += 2) {
+#pragma unroll
+          for (int q = m; q < m + 2; ++q) s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              uint32_t a0, a1, a2, a3;
-              decode4<FMT>(word(kr[m][0][h], i), a0, a2);
-              decode4<FMT>(word(kr[m][1][h], i), a1, a3);
               const uint2 qf = ld_shared2(q_at + (4 * h + i) * 256);
-              mma_f16(s[m], a0, a1, a2, a3, qf.x, qf.y);
+#pragma unroll
+              for (int q = m; q < m + 2; ++q) {
+                uint32_t a0, a1, a2, a3;
+                decode4<FMT>(word(kr[q][0][h], i), a0, a2);
+                decode4<FMT>(word(kr[q][1][h], i), a1, a3);
+                mma_f16(s[q], a0, a1, a2, a3, qf.x, qf.y);
+              }
             }
 #pragma unroll
-          for (int d = 2 * m; d < 2 * m + 2; ++d)
+          for (int d = 2 * m; d < 2 * m + 4; ++d)
 #pragma unroll
             for (int e = 0; e < 2; ++e) vr[d][e] = ld_codes(vp + (16 * d + 8 * e) * kPage, v_in);
         }
@@ -377,16 +382,18 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
         uint32_t pb[4][2];
         weigh<4>(R, s, c, sc, ks, vs, whole, have, p * kPage + key0, pb);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
+        for (int d = 0; d < 8; d += 2) {
 #pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            uint32_t a0, a1, a2, a3;
-            decode4<FMT>(word(vr[d][0], m), a0, a2);
-            decode4<FMT>(word(vr[d][1], m), a1, a3);
-            mma_f16(R.o[d], a0, a1, a2, a3, pb[m][0], pb[m][1]);
-          }
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int q = d; q < d + 2; ++q) {
+              uint32_t a0, a1, a2, a3;
+              decode4<FMT>(word(vr[q][0], m), a0, a2);
+              decode4<FMT>(word(vr[q][1], m), a1, a3);
+              mma_f16(R.o[q], a0, a1, a2, a3, pb[m][0], pb[m][1]);
+            }
           // the next page's keys (zeros behind the last) take the values' registers
-          if (d & 1) load_k(kr[d >> 1], d >> 1, p + kWarps, page);
+          load_k(kr[d >> 1], d >> 1, p + kWarps, page);
         }
       }
     }
@@ -691,6 +698,10 @@ extern "C" int hier_paged8_attn_workspace(int32_t rows, int32_t heads, int32_t k
   clear_error();
   int rc = check_paged8(rows, heads, kv_heads, n, width);
   if (rc) return rc;
+  if (!floats) {
+    set_error(HIER_EVALUE, "no place for the workspace size");
+    return HIER_EVALUE;
+  }
   *floats = rows ? shape_of(rows, heads / kv_heads, kv_heads, n, width, max_rows).floats : 0;
   return HIER_OK;
 }

@@ -24,19 +24,21 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_ptr
+from ._lib import check, raw_stream
 
 __all__ = ["PAGE_TOKENS", "Paged8Cache", "PageStep", "page_step", "paged8_append",
            "paged8_attention"]
 
 PAGE_TOKENS = 64
 HEAD_DIM = 128
+_I32, _BF16 = torch.int32, torch.bfloat16
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _STATUS = {}
 
@@ -57,18 +59,23 @@ def on_device(dev):
     return torch.cuda.device(dev)
 
 
-def _need(name, t, dtype, dev, dim):
-    if t.dtype != dtype or t.dim() != dim:
-        raise ValueError(f"{name} must be {dtype} with {dim} dimension(s), got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, expected {dev}")
-
-
 def _vector(name, t, n, dev):
-    _need(name, t, torch.int32, dev, 1)
-    if t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 [{n}], got {tuple(t.shape)}")
+    if (t.dtype is not _I32 or t.dim() != 1 or t.shape[0] != n or t.device != dev
+            or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous int32 [{n}] on {dev}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+
+
+def _table(t, dev):
+    """(requests, width, row stride) of a block table."""
+    if t.dtype is not _I32 or t.dim() != 2 or t.device != dev:
+        raise ValueError(f"table must be int32 [requests, width] on {dev}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    n, width = t.shape
+    stride, inner = t.stride()
+    if n and width and (inner != 1 or stride < width):
+        raise ValueError("table must be row-major")
+    return n, width, stride if stride > width else width
 
 
 def _cuda(what, dev):
@@ -87,9 +94,10 @@ def token_rows(name, x, width):
         x = x[0]
     if x.dim() != 2 or x.shape[1] != width:
         raise ValueError(f"{name} must be [T, {width}], got {tuple(x.shape)}")
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not _BF16:
         raise NotImplementedError(f"{name} must be bf16; got {x.dtype}")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < width or x.data_ptr() % 16:
+    stride, inner = x.stride()
+    if inner != 1 or stride % 8 or stride < width or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -123,7 +131,7 @@ class Paged8Cache:
     def _set(self, k, v, k_scale, v_scale, status):
         self.k, self.v, self.k_scale, self.v_scale, self.status = k, v, k_scale, v_scale, status
         self.num_pages, self.num_heads = k.shape[0], k.shape[1]
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.format = k.dtype, k.device, _FORMATS[k.dtype]
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale, status=None) -> "Paged8Cache":
@@ -203,13 +211,10 @@ def page_step(lengths, add, table, free_pages, free_count, rows: int, *,
     :meth:`PageStep.check` reports it.  ``in_place`` writes the new lengths and
     count over the old ones (a captured step)."""
     dev = table.device
-    _need("table", table, torch.int32, dev, 2)
-    n, width = table.shape
-    if n and width and (table.stride(1) != 1 or table.stride(0) < width):
-        raise ValueError("table must be row-major")
+    n, width, stride = _table(table, dev)
     _vector("lengths", lengths, n, dev)
     _vector("add", add, n, dev)
-    _vector("free_pages", free_pages, free_pages.shape[0], dev)
+    _vector("free_pages", free_pages, free_pages.shape[0] if free_pages.dim() else 0, dev)
     _vector("free_count", free_count, 1, dev)
     rows = int(rows)
     if rows < 0 or rows >= 1 << 31:
@@ -217,29 +222,37 @@ def page_step(lengths, add, table, free_pages, free_count, rows: int, *,
     if most_new is not None and most_new < 0:
         raise ValueError(f"most_new must not be negative, got {most_new}")
     _cuda("page_step", dev)
-    held, count = (0, 0) if in_place else (n, 1)
     with on_device(dev):
-        out = torch.empty(held + count + n + 2 + 2 * rows, dtype=torch.int32, device=dev)
-        new_len, new_count, q_start, status, slots, positions = out.split(
-            (held, count, n + 1, 1, rows, rows))
         if in_place:
+            q_start, status, slots, positions = torch.empty(
+                n + 2 + 2 * rows, dtype=_I32, device=dev).split((n + 1, 1, rows, rows))
             new_len, new_count = lengths, free_count
-        check(_lib.lib().hier_page_step(
-            ptr(lengths), ptr(add), n, ptr(table), max(table.stride(0), width), width,
-            ptr(free_pages), free_pages.shape[0], ptr(free_count), rows,
-            -1 if most_new is None else int(most_new), ptr(new_len), ptr(new_count), ptr(q_start),
-            ptr(slots), ptr(positions), ptr(status), stream_ptr(dev)))
+        else:
+            new_len, new_count, q_start, status, slots, positions = torch.empty(
+                2 * n + 3 + 2 * rows, dtype=_I32, device=dev).split((n, 1, n + 1, 1, rows, rows))
+        rc = _lib.lib().hier_page_step(
+            lengths.data_ptr(), add.data_ptr(), n, table.data_ptr(), stride, width,
+            free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), rows,
+            -1 if most_new is None else int(most_new), new_len.data_ptr(), new_count.data_ptr(),
+            q_start.data_ptr(), slots.data_ptr(), positions.data_ptr(), status.data_ptr(),
+            raw_stream(dev.index))
+    if rc:
+        check(rc)
     return PageStep(new_len, new_count, q_start, slots, positions, status)
 
 
 def _requests(cache, table, lengths, q_start):
-    _need("table", table, torch.int32, cache.device, 2)
-    n, width = table.shape
-    if n and width and (table.stride(1) != 1 or table.stride(0) < width):
-        raise ValueError("table must be row-major")
+    n, width, stride = _table(table, cache.device)
     _vector("lengths", lengths, n, cache.device)
     _vector("q_start", q_start, n + 1, cache.device)
-    return n, width
+    return n, width, stride
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_floats(*sizes):
+    floats = ctypes.c_int64()
+    check(_lib.lib().hier_paged8_attn_workspace(*sizes, ctypes.byref(floats)))
+    return floats.value
 
 
 def paged8_append(cache: Paged8Cache, k, v, table, lengths, q_start):
@@ -252,16 +265,20 @@ def paged8_append(cache: Paged8Cache, k, v, table, lengths, q_start):
     k, v = token_rows("k", k, width_k), token_rows("v", v, width_k)
     if k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} disagree")
-    n, width = _requests(cache, table, lengths, q_start)
-    _cuda("paged8_append", cache.device)
-    if k.device != cache.device or v.device != cache.device:
-        raise ValueError(f"k, v must be on {cache.device}")
-    with on_device(cache.device):
-        check(_lib.lib().hier_paged8_append(
-            ptr(k), k.stride(0), ptr(v), v.stride(0), k.shape[0], cache.num_heads,
-            _FORMATS[cache.dtype], ptr(cache.k), ptr(cache.v), ptr(cache.k_scale),
-            ptr(cache.v_scale), cache.num_pages, ptr(table), max(table.stride(0), width), width,
-            ptr(lengths), ptr(q_start), n, ptr(cache.status), stream_ptr(cache.device)))
+    n, width, stride = _requests(cache, table, lengths, q_start)
+    dev = cache.device
+    _cuda("paged8_append", dev)
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"k, v must be on {dev}")
+    with on_device(dev):
+        rc = _lib.lib().hier_paged8_append(
+            k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), k.shape[0], cache.num_heads,
+            cache.format, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
+            lengths.data_ptr(), q_start.data_ptr(), n, cache.status.data_ptr(),
+            raw_stream(dev.index))
+    if rc:
+        check(rc)
 
 
 def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: int, *,
@@ -298,37 +315,41 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
         raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
     dim = num_heads * HEAD_DIM
     q = token_rows("q", q, dim)
-    n, width = _requests(cache, table, lengths, q_start)
+    n, width, stride = _requests(cache, table, lengths, q_start)
     dev, T = cache.device, q.shape[0]
-    if out is not None and (out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != dev
+    if out is not None and (out.dtype is not _BF16 or out.shape != q.shape or out.device != dev
                             or out.stride(1) != 1 or (T > 1 and out.stride(0) < dim)):
         raise ValueError(f"out must be bf16 {tuple(q.shape)} rows on {dev}")
     _cuda("paged8_attention", dev)
     if q.device != dev:
         raise ValueError(f"q must be on {dev}")
-    zero_tail = out is None
-    most = 0 if max_rows is None else int(max_rows)
     from .attention import _dev_err
 
-    L = _lib.lib()
+    most = 0 if max_rows is None else int(max_rows)
+    lse = ws = None
     with on_device(dev):
-        given = out
         if out is None:
-            out = torch.empty((T, dim), dtype=torch.bfloat16, device=dev)
+            o = torch.empty((T, dim), dtype=_BF16, device=dev)
         elif out.data_ptr() % 16 or out.stride(0) % 8:  # rows the kernels cannot store to
-            out = out.clone(memory_format=torch.contiguous_format)
-        lse = torch.empty((T, num_heads), dtype=torch.float32, device=dev) if return_lse else None
-        floats = ctypes.c_int64()
-        check(L.hier_paged8_attn_workspace(T, num_heads, cache.num_heads, n, width, most,
-                                           ctypes.byref(floats)))
-        ws = (torch.empty(floats.value, dtype=torch.float32, device=dev) if floats.value else None)
-        check(L.hier_paged8_attn(
-            ptr(q), q.stride(0), T, num_heads, cache.num_heads, HEAD_DIM, _FORMATS[cache.dtype],
-            ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), cache.num_pages,
-            ptr(table), max(table.stride(0), width), width, ptr(lengths), ptr(q_start), n,
-            int(tokens_per_frame), int(block_frames), int(window), scale, most, ptr(out),
-            out.stride(0), ptr(lse), int(zero_tail), ptr(ws), ptr(cache.status),
-            ptr(_dev_err(dev)), stream_ptr(dev)))
-        if given is not None and out is not given:
-            out = given.copy_(out)
-    return (out, lse) if return_lse else out
+            o = out.clone(memory_format=torch.contiguous_format)
+        else:
+            o = out
+        if return_lse:
+            lse = torch.empty((T, num_heads), dtype=torch.float32, device=dev)
+        floats = _workspace_floats(T, num_heads, cache.num_heads, n, width, most)
+        if floats:
+            ws = torch.empty(floats, dtype=torch.float32, device=dev)
+        rc = _lib.lib().hier_paged8_attn(
+            q.data_ptr(), q.stride(0), T, num_heads, cache.num_heads, HEAD_DIM, cache.format,
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
+            lengths.data_ptr(), q_start.data_ptr(), n, int(tokens_per_frame), int(block_frames), int(window), scale,
+            most, o.data_ptr(), o.stride(0), None if lse is None else lse.data_ptr(),
+            int(out is None), None if ws is None else ws.data_ptr(), cache.status.data_ptr(),
+            _dev_err(dev).data_ptr(), raw_stream(dev.index))
+        if rc:
+            check(rc)
+        if out is not None and o is not out:
+            out.copy_(o)
+            o = out
+    return (o, lse) if return_lse else o

@@ -19,6 +19,7 @@ is recording.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -27,6 +28,7 @@ from . import _lib
 from ._lib import check, ptr, stream_ptr
 from .attention import _dev_err, _rows
 from .hier_masks import HierBlockMask
+from .paged8 import on_device, token_rows
 
 __all__ = ["BlockPlanGrad", "block_plan_grad", "hier_block_attention_grad", "plan_attention_grad",
            "prologue_grad", "head_norm_rope_grad"]
@@ -238,42 +240,52 @@ class _HeadNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, wq, wk, ft, positions, num_heads, num_kv_heads, eps):
-        from .attention import hier_head_norm_rope
+        from .attention import head_norm_args, head_norm_launch
 
-        ctx.save_for_backward(q, k, wq, wk, ft, positions)
-        ctx.sizes = num_heads, num_kv_heads, eps
-        return hier_head_norm_rope(q, k, ft, num_heads, num_kv_heads, q_weight=wq, k_weight=wk,
-                                   positions=positions, eps=eps)
+        args = head_norm_args(q, k, ft, num_heads, num_kv_heads, wq, wk, positions)
+        q2, k2, D, w1, w2, ft, pos = args
+        ctx.save_for_backward(q2, k2, w1, w2, ft, pos)
+        ctx.sizes = num_heads, num_kv_heads, D, eps
+        ctx.like = q.shape, k.shape, wq.dtype, wk.dtype
+        return head_norm_launch(args, num_heads, num_kv_heads, eps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        from .attention import head_norm_args
-        from .paged8 import on_device, token_rows
-
-        q, k, wq0, wk0, ft, positions = ctx.saved_tensors
-        H, Hk, eps = ctx.sizes
-        q2, k2, D, wq, wk, ft, pos = head_norm_args(q, k, ft, H, Hk, wq0, wk0, positions)
-        T, dev = q2.shape[0], q2.device
+        q2, k2, wq, wk, ft, pos = ctx.saved_tensors
+        H, Hk, D, eps = ctx.sizes
+        q_shape, k_shape, wq_dtype, wk_dtype = ctx.like
+        T, dev, bf = q2.shape[0], q2.device, torch.bfloat16
         L = _lib.lib()
         with on_device(dev):
-            gq = (torch.zeros((T, H * D), dtype=torch.bfloat16, device=dev) if gq is None
-                  else token_rows("gradient of q", gq.to(torch.bfloat16), H * D))
-            gk = (torch.zeros((T, Hk * D), dtype=torch.bfloat16, device=dev) if gk is None
-                  else token_rows("gradient of k", gk.to(torch.bfloat16), Hk * D))
-            dq = torch.empty((T, H * D), dtype=torch.bfloat16, device=dev)
-            dk = torch.empty((T, Hk * D), dtype=torch.bfloat16, device=dev)
+            gq = (torch.zeros((T, H * D), dtype=bf, device=dev) if gq is None
+                  else token_rows("gradient of q", gq.to(bf), H * D))
+            gk = (torch.zeros((T, Hk * D), dtype=bf, device=dev) if gk is None
+                  else token_rows("gradient of k", gk.to(bf), Hk * D))
+            dq = torch.empty(q_shape, dtype=bf, device=dev)
+            dk = torch.empty(k_shape, dtype=bf, device=dev)
             dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
-            n = ctypes.c_int32()
-            check(L.hier_head_norm_rope_bwd_partials(T, H, Hk, D, ctypes.byref(n)))
-            part = torch.empty((n.value, 2, D), dtype=torch.float32, device=dev)
-            check(L.hier_head_norm_rope_bwd(
-                ptr(q2), q2.stride(0), ptr(k2), k2.stride(0), T, H, Hk, D, ptr(wq), ptr(wk),
-                int(wq.dtype == torch.float32), ptr(ft), ft.shape[0], ptr(pos), float(eps), ptr(gq),
-                gq.stride(0), ptr(gk), gk.stride(0), ptr(dq), dq.stride(0), ptr(dk), dk.stride(0),
-                ptr(part), n.value, ptr(dwq), ptr(dwk), ptr(_dev_err(dev)), stream_ptr(dev)))
-            return (dq.view(q.shape), dk.view(k.shape), dwq.to(wq0.dtype), dwk.to(wk0.dtype), None,
-                    None, None, None, None)
+            blocks = _head_norm_blocks(T, H, Hk, D)
+            part = torch.empty((blocks, 2, D), dtype=torch.float32, device=dev)
+            rc = L.hier_head_norm_rope_bwd(
+                q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, H, Hk, D,
+                wq.data_ptr(), wk.data_ptr(), int(wq.dtype is torch.float32), ft.data_ptr(),
+                ft.shape[0], None if pos is None else pos.data_ptr(), float(eps), gq.data_ptr(),
+                gq.stride(0), gk.data_ptr(), gk.stride(0), dq.data_ptr(), H * D,
+                dk.data_ptr(), Hk * D, part.data_ptr(), blocks, dwq.data_ptr(),
+                dwk.data_ptr(), _dev_err(dev).data_ptr(), _lib.raw_stream(dev.index))
+            if rc:
+                check(rc)
+            if wq.dtype is not wq_dtype or wk.dtype is not wk_dtype:
+                dwq, dwk = dwq.to(wq_dtype), dwk.to(wk_dtype)
+            return dq, dk, dwq, dwk, None, None, None, None, None
+
+
+@functools.lru_cache(maxsize=256)
+def _head_norm_blocks(*sizes):
+    n = ctypes.c_int32()
+    check(_lib.lib().hier_head_norm_rope_bwd_partials(*sizes, ctypes.byref(n)))
+    return n.value
 
 
 def head_norm_rope_grad(q, k, freqs, num_heads: int, num_kv_heads: int, *, q_weight, k_weight,
