@@ -112,35 +112,38 @@ __device__ __forceinline__ bool uses(const Job& J, int h, int p) {
   return p * kPage < (h ? J.hi[1] : J.hi[0]) && (p + 2) * kPage > (h ? J.lo[1] : J.lo[0]);
 }
 
-__device__ __forceinline__ int page_of(const Paged8Args& a, const Job& J, int p) {
-  if (p >= J.page_end) return -1;
-  const int page = J.row[p];
-  return page >= 0 && page < a.n_pages ? page : -1;
+// Table entries are read ahead of their use and checked there, so that no role
+// waits for one: -1 behind the part's pages.
+__device__ __forceinline__ int entry(const Job& J, int p) {
+  return p < J.page_end ? __ldg(J.row + p) : -1;
+}
+__device__ __forceinline__ bool in_pool(const Paged8Args& a, int page) {
+  return page >= 0 && page < a.n_pages;
 }
 
 __device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uint8_t* smem,
                                           const Bars& B) {
-  int pg[2] = {page_of(a, J, J.page0), page_of(a, J, J.page0 + 1)};
+  int pg[2] = {entry(J, J.page0), entry(J, J.page0 + 1)};
   for (int j = 0; j < J.n_kv; ++j) {
     const int p = J.page0 + 2 * j;
-    const int now[2] = {pg[0], pg[1]};
-    if (now[0] < 0 || (now[1] < 0 && p + 1 < J.page_end)) atomicOr(a.status, P8_BAD_PAGE);
-    if (j + 1 < J.n_kv) pg[0] = page_of(a, J, p + 2), pg[1] = page_of(a, J, p + 3);
+    const int now0 = pg[0], now1 = pg[1];
+    pg[0] = entry(J, p + 2), pg[1] = entry(J, p + 3);
+    const bool have0 = in_pool(a, now0), have1 = in_pool(a, now1);
+    if (!have0 || (!have1 && p + 1 < J.page_end)) atomicOr(a.status, P8_BAD_PAGE);
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
       if (j > 0 && !mbar_wait(B.raw_empty + kind, (j - 1) & 1, a.err, 40 + kind)) return;
-      const uint32_t bytes = ((now[0] >= 0) + (now[1] >= 0)) * kPageHeadBytes;
+      const uint32_t bytes = (have0 + have1) * kPageHeadBytes;
       if (bytes)
         mbar_arrive_expect_tx(B.raw_full + kind, bytes);
       else
         mbar_arrive(B.raw_full + kind);
-      const uint8_t* src = kind ? a.v : a.k;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (now[i] >= 0)
-          bulk_load(smem + kSmemRaw + kind * kRawTile + i * kPageHeadBytes,
-                    src + ((int64_t)now[i] * a.kv_heads + J.kvh) * kPageHeadBytes, kPageHeadBytes,
-                    B.raw_full + kind);
+      const uint8_t* src = (kind ? a.v : a.k) + (int64_t)J.kvh * kPageHeadBytes;
+      const int64_t page_bytes = (int64_t)a.kv_heads * kPageHeadBytes;
+      uint8_t* dst = smem + kSmemRaw + kind * kRawTile;
+      if (have0) bulk_load(dst, src + now0 * page_bytes, kPageHeadBytes, B.raw_full + kind);
+      if (have1)
+        bulk_load(dst + kPageHeadBytes, src + now1 * page_bytes, kPageHeadBytes, B.raw_full + kind);
     }
   }
 }
@@ -205,7 +208,7 @@ template <int FMT>
 __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, bool values,
                                              bool have0, bool have1, int tid) {
   const int t = tid & 3, line0 = tid >> 2;
-#pragma unroll 4
+#pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int page = i >> 2, line = line0 + 32 * (i & 3);
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -226,9 +229,11 @@ __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, b
 template <int FMT>
 __device__ __forceinline__ void convert_role(const Paged8Args& a, const Job& J, uint8_t* smem,
                                              const Bars& B, int tid) {
+  int pg[2] = {entry(J, J.page0), entry(J, J.page0 + 1)};
   for (int j = 0; j < J.n_kv; ++j) {
     const int st = j % kStages, p = J.page0 + 2 * j;
-    const bool have0 = page_of(a, J, p) >= 0, have1 = page_of(a, J, p + 1) >= 0;
+    const bool have0 = in_pool(a, pg[0]), have1 = in_pool(a, pg[1]);
+    pg[0] = entry(J, p + 2), pg[1] = entry(J, p + 3);
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
       uint64_t* empty = (kind ? B.v_empty : B.k_empty) + st;
@@ -250,6 +255,13 @@ __device__ __forceinline__ uint32_t key_bits(int lo, int hi, int k) {
   return below_b & ~below_a;
 }
 
+// 32 bytes to a 32-byte aligned global address
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 __device__ __forceinline__ void rescale_o(uint32_t o_col, float alpha) {
 #pragma unroll 1
   for (int q = 0; q < 16; ++q) {
@@ -268,48 +280,59 @@ __device__ __forceinline__ void rescale_o(uint32_t o_col, float alpha) {
   }
 }
 
-// The pair's query row into the swizzled fp16 tile; returns the factor of its
-// scores: scale * log2(e) over the power of two it was multiplied by.
-__device__ __forceinline__ float stage_query(const Paged8Args& a, const __nv_bfloat16* q, bool in,
-                                             uint8_t* tile, int row) {
+// The 32 query rows of a warp (its lanes' pairs) into the swizzled fp16 tile:
+// half a warp reads a row, 512 bytes per load, all loads in flight together.
+// Returns the factor of the lane's scores: scale * log2(e) over the power of
+// two its row was multiplied by.  at: element offset of the lane's row in q, < 0
+// for none.
+__device__ __forceinline__ float stage_queries(const Paged8Args& a, int64_t at, uint8_t* tile, int row0,
+                                               int lane) {
+  const int c = lane & 15;  // 16-byte column of a row
   uint4 v[16];
-  float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    v[i] = in ? reinterpret_cast<const uint4*>(q)[i] : make_uint4(0u, 0u, 0u, 0u);
+    const int64_t from = __shfl_sync(0xffffffffu, at, 2 * i + (lane >> 4));
+    v[i] = from >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q + from) + c) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[i]);
+    float amax = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[j] << 16)),
                                fabsf(__uint_as_float(w[j] & 0xffff0000u))));
-  }
-  const int sh = fp16_shift(amax);
-  const float f = exp2_int(sh);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[i]);
+    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const int sh = fp16_shift(amax);
+    const float f = exp2_int(sh);
+    const int other = __shfl_sync(0xffffffffu, sh, 16 * (lane & 1));
+    if ((lane >> 1) == i) mine = other;  // rows 2i and 2i + 1 are lanes 2i and 2i + 1
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       o[j] = pack_f16x2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
-    *reinterpret_cast<uint4*>(tile + (i >> 3) * kHalf + row * 128 + (((i & 7) ^ (row & 7)) << 4)) =
+    const int r = row0 + 2 * i + (lane >> 4);
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
         make_uint4(o[0], o[1], o[2], o[3]);
   }
-  return a.scale_log2 * exp2_int(-sh);
+  return a.scale_log2 * exp2_int(-mine);
 }
 
+// A page's scales as read; what is derived from them is computed at their use.
 struct PageScale {
-  float ks, ve, unscale;  // key scale, log2 of the value scale, 2^-ve
+  float ks, vs;
+  bool have;
 };
 
 __device__ __forceinline__ PageScale page_scale(const Paged8Args& a, const Job& J, int page) {
-  PageScale s = {0.f, 0.f, 0.f};
-  if (page < 0) return s;
-  const int64_t at = (int64_t)page * a.kv_heads + J.kvh;
-  const int ve = scale_log2_of(a.v_scale[at]);
-  s.ks = a.k_scale[at];
-  s.ve = (float)ve;
-  s.unscale = exp2_int(max(-126, min(126, -ve)));
+  PageScale s = {0.f, 1.f, in_pool(a, page)};
+  if (s.have) {
+    const int64_t at = (int64_t)page * a.kv_heads + J.kvh;
+    s.ks = __ldg(a.k_scale + at);
+    s.vs = __ldg(a.v_scale + at);
+  }
   return s;
 }
 
@@ -329,8 +352,8 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
   float m_run = -INFINITY, l_run = 0.f;
   int c = 0;
   if (J.n_kv > 0) {
-    const float sc = stage_query(a, a.q + grow * a.q_stride + head * 128, in_row && J.tl.b < a.n,
-                                 smem + kSmemQ + h * kTile, row);
+    const float sc = stage_queries(a, in_row ? grow * a.q_stride + head * 128 : -1,
+                                   smem + kSmemQ + h * kTile, row & ~31, lane_id());
     fence_proxy_async_smem();
     mbar_arrive(B.q_full);
     int lo = 0, hi = 0;
@@ -345,22 +368,18 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
         row_keys(a, J.tl.rq, first / a.group, unused, all_hi);
       }
     }
-    int pg0 = page_of(a, J, J.page0), pg1 = page_of(a, J, J.page0 + 1);
-    PageScale n0 = page_scale(a, J, pg0), n1 = page_scale(a, J, pg1);
-    bool nb0 = pg0 >= 0, nb1 = pg1 >= 0;
-    if (J.n_kv > 1) pg0 = page_of(a, J, J.page0 + 2), pg1 = page_of(a, J, J.page0 + 3);
+    PageScale n0 = page_scale(a, J, entry(J, J.page0)), n1 = page_scale(a, J, entry(J, J.page0 + 1));
+    int pg0 = entry(J, J.page0 + 2), pg1 = entry(J, J.page0 + 3);
     for (int j = 0; j < J.n_kv; ++j) {
       const int p = J.page0 + 2 * j;
       // scales one tile ahead, table entries two
       const PageScale e0 = n0, e1 = n1;
-      const bool b0 = nb0, b1 = nb1;
-      if (j + 1 < J.n_kv) {
-        n0 = page_scale(a, J, pg0), n1 = page_scale(a, J, pg1);
-        nb0 = pg0 >= 0, nb1 = pg1 >= 0;
-        if (j + 2 < J.n_kv) pg0 = page_of(a, J, p + 4), pg1 = page_of(a, J, p + 5);
-      }
+      n0 = page_scale(a, J, pg0), n1 = page_scale(a, J, pg1);
+      pg0 = entry(J, p + 4), pg1 = entry(J, p + 5);
       if (!uses(J, h, p)) continue;
+      const bool b0 = e0.have, b1 = e1.have;
       const float c0 = fmaxf(sc * e0.ks, FLT_MIN), c1 = fmaxf(sc * e1.ks, FLT_MIN);
+      const int ve0 = scale_log2_of(e0.vs), ve1 = scale_log2_of(e1.vs);
       const int k0 = p * kPage;
       const bool partial = !(k0 >= all_lo && k0 + 2 * kPage <= all_hi && b0 && b1);
       // S_h is committed after the half's previous PV, so once it is visible O
@@ -391,8 +410,8 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
         m8[i & 3] = fmaxf(m8[i & 3], sv[i]);
         m8[4 + (i & 3)] = fmaxf(m8[4 + (i & 3)], sv[64 + i]);
       }
-      const float mx = fmaxf(fmaf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), c0, e0.ve),
-                             fmaf(fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])), c1, e1.ve));
+      const float mx = fmaxf(fmaf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), c0, (float)ve0),
+                             fmaf(fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])), c1, (float)ve1));
       const bool grow_max = mx > m_run + kRescaleThreshold;
       const bool need_rescale = grow_max && m_run != -INFINITY;
       if (__any_sync(0xffffffffu, need_rescale)) {
@@ -404,7 +423,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
       const float nref = m_run == -INFINITY ? 0.f : -m_run;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float ch = half ? c1 : c0, rh = nref + (half ? e1.ve : e0.ve);
+        const float ch = half ? c1 : c0, rh = nref + (float)(half ? ve1 : ve0);
         const uint64_t sc2 = f2_pack(ch, ch), ref2 = f2_pack(rh, rh);
         uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
         uint32_t pk[32];
@@ -425,7 +444,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
         }
         float s0, s1;
         f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
-        l_run = fmaf(s0 + s1, half ? e1.unscale : e0.unscale, l_run);
+        l_run = fmaf(s0 + s1, exp2_int(max(-126, min(126, half ? -ve1 : -ve0))), l_run);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -465,10 +484,15 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
-      uint4* dst = reinterpret_cast<uint4*>(orow + q * 32);
+      if ((reinterpret_cast<uintptr_t>(orow) & 31) == 0) {
+        st_global_v8(orow + q * 32, w);
+        st_global_v8(orow + q * 32 + 16, w + 8);
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(orow + q * 32);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        for (int k = 0; k < 4; ++k)
+          dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+      }
     } else {
       uint4* dst = reinterpret_cast<uint4*>(a.part_o + at * 128 + q * 32);
 #pragma unroll
@@ -485,34 +509,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = warp_id(), lane = lane_id();
-  // the last tiles of a request see the most keys: they come first
-  const int split = blockIdx.x % a.splits;
-  Job J;
-  J.kvh = blockIdx.x / a.splits % a.kv_heads;
-  const int64_t tile = tiles - 1 - blockIdx.x / ((int64_t)a.splits * a.kv_heads);
-  J.tl = paged8_tile<kRows>(a, tile, threadIdx.x == 0 && split == 0 && J.kvh == 0);
-  if (!J.tl.live) return;
-  const bool tail = J.tl.b == a.n;
-  if (tail ? !a.zero_tail : J.tl.pairs <= a.row_limit) return;
-  const int kv_all = (J.tl.np + 1) / 2;
-  const int parts = parts_of<kPaged8LargeMin>(kv_all, a.splits);
-  if (split >= parts) return;
-  const int t0 = (int)((int64_t)kv_all * split / parts), t1 = (int)((int64_t)kv_all * (split + 1) / parts);
-  J.page0 = J.tl.p0 + 2 * t0;
-  J.n_kv = t1 - t0;
-  J.page_end = min(J.tl.p0 + J.tl.np, J.tl.p0 + 2 * t1);
-  J.row = tail ? a.table : a.table + J.tl.b * a.table_stride;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int first = J.tl.rho0 + 128 * h, last = min(first + 128, J.tl.pairs) - 1;
-    J.lo[h] = J.hi[h] = 0;
-    int unused;
-    if (first <= last && !tail) {
-      row_keys(a, J.tl.rq, first / a.group, J.lo[h], unused);
-      row_keys(a, J.tl.rq, last / a.group, unused, J.hi[h]);
-      if (J.hi[h] <= J.lo[h]) J.lo[h] = J.hi[h] = 0;
-    }
-  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBar);
   Bars B;
   B.q_full = bars;
@@ -544,6 +540,34 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
       mbar_init(B.o_final + i, 1);
     }
     fence_mbar_init();
+  }
+  // the last tiles of a request see the most keys: they come first
+  const int split = blockIdx.x % a.splits;
+  Job J;
+  J.kvh = blockIdx.x / a.splits % a.kv_heads;
+  const int64_t tile = tiles - 1 - blockIdx.x / ((int64_t)a.splits * a.kv_heads);
+  J.tl = paged8_tile<kRows>(a, tile, threadIdx.x == 0 && split == 0 && J.kvh == 0);
+  if (!J.tl.live) return;
+  const bool tail = J.tl.b == a.n;
+  if (tail ? !a.zero_tail : J.tl.pairs <= a.row_limit) return;
+  const int kv_all = (J.tl.np + 1) / 2;
+  const int parts = parts_of<kPaged8LargeMin>(kv_all, a.splits);
+  if (split >= parts) return;
+  const int t0 = (int)((int64_t)kv_all * split / parts), t1 = (int)((int64_t)kv_all * (split + 1) / parts);
+  J.page0 = J.tl.p0 + 2 * t0;
+  J.n_kv = t1 - t0;
+  J.page_end = min(J.tl.p0 + J.tl.np, J.tl.p0 + 2 * t1);
+  J.row = tail ? a.table : a.table + J.tl.b * a.table_stride;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int first = J.tl.rho0 + 128 * h, last = min(first + 128, J.tl.pairs) - 1;
+    J.lo[h] = J.hi[h] = 0;
+    int unused;
+    if (first <= last && !tail) {
+      row_keys(a, J.tl.rq, first / a.group, J.lo[h], unused);
+      row_keys(a, J.tl.rq, last / a.group, unused, J.hi[h]);
+      if (J.hi[h] <= J.lo[h]) J.lo[h] = J.hi[h] = 0;
+    }
   }
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();

@@ -75,22 +75,27 @@ struct Paged8Request {
   bool ok;
 };
 
-__device__ __forceinline__ Paged8Request paged8_request(const int32_t* q_start,
-                                                        const int32_t* lengths, int b, int rows,
+__device__ __forceinline__ Paged8Request paged8_request(int row0, int row1, int held, int rows,
                                                         int width, bool rows_are_held,
                                                         int32_t* status) {
   Paged8Request r;
-  r.row0 = q_start[b];
-  const int end = q_start[b + 1];
-  r.held = lengths[b];
-  r.n = end - r.row0;
+  r.row0 = row0;
+  r.held = held;
+  r.n = row1 - row0;
   int bad = 0;
-  if (r.row0 < 0 || end < r.row0 || end > rows) bad |= P8_BAD_ROWS;
-  if (r.held < 0 || r.held > (int64_t)width * kPage || (rows_are_held && !bad && r.n > r.held))
+  if (row0 < 0 || row1 < row0 || row1 > rows) bad |= P8_BAD_ROWS;
+  if (held < 0 || held > (int64_t)width * kPage || (rows_are_held && !bad && r.n > held))
     bad |= P8_BAD_LENGTH;
   r.ok = bad == 0;
   if (bad && status) atomicOr(status, bad);
   return r;
+}
+
+__device__ __forceinline__ Paged8Request paged8_request(const int32_t* q_start,
+                                                        const int32_t* lengths, int b, int rows,
+                                                        int width, bool rows_are_held,
+                                                        int32_t* status) {
+  return paged8_request(q_start[b], q_start[b + 1], lengths[b], rows, width, rows_are_held, status);
 }
 
 // ---- codes to fp16 pairs ----------------------------------------------------

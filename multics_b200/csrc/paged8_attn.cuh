@@ -101,21 +101,34 @@ __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t t
   Paged8Tile t;
   const int32_t* qs = a.q_start;
   const int64_t G = a.group;
-  t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
   t.live = false;
   t.rho0 = t.pairs = t.lo = t.hi = t.p0 = t.np = 0;
-  const int64_t first = qs[t.b] * G / kRows + t.b;
+  int row0, row1, held;
+  if (a.n < 32) {  // one read of everything
+    const int lane = threadIdx.x & 31, i = min(lane, a.n);
+    const int q = qs[i], len = a.n ? a.lengths[min(lane, a.n - 1)] : 0;
+    const unsigned le = __ballot_sync(0xffffffffu, lane <= a.n && q * G / kRows + lane <= tile);
+    t.b = 31 - __clz(le | 1u);
+    row0 = __shfl_sync(0xffffffffu, q, t.b);
+    row1 = __shfl_sync(0xffffffffu, q, min(t.b + 1, 31));
+    held = __shfl_sync(0xffffffffu, len, t.b);
+  } else {
+    t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
+    row0 = qs[t.b];
+    row1 = t.b < a.n ? qs[t.b + 1] : 0;
+    held = t.b < a.n ? a.lengths[t.b] : 0;
+  }
+  const int64_t first = row0 * G / kRows + t.b;
   if (tile < first) return t;
   const int64_t rho0 = (tile - first) * kRows;
   if (t.b == a.n) {  // rows behind the last request
-    t.rq.row0 = qs[a.n];
+    t.rq.row0 = row0;
     t.rq.n = a.rows - t.rq.row0;
     t.rq.held = 0;
     t.rq.ok = t.rq.row0 >= 0 && t.rq.n > 0;
     if (!t.rq.ok || rho0 >= t.rq.n * G) return t;
   } else {
-    t.rq = paged8_request(a.q_start, a.lengths, t.b, a.rows, a.width, false,
-                          report ? a.status : nullptr);
+    t.rq = paged8_request(row0, row1, held, a.rows, a.width, false, report ? a.status : nullptr);
     if (t.rq.row0 < 0 || t.rq.n <= 0 || t.rq.row0 + (int64_t)t.rq.n > a.rows ||
         rho0 >= t.rq.n * G)
       return t;
