@@ -7,6 +7,10 @@
 //
 //   S0(0) S1(0) | PV0(0) S0(1) PV1(0) S1(1) | PV0(1) S0(2) PV1(1) S1(2) | ...
 //
+// A tile of at most 128 pairs has no second half: both halves then take the
+// same pairs and every other key tile, S0(0) S1(1) | PV0(0) S0(2) | PV1(1) S1(3)
+// | ..., and are joined through shared memory at the end.
+//
 // What differs is the operands.  Codes are exact in fp16, so keys and values
 // are turned into fp16 tiles in shared memory by a warpgroup of their own and
 // both products run as kind::f16 on fp16 operands: the queries are brought
@@ -19,7 +23,8 @@
 //
 // Warp roles (512 threads, four warpgroups):
 //   warp 0       loads pages: bulk copies of 8 KiB (page, head) blocks, one
-//                16 KiB stage for keys and one for values
+//                16 KiB stage for keys and one for values, two of each for a
+//                dual tile, which has no second query tile
 //   warp 1       MMA issuer (one lane), TMEM allocator
 //   warps 4-7    codes -> fp16 tiles (two stages of each)
 //   warps 8-11   queries and softmax of half 0, one pair per thread
@@ -29,6 +34,8 @@
 // Every mbarrier wait is bounded and records a timeout in dev_err.
 
 #include <float.h>
+
+#include <type_traits>
 
 #include "paged8_attn.cuh"
 #include "tile_mma.cuh"
@@ -45,7 +52,7 @@ constexpr int kSmemV = kSmemK + kStages * kTile;
 constexpr int kSmemRaw = kSmemV + kStages * kTile;  // codes of a key tile, of a value tile
 constexpr int kRawTile = 2 * kPageHeadBytes;
 constexpr int kSmemBar = kSmemRaw + 2 * kRawTile;
-constexpr int kNumBars = 1 + 4 * kStages + 4 + 8;
+constexpr int kNumBars = 1 + 4 * kStages + 8 + 8;
 constexpr int kSmemBytes = kSmemBar + 256 + 1024;  // + slack for 1024-byte alignment
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 static_assert(kNumBars * 8 + 8 <= 256, "barriers and the TMEM slot");
@@ -65,7 +72,7 @@ struct Bars {
   uint64_t* k_empty;
   uint64_t* v_full;
   uint64_t* v_empty;
-  uint64_t* raw_full;   // [keys, values]
+  uint64_t* raw_full;   // [stage][keys, values]
   uint64_t* raw_empty;
   uint64_t* s_full;     // [half]
   uint64_t* p_full;
@@ -104,11 +111,15 @@ struct Job {
   int page0, n_kv;       // first page, 128-key tiles of this part
   int page_end;          // pages from here on are not this part's
   int lo[2], hi[2];      // keys that a half's rows see between them (lo = hi: none)
+  bool dual;             // one half's pairs, the key tiles shared out to both
+  int raw_stages;        // stages of codes: 2 where the second query tile's place is free
   const int32_t* row;    // block table row
 };
 
-// a half has rows that see some key of the tile that starts at page p
+// the half works on the tile that starts at page p: its rows see some key of
+// it, or the tile is the half's share
 __device__ __forceinline__ bool uses(const Job& J, int h, int p) {
+  if (J.dual) return (((p - J.page0) >> 1) & 1) == h;
   return p * kPage < (h ? J.hi[1] : J.hi[0]) && (p + 2) * kPage > (h ? J.lo[1] : J.lo[0]);
 }
 
@@ -116,6 +127,9 @@ __device__ __forceinline__ bool uses(const Job& J, int h, int p) {
 // waits for one: -1 behind the part's pages.
 __device__ __forceinline__ int entry(const Job& J, int p) {
   return p < J.page_end ? __ldg(J.row + p) : -1;
+}
+__device__ __forceinline__ uint8_t* raw_stage(uint8_t* smem, int stage, int kind) {
+  return smem + (stage ? kSmemQ + kTile : kSmemRaw) + kind * kRawTile;
 }
 __device__ __forceinline__ bool in_pool(const Paged8Args& a, int page) {
   return page >= 0 && page < a.n_pages;
@@ -126,24 +140,26 @@ __device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uin
   int pg[2] = {entry(J, J.page0), entry(J, J.page0 + 1)};
   for (int j = 0; j < J.n_kv; ++j) {
     const int p = J.page0 + 2 * j;
+    const int raw = j % J.raw_stages, raw_phase = ((j / J.raw_stages) - 1) & 1;
     const int now0 = pg[0], now1 = pg[1];
     pg[0] = entry(J, p + 2), pg[1] = entry(J, p + 3);
     const bool have0 = in_pool(a, now0), have1 = in_pool(a, now1);
     if (!have0 || (!have1 && p + 1 < J.page_end)) atomicOr(a.status, P8_BAD_PAGE);
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
-      if (j > 0 && !mbar_wait(B.raw_empty + kind, (j - 1) & 1, a.err, 40 + kind)) return;
+      uint64_t* full = B.raw_full + 2 * raw + kind;
+      if (j >= J.raw_stages && !mbar_wait(B.raw_empty + 2 * raw + kind, raw_phase, a.err, 40 + kind))
+        return;
       const uint32_t bytes = (have0 + have1) * kPageHeadBytes;
       if (bytes)
-        mbar_arrive_expect_tx(B.raw_full + kind, bytes);
+        mbar_arrive_expect_tx(full, bytes);
       else
-        mbar_arrive(B.raw_full + kind);
+        mbar_arrive(full);
       const uint8_t* src = (kind ? a.v : a.k) + (int64_t)J.kvh * kPageHeadBytes;
       const int64_t page_bytes = (int64_t)a.kv_heads * kPageHeadBytes;
-      uint8_t* dst = smem + kSmemRaw + kind * kRawTile;
-      if (have0) bulk_load(dst, src + now0 * page_bytes, kPageHeadBytes, B.raw_full + kind);
-      if (have1)
-        bulk_load(dst + kPageHeadBytes, src + now1 * page_bytes, kPageHeadBytes, B.raw_full + kind);
+      uint8_t* dst = raw_stage(smem, raw, kind);
+      if (have0) bulk_load(dst, src + now0 * page_bytes, kPageHeadBytes, full);
+      if (have1) bulk_load(dst + kPageHeadBytes, src + now1 * page_bytes, kPageHeadBytes, full);
     }
   }
 }
@@ -151,11 +167,46 @@ __device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uin
 __device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint32_t tbase,
                                          uint8_t* smem, const Bars& B) {
   const uint32_t q_lo[2] = {sdesc_lo_kmajor(smem_u32(smem + kSmemQ)),
-                            sdesc_lo_kmajor(smem_u32(smem + kSmemQ + kTile))};
+                            sdesc_lo_kmajor(smem_u32(smem + kSmemQ + (J.dual ? 0 : kTile)))};
   const uint32_t k_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemK));
   const uint32_t v_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemV));
   int cp[2] = {0, 0};  // PVs issued per half
   if (!mbar_wait(B.q_full, 0, a.err, 42)) return;
+  if (J.dual) {
+    // tile j is half j % 2's, and so are the stages it passes through
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (j >= J.n_kv) break;
+      if (!mbar_wait(B.k_full + j, 0, a.err, 43)) return;
+      tc_fence_after();
+      issue_s_f16(tbase + j * kBN, q_lo[j], k_lo0 + ((j * kTile) >> 4));
+      umma_commit(B.s_full + j);
+      umma_commit(B.k_empty + j);
+    }
+    for (int j = 0; j < J.n_kv; ++j) {
+      const int h = j & 1, phase = (j >> 1) & 1;
+      const uint32_t o_t = tbase + kColO + h * kBN, p_t = tbase + h * kBN;
+      const uint32_t v_lo = v_lo0 + ((h * kTile) >> 4);
+      if (!mbar_wait(B.v_full + h, phase, a.err, 44)) return;
+      if (!mbar_wait(B.p_lo + h, phase, a.err, 45)) return;
+      tc_fence_after();
+      issue_pv_f16<0>(o_t, p_t, v_lo, j > 1);
+      if (!mbar_wait(B.p_full + h, phase, a.err, 46)) return;
+      tc_fence_after();
+      issue_pv_f16<1>(o_t, p_t, v_lo, true);
+      umma_commit(B.v_empty + h);
+      if (j + 2 < J.n_kv) {
+        if (!mbar_wait(B.k_full + h, ((j + 2) / kStages) & 1, a.err, 43)) return;
+        tc_fence_after();
+        issue_s_f16(p_t, q_lo[h], k_lo0 + ((h * kTile) >> 4));
+        umma_commit(B.s_full + h);
+        umma_commit(B.k_empty + h);
+      }
+    }
+    umma_commit(B.o_final);
+    umma_commit(B.o_final + 1);
+    return;
+  }
   // every phase of the stage barriers is waited for, used or not
   if (!mbar_wait(B.k_full, 0, a.err, 43)) return;
   tc_fence_after();
@@ -203,49 +254,61 @@ __device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint
 // A page's 128 lines of 64 codes (keys: 64 of each dimension half; values: one
 // per dimension) become lines of 128 bytes in the swizzled tile.  Eight lanes
 // read two lines of codes (128 bytes) and write two lines of eight different
-// 16-byte columns: no bank conflicts either way.
-template <int FMT>
-__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, bool values,
-                                             bool have0, bool have1, int tid) {
+// 16-byte columns: no bank conflicts either way.  A thread takes 16 bytes of
+// lines line0, line0 + 32, .. of both pages; pages that are not there are zeros.
+template <int FMT, bool kValues>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, bool have0, bool have1,
+                                             int tid) {
   const int t = tid & 3, line0 = tid >> 2;
+  const uint8_t* src = raw + tid * 16;
+  // (the line's swizzle is that of line0: the others are multiples of 8 away)
+  uint8_t* lo = dst + line0 * 128 + (((2 * t) ^ (line0 & 7)) << 4);
+  uint8_t* hi = dst + line0 * 128 + (((2 * t + 1) ^ (line0 & 7)) << 4);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int page = i >> 2, line = line0 + 32 * (i & 3);
+    const int page = i >> 2, line = 32 * (i & 3);  // + line0
+    const int off = kValues ? page * kHalf + line * 128 : (line >> 6) * kHalf + (64 * page + (line & 63)) * 128;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (page ? have1 : have0)
-      v = *reinterpret_cast<const uint4*>(raw + page * kPageHeadBytes + line * 64 + t * 16);
+      v = *reinterpret_cast<const uint4*>(src + page * kPageHeadBytes + line * 64);
     uint32_t o[8];
     decode4<FMT>(v.x, o[0], o[1]);
     decode4<FMT>(v.y, o[2], o[3]);
     decode4<FMT>(v.z, o[4], o[5]);
     decode4<FMT>(v.w, o[6], o[7]);
-    const int r = values ? line : 64 * page + (line & 63);
-    uint8_t* d = dst + (values ? page : line >> 6) * kHalf + r * 128;
-    *reinterpret_cast<uint4*>(d + (((2 * t) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-    *reinterpret_cast<uint4*>(d + (((2 * t + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+    *reinterpret_cast<uint4*>(lo + off) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(hi + off) = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
+// The proxy fence also ends the reads of the codes before their stage is given
+// back to the copies.
 template <int FMT>
 __device__ __forceinline__ void convert_role(const Paged8Args& a, const Job& J, uint8_t* smem,
                                              const Bars& B, int tid) {
-  int pg[2] = {entry(J, J.page0), entry(J, J.page0 + 1)};
+  int pg0 = entry(J, J.page0), pg1 = entry(J, J.page0 + 1);
   for (int j = 0; j < J.n_kv; ++j) {
-    const int st = j % kStages, p = J.page0 + 2 * j;
-    const bool have0 = in_pool(a, pg[0]), have1 = in_pool(a, pg[1]);
-    pg[0] = entry(J, p + 2), pg[1] = entry(J, p + 3);
-#pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {
-      uint64_t* empty = (kind ? B.v_empty : B.k_empty) + st;
-      if (j >= kStages && !mbar_wait(empty, ((j / kStages) - 1) & 1, a.err, 47)) return;
-      if (!mbar_wait(B.raw_full + kind, j & 1, a.err, 48)) return;
-      convert_tile<FMT>(smem + kSmemRaw + kind * kRawTile,
-                        smem + (kind ? kSmemV : kSmemK) + st * kTile, kind == 1, have0, have1, tid);
+    const int st = j % kStages, raw = j % J.raw_stages, raw_phase = (j / J.raw_stages) & 1;
+    const bool have0 = in_pool(a, pg0), have1 = in_pool(a, pg1);
+    pg0 = entry(J, J.page0 + 2 * j + 2), pg1 = entry(J, J.page0 + 2 * j + 3);
+    const auto one = [&](auto values) -> bool {
+      constexpr bool kValues = decltype(values)::value;
+      uint64_t* empty = (kValues ? B.v_empty : B.k_empty) + st;
+      if (j >= kStages && !mbar_wait(empty, ((j / kStages) - 1) & 1, a.err, 47)) return false;
+      if (!mbar_wait(B.raw_full + 2 * raw + kValues, raw_phase, a.err, 48)) return false;
+      convert_tile<FMT, kValues>(raw_stage(smem, raw, kValues),
+                                 smem + (kValues ? kSmemV : kSmemK) + st * kTile, have0, have1, tid);
       fence_proxy_async_smem();
-      mbar_arrive((kind ? B.v_full : B.k_full) + st);
-      mbar_arrive(B.raw_empty + kind);
-    }
+      mbar_arrive((kValues ? B.v_full : B.k_full) + st);
+      mbar_arrive(B.raw_empty + 2 * raw + kValues);
+      return true;
+    };
+    if (!one(std::false_type{}) || !one(std::true_type{})) return;
   }
+}
+
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // bits [a, b) of the 32 keys that start at key k
@@ -344,16 +407,18 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
   const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
   const uint32_t s_col = tbase + lane_base + h * kBN;
   const uint32_t o_col = tbase + lane_base + kColO + h * kBN;
-  const int rho = J.tl.rho0 + 128 * h + row;
+  const int half0 = J.tl.rho0 + (J.dual ? 0 : 128 * h);  // first pair of the half
+  const int rho = half0 + row;
   const bool in_row = rho < J.tl.pairs;
   const int qi = (in_row ? rho : 0) / a.group;
   const int head = J.kvh * a.group + (in_row ? rho : 0) % a.group;
   const int64_t grow = J.tl.rq.row0 + (int64_t)qi;
   float m_run = -INFINITY, l_run = 0.f;
   int c = 0;
+  bool lost = false;  // a wait ran out: nothing more is waited for or written
   if (J.n_kv > 0) {
     const float sc = stage_queries(a, in_row ? grow * a.q_stride + head * 128 : -1,
-                                   smem + kSmemQ + h * kTile, row & ~31, lane_id());
+                                   smem + kSmemQ + (J.dual ? 0 : h * kTile), row & ~31, lane_id());
     fence_proxy_async_smem();
     mbar_arrive(B.q_full);
     int lo = 0, hi = 0;
@@ -361,7 +426,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
     // tiles that every row of the half sees whole need no mask
     int all_lo, all_hi, unused;
     {
-      const int first = J.tl.rho0 + 128 * h, last = min(first + 128, J.tl.pairs) - 1;
+      const int first = half0, last = min(first + 128, J.tl.pairs) - 1;
       all_lo = INT_MAX, all_hi = 0;
       if (first <= last) {
         row_keys(a, J.tl.rq, last / a.group, all_lo, unused);
@@ -384,7 +449,10 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
       const bool partial = !(k0 >= all_lo && k0 + 2 * kPage <= all_hi && b0 && b1);
       // S_h is committed after the half's previous PV, so once it is visible O
       // holds every earlier product and can be rescaled without another wait
-      if (!mbar_wait(B.s_full + h, c & 1, a.err, 49)) return;
+      if (!mbar_wait(B.s_full + h, c & 1, a.err, 49)) {
+        lost = true;
+        break;
+      }
       tc_fence_after();
       float sv[kBN];
       {
@@ -452,15 +520,49 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
       ++c;
     }
   }
-  if (c > 0) {
-    if (!mbar_wait(B.o_final + h, 0, a.err, 50)) return;
+  if (c > 0 && !lost) {
+    lost = !mbar_wait(B.o_final + h, 0, a.err, 50);
     tc_fence_after();
   }
+  // The halves of a dual tile joined: the second leaves its rows, column by
+  // column, where the queries were (every product is done), the first adds them.
+  float* other = reinterpret_cast<float*>(smem + kSmemQ) + row;
+  float2* other_ml = reinterpret_cast<float2*>(smem + kSmemRaw) + row;
+  float keep = 1.f, add = 0.f;
+  if (J.dual && J.n_kv > 0) {
+    named_barrier(1, 256);
+    if (h == 1) {
+      if (!lost) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t r[32];
+          if (c > 0) {
+            tmem_ld32(o_col + q * 32, r);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            other[(32 * q + i) * 128] = c > 0 ? __uint_as_float(r[i]) : 0.f;
+        }
+      }
+      *other_ml = make_float2(m_run, l_run);
+    }
+    named_barrier(1, 256);
+    if (h == 1) return;
+    const float2 ml = *other_ml;
+    const float M = fmaxf(m_run, ml.x), ref = M == -INFINITY ? 0.f : M;
+    keep = ex2_approx(m_run - ref), add = ex2_approx(ml.x - ref);
+    l_run = fmaf(l_run, keep, ml.y * add);
+    m_run = M;
+  } else if (J.dual && h == 1) {
+    return;
+  }
+  if (lost) return;
   const bool whole = parts == 1;
   const float inv = whole ? (l_run > 0.f ? 1.f / l_run : l_run == 0.f ? 0.f : l_run) : 1.f;
+  keep *= inv, add *= inv;
   __nv_bfloat16* orow = a.out + grow * a.out_stride + head * 128;
-  const int64_t at = whole ? 0
-                           : ((int64_t)blockIdx.x * kRows + 128 * h + row);
+  const int64_t at = whole ? 0 : ((int64_t)blockIdx.x * kRows + (rho - J.tl.rho0));
   if (in_row) {
     if (whole) {
       if (a.lse) a.lse[grow * a.heads + head] = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
@@ -479,11 +581,17 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
       for (int i = 0; i < 32; ++i) r[i] = 0u;
     }
     if (!in_row) continue;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float v = __uint_as_float(r[i]) * keep;
+      if (J.dual && J.n_kv > 0) v = fmaf(other[(32 * q + i) * 128], add, v);
+      r[i] = __float_as_uint(v);
+    }
     if (whole) {
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
+        w[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
       if ((reinterpret_cast<uintptr_t>(orow) & 31) == 0) {
         st_global_v8(orow + q * 32, w);
         st_global_v8(orow + q * 32 + 16, w + 8);
@@ -517,8 +625,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   B.v_full = B.k_empty + kStages;
   B.v_empty = B.v_full + kStages;
   B.raw_full = B.v_empty + kStages;
-  B.raw_empty = B.raw_full + 2;
-  B.s_full = B.raw_empty + 2;
+  B.raw_empty = B.raw_full + 4;
+  B.s_full = B.raw_empty + 4;
   B.p_full = B.s_full + 2;
   B.p_lo = B.p_full + 2;
   B.o_final = B.p_lo + 2;
@@ -531,9 +639,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
       mbar_init(B.v_full + s, 128);
       mbar_init(B.v_empty + s, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(B.raw_full + i, 1);
       mbar_init(B.raw_empty + i, 128);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(B.s_full + i, 1);
       mbar_init(B.p_full + i, 128);
       mbar_init(B.p_lo + i, 128);
@@ -557,6 +667,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   J.page0 = J.tl.p0 + 2 * t0;
   J.n_kv = t1 - t0;
   J.page_end = min(J.tl.p0 + J.tl.np, J.tl.p0 + 2 * t1);
+  J.dual = J.tl.pairs - J.tl.rho0 <= 128;
+  J.raw_stages = J.dual ? 2 : 1;
   J.row = tail ? a.table : a.table + J.tl.b * a.table_stride;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {

@@ -376,6 +376,17 @@ def test_attention_long_keys_few_heads(dtype, lengths, counts):
     _check(c, table, lengths, counts, 4, g, max_rows=max(counts))
 
 
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("counts", [[17, 128, 127, 64, 65], [100, 129, 256, 64, 1], [257, 200, 120, 33, 40]])
+@pytest.mark.parametrize("heads", [1, 4])
+def test_attention_tiles_of_one_half(dtype, counts, heads):
+    """Up to 128 pairs in a tile, one, two and many key tiles, whole and split."""
+    lengths = [1500, 700, 400, 64, 130]
+    c, table, g = _filled(lengths, 1, dtype, seed=heads)
+    for mask in ((1, 1, -1), (3, 0, -1), (10, 2, 9)):
+        _check(c, table, lengths, counts, heads, g, frame=mask[0], block=mask[1], window=mask[2])
+
+
 @pytest.mark.parametrize("width", [None, 90])
 def test_attention_max_rows_chooses_kernels_not_results(width):
     """Requests of more rows than the caller said, short and split keys."""
@@ -513,6 +524,20 @@ def test_attention_mixed_batch_is_each_request_alone():
     c, table, g = _filled(lengths, 3, torch.float8_e4m3fn)
     table[1][:5] = table[0][:5]
     _check(c, table, lengths, counts, 6, g)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+def test_attention_of_new_data_is_that_of_old(dtype):
+    """The first call on a cache just written gives the bits of the calls after
+    it, when its pages are in the L2 cache: no load is used before it is there."""
+    for seed in range(60):
+        lengths, counts = [700, 64, 130, 333], [300, 3, 130, 17]
+        c, table, g = _filled(lengths, 2, dtype, seed=seed)
+        q = (torch.randn(450, 256, generator=g) * 1.5).to(BF)
+        args = (q.cuda(), c, _i32(table), _i32(lengths), _i32([0, 300, 303, 433, 450]), 2)
+        kw = dict(tokens_per_frame=1 + seed % 7, block_frames=seed % 3)
+        first, second = (paged8_attention(*args, **kw) for _ in range(2))
+        assert torch.equal(first, second), seed
 
 
 def test_attention_on_two_streams_at_once():
