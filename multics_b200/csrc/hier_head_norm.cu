@@ -49,7 +49,7 @@ struct HeadNormArgs {
 
 // Table row of row r: < 0 skips the row.
 __device__ __forceinline__ int64_t table_row(const HeadNormArgs& a, int64_t r) {
-  if (!a.positions) return r % a.freqs_rows;
+  if (!a.positions) return (uint32_t)r % (uint32_t)a.freqs_rows;
   const int p = a.positions[r];
   if (p >= a.freqs_rows) {
     if (a.err) atomicCAS(a.err, 0, DEV_BAD_INDEX);
@@ -91,11 +91,11 @@ __global__ void __launch_bounds__(kWarps * 32) head_norm_kernel(HeadNormArgs a) 
   constexpr int LPH = D / 8, HPW = 32 / LPH;
   const int lane = threadIdx.x & 31;
   const int sub = lane / LPH, d = (lane % LPH) * 8;
-  const int per_row = a.chunks[0] + a.chunks[1];
-  const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (item >= a.rows * per_row) return;
+  const uint32_t per_row = a.chunks[0] + a.chunks[1];
+  const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (item >= (uint32_t)a.rows * per_row) return;
   const int64_t r = item / per_row;
-  int c = (int)(item - r * per_row);
+  int c = (int)(item - (uint32_t)r * per_row);
   const int kind = c >= a.chunks[0];
   if (kind) c -= a.chunks[0];
   const int h0 = c * (kUnroll * HPW) + sub, heads = a.heads[kind];
@@ -163,13 +163,12 @@ __global__ void __launch_bounds__(kWarps * 32) head_norm_bwd_kernel(HeadNormArgs
   __shared__ float sums[kWarps][2][HPW][D];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane / LPH, d = (lane % LPH) * 8;
-  const int per_row = a.chunks[0] + a.chunks[1];
-  const int64_t items = a.rows * per_row;
+  const uint32_t per_row = a.chunks[0] + a.chunks[1];
+  const uint32_t items = (uint32_t)a.rows * per_row;
   float acc[2][8] = {};
-  for (int64_t item = (int64_t)blockIdx.x * kWarps + warp; item < items;
-       item += (int64_t)gridDim.x * kWarps) {
+  for (uint32_t item = blockIdx.x * kWarps + warp; item < items; item += gridDim.x * kWarps) {
     const int64_t r = item / per_row;
-    int c = (int)(item - r * per_row);
+    int c = (int)(item - (uint32_t)r * per_row);
     const int kind = c >= a.chunks[0];
     if (kind) c -= a.chunks[0];
     const int h0 = c * (kU * HPW) + sub, heads = a.heads[kind];
@@ -295,6 +294,11 @@ int check_sizes(int64_t rows, int hq, int hk, int D, int64_t freqs_rows, const v
               (long long)rows, hq, hk, (long long)freqs_rows);
     return HIER_EVALUE;
   }
+  if (rows * ((hq + 3) / 4 + (hk + 3) / 4) > INT32_MAX || freqs_rows > INT32_MAX) {
+    set_error(HIER_EVALUE, "too many rows (%lld) or table rows (%lld)", (long long)rows,
+              (long long)freqs_rows);
+    return HIER_EVALUE;
+  }
   if (!positions && rows % freqs_rows) {
     set_error(HIER_EVALUE, "without positions the %lld table rows must divide the %lld rows",
               (long long)freqs_rows, (long long)rows);
@@ -349,10 +353,6 @@ extern "C" int hier_head_norm_rope(const void* q, int64_t q_stride, const void* 
   const int per = kUnroll * (256 / D);
   a.chunks[0] = (hq + per - 1) / per, a.chunks[1] = (hk + per - 1) / per;
   const int64_t blocks = (rows * (a.chunks[0] + a.chunks[1]) + kWarps - 1) / kWarps;
-  if (blocks > INT32_MAX) {
-    set_error(HIER_EVALUE, "too many rows");
-    return HIER_EVALUE;
-  }
   cudaStream_t st = (cudaStream_t)stream;
   if (D == 64)
     head_norm_kernel<64><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a);

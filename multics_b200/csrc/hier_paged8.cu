@@ -429,9 +429,9 @@ template <int FMT>
 __global__ void __launch_bounds__(128) paged8_append_pages_kernel(AppendArgs a) {
   __shared__ float most[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int head = (int)(blockIdx.x % a.heads);
-  const int kv = (int)(blockIdx.x / a.heads % 2);
-  const int64_t vp = blockIdx.x / (2 * a.heads);  // virtual page: see hier_paged8_append
+  const int part = blockIdx.x / a.heads, head = blockIdx.x - part * a.heads;
+  const int kv = part & 1;
+  const int64_t vp = part >> 1;  // virtual page: see hier_paged8_append
   const int32_t* qs = a.q_start;
   const int b = warp_find(a.n, vp, [=](int i) { return (int64_t)(qs[i] >> 6) + 2 * (int64_t)i; });
   const Paged8Request rq = paged8_request(a.q_start, a.lengths, b, a.rows, a.width, true,
@@ -504,13 +504,12 @@ __device__ __forceinline__ void regrow(const AppendItem& it, int kv, float ratio
 // N tokens at a time: 4, values written byte by byte, or 16, values merged 16
 // bytes at a time.
 template <int FMT, int N>
-__global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, int64_t units) {
+__global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, int units) {
   const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (unit >= units) return;
-  const int head = (int)(unit % a.heads);
-  const int kv = (int)(unit / a.heads % 2);
-  const int b = (int)(unit / (2 * (int64_t)a.heads));
+  const int part = unit / a.heads, head = unit - part * a.heads;
+  const int b = part >> 1, kv = part & 1;
   const Paged8Request rq = paged8_request(a.q_start, a.lengths, b, a.rows, a.width, true,
                                           lane == 0 && head == 0 ? a.status : nullptr);
   if (!rq.ok || rq.n == 0) return;
@@ -646,7 +645,7 @@ extern "C" int hier_paged8_append(const void* k, int64_t k_stride, const void* v
                     (rows > 4 * (int64_t)n && (int64_t)n * heads * 2 <= 148 * 8);
   const int64_t units = (many ? rows / kPage + 2 * (int64_t)n : (int64_t)n) * heads * 2;
   const int64_t blocks = many ? units : (units + 3) / 4;
-  if (blocks > INT32_MAX) {
+  if (units > INT32_MAX - 4) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
   }
@@ -660,7 +659,7 @@ extern "C" int hier_paged8_append(const void* k, int64_t k_stride, const void* v
                                             : paged8_append_rows_kernel<P8_INT8, 16>)
                                      : (few ? paged8_append_rows_kernel<P8_E4M3, 4>
                                             : paged8_append_rows_kernel<P8_E4M3, 16>);
-    kernel<<<(unsigned)blocks, 128, 0, st>>>(a, units);
+    kernel<<<(unsigned)blocks, 128, 0, st>>>(a, (int)units);
   }
   HIER_CHECK_CUDA(cudaGetLastError(), "paged8_append launch");
   return HIER_OK;

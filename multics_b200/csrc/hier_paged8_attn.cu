@@ -298,9 +298,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
   asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int split = (int)(blockIdx.x % a.splits);
-  const int kvh = (int)(blockIdx.x / a.splits % a.kv_heads);
-  const int tile = (int)(blockIdx.x / a.splits / a.kv_heads);
+  const int unit = blockIdx.x / a.splits, split = blockIdx.x - unit * a.splits;
+  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads;
   const int b = tile / a.direct, first = tile % a.direct * kRows;
   if (a.zero_tail && split == 0)
     zero_tail(a, kvh, (int64_t)tile * kWarps + w, (int64_t)a.n * a.direct * kWarps, lane);
@@ -311,8 +310,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
     if (!tl.live) return;
     const int parts = rho0 == first ? parts_of<kMinPages>(tl.np, a.splits) : 1;
     if (split >= parts) return;
-    const int p_end = tl.p0 + (int)((int64_t)tl.np * (split + 1) / parts);
-    int p = tl.p0 + (int)((int64_t)tl.np * split / parts) + w;
+    const int p_end = tl.p0 + tl.np * (split + 1) / parts;
+    int p = tl.p0 + tl.np * split / parts + w;
     Running R;
     start(R);
     if (p < p_end) {
@@ -492,13 +491,13 @@ __device__ __forceinline__ void short_keys(const Paged8Args& a, const Columns& c
 }
 
 template <int FMT>
-__global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args a, int64_t units) {
+__global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args a, int units) {
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
   __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t unit = (int64_t)blockIdx.x * kWarps + w;
+  const int unit = blockIdx.x * kWarps + w;
   if (unit >= units) return;
-  const int kvh = (int)(unit % a.kv_heads), tile = (int)(unit / a.kv_heads);
+  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads;
   const int b = tile / a.direct;
   if (a.zero_tail) zero_tail(a, kvh, tile, (int64_t)a.n * a.direct, lane);
   for (int rho0 = tile % a.direct * kRows;; rho0 += a.direct * kRows) {
@@ -542,12 +541,11 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
   constexpr bool kLarge = kTileRows == kPaged8LargeRows;
   constexpr int kGroups = kTileRows / 8;
   const int lane = threadIdx.x & 31;
-  const int64_t unit = blockIdx.x / kGroups;  // (tile, key head) as its kernel numbers them
+  const int unit = blockIdx.x / kGroups;  // (tile, key head) as its kernel numbers them
   const int r = (int)(blockIdx.x % kGroups) * 8 + (threadIdx.x >> 5);
-  const int kvh = (int)(unit % a.kv_heads);
-  const int64_t tile = unit / a.kv_heads;
+  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads;
   const Paged8Tile tl = kLarge ? paged8_tile<kTileRows>(a, tiles - 1 - tile, false)
-                               : small_tile(a, (int)(tile / a.direct), (int)(tile % a.direct) * kRows, false);
+                               : small_tile(a, tile / a.direct, tile % a.direct * kRows, false);
   // every block waits: what follows this kernel on the stream needs the attention done
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!tl.live || (kLarge && (tl.b == a.n || tl.pairs <= a.row_limit))) return;
@@ -555,7 +553,7 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
                            : parts_of<kMinPages>(tl.np, a.splits);
   const int pr = tl.rho0 + r;
   if (parts == 1 || pr >= tl.pairs) return;
-  const int64_t at = unit * a.splits * kTileRows + r;
+  const int64_t at = (int64_t)unit * a.splits * kTileRows + r;
   // lane s holds part s's maximum and sum (at most 32 parts)
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < parts) ml = *reinterpret_cast<const float2*>(a.part_ml + (at + (int64_t)lane * kTileRows) * 2);
@@ -650,13 +648,13 @@ int launch_merge(const Paged8Args& a, int64_t tiles, cudaStream_t st) {
 
 int launch_small(const Paged8Args& a, int format, int64_t tiles, cudaStream_t st) {
   const int64_t units = tiles * a.kv_heads * a.splits;
-  if (units > INT32_MAX) {
+  if (units > INT32_MAX - kWarps) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
   }
   if (a.width <= kShortPages) {
     auto* kernel = format == P8_INT8 ? paged8_short_kernel<P8_INT8> : paged8_short_kernel<P8_E4M3>;
-    kernel<<<(unsigned)((units + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(a, units);
+    kernel<<<(unsigned)((units + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(a, (int)units);
     HIER_CHECK_CUDA(cudaGetLastError(), "paged8_short_kernel launch");
     return HIER_OK;
   }

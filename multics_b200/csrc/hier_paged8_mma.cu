@@ -361,14 +361,12 @@ __device__ __forceinline__ float stage_queries(const Paged8Args& a, int64_t at, 
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[i]);
-    float amax = 0.f;
+    // the largest magnitude as bits: pairs of 16 (NaN above infinity)
+    uint32_t big = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                            __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[j] << 16)),
-                               fabsf(__uint_as_float(w[j] & 0xffff0000u))));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const int sh = fp16_shift(amax);
+    for (int o = 8; o > 0; o >>= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, o));
+    const int sh = fp16_shift(__uint_as_float(max(big << 16, big & 0xffff0000u)));
     const float f = exp2_int(sh);
     const int other = __shfl_sync(0xffffffffu, sh, 16 * (lane & 1));
     if ((lane >> 1) == i) mine = other;  // rows 2i and 2i + 1 are lanes 2i and 2i + 1
@@ -652,10 +650,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
     fence_mbar_init();
   }
   // the last tiles of a request see the most keys: they come first
-  const int split = blockIdx.x % a.splits;
+  const int unit = blockIdx.x / a.splits, split = blockIdx.x - unit * a.splits;
+  const int64_t tile = tiles - 1 - unit / a.kv_heads;
   Job J;
-  J.kvh = blockIdx.x / a.splits % a.kv_heads;
-  const int64_t tile = tiles - 1 - blockIdx.x / ((int64_t)a.splits * a.kv_heads);
+  J.kvh = unit % a.kv_heads;
   J.tl = paged8_tile<kRows>(a, tile, threadIdx.x == 0 && split == 0 && J.kvh == 0);
   if (!J.tl.live) return;
   const bool tail = J.tl.b == a.n;
@@ -663,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   const int kv_all = (J.tl.np + 1) / 2;
   const int parts = parts_of<kPaged8LargeMin>(kv_all, a.splits);
   if (split >= parts) return;
-  const int t0 = (int)((int64_t)kv_all * split / parts), t1 = (int)((int64_t)kv_all * (split + 1) / parts);
+  const int t0 = kv_all * split / parts, t1 = kv_all * (split + 1) / parts;
   J.page0 = J.tl.p0 + 2 * t0;
   J.n_kv = t1 - t0;
   J.page_end = min(J.tl.p0 + J.tl.np, J.tl.p0 + 2 * t1);

@@ -58,13 +58,13 @@ struct Paged8Mask {
   int frame, block, window;
   __device__ __forceinline__ int first(int pos) const {
     if (window < 0) return 0;
-    const int64_t f = pos / frame;
-    return (int)max((int64_t)0, (f - window + 1) * frame);
+    const int f = pos / frame;  // (32-bit divisions: a 64-bit one is a hundred instructions)
+    return f < window ? 0 : (f - window + 1) * frame;
   }
   __device__ __forceinline__ int end(int pos, int held) const {
     if (block == 0) return held;
-    const int64_t f = pos / frame;
-    return (int)min((int64_t)held, (f / block + 1) * block * frame);
+    const int f = pos / frame;
+    return (int)min((int64_t)held, (int64_t)(f / block + 1) * block * frame);
   }
 };
 

@@ -150,8 +150,8 @@ __device__ __forceinline__ int parts_of(int np, int splits) {
 // power of two that brings a row's largest magnitude into [2^14, 2^15) in
 // fp16: bf16 values keep all their bits there down to 2^-28 of the largest
 __device__ __forceinline__ int fp16_shift(float amax) {
-  if (!(amax > 0.f) || !(amax < INFINITY)) return 0;
-  return min(120, 14 - ilogbf(amax));
+  const int e = (int)(__float_as_uint(amax) >> 23);  // biased; 0: zero or a bf16 subnormal
+  return e >= 255 ? 0 : min(120, 14 + 127 - e);
 }
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
