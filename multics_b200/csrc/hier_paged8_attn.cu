@@ -83,12 +83,8 @@ __device__ __forceinline__ int page_at(const Paged8Args& a, const int32_t* row, 
 
 // row of a request and head of the group of pair rho
 __device__ __forceinline__ void split_pair(const Paged8Args& a, int rho, int& row, int& g) {
-  if (a.group == 1) {
-    row = rho, g = 0;
-  } else {
-    row = rho / a.group;
-    g = rho - row * a.group;
-  }
+  row = rho / a.group;
+  g = rho - row * a.group.d;
 }
 
 // The 8 pairs of tile i of request b, from pair rho0.
@@ -298,8 +294,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
   asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int unit = blockIdx.x / a.splits, split = blockIdx.x - unit * a.splits;
-  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads;
+  const int unit = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - unit * a.splits.d;
+  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const int b = tile / a.direct, first = tile % a.direct * kRows;
   if (a.zero_tail && split == 0)
     zero_tail(a, kvh, (int64_t)tile * kWarps + w, (int64_t)a.n * a.direct * kWarps, lane);
@@ -497,7 +493,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int unit = blockIdx.x * kWarps + w;
   if (unit >= units) return;
-  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads;
+  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const int b = tile / a.direct;
   if (a.zero_tail) zero_tail(a, kvh, tile, (int64_t)a.n * a.direct, lane);
   for (int rho0 = tile % a.direct * kRows;; rho0 += a.direct * kRows) {
@@ -543,7 +539,7 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
   const int lane = threadIdx.x & 31;
   const int unit = blockIdx.x / kGroups;  // (tile, key head) as its kernel numbers them
   const int r = (int)(blockIdx.x % kGroups) * 8 + (threadIdx.x >> 5);
-  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads;
+  const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const Paged8Tile tl = kLarge ? paged8_tile<kTileRows>(a, tiles - 1 - tile, false)
                                : small_tile(a, tile / a.direct, tile % a.direct * kRows, false);
   // every block waits: what follows this kernel on the stream needs the attention done
@@ -745,13 +741,14 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
   Paged8Args a = {};
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
   a.q_stride = q_stride;
-  a.rows = rows, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+  a.rows = rows, a.heads = heads, a.kv_heads = divisor(kv_heads), a.group = divisor(heads / kv_heads);
   a.k = reinterpret_cast<const uint8_t*>(k_codes), a.v = reinterpret_cast<const uint8_t*>(v_codes);
   a.k_scale = k_scale, a.v_scale = v_scale;
   a.n_pages = n_pages;
   a.table = table, a.table_stride = table_stride, a.width = width;
   a.lengths = lengths, a.q_start = q_start, a.n = n;
-  a.mask.frame = frame, a.mask.block = block, a.mask.window = window;
+  a.mask.frame = divisor(frame), a.mask.block = divisor(block ? block : 1), a.mask.blocks = block;
+  a.mask.window = window;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.out_stride = out_stride;
@@ -769,7 +766,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
   a.row_limit = !s.large ? INT32_MAX : s.small ? kSmallPairs : 0;
   if (s.large) {
     a.zero_tail = zero_tail;
-    a.splits = s.large_splits;
+    a.splits = divisor(s.large_splits);
     a.part_o = workspace + s.small_floats;
     a.part_ml = a.part_o + (s.floats - s.small_floats) / 130 * 128;
     rc = paged8_launch_large(a, format, s.large_tiles, st);
@@ -778,8 +775,8 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
   }
   if (s.small) {
     a.zero_tail = s.large ? 0 : zero_tail;
-    a.direct = s.direct;
-    a.splits = s.small_splits;
+    a.direct = divisor(s.direct);
+    a.splits = divisor(s.small_splits);
     a.part_o = workspace;
     a.part_ml = workspace + s.small_floats / 130 * 128;
     rc = launch_small(a, format, s.small_tiles, st);

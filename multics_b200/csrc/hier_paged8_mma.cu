@@ -104,6 +104,10 @@ __device__ __forceinline__ void issue_pv_f16(uint32_t o, uint32_t p, uint32_t vl
   pv_step<4 * H + 2>(o, p, vlo, acc), pv_step<4 * H + 3>(o, p, vlo, acc);
 }
 
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // What every role of a CTA works from.
 struct Job {
   Paged8Tile tl;
@@ -307,10 +311,6 @@ __device__ __forceinline__ void convert_role(const Paged8Args& a, const Job& J, 
   }
 }
 
-__device__ __forceinline__ void named_barrier(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 // bits [a, b) of the 32 keys that start at key k
 __device__ __forceinline__ uint32_t key_bits(int lo, int hi, int k) {
   const int a = min(32, max(0, lo - k)), b = min(32, max(0, hi - k));
@@ -343,42 +343,67 @@ __device__ __forceinline__ void rescale_o(uint32_t o_col, float alpha) {
   }
 }
 
-// The 32 query rows of a warp (its lanes' pairs) into the swizzled fp16 tile:
-// half a warp reads a row, 512 bytes per load, all loads in flight together.
-// Returns the factor of the lane's scores: scale * log2(e) over the power of
-// two its row was multiplied by.  at: element offset of the lane's row in q, < 0
-// for none.
-__device__ __forceinline__ float stage_queries(const Paged8Args& a, int64_t at, uint8_t* tile, int row0,
-                                               int lane) {
-  const int c = lane & 15;  // 16-byte column of a row
-  uint4 v[16];
+// The 32 query rows of a warp (its lanes' pairs) to registers, a lane column
+// lane % 16 of row 2i + lane / 16: half a warp copies a row, all copies in flight
+// together.  They go through the tile's place in shared memory: what is left of
+// the L1 cache beside 227 KB of it could not hold 64 KB of loads in flight.
+// at: element offset of the lane's row in q, < 0 for none.
+__device__ __forceinline__ void read_queries(const Paged8Args& a, int64_t at, uint8_t* tile, int row0,
+                                             int lane, uint4 (&v)[16]) {
+  uint8_t* dst = tile + (row0 + (lane >> 4)) * 256 + (lane & 15) * 16;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int64_t from = __shfl_sync(0xffffffffu, at, 2 * i + (lane >> 4));
-    v[i] = from >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q + from) + c) : make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + i * 512)),
+                 "l"(a.q + (from >= 0 ? from : 0) + (lane & 15) * 8), "r"(from >= 0 ? 16 : 0)
+                 : "memory");
   }
-  int mine = 0;
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = *reinterpret_cast<const uint4*>(dst + i * 512);
+}
+
+// Returns the factor of the lane's scores: scale * log2(e) over the power of
+// two its row is multiplied by.
+__device__ __forceinline__ float stage_queries(const Paged8Args& a, const uint4 (&v)[16], uint8_t* tile,
+                                               int row0, int lane) {
+  const int c = lane & 15;  // 16-byte column of the rows 2i + (lane >> 4)
+  // the largest magnitudes as bits, pairs of 16 (NaN above infinity)
+  uint32_t big[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    big[i] = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                      __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+  // sixteen rows over sixteen lanes: each step halves the rows that a lane keeps,
+  // and column c ends with row 2c + (lane >> 4)
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const bool up = (c & o) != 0;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const uint32_t give = up ? big[i] : big[i + o], keep = up ? big[i + o] : big[i];
+      big[i] = __vmaxu2(keep, __shfl_xor_sync(0xffffffffu, give, o));
+    }
+  }
+  const int sh = fp16_shift(__uint_as_float(max(big[0] << 16, big[0] & 0xffff0000u)));
+  const float mine = exp2_int(sh), factor = a.scale_log2 * exp2_int(-sh);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
+    const float f = __shfl_sync(0xffffffffu, mine, (lane & 16) + i);
+    const uint64_t f2 = f2_pack(f, f);
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[i]);
-    // the largest magnitude as bits: pairs of 16 (NaN above infinity)
-    uint32_t big = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
-                            __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, o));
-    const int sh = fp16_shift(__uint_as_float(max(big << 16, big & 0xffff0000u)));
-    const float f = exp2_int(sh);
-    const int other = __shfl_sync(0xffffffffu, sh, 16 * (lane & 1));
-    if ((lane >> 1) == i) mine = other;  // rows 2i and 2i + 1 are lanes 2i and 2i + 1
     uint32_t o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o[j] = pack_f16x2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
+    for (int j = 0; j < 4; ++j) {
+      float x, y;
+      f2_unpack(f2_mul(f2_pack(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)), f2), x, y);
+      o[j] = pack_f16x2(x, y);
+    }
     const int r = row0 + 2 * i + (lane >> 4);
     *reinterpret_cast<uint4*>(tile + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
         make_uint4(o[0], o[1], o[2], o[3]);
   }
-  return a.scale_log2 * exp2_int(-mine);
+  return __shfl_sync(0xffffffffu, factor, ((lane & 1) << 4) + (lane >> 1));
 }
 
 // A page's scales as read; what is derived from them is computed at their use.
@@ -409,14 +434,18 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
   const int rho = half0 + row;
   const bool in_row = rho < J.tl.pairs;
   const int qi = (in_row ? rho : 0) / a.group;
-  const int head = J.kvh * a.group + (in_row ? rho : 0) % a.group;
+  const int head = J.kvh * a.group.d + (in_row ? rho - qi * a.group.d : 0);
   const int64_t grow = J.tl.rq.row0 + (int64_t)qi;
   float m_run = -INFINITY, l_run = 0.f;
   int c = 0;
   bool lost = false;  // a wait ran out: nothing more is waited for or written
   if (J.n_kv > 0) {
-    const float sc = stage_queries(a, in_row ? grow * a.q_stride + head * 128 : -1,
-                                   smem + kSmemQ + (J.dual ? 0 : h * kTile), row & ~31, lane_id());
+    uint4 qv[16];
+    uint8_t* q_tile = smem + kSmemQ + (J.dual ? 0 : h * kTile);
+    read_queries(a, in_row && J.tl.b < a.n ? grow * a.q_stride + head * 128 : -1, q_tile, row & ~31,
+                 lane_id(), qv);
+    named_barrier(1, 256);  // every row is in registers: the tile may be written
+    const float sc = stage_queries(a, qv, q_tile, row & ~31, lane_id());
     fence_proxy_async_smem();
     mbar_arrive(B.q_full);
     int lo = 0, hi = 0;
@@ -650,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
     fence_mbar_init();
   }
   // the last tiles of a request see the most keys: they come first
-  const int unit = blockIdx.x / a.splits, split = blockIdx.x - unit * a.splits;
+  const int unit = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - unit * a.splits.d;
   const int64_t tile = tiles - 1 - unit / a.kv_heads;
   Job J;
   J.kvh = unit % a.kv_heads;

@@ -51,20 +51,37 @@ __device__ __forceinline__ int warp_find(int n, int64_t i, F base) {
   return lo;
 }
 
+// A divisor known to the host: n / d for 0 <= n < 2^31 in three instructions.
+struct Divisor {
+  int d;
+  uint32_t mul, shift;
+  __host__ __device__ operator int() const { return d; }
+};
+inline Divisor divisor(int d) {
+  uint32_t s = 0;
+  while (s < 31 && (1u << s) < (uint32_t)d) ++s;
+  return {d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - d)) / d + 1), s};
+}
+__device__ __forceinline__ int operator/(int n, const Divisor& v) {
+  return (int)((__umulhi((uint32_t)n, v.mul) + (uint32_t)n) >> v.shift);
+}
+__device__ __forceinline__ int operator%(int n, const Divisor& v) { return n - n / v * v.d; }
+
 // What the rows of a call may see: frames of `frame` tokens in causal blocks
 // of `block` frames (0: every held key), at most `window` frames back (< 0: no
 // limit).  Both ends ascend with the position.
 struct Paged8Mask {
-  int frame, block, window;
+  Divisor frame, block;  // (block: 1 where blocks is 0)
+  int blocks, window;
   __device__ __forceinline__ int first(int pos) const {
     if (window < 0) return 0;
-    const int f = pos / frame;  // (32-bit divisions: a 64-bit one is a hundred instructions)
-    return f < window ? 0 : (f - window + 1) * frame;
+    const int f = pos / frame;
+    return f < window ? 0 : (f - window + 1) * frame.d;
   }
   __device__ __forceinline__ int end(int pos, int held) const {
-    if (block == 0) return held;
+    if (blocks == 0) return held;
     const int f = pos / frame;
-    return (int)min((int64_t)held, (int64_t)(f / block + 1) * block * frame);
+    return (int)min((int64_t)held, (int64_t)(f / block + 1) * block.d * frame.d);
   }
 };
 

@@ -23,7 +23,8 @@ namespace hier {
 struct Paged8Args {
   const __nv_bfloat16* q;
   int64_t q_stride;
-  int rows, heads, kv_heads, group;
+  int rows, heads;
+  Divisor kv_heads, group;  // key heads, query heads of each
   const uint8_t* k;
   const uint8_t* v;
   const float* k_scale;
@@ -41,12 +42,12 @@ struct Paged8Args {
   int64_t out_stride;
   float* lse;       // [rows][heads] log2-sum-exp, or NULL
   int zero_tail;    // write zeros to the rows behind the last request
-  int splits;       // most parts a tile's keys are cut into
+  Divisor splits;   // most parts a tile's keys are cut into
   float* part_o;    // [tile][kv head][split][kRows][128]
   float* part_ml;   // [tile][kv head][split][kRows][2]
   int row_limit;    // requests of up to row_limit pairs are the small kernel's, the others the
                     // large one's (INT_MAX: all the small one's, 0: all the large one's)
-  int direct;       // small kernel: its tile t is tile t % direct of request t / direct
+  Divisor direct;   // small kernel: its tile t is tile t % direct of request t / direct
   int32_t* status;
   int* err;         // bounded waits
 };
@@ -80,7 +81,7 @@ __device__ __forceinline__ void row_keys(const Paged8Args& a, const Paged8Reques
     hi = a.mask.end(pos, r.held);
   } else {  // rows beyond the held tokens see keys only where positions do not matter
     lo = 0;
-    hi = a.mask.block == 0 && a.mask.window < 0 ? r.held : 0;
+    hi = a.mask.blocks == 0 && a.mask.window < 0 ? r.held : 0;
   }
 }
 
@@ -100,7 +101,7 @@ template <int kRows>
 __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t tile, bool report) {
   Paged8Tile t;
   const int32_t* qs = a.q_start;
-  const int64_t G = a.group;
+  const int64_t G = a.group.d;
   t.live = false;
   t.rho0 = t.pairs = t.lo = t.hi = t.p0 = t.np = 0;
   int row0, row1, held;
