@@ -751,7 +751,7 @@ int hier_head_norm_rope(const void* q, int64_t q_stride, const void* k, int64_t 
 
 /* Backward of hier_head_norm_rope without row maps: dq, dk from the gradients
  * gq, gk of its outputs (all bf16), dwq, dwk [D] in the weights' type.
- * partials float [blocks][2][D], blocks from ..._bwd_partials: the sums are
+ * partials float [blocks][D], blocks from ..._bwd_partials: the sums are
  * added in a fixed order.  Skipped rows get zero gradients. */
 int hier_head_norm_rope_bwd_partials(int64_t rows, int32_t hq, int32_t hk, int32_t D,
                                      int32_t* blocks);

@@ -11,9 +11,13 @@
 // Memory bound: 4 bytes per value forward, 8 backward.  A head is D/8 lanes of
 // 8 values (16 bytes), so a warp holds 32*8/D heads at once and the sum of
 // squares is a few shuffles.  A warp takes up to kUnroll such groups of one
-// row's heads: their loads are all in flight together (4 KiB per warp), the
+// row's heads: their loads are all in flight together (3 KiB per warp), the
 // lane's four (cos, sin) pairs are read once per row and are the same for all
-// of its heads.
+// of its heads.  Results are stored past the caches' reuse (written once, 165
+// against 183 us).  38 556 rows of 24 + 24 heads of 128: 150 us = 6.3 TB/s, 0.97
+// of the measured copy bandwidth (8 groups per warp: 165 us, 4: 162, 2: 200).
+// Backward on 9 241 rows of 24 + 8 heads: about 50 us = 4.5 TB/s, bound by its
+// arithmetic and two reductions per head.
 
 #include "common.cuh"
 
@@ -21,7 +25,7 @@ namespace hier {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kUnroll = 8;
+constexpr int kUnroll = 6;
 
 struct HeadNormArgs {
   const __nv_bfloat16* x[2];  // q, k
@@ -44,7 +48,7 @@ struct HeadNormArgs {
   // backward
   const __nv_bfloat16* g[2];
   int64_t g_stride[2];
-  float* part;  // [blocks][2][D]
+  float* part;  // [blocks][D]
 };
 
 // Table row of row r: < 0 skips the row.
@@ -150,28 +154,32 @@ __global__ void __launch_bounds__(kWarps * 32) head_norm_kernel(HeadNormArgs a) 
       o[i] = pack_bf16x2(fmaf(p, cs[i], -q * sn[i]), fmaf(p, sn[i], q * cs[i]));
     }
     if (h < heads)
-      *reinterpret_cast<uint4*>(y + (int64_t)h * D) = make_uint4(o[0], o[1], o[2], o[3]);
+      __stcs(reinterpret_cast<uint4*>(y + (int64_t)h * D), make_uint4(o[0], o[1], o[2], o[3]));
   }
 }
 
-// dw: every lane keeps the sums of its 8 channels over the items it walks, for
-// q and for k; a block adds its warps' sums in a fixed order and writes one
-// partial row of each, which head_norm_dw_kernel adds in block order.
+// dw: a block works on q or on k; every lane keeps the sums of its 8 channels
+// over the heads it walks.  The block adds its lanes' sums in a fixed order and
+// writes one partial row, which head_norm_dw_kernel adds in block order.
+constexpr int kBwdUnroll = 4;
+
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) head_norm_bwd_kernel(HeadNormArgs a) {
-  constexpr int LPH = D / 8, HPW = 32 / LPH, kU = 4;
-  __shared__ float sums[kWarps][2][HPW][D];
+__global__ void __launch_bounds__(kWarps * 32, 2) head_norm_bwd_kernel(HeadNormArgs a, int q_blocks) {
+  constexpr int LPH = D / 8, HPW = 32 / LPH, kU = kBwdUnroll;
+  __shared__ float sums[kWarps][HPW][D];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane / LPH, d = (lane % LPH) * 8;
-  const uint32_t per_row = a.chunks[0] + a.chunks[1];
-  const uint32_t items = (uint32_t)a.rows * per_row;
-  float acc[2][8] = {};
-  for (uint32_t item = blockIdx.x * kWarps + warp; item < items; item += gridDim.x * kWarps) {
+  const int kind = (int)blockIdx.x >= q_blocks;
+  const int block = kind ? blockIdx.x - q_blocks : blockIdx.x;
+  const int blocks = kind ? gridDim.x - q_blocks : q_blocks;
+  const uint32_t per_row = a.chunks[kind], items = (uint32_t)a.rows * per_row;
+  const int heads = a.heads[kind];
+  float w[8], acc[8] = {};
+  load_weight(a, kind, d, w);
+  for (uint32_t item = block * kWarps + warp; item < items; item += blocks * kWarps) {
     const int64_t r = item / per_row;
-    int c = (int)(item - (uint32_t)r * per_row);
-    const int kind = c >= a.chunks[0];
-    if (kind) c -= a.chunks[0];
-    const int h0 = c * (kU * HPW) + sub, heads = a.heads[kind];
+    const int c = (int)(item - (uint32_t)r * per_row);
+    const int h0 = c * (kU * HPW) + sub;
     const __nv_bfloat16* x = a.x[kind] + r * a.x_stride[kind] + d;
     const __nv_bfloat16* g = a.g[kind] + r * a.g_stride[kind] + d;
     __nv_bfloat16* y = a.y[kind] + r * a.y_stride[kind] + d;
@@ -195,8 +203,6 @@ __global__ void __launch_bounds__(kWarps * 32) head_norm_bwd_kernel(HeadNormArgs
     const float4* fr = reinterpret_cast<const float4*>(a.freqs + t * (D / 2) + d / 2);
     const float4 f0 = fr[0], f1 = fr[1];
     const float cs[4] = {f0.x, f0.z, f1.x, f1.z}, sn[4] = {f0.y, f0.w, f1.y, f1.w};
-    float w[8];
-    load_weight(a, kind, d, w);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int h = h0 + u * HPW;
@@ -215,13 +221,8 @@ __global__ void __launch_bounds__(kWarps * 32) head_norm_bwd_kernel(HeadNormArgs
         const float g1 = fmaf(q[2 * i + 1], cs[i], -q[2 * i] * sn[i]);
         f[2 * i] *= rs;
         f[2 * i + 1] *= rs;
-        if (kind) {
-          acc[1][2 * i] = fmaf(g0, f[2 * i], acc[1][2 * i]);
-          acc[1][2 * i + 1] = fmaf(g1, f[2 * i + 1], acc[1][2 * i + 1]);
-        } else {
-          acc[0][2 * i] = fmaf(g0, f[2 * i], acc[0][2 * i]);
-          acc[0][2 * i + 1] = fmaf(g1, f[2 * i + 1], acc[0][2 * i + 1]);
-        }
+        acc[2 * i] = fmaf(g0, f[2 * i], acc[2 * i]);
+        acc[2 * i + 1] = fmaf(g1, f[2 * i + 1], acc[2 * i + 1]);
         q[2 * i] = g0 * w[2 * i];
         q[2 * i + 1] = g1 * w[2 * i + 1];
         dot = fmaf(q[2 * i], f[2 * i], dot);
@@ -234,49 +235,59 @@ __global__ void __launch_bounds__(kWarps * 32) head_norm_bwd_kernel(HeadNormArgs
         o[i] = pack_bf16x2(rs * fmaf(-f[2 * i], dot, q[2 * i]),
                            rs * fmaf(-f[2 * i + 1], dot, q[2 * i + 1]));
       if (h < heads)
-        *reinterpret_cast<uint4*>(y + (int64_t)h * D) = make_uint4(o[0], o[1], o[2], o[3]);
+        __stcs(reinterpret_cast<uint4*>(y + (int64_t)h * D), make_uint4(o[0], o[1], o[2], o[3]));
     }
   }
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sums[warp][kind][sub][d + i] = acc[kind][i];
+  for (int i = 0; i < 8; ++i) sums[warp][sub][d + i] = acc[i];
   __syncthreads();
-  for (int e = threadIdx.x; e < 2 * D; e += blockDim.x) {
-    const int kind = e / D, ch = e % D;
+  for (int ch = threadIdx.x; ch < D; ch += blockDim.x) {
     float s = 0.f;
     for (int q = 0; q < kWarps; ++q)
-      for (int p = 0; p < HPW; ++p) s += sums[q][kind][p][ch];
-    a.part[((int64_t)blockIdx.x * 2 + kind) * D + ch] = s;
+      for (int p = 0; p < HPW; ++p) s += sums[q][p][ch];
+    a.part[(int64_t)blockIdx.x * D + ch] = s;
   }
 }
 
-// dw[kind][ch] = sum over blocks of the partial rows: one warp per channel,
-// lanes over the blocks, then a fixed tree.
-__global__ void head_norm_dw_kernel(const float* part, int blocks, int D, int f32, void* dwq,
+// dw[ch] = sum over q's blocks, or over k's, of the partial rows: one warp per
+// channel, lanes over the blocks, then a fixed tree.
+__global__ void head_norm_dw_kernel(const float* part, int q_blocks, int blocks, int D, int f32, void* dwq,
                                     void* dwk) {
-  const int ch = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (ch >= 2 * D) return;
+  const int e = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (e >= 2 * D) return;
+  const int kind = e >= D, ch = kind ? e - D : e;
+  const int from = kind ? q_blocks : 0, to = kind ? blocks : q_blocks;
   float s = 0.f;
-  for (int b = lane; b < blocks; b += 32) s += part[(int64_t)b * 2 * D + ch];
+  for (int b = from + lane; b < to; b += 32) s += part[(int64_t)b * D + ch];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane) return;
-  void* out = ch < D ? dwq : dwk;
-  const int c = ch % D;
+  void* out = kind ? dwk : dwq;
   if (f32)
-    reinterpret_cast<float*>(out)[c] = s;
+    reinterpret_cast<float*>(out)[ch] = s;
   else
-    reinterpret_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(s);
+    reinterpret_cast<__nv_bfloat16*>(out)[ch] = __float2bfloat16_rn(s);
 }
 
 constexpr int kMaxBwdBlocks = 148 * 4;
 
-int bwd_blocks(int64_t rows, int hq, int hk, int D) {
-  const int hpw = 256 / D, per = 4 * hpw;
-  const int64_t items = rows * ((hq + per - 1) / per + (hk + per - 1) / per);
-  const int64_t b = (items + kWarps - 1) / kWarps;
-  return (int)(b < 1 ? 1 : b > kMaxBwdBlocks ? kMaxBwdBlocks : b);
+// Blocks of the backward on q and on k: what their items fill, at most
+// kMaxBwdBlocks together, shared out by the items.
+struct BwdBlocks {
+  int q, k;
+};
+BwdBlocks bwd_blocks(int64_t rows, int hq, int hk, int D) {
+  const int per = kBwdUnroll * (256 / D);
+  const int64_t iq = rows * ((hq + per - 1) / per), ik = rows * ((hk + per - 1) / per);
+  const auto fill = [](int64_t items) { return items < kWarps ? 1 : (items + kWarps - 1) / kWarps; };
+  int64_t bq = fill(iq), bk = fill(ik);
+  if (bq + bk > kMaxBwdBlocks) {
+    bq = kMaxBwdBlocks * iq / (iq + ik);
+    if (bq < 1) bq = 1;
+    if (bq > kMaxBwdBlocks - 1) bq = kMaxBwdBlocks - 1;
+    bk = kMaxBwdBlocks - bq;
+  }
+  return {(int)bq, (int)bk};
 }
 
 bool aligned_rows(const void* p, int64_t stride) {
@@ -294,7 +305,7 @@ int check_sizes(int64_t rows, int hq, int hk, int D, int64_t freqs_rows, const v
               (long long)rows, hq, hk, (long long)freqs_rows);
     return HIER_EVALUE;
   }
-  if (rows * ((hq + 3) / 4 + (hk + 3) / 4) > INT32_MAX || freqs_rows > INT32_MAX) {
+  if (rows * ((hq + 1) / 2 + (hk + 1) / 2) > INT32_MAX || freqs_rows > INT32_MAX) {
     set_error(HIER_EVALUE, "too many rows (%lld) or table rows (%lld)", (long long)rows,
               (long long)freqs_rows);
     return HIER_EVALUE;
@@ -373,7 +384,8 @@ extern "C" int hier_head_norm_rope_bwd_partials(int64_t rows, int32_t hq, int32_
     set_error(HIER_EVALUE, "no place for the number of partial rows");
     return HIER_EVALUE;
   }
-  *blocks = bwd_blocks(rows, hq, hk, D);
+  const BwdBlocks b = bwd_blocks(rows, hq, hk, D);
+  *blocks = b.q + b.k;
   return HIER_OK;
 }
 
@@ -394,8 +406,9 @@ extern "C" int hier_head_norm_rope_bwd(const void* q, int64_t q_stride, const vo
     set_error(HIER_EVALUE, "rows must be 16-byte aligned with 16-byte row strides");
     return HIER_EVALUE;
   }
-  if (blocks != bwd_blocks(rows, hq, hk, D)) {
-    set_error(HIER_EVALUE, "partials must have %d blocks; got %d", bwd_blocks(rows, hq, hk, D), blocks);
+  const BwdBlocks b = bwd_blocks(rows, hq, hk, D);
+  if (blocks != b.q + b.k) {
+    set_error(HIER_EVALUE, "partials must have %d blocks; got %d", b.q + b.k, blocks);
     return HIER_EVALUE;
   }
   HeadNormArgs a = {};
@@ -415,17 +428,17 @@ extern "C" int hier_head_norm_rope_bwd(const void* q, int64_t q_stride, const vo
   a.g_stride[0] = gq_stride, a.g_stride[1] = gk_stride;
   a.part = partials;
   a.err = dev_err;
-  const int per = 4 * (256 / D);
+  const int per = kBwdUnroll * (256 / D);
   a.chunks[0] = (hq + per - 1) / per, a.chunks[1] = (hk + per - 1) / per;
   cudaStream_t st = (cudaStream_t)stream;
   if (D == 64)
-    head_norm_bwd_kernel<64><<<blocks, kWarps * 32, 0, st>>>(a);
+    head_norm_bwd_kernel<64><<<blocks, kWarps * 32, 0, st>>>(a, b.q);
   else if (D == 128)
-    head_norm_bwd_kernel<128><<<blocks, kWarps * 32, 0, st>>>(a);
+    head_norm_bwd_kernel<128><<<blocks, kWarps * 32, 0, st>>>(a, b.q);
   else
-    head_norm_bwd_kernel<256><<<blocks, kWarps * 32, 0, st>>>(a);
+    head_norm_bwd_kernel<256><<<blocks, kWarps * 32, 0, st>>>(a, b.q);
   HIER_CHECK_CUDA(cudaGetLastError(), "head_norm_bwd_kernel launch");
-  head_norm_dw_kernel<<<(2 * D + 7) / 8, 256, 0, st>>>(partials, blocks, D, w_f32, dwq, dwk);
+  head_norm_dw_kernel<<<(2 * D + 7) / 8, 256, 0, st>>>(partials, b.q, blocks, D, w_f32, dwq, dwk);
   HIER_CHECK_CUDA(cudaGetLastError(), "head_norm_dw_kernel launch");
   return HIER_OK;
 }

@@ -266,7 +266,7 @@ class _HeadNormFn(torch.autograd.Function):
             dk = torch.empty(k_shape, dtype=bf, device=dev)
             dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
             blocks = _head_norm_blocks(T, H, Hk, D)
-            part = torch.empty((blocks, 2, D), dtype=torch.float32, device=dev)
+            part = torch.empty((blocks, D), dtype=torch.float32, device=dev)
             rc = L.hier_head_norm_rope_bwd(
                 q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, H, Hk, D,
                 wq.data_ptr(), wk.data_ptr(), int(wq.dtype is torch.float32), ft.data_ptr(),
