@@ -271,9 +271,32 @@ def stream_ptr(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_DEV_ERR = {}
+
+
+def dev_err(device):
+    """The device's sticky error word of the kernels' bounded waits."""
+    import torch
+
+    key = device.index if isinstance(device, torch.device) else torch.device(device).index
+    if key is None:  # "cuda" is the current device, whose tensors carry its index
+        key = torch.cuda.current_device()
+    t = _DEV_ERR.get(key)
+    if t is None:
+        t = _DEV_ERR[key] = torch.zeros(1, dtype=torch.int32, device=device)
+    return t
+
+
 def raw_stream(index):
     """Handle of the current stream of device ``index`` (an int: what
     ``current_stream(device).cuda_stream`` gives, without the objects)."""
     import torch
 
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def is_current(dev):
+    """Whether ``dev`` (a CUDA device with an index) is the current device."""
+    import torch
+
+    return dev.index == torch._C._cuda_getDevice()

@@ -26,9 +26,10 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from ._lib import check, ptr, stream_ptr
+from ._lib import check, is_current, ptr, stream_ptr
+from ._lib import dev_err as _dev_err
 from .hier_masks import HierBlockMask, block_mask_for_spec, build_dense_block_plan
-from .paged8 import on_device, token_rows
+from .paged8 import token_rows
 
 __all__ = ["hier_prep_qk", "hier_block_attention", "freqs_table", "RMSNorm", "SelfAttention",
            "AttentionPlan", "attention_from_plan", "HierSequencePlan", "sequence_plan",
@@ -38,20 +39,6 @@ __all__ = ["hier_prep_qk", "hier_block_attention", "freqs_table", "RMSNorm", "Se
 # HierSequencePlan wherever the grouping allows it) or "blocks" (always the
 # 128x128 block plan of the HierBlockMask).
 FULL_SEQUENCE_PLAN_ENV = "MULTICS_B200_FULL_SEQUENCE_PLAN"
-
-_DEV_ERR = {}
-
-
-def _dev_err(device):
-    key = device.index if isinstance(device, torch.device) else torch.device(device).index
-    if key is None:  # "cuda" is the current device, whose tensors carry its index
-        key = torch.cuda.current_device()
-    t = _DEV_ERR.get(key)
-    if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
-        _DEV_ERR[key] = t
-    return t
-
 
 def device_error(device=None) -> int:
     """Sticky device error word of the attention kernels (0 = no timeout)."""
@@ -210,25 +197,27 @@ def head_norm_launch(args, num_heads, num_kv_heads, eps, out=None, q_rows=None, 
         if m is not None and (m.dtype != torch.int32 or tuple(m.shape) != (T,) or m.device != dev
                               or not m.is_contiguous()):
             raise ValueError(f"out_rows and k_out_rows must be int32 [{T}] on {dev}")
-    with on_device(dev):
-        if out is None:
-            q_out = torch.empty((T, num_heads * D), dtype=torch.bfloat16, device=dev)
-            k_out = torch.empty((T, num_kv_heads * D), dtype=torch.bfloat16, device=dev)
-        else:
-            q_out, k_out = out
-            for name, t, w, m in (("q_out", q_out, num_heads * D, q_rows),
-                                  ("k_out", k_out, num_kv_heads * D, k_rows)):
-                if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != w or t.device != dev \
-                        or t.stride(1) != 1 or (m is None and t.shape[0] < T):
-                    raise ValueError(f"{name} must be bf16 [{T}, {w}] rows on {dev}, got {t.dtype} "
-                                     f"{tuple(t.shape)}")
-        rc = _lib.lib().hier_head_norm_rope(
-            q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, num_heads, num_kv_heads,
-            D, wq.data_ptr(), wk.data_ptr(), int(wq.dtype is torch.float32), ft.data_ptr(),
-            ft.shape[0], None if pos is None else pos.data_ptr(), float(eps), q_out.data_ptr(),
-            q_out.stride(0), None if q_rows is None else q_rows.data_ptr(), q_out.shape[0],
-            k_out.data_ptr(), k_out.stride(0), None if k_rows is None else k_rows.data_ptr(),
-            k_out.shape[0], int(out is None), _dev_err(dev).data_ptr(), _lib.raw_stream(dev.index))
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return head_norm_launch(args, num_heads, num_kv_heads, eps, out, q_rows, k_rows)
+    if out is None:
+        q_out = torch.empty((T, num_heads * D), dtype=torch.bfloat16, device=dev)
+        k_out = torch.empty((T, num_kv_heads * D), dtype=torch.bfloat16, device=dev)
+    else:
+        q_out, k_out = out
+        for name, t, w, m in (("q_out", q_out, num_heads * D, q_rows),
+                              ("k_out", k_out, num_kv_heads * D, k_rows)):
+            if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != w or t.device != dev \
+                    or t.stride(1) != 1 or (m is None and t.shape[0] < T):
+                raise ValueError(f"{name} must be bf16 [{T}, {w}] rows on {dev}, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+    rc = _lib.lib().hier_head_norm_rope(
+        q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, num_heads, num_kv_heads, D,
+        wq.data_ptr(), wk.data_ptr(), wq.dtype is torch.float32, ft.data_ptr(), ft.shape[0],
+        None if pos is None else pos.data_ptr(), eps, q_out.data_ptr(), q_out.stride(0),
+        None if q_rows is None else q_rows.data_ptr(), q_out.shape[0], k_out.data_ptr(),
+        k_out.stride(0), None if k_rows is None else k_rows.data_ptr(), k_out.shape[0],
+        out is None, _dev_err(dev).data_ptr(), _lib.raw_stream(dev.index))
     if rc:
         check(rc)
     return q_out, k_out

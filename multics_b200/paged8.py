@@ -22,7 +22,6 @@ length outside the table) it skips and records in the cache's status word
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import math
@@ -31,7 +30,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from ._lib import check, raw_stream
+from ._lib import check, dev_err, is_current, raw_stream
 
 __all__ = ["PAGE_TOKENS", "Paged8Cache", "PageStep", "page_step", "paged8_append",
            "paged8_attention"]
@@ -50,13 +49,6 @@ _STEP_BITS = ((1, "too few free pages"), (2, "more new tokens than rows"),
               (4, "a length leaves the block table"),
               (8, "an addition is below -length or above the step's most"),
               (16, "the free count leaves the free list"))
-
-
-def on_device(dev):
-    """A context in which ``dev`` is the current device (none when it is)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
 
 
 def _vector(name, t, n, dev):
@@ -140,24 +132,27 @@ class Paged8Cache:
         way share one word per device."""
         if k.dtype not in _FORMATS or v.dtype != k.dtype:
             raise ValueError(f"codes must both be int8 or float8_e4m3fn, got {k.dtype}, {v.dtype}")
-        if k.dim() != 5 or tuple(k.shape[2:]) != (2, PAGE_TOKENS, 64):
+        pool = k.shape[:2]
+        if k.dim() != 5 or k.shape[2:] != (2, PAGE_TOKENS, 64):
             raise ValueError(f"k must be [pages, heads, 2, 64, 64], got {tuple(k.shape)}")
-        if tuple(v.shape) != (*k.shape[:2], HEAD_DIM, PAGE_TOKENS):
+        if v.shape != (*pool, HEAD_DIM, PAGE_TOKENS):
             raise ValueError(f"v must be [pages, heads, 128, 64] like k {tuple(k.shape)}, got "
                              f"{tuple(v.shape)}")
-        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if s.dtype != torch.float32 or s.shape != k.shape[:2]:
-                raise ValueError(f"{name} must be float32 {tuple(k.shape[:2])}, got {s.dtype} "
-                                 f"{tuple(s.shape)}")
-        for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
-            if not t.is_contiguous() or t.device != k.device:
-                raise ValueError(f"{name} must be contiguous on {k.device}")
+        if (k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32
+                or k_scale.shape != pool or v_scale.shape != pool):
+            raise ValueError(f"k_scale and v_scale must be float32 {tuple(pool)}, got "
+                             f"{k_scale.dtype} {tuple(k_scale.shape)}, {v_scale.dtype} "
+                             f"{tuple(v_scale.shape)}")
+        dev = k.device
+        for t in (k, v, k_scale, v_scale):
+            if not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"codes and scales must be contiguous on {dev}")
         if status is None:
-            status = _STATUS.get(k.device)
+            status = _STATUS.get(dev)
             if status is None:
-                status = _STATUS[k.device] = torch.zeros(1, dtype=torch.int32, device=k.device)
+                status = _STATUS[dev] = torch.zeros(1, dtype=_I32, device=dev)
         else:
-            _vector("status", status, 1, k.device)
+            _vector("status", status, 1, dev)
         self = cls.__new__(cls)
         self._set(k, v, k_scale, v_scale, status)
         return self
@@ -222,20 +217,23 @@ def page_step(lengths, add, table, free_pages, free_count, rows: int, *,
     if most_new is not None and most_new < 0:
         raise ValueError(f"most_new must not be negative, got {most_new}")
     _cuda("page_step", dev)
-    with on_device(dev):
-        if in_place:
-            q_start, status, slots, positions = torch.empty(
-                n + 2 + 2 * rows, dtype=_I32, device=dev).split((n + 1, 1, rows, rows))
-            new_len, new_count = lengths, free_count
-        else:
-            new_len, new_count, q_start, status, slots, positions = torch.empty(
-                2 * n + 3 + 2 * rows, dtype=_I32, device=dev).split((n, 1, n + 1, 1, rows, rows))
-        rc = _lib.lib().hier_page_step(
-            lengths.data_ptr(), add.data_ptr(), n, table.data_ptr(), stride, width,
-            free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), rows,
-            -1 if most_new is None else int(most_new), new_len.data_ptr(), new_count.data_ptr(),
-            q_start.data_ptr(), slots.data_ptr(), positions.data_ptr(), status.data_ptr(),
-            raw_stream(dev.index))
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return page_step(lengths, add, table, free_pages, free_count, rows, most_new=most_new,
+                             in_place=in_place)
+    if in_place:
+        q_start, status, slots, positions = torch.empty(
+            n + 2 + 2 * rows, dtype=_I32, device=dev).split((n + 1, 1, rows, rows))
+        new_len, new_count = lengths, free_count
+    else:
+        new_len, new_count, q_start, status, slots, positions = torch.empty(
+            2 * n + 3 + 2 * rows, dtype=_I32, device=dev).split((n, 1, n + 1, 1, rows, rows))
+    rc = _lib.lib().hier_page_step(
+        lengths.data_ptr(), add.data_ptr(), n, table.data_ptr(), stride, width,
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), rows,
+        -1 if most_new is None else int(most_new), new_len.data_ptr(), new_count.data_ptr(),
+        q_start.data_ptr(), slots.data_ptr(), positions.data_ptr(), status.data_ptr(),
+        raw_stream(dev.index))
     if rc:
         check(rc)
     return PageStep(new_len, new_count, q_start, slots, positions, status)
@@ -270,13 +268,14 @@ def paged8_append(cache: Paged8Cache, k, v, table, lengths, q_start):
     _cuda("paged8_append", dev)
     if k.device != dev or v.device != dev:
         raise ValueError(f"k, v must be on {dev}")
-    with on_device(dev):
-        rc = _lib.lib().hier_paged8_append(
-            k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), k.shape[0], cache.num_heads,
-            cache.format, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
-            lengths.data_ptr(), q_start.data_ptr(), n, cache.status.data_ptr(),
-            raw_stream(dev.index))
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return paged8_append(cache, k, v, table, lengths, q_start)
+    rc = _lib.lib().hier_paged8_append(
+        k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), k.shape[0], cache.num_heads,
+        cache.format, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+        cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
+        lengths.data_ptr(), q_start.data_ptr(), n, cache.status.data_ptr(), raw_stream(dev.index))
     if rc:
         check(rc)
 
@@ -323,33 +322,37 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
     _cuda("paged8_attention", dev)
     if q.device != dev:
         raise ValueError(f"q must be on {dev}")
-    from .attention import _dev_err
-
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return paged8_attention(q, cache, table, lengths, q_start, num_heads,
+                                    tokens_per_frame=tokens_per_frame, block_frames=block_frames,
+                                    window=window, softmax_scale=scale, max_rows=max_rows, out=out,
+                                    return_lse=return_lse)
     most = 0 if max_rows is None else int(max_rows)
     lse = ws = None
-    with on_device(dev):
-        if out is None:
-            o = torch.empty((T, dim), dtype=_BF16, device=dev)
-        elif out.data_ptr() % 16 or out.stride(0) % 8:  # rows the kernels cannot store to
-            o = out.clone(memory_format=torch.contiguous_format)
-        else:
-            o = out
-        if return_lse:
-            lse = torch.empty((T, num_heads), dtype=torch.float32, device=dev)
-        floats = _workspace_floats(T, num_heads, cache.num_heads, n, width, most)
-        if floats:
-            ws = torch.empty(floats, dtype=torch.float32, device=dev)
-        rc = _lib.lib().hier_paged8_attn(
-            q.data_ptr(), q.stride(0), T, num_heads, cache.num_heads, HEAD_DIM, cache.format,
-            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
-            lengths.data_ptr(), q_start.data_ptr(), n, int(tokens_per_frame), int(block_frames), int(window), scale,
-            most, o.data_ptr(), o.stride(0), None if lse is None else lse.data_ptr(),
-            int(out is None), None if ws is None else ws.data_ptr(), cache.status.data_ptr(),
-            _dev_err(dev).data_ptr(), raw_stream(dev.index))
-        if rc:
-            check(rc)
-        if out is not None and o is not out:
-            out.copy_(o)
-            o = out
+    if out is None:
+        o = torch.empty((T, dim), dtype=_BF16, device=dev)
+    elif out.data_ptr() % 16 or out.stride(0) % 8:  # rows the kernels cannot store to
+        o = out.clone(memory_format=torch.contiguous_format)
+    else:
+        o = out
+    if return_lse:
+        lse = torch.empty((T, num_heads), dtype=torch.float32, device=dev)
+    floats = _workspace_floats(T, num_heads, cache.num_heads, n, width, most)
+    if floats:
+        ws = torch.empty(floats, dtype=torch.float32, device=dev)
+    rc = _lib.lib().hier_paged8_attn(
+        q.data_ptr(), q.stride(0), T, num_heads, cache.num_heads, HEAD_DIM, cache.format,
+        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+        cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
+        lengths.data_ptr(), q_start.data_ptr(), n, int(tokens_per_frame), int(block_frames),
+        int(window), scale, most, o.data_ptr(), o.stride(0),
+        None if lse is None else lse.data_ptr(), out is None,
+        None if ws is None else ws.data_ptr(), cache.status.data_ptr(),
+        dev_err(dev).data_ptr(), raw_stream(dev.index))
+    if rc:
+        check(rc)
+    if out is not None and o is not out:
+        out.copy_(o)
+        o = out
     return (o, lse) if return_lse else o

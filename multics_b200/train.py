@@ -18,6 +18,7 @@ is recording.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -26,9 +27,9 @@ import torch
 
 from . import _lib
 from ._lib import check, ptr, stream_ptr
-from .attention import _dev_err, _rows
+from .attention import _dev_err, _rows, head_norm_args, head_norm_launch
 from .hier_masks import HierBlockMask
-from .paged8 import on_device, token_rows
+from .paged8 import token_rows
 
 __all__ = ["BlockPlanGrad", "block_plan_grad", "hier_block_attention_grad", "plan_attention_grad",
            "prologue_grad", "head_norm_rope_grad"]
@@ -240,8 +241,6 @@ class _HeadNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, wq, wk, ft, positions, num_heads, num_kv_heads, eps):
-        from .attention import head_norm_args, head_norm_launch
-
         args = head_norm_args(q, k, ft, num_heads, num_kv_heads, wq, wk, positions)
         q2, k2, D, w1, w2, ft, pos = args
         ctx.save_for_backward(q2, k2, w1, w2, ft, pos)
@@ -256,29 +255,28 @@ class _HeadNormFn(torch.autograd.Function):
         H, Hk, D, eps = ctx.sizes
         q_shape, k_shape, wq_dtype, wk_dtype = ctx.like
         T, dev, bf = q2.shape[0], q2.device, torch.bfloat16
-        L = _lib.lib()
-        with on_device(dev):
+        with contextlib.nullcontext() if _lib.is_current(dev) else torch.cuda.device(dev):
             gq = (torch.zeros((T, H * D), dtype=bf, device=dev) if gq is None
-                  else token_rows("gradient of q", gq.to(bf), H * D))
+                  else token_rows("gradient of q", gq if gq.dtype is bf else gq.to(bf), H * D))
             gk = (torch.zeros((T, Hk * D), dtype=bf, device=dev) if gk is None
-                  else token_rows("gradient of k", gk.to(bf), Hk * D))
+                  else token_rows("gradient of k", gk if gk.dtype is bf else gk.to(bf), Hk * D))
             dq = torch.empty(q_shape, dtype=bf, device=dev)
             dk = torch.empty(k_shape, dtype=bf, device=dev)
             dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
             blocks = _head_norm_blocks(T, H, Hk, D)
             part = torch.empty((blocks, D), dtype=torch.float32, device=dev)
-            rc = L.hier_head_norm_rope_bwd(
+            rc = _lib.lib().hier_head_norm_rope_bwd(
                 q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, H, Hk, D,
-                wq.data_ptr(), wk.data_ptr(), int(wq.dtype is torch.float32), ft.data_ptr(),
-                ft.shape[0], None if pos is None else pos.data_ptr(), float(eps), gq.data_ptr(),
-                gq.stride(0), gk.data_ptr(), gk.stride(0), dq.data_ptr(), H * D,
-                dk.data_ptr(), Hk * D, part.data_ptr(), blocks, dwq.data_ptr(),
-                dwk.data_ptr(), _dev_err(dev).data_ptr(), _lib.raw_stream(dev.index))
-            if rc:
-                check(rc)
-            if wq.dtype is not wq_dtype or wk.dtype is not wk_dtype:
-                dwq, dwk = dwq.to(wq_dtype), dwk.to(wk_dtype)
-            return dq, dk, dwq, dwk, None, None, None, None, None
+                wq.data_ptr(), wk.data_ptr(), wq.dtype is torch.float32, ft.data_ptr(),
+                ft.shape[0], None if pos is None else pos.data_ptr(), eps, gq.data_ptr(),
+                gq.stride(0), gk.data_ptr(), gk.stride(0), dq.data_ptr(), H * D, dk.data_ptr(),
+                Hk * D, part.data_ptr(), blocks, dwq.data_ptr(), dwk.data_ptr(),
+                _dev_err(dev).data_ptr(), _lib.raw_stream(dev.index))
+        if rc:
+            check(rc)
+        if wq.dtype is not wq_dtype or wk.dtype is not wk_dtype:
+            dwq, dwk = dwq.to(wq_dtype), dwk.to(wk_dtype)
+        return dq, dk, dwq, dwk, None, None, None, None, None
 
 
 @functools.lru_cache(maxsize=256)
