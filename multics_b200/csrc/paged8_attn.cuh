@@ -45,6 +45,7 @@ struct Paged8Args {
   Divisor splits;   // most parts a tile's keys are cut into
   float* part_o;    // [tile][kv head][split][kRows][128]
   float* part_ml;   // [tile][kv head][split][kRows][2]
+  int cluster;      // the parts of a small tile are the blocks of a cluster
   int row_limit;    // requests of up to row_limit pairs are the small kernel's, the others the
                     // large one's (INT_MAX: all the small one's, 0: all the large one's)
   Divisor direct;   // small kernel: its tile t is tile t % direct of request t / direct
