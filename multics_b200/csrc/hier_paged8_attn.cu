@@ -625,10 +625,15 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
 }
 
 // How a call is cut, from the sizes the host knows (the same for every content
-// of the device tables).  Requests of up to kSmallPairs (row, head) pairs per
-// key head run on the small kernel, longer ones on the large one; a call that
+// of the device tables).  Requests of up to small_pairs() (row, head) pairs per
+// key head run on the small kernels, longer ones on the large one; a call that
 // may hold both runs both, each leaving the other's requests.
-constexpr int kSmallPairs = 16;
+//
+// Per SM and 8 pairs the small kernels take about 0.3 us and 0.25 us a page, the
+// large one 11 us and 0.67 us a page for up to 128 pairs (651 x 56 pairs over one
+// page, 2 key heads: 101 us on the large kernel): the sides meet at 169 pairs for
+// one page, 84 for four, 22 for hundreds.  Pages are those a table row can list.
+int small_pairs(int width) { return (int)(8 * (440 + 27 * (int64_t)width) / (12 + 10 * (int64_t)width)); }
 constexpr int kShortPages = 4;
 constexpr int kMaxCluster = 8;
 
@@ -639,6 +644,7 @@ struct Shape {
   int64_t floats;  // workspace: the small kernel's parts, then the large one's
   int64_t small_floats;
   bool cluster;    // the small kernel's parts are a cluster's
+  int limit;       // small_pairs
 };
 
 int clamp_int(int64_t v, int64_t lo, int64_t hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
@@ -648,11 +654,13 @@ Shape shape_of(int64_t rows, int group, int kv_heads, int n, int width, int max_
   const int64_t most = max_rows > 0 && max_rows < rows ? max_rows : rows;
   const int64_t some = n < rows ? n : rows;  // requests that can have rows
   s.large_splits = 1;
-  s.small = n > 0 && (most * group <= kSmallPairs || n > 1);
-  s.large = n == 0 || most * group > kSmallPairs;
+  s.limit = small_pairs(width);
+  s.small = n > 0 && (most * group <= s.limit || n > 1);
+  s.large = n == 0 || most * group > s.limit;
   if (s.small) {
-    const int64_t pairs = s.large ? kSmallPairs : most * group;
-    s.direct = (int)((pairs + kRows - 1) / kRows);
+    // (beside the large kernel most requests may be its own: two tiles each, the
+    // others in turn)
+    s.direct = s.large ? 2 : (int)((most * group + kRows - 1) / kRows);
     s.small_tiles = (int64_t)n * s.direct;
     s.small_splits = 1;
     if (width > kShortPages) {
@@ -674,8 +682,9 @@ Shape shape_of(int64_t rows, int group, int kv_heads, int n, int width, int max_
   }
   if (s.large) {
     s.large_tiles = paged8_tiles<kPaged8LargeRows>(rows, group, n);
-    const int64_t real = (rows * group + kPaged8LargeRows - 1) / kPaged8LargeRows;
-    const int64_t work = real * kv_heads;
+    // tiles that are likely there: every request has one
+    const int64_t full = (rows * group + kPaged8LargeRows - 1) / kPaged8LargeRows;
+    const int64_t work = std::max<int64_t>({full, some, 1}) * kv_heads;
     s.large_splits = clamp_int(148 / work, 1, clamp_int(width / (2 * kPaged8LargeMin), 1, 16));
   }
   s.floats = s.small_floats;
@@ -835,7 +844,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
   }
   // both kernels: one rule for whose a request is, and the rows behind the last
   // request are the large one's
-  a.row_limit = !s.large ? INT32_MAX : s.small ? kSmallPairs : 0;
+  a.row_limit = !s.large ? INT32_MAX : s.small ? s.limit : 0;
   if (s.large) {
     a.zero_tail = zero_tail;
     a.splits = divisor(s.large_splits);

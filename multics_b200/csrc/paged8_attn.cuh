@@ -55,7 +55,7 @@ struct Paged8Args {
 
 constexpr int kPaged8SmallRows = 8;
 constexpr int kPaged8LargeRows = 256;
-constexpr int kPaged8LargeMin = 4;  // 128-key tiles of a part at least
+constexpr int kPaged8LargeMin = 8;  // 128-key tiles of a part at least
 
 template <int kRows>
 __host__ __device__ inline int64_t paged8_tiles(int64_t rows, int group, int n) {
