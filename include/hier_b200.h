@@ -815,9 +815,9 @@ int hier_paged8_append(const void* k, int64_t k_stride, const void* v, int64_t v
  *   block == 0, or j / frame / block <= p / frame / block, and
  *   window < 0, or p / frame - j / frame < window
  * (frames of `frame` tokens, causal blocks of `block` frames, window in
- * frames).  out bf16 [rows][heads*128] is 0 for rows that see nothing; rows
- * behind the last request are left, or zeroed with zero_tail.  lse (or NULL):
- * float [rows][heads], log2-sum-exp of the scaled scores.  max_rows: the most
+ * frames).  out bf16 [rows][heads*128] (may be q) is 0 for rows that see
+ * nothing; rows of no request are left, or zeroed with zero_rest.  lse (or
+ * NULL): float [rows][heads], log2-sum-exp of the scaled scores.  max_rows: the most
  * rows a request has, as far as the caller knows (it chooses kernels, not
  * results); <= 0: unknown.  softmax_scale is positive and finite.  workspace:
  * floats of ..._workspace for the same sizes.  dev_err: the kernels' sticky
@@ -830,7 +830,7 @@ int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, int32_t head
                      int32_t n_pages, const int32_t* table, int64_t table_stride, int32_t width,
                      const int32_t* lengths, const int32_t* q_start, int32_t n, int32_t frame,
                      int32_t block, int32_t window, float softmax_scale, int32_t max_rows,
-                     void* out, int64_t out_stride, float* lse, int32_t zero_tail,
+                     void* out, int64_t out_stride, float* lse, int32_t zero_rest,
                      float* workspace, int32_t* status, int32_t* dev_err, void* stream);
 
 /* ---------------------------------------------------------------------------

@@ -179,9 +179,10 @@ def hier_head_norm_rope(q, k, freqs, num_heads, num_kv_heads, *, q_weight, k_wei
     (int32 on the device; ``r % F`` without them).  Rows with a negative
     position are zeros, or left as they were in a given ``out``; a position past
     the table counts as negative and sets :func:`device_error`.  ``out``:
-    ``(q_out, k_out)`` to write to (16-byte aligned rows), ``out_rows`` / ``k_out_rows`` (int32 ``[T]``)
-    the row of each token in them (``k_out_rows`` for k alone, e.g. the slots of
-    a paged pool; negative: not written)."""
+    ``(q_out, k_out)`` to write to (16-byte aligned rows; ``q`` and ``k``
+    themselves where no row moves), ``out_rows`` / ``k_out_rows`` (int32
+    ``[T]``) the row of each token in them (``k_out_rows`` for k alone, e.g. the
+    slots of a paged pool; negative: not written)."""
     args = head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight, k_weight, positions)
     if out is None and k_out_rows is not None:
         raise ValueError("k_out_rows needs out=(q_out, k_out)")

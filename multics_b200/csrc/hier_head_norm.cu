@@ -221,8 +221,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) head_norm_bwd_kernel(HeadNormA
         const float g1 = fmaf(q[2 * i + 1], cs[i], -q[2 * i] * sn[i]);
         f[2 * i] *= rs;
         f[2 * i + 1] *= rs;
-        acc[2 * i] = fmaf(g0, f[2 * i], acc[2 * i]);
-        acc[2 * i + 1] = fmaf(g1, f[2 * i + 1], acc[2 * i + 1]);
+        if (h < heads) {  // (lanes without a head: 0 x rsqrt(eps), eps may be 0)
+          acc[2 * i] = fmaf(g0, f[2 * i], acc[2 * i]);
+          acc[2 * i + 1] = fmaf(g1, f[2 * i + 1], acc[2 * i + 1]);
+        }
         q[2 * i] = g0 * w[2 * i];
         q[2 * i + 1] = g1 * w[2 * i + 1];
         dot = fmaf(q[2 * i], f[2 * i], dot);

@@ -611,7 +611,7 @@ extern "C" int hier_paged8_append(const void* k, int64_t k_stride, const void* v
     set_error(HIER_EVALUE, "cache format must be 0 (int8) or 1 (e4m3); got %d", format);
     return HIER_EVALUE;
   }
-  if (rows < 0 || heads < 1 || n_pages < 0 || n < 0 || width < 0 || table_stride < width ||
+  if (rows < 0 || heads < 1 || n_pages < 1 || n < 0 || width < 0 || table_stride < width ||
       (int64_t)width * kPage > INT32_MAX) {
     set_error(HIER_EVALUE, "invalid rows=%d, heads=%d, pages=%d, requests=%d or table width=%d", rows,
               heads, n_pages, n, width);

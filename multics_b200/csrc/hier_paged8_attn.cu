@@ -274,19 +274,7 @@ __device__ __forceinline__ void write_pair(const Paged8Args& a, const Paged8Tile
   const int h = kvh * a.group + g;
   *reinterpret_cast<uint2*>(a.out + r * a.out_stride + h * 128 + 4 * lane) = make_uint2(
       pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-  if (a.lse && lane == 0) a.lse[r * a.heads + h] = L > 0.f ? M + log2f(L) : -INFINITY;
-}
-
-// zeros to the rows behind the last request, worker i of n taking every n-th
-__device__ __forceinline__ void zero_tail(const Paged8Args& a, int kvh, int64_t i, int64_t n, int lane) {
-  const int end = a.q_start[a.n];
-  if (end < 0) return;
-  for (int64_t r = end + i; r < a.rows; r += n) {
-    uint4* dst = reinterpret_cast<uint4*>(a.out + r * a.out_stride + kvh * a.group * 128);
-    for (int e = lane; e < a.group * 16; e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
-    if (a.lse)
-      for (int e = lane; e < a.group; e += 32) a.lse[r * a.heads + kvh * a.group + e] = -INFINITY;
-  }
+  if (a.lse && lane == 0) a.lse[r * a.heads + h] = row_lse(M, L);
 }
 
 constexpr int kMinPages = 2 * kWarps;  // of a part at least
@@ -326,8 +314,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
   const int unit = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - unit * a.splits.d;
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const int b = tile / a.direct, first = tile % a.direct * kRows;
-  if (a.zero_tail && split == 0)
-    zero_tail(a, kvh, (int64_t)tile * kWarps + w, (int64_t)a.n * a.direct * kWarps, lane);
+  if (a.zero_rest && split == 0)
+    zero_rest(a, kvh, (int64_t)tile * kWarps + w, (int64_t)a.n * a.direct * kWarps, lane);
   // Tiles beyond those the launch counted on (a request of more rows than
   // max_rows said) follow in the same block, their keys in one part.
   for (int rho0 = first;; rho0 += a.direct * kRows) {
@@ -548,7 +536,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args
   if (unit >= units) return;
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const int b = tile / a.direct;
-  if (a.zero_tail) zero_tail(a, kvh, tile, (int64_t)a.n * a.direct, lane);
+  if (a.zero_rest) zero_rest(a, kvh, tile, (int64_t)a.n * a.direct, lane);
   for (int rho0 = tile % a.direct * kRows;; rho0 += a.direct * kRows) {
     const Paged8Tile tl = small_tile(a, b, rho0, kvh == 0 && lane == 0);
     if (!tl.live) return;
@@ -597,7 +585,7 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
                                : small_tile(a, tile / a.direct, tile % a.direct * kRows, false);
   // every block waits: what follows this kernel on the stream needs the attention done
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!tl.live || (kLarge && (tl.b == a.n || tl.pairs <= a.row_limit))) return;
+  if (!tl.live || (kLarge && tl.pairs <= a.row_limit)) return;
   const int parts = kLarge ? parts_of<kPaged8LargeMin>((tl.np + 1) / 2, a.splits)
                            : parts_of<kMinPages>(tl.np, a.splits);
   const int pr = tl.rho0 + r;
@@ -670,7 +658,9 @@ Shape shape_of(int64_t rows, int group, int kv_heads, int n, int width, int max_
       const int64_t work = some * s.direct * kv_heads;
       const int64_t one = std::min<int64_t>(kWave / work, width / kMinPages);
       const int64_t four = std::min<int64_t>(4 * kWave / work, width / (2 * kMinPages));
-      s.small_splits = clamp_int(std::max(one, four), 1, 32);
+      // (requests without rows have places in the workspace too: 68 MB of it at most)
+      s.small_splits =
+          clamp_int(std::max(one, four), 1, clamp_int((1 << 14) / (s.small_tiles * kv_heads), 1, 32));
       if (s.small_splits > 1 && work * std::min(s.small_splits, kMaxCluster) <= kWave) {
         s.cluster = true;
         while (s.small_splits > kMaxCluster || (s.small_splits & (s.small_splits - 1)))
@@ -788,7 +778,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
                                 int32_t width, const int32_t* lengths, const int32_t* q_start,
                                 int32_t n, int32_t frame, int32_t block, int32_t window,
                                 float softmax_scale, int32_t max_rows, void* out,
-                                int64_t out_stride, float* lse, int32_t zero_tail,
+                                int64_t out_stride, float* lse, int32_t zero_rest,
                                 float* workspace, int32_t* status, int32_t* dev_err,
                                 void* stream) {
   clear_error();
@@ -802,7 +792,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
     set_error(HIER_EVALUE, "cache format must be 0 (int8) or 1 (e4m3); got %d", format);
     return HIER_EVALUE;
   }
-  if (n_pages < 0 || table_stride < width || frame < 1 || frame > (1 << 30) || block < 0 ||
+  if (n_pages < 1 || table_stride < width || frame < 1 || frame > (1 << 30) || block < 0 ||
       block > (1 << 30) || window == 0 || window > (1 << 30)) {
     set_error(HIER_EVALUE, "invalid pages=%d, table stride=%lld, frame=%d, block=%d or window=%d",
               n_pages, (long long)table_stride, frame, block, window);
@@ -842,11 +832,11 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
     set_error(HIER_EVALUE, "this call needs a workspace (hier_paged8_attn_workspace)");
     return HIER_EVALUE;
   }
-  // both kernels: one rule for whose a request is, and the rows behind the last
-  // request are the large one's
+  // both kernels: one rule for whose a request is; the rows of no request are the
+  // small one's where it runs
   a.row_limit = !s.large ? INT32_MAX : s.small ? s.limit : 0;
   if (s.large) {
-    a.zero_tail = zero_tail;
+    a.zero_rest = zero_rest && !s.small;
     a.splits = divisor(s.large_splits);
     a.part_o = workspace + s.small_floats;
     a.part_ml = a.part_o + (s.floats - s.small_floats) / 130 * 128;
@@ -855,7 +845,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
     if (rc) return rc;
   }
   if (s.small) {
-    a.zero_tail = s.large ? 0 : zero_tail;
+    a.zero_rest = zero_rest;
     a.direct = divisor(s.direct);
     a.splits = divisor(s.small_splits);
     a.cluster = s.cluster;

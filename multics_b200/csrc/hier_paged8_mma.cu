@@ -52,7 +52,7 @@ constexpr int kSmemV = kSmemK + kStages * kTile;
 constexpr int kSmemRaw = kSmemV + kStages * kTile;  // codes of a key tile, of a value tile
 constexpr int kRawTile = 2 * kPageHeadBytes;
 constexpr int kSmemBar = kSmemRaw + 2 * kRawTile;
-constexpr int kNumBars = 1 + 4 * kStages + 8 + 8;
+constexpr int kNumBars = 1 + 4 * kStages + 8 + 8 + 1;
 constexpr int kSmemBytes = kSmemBar + 256 + 1024;  // + slack for 1024-byte alignment
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 static_assert(kNumBars * 8 + 8 <= 256, "barriers and the TMEM slot");
@@ -78,6 +78,7 @@ struct Bars {
   uint64_t* p_full;
   uint64_t* p_lo;
   uint64_t* o_final;
+  uint64_t* drained;    // a failed issuer's products are over
 };
 
 // fp16 operands, fp32 accumulation, both K-major
@@ -142,6 +143,7 @@ __device__ __forceinline__ bool in_pool(const Paged8Args& a, int page) {
 __device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uint8_t* smem,
                                           const Bars& B) {
   int pg[2] = {entry(J, J.page0), entry(J, J.page0 + 1)};
+  int issued[2] = {0, 0};  // tiles of keys, of values
   for (int j = 0; j < J.n_kv; ++j) {
     const int p = J.page0 + 2 * j;
     const int raw = j % J.raw_stages, raw_phase = ((j / J.raw_stages) - 1) & 1;
@@ -153,7 +155,7 @@ __device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uin
     for (int kind = 0; kind < 2; ++kind) {
       uint64_t* full = B.raw_full + 2 * raw + kind;
       if (j >= J.raw_stages && !mbar_wait(B.raw_empty + 2 * raw + kind, raw_phase, a.err, 40 + kind))
-        return;
+        break;
       const uint32_t bytes = (have0 + have1) * kPageHeadBytes;
       if (bytes)
         mbar_arrive_expect_tx(full, bytes);
@@ -164,24 +166,32 @@ __device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uin
       uint8_t* dst = raw_stage(smem, raw, kind);
       if (have0) bulk_load(dst, src + now0 * page_bytes, kPageHeadBytes, full);
       if (have1) bulk_load(dst + kPageHeadBytes, src + now1 * page_bytes, kPageHeadBytes, full);
+      ++issued[kind];
     }
+    if (issued[1] <= j) break;
   }
+  // no copy outlives the block, whoever else gave up
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind)
+    for (int j = max(0, issued[kind] - J.raw_stages); j < issued[kind]; ++j)
+      mbar_wait(B.raw_full + 2 * (j % J.raw_stages) + kind, (j / J.raw_stages) & 1, a.err, 52);
 }
 
-__device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint32_t tbase,
+// False: a wait ran out, with products perhaps still running.
+__device__ __forceinline__ bool mma_role(const Paged8Args& a, const Job& J, uint32_t tbase,
                                          uint8_t* smem, const Bars& B) {
   const uint32_t q_lo[2] = {sdesc_lo_kmajor(smem_u32(smem + kSmemQ)),
                             sdesc_lo_kmajor(smem_u32(smem + kSmemQ + (J.dual ? 0 : kTile)))};
   const uint32_t k_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemK));
   const uint32_t v_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemV));
   int cp[2] = {0, 0};  // PVs issued per half
-  if (!mbar_wait(B.q_full, 0, a.err, 42)) return;
+  if (!mbar_wait(B.q_full, 0, a.err, 42)) return false;
   if (J.dual) {
     // tile j is half j % 2's, and so are the stages it passes through
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (j >= J.n_kv) break;
-      if (!mbar_wait(B.k_full + j, 0, a.err, 43)) return;
+      if (!mbar_wait(B.k_full + j, 0, a.err, 43)) return false;
       tc_fence_after();
       issue_s_f16(tbase + j * kBN, q_lo[j], k_lo0 + ((j * kTile) >> 4));
       umma_commit(B.s_full + j);
@@ -191,16 +201,16 @@ __device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint
       const int h = j & 1, phase = (j >> 1) & 1;
       const uint32_t o_t = tbase + kColO + h * kBN, p_t = tbase + h * kBN;
       const uint32_t v_lo = v_lo0 + ((h * kTile) >> 4);
-      if (!mbar_wait(B.v_full + h, phase, a.err, 44)) return;
-      if (!mbar_wait(B.p_lo + h, phase, a.err, 45)) return;
+      if (!mbar_wait(B.v_full + h, phase, a.err, 44)) return false;
+      if (!mbar_wait(B.p_lo + h, phase, a.err, 45)) return false;
       tc_fence_after();
       issue_pv_f16<0>(o_t, p_t, v_lo, j > 1);
-      if (!mbar_wait(B.p_full + h, phase, a.err, 46)) return;
+      if (!mbar_wait(B.p_full + h, phase, a.err, 46)) return false;
       tc_fence_after();
       issue_pv_f16<1>(o_t, p_t, v_lo, true);
       umma_commit(B.v_empty + h);
       if (j + 2 < J.n_kv) {
-        if (!mbar_wait(B.k_full + h, ((j + 2) / kStages) & 1, a.err, 43)) return;
+        if (!mbar_wait(B.k_full + h, ((j + 2) / kStages) & 1, a.err, 43)) return false;
         tc_fence_after();
         issue_s_f16(p_t, q_lo[h], k_lo0 + ((h * kTile) >> 4));
         umma_commit(B.s_full + h);
@@ -209,10 +219,10 @@ __device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint
     }
     umma_commit(B.o_final);
     umma_commit(B.o_final + 1);
-    return;
+    return true;
   }
   // every phase of the stage barriers is waited for, used or not
-  if (!mbar_wait(B.k_full, 0, a.err, 43)) return;
+  if (!mbar_wait(B.k_full, 0, a.err, 43)) return false;
   tc_fence_after();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -225,22 +235,22 @@ __device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint
     const bool more = j + 1 < J.n_kv;
     const int p = J.page0 + 2 * j;
     const int stv = j % kStages, stk = (j + 1) % kStages;
-    if (!mbar_wait(B.v_full + stv, (j / kStages) & 1, a.err, 44)) return;
+    if (!mbar_wait(B.v_full + stv, (j / kStages) & 1, a.err, 44)) return false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (uses(J, h, p)) {
         const uint32_t o_t = tbase + kColO + h * kBN, p_t = tbase + h * kBN;
         const uint32_t v_lo = v_lo0 + ((stv * kTile) >> 4);
-        if (!mbar_wait(B.p_lo + h, cp[h] & 1, a.err, 45)) return;
+        if (!mbar_wait(B.p_lo + h, cp[h] & 1, a.err, 45)) return false;
         tc_fence_after();
         issue_pv_f16<0>(o_t, p_t, v_lo, cp[h] > 0);
-        if (!mbar_wait(B.p_full + h, cp[h] & 1, a.err, 46)) return;
+        if (!mbar_wait(B.p_full + h, cp[h] & 1, a.err, 46)) return false;
         tc_fence_after();
         issue_pv_f16<1>(o_t, p_t, v_lo, true);
         ++cp[h];
       }
       if (!more) continue;
-      if (h == 0 && !mbar_wait(B.k_full + stk, ((j + 1) / kStages) & 1, a.err, 43)) return;
+      if (h == 0 && !mbar_wait(B.k_full + stk, ((j + 1) / kStages) & 1, a.err, 43)) return false;
       if (uses(J, h, p + 2)) {
         tc_fence_after();
         issue_s_f16(tbase + h * kBN, q_lo[h], k_lo0 + ((stk * kTile) >> 4));
@@ -253,6 +263,7 @@ __device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (cp[h] > 0) umma_commit(B.o_final + h);
+  return true;
 }
 
 // A page's 128 lines of 64 codes (keys: 64 of each dimension half; values: one
@@ -442,14 +453,14 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
   if (J.n_kv > 0) {
     uint4 qv[16];
     uint8_t* q_tile = smem + kSmemQ + (J.dual ? 0 : h * kTile);
-    read_queries(a, in_row && J.tl.b < a.n ? grow * a.q_stride + head * 128 : -1, q_tile, row & ~31,
+    read_queries(a, in_row ? grow * a.q_stride + head * 128 : -1, q_tile, row & ~31,
                  lane_id(), qv);
     named_barrier(1, 256);  // every row is in registers: the tile may be written
     const float sc = stage_queries(a, qv, q_tile, row & ~31, lane_id());
     fence_proxy_async_smem();
     mbar_arrive(B.q_full);
     int lo = 0, hi = 0;
-    if (in_row && J.tl.b < a.n) row_keys(a, J.tl.rq, qi, lo, hi);
+    if (in_row) row_keys(a, J.tl.rq, qi, lo, hi);
     // tiles that every row of the half sees whole need no mask
     int all_lo, all_hi, unused;
     {
@@ -592,7 +603,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
   const int64_t at = whole ? 0 : ((int64_t)blockIdx.x * kRows + (rho - J.tl.rho0));
   if (in_row) {
     if (whole) {
-      if (a.lse) a.lse[grow * a.heads + head] = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
+      if (a.lse) a.lse[grow * a.heads + head] = row_lse(m_run, l_run);
     } else {
       *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_run, l_run);
     }
@@ -657,9 +668,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   B.p_full = B.s_full + 2;
   B.p_lo = B.p_full + 2;
   B.o_final = B.p_lo + 2;
+  B.drained = B.o_final + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
   if (threadIdx.x == 0) {
     mbar_init(B.q_full, 256);
+    mbar_init(B.drained, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(B.k_full + s, 128);
       mbar_init(B.k_empty + s, 1);
@@ -684,9 +697,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   Job J;
   J.kvh = unit % a.kv_heads;
   J.tl = paged8_tile<kRows>(a, tile, threadIdx.x == 0 && split == 0 && J.kvh == 0);
-  if (!J.tl.live) return;
-  const bool tail = J.tl.b == a.n;
-  if (tail ? !a.zero_tail : J.tl.pairs <= a.row_limit) return;
+  const bool rest = a.zero_rest && split == 0 && (warp & ~1) == 2;  // warps 2 and 3
+  const int64_t rest0 = 2 * (int64_t)(unit / a.kv_heads) + (warp & 1);
+  if (!J.tl.live || J.tl.pairs <= a.row_limit) {
+    if (rest) zero_rest(a, J.kvh, rest0, 2 * tiles, lane);
+    return;
+  }
   const int kv_all = (J.tl.np + 1) / 2;
   const int parts = parts_of<kPaged8LargeMin>(kv_all, a.splits);
   if (split >= parts) return;
@@ -696,13 +712,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   J.page_end = min(J.tl.p0 + J.tl.np, J.tl.p0 + 2 * t1);
   J.dual = J.tl.pairs - J.tl.rho0 <= 128;
   J.raw_stages = J.dual ? 2 : 1;
-  J.row = tail ? a.table : a.table + J.tl.b * a.table_stride;
+  J.row = a.table + J.tl.b * a.table_stride;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int first = J.tl.rho0 + 128 * h, last = min(first + 128, J.tl.pairs) - 1;
     J.lo[h] = J.hi[h] = 0;
     int unused;
-    if (first <= last && !tail) {
+    if (first <= last) {
       row_keys(a, J.tl.rq, first / a.group, J.lo[h], unused);
       row_keys(a, J.tl.rq, last / a.group, unused, J.hi[h]);
       if (J.hi[h] <= J.lo[h]) J.lo[h] = J.hi[h] = 0;
@@ -723,8 +739,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     if (J.n_kv > 0 && lane == 0) {
       if (warp == 0) load_role(a, J, smem, B);
-      if (warp == 1) mma_role(a, J, tbase, smem, B);
+      if (warp == 1 && !mma_role(a, J, tbase, smem, B)) {
+        umma_commit(B.drained);
+        mbar_wait(B.drained, 0, a.err, 51);
+      }
     }
+    if (rest) zero_rest(a, J.kvh, rest0, 2 * tiles, lane);
   }
   tc_fence_before();
   __syncthreads();

@@ -4,9 +4,10 @@
 // out[r, h] = sum_j softmax_j(scale q[r, h] . (sk K8[j])) sv V8[j] over the keys
 // that row r sees.  A tile is `kRows` consecutive (row, head of the key head's
 // group) pairs of one request, row-major: rho = row * G + g.  Tile t of request
-// b is number q_start[b] * G / kRows + b + t, so a launch needs no count from
-// the device; numbers between the requests' tiles are empty.  The rows behind
-// the last request are tiles of the "request" n.
+// b is number q_start[b] * G / kRows + min(b, q_start[b]) + t, so a launch needs
+// no count from the device; numbers between the requests' tiles are empty.
+// (Before a request with rows there are at most that many others with rows, so
+// requests without any take no numbers.)
 //
 // The page scales never touch the codes: a page's key scale multiplies its
 // scores, and its value scale 2^ve is added to their exponents, so that with
@@ -41,7 +42,7 @@ struct Paged8Args {
   __nv_bfloat16* out;
   int64_t out_stride;
   float* lse;       // [rows][heads] log2-sum-exp, or NULL
-  int zero_tail;    // write zeros to the rows behind the last request
+  int zero_rest;    // write zeros to the rows of no request
   Divisor splits;   // most parts a tile's keys are cut into
   float* part_o;    // [tile][kv head][split][kRows][128]
   float* part_ml;   // [tile][kv head][split][kRows][2]
@@ -59,7 +60,7 @@ constexpr int kPaged8LargeMin = 8;  // 128-key tiles of a part at least
 
 template <int kRows>
 __host__ __device__ inline int64_t paged8_tiles(int64_t rows, int group, int n) {
-  return rows * group / kRows + n + 1;
+  return rows * group / kRows + (n < rows ? n : rows) + 1;
 }
 
 struct Paged8Tile {
@@ -109,38 +110,52 @@ __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t t
   if (a.n < 32) {  // one read of everything
     const int lane = threadIdx.x & 31, i = min(lane, a.n);
     const int q = qs[i], len = a.n ? a.lengths[min(lane, a.n - 1)] : 0;
-    const unsigned le = __ballot_sync(0xffffffffu, lane <= a.n && q * G / kRows + lane <= tile);
+    const unsigned le =
+        __ballot_sync(0xffffffffu, lane <= a.n && q * G / kRows + min(lane, q) <= tile);
     t.b = 31 - __clz(le | 1u);
     row0 = __shfl_sync(0xffffffffu, q, t.b);
     row1 = __shfl_sync(0xffffffffu, q, min(t.b + 1, 31));
     held = __shfl_sync(0xffffffffu, len, t.b);
   } else {
-    t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + i; });
+    t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + min(i, qs[i]); });
     row0 = qs[t.b];
     row1 = t.b < a.n ? qs[t.b + 1] : 0;
     held = t.b < a.n ? a.lengths[t.b] : 0;
   }
-  const int64_t first = row0 * G / kRows + t.b;
-  if (tile < first) return t;
+  const int64_t first = row0 * G / kRows + min(t.b, row0);
+  if (tile < first || t.b == a.n) return t;  // rows of no request
   const int64_t rho0 = (tile - first) * kRows;
-  if (t.b == a.n) {  // rows behind the last request
-    t.rq.row0 = row0;
-    t.rq.n = a.rows - t.rq.row0;
-    t.rq.held = 0;
-    t.rq.ok = t.rq.row0 >= 0 && t.rq.n > 0;
-    if (!t.rq.ok || rho0 >= t.rq.n * G) return t;
-  } else {
-    t.rq = paged8_request(row0, row1, held, a.rows, a.width, false, report ? a.status : nullptr);
-    if (t.rq.row0 < 0 || t.rq.n <= 0 || t.rq.row0 + (int64_t)t.rq.n > a.rows ||
-        rho0 >= t.rq.n * G)
-      return t;
-    if (!t.rq.ok) t.rq.held = 0;  // a length outside the table: the rows see nothing
-  }
+  t.rq = paged8_request(row0, row1, held, a.rows, a.width, false, report ? a.status : nullptr);
+  if (t.rq.row0 < 0 || t.rq.n <= 0 || t.rq.row0 + (int64_t)t.rq.n > a.rows || rho0 >= t.rq.n * G)
+    return t;
+  if (!t.rq.ok) t.rq.held = 0;  // a length outside the table: the rows see nothing
   t.live = true;
   t.rho0 = (int)rho0;
   t.pairs = (int)(t.rq.n * G);
-  if (t.b < a.n) paged8_span(a, t, kRows);
+  paged8_span(a, t, kRows);
   return t;
+}
+
+// Zeros to the rows before the first request and behind the last one, a warp's
+// heads of key head kvh; worker i of n takes every n-th row.
+__device__ __forceinline__ void zero_rest(const Paged8Args& a, int kvh, int64_t i, int64_t n, int lane) {
+  const int first = a.q_start[0], end = a.q_start[a.n];
+  if (first < 0 || end < first) return;
+  const int64_t rest = (int64_t)a.rows - (end - first);
+  for (int64_t j = i; j < rest; j += n) {
+    const int64_t r = j < first ? j : j + (end - first);
+    if (r >= a.rows) return;
+    uint4* dst = reinterpret_cast<uint4*>(a.out + r * a.out_stride + kvh * a.group.d * 128);
+    for (int e = lane; e < a.group.d * 16; e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
+    if (a.lse)
+      for (int e = lane; e < a.group.d; e += 32) a.lse[r * a.heads + kvh * a.group.d + e] = -INFINITY;
+  }
+}
+
+// log2-sum-exp of a pair from its maximum and sum: -inf where nothing was seen,
+// NaN where the sum is
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
 }
 
 // parts that np pages are really cut into: at least kMin pages each

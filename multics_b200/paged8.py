@@ -128,11 +128,14 @@ class Paged8Cache:
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale, status=None) -> "Paged8Cache":
         """A cache over tensors in the layout above (finite codes, power-of-two
-        scales).  Without ``status`` (int32 ``[1]``, zero) the caches made this
-        way share one word per device."""
+        scales, in ``[2^-126, 2^126]``).  Without ``status`` (int32 ``[1]``, zero)
+        the caches made this way share one word per device; one made while a
+        graph is captured has a word of that graph."""
         if k.dtype not in _FORMATS or v.dtype != k.dtype:
             raise ValueError(f"codes must both be int8 or float8_e4m3fn, got {k.dtype}, {v.dtype}")
         pool = k.shape[:2]
+        if k.dim() == 5 and 0 in pool:
+            raise ValueError(f"k {tuple(k.shape)} has no pages or no heads")
         if k.dim() != 5 or k.shape[2:] != (2, PAGE_TOKENS, 64):
             raise ValueError(f"k must be [pages, heads, 2, 64, 64], got {tuple(k.shape)}")
         if v.shape != (*pool, HEAD_DIM, PAGE_TOKENS):
@@ -150,7 +153,9 @@ class Paged8Cache:
         if status is None:
             status = _STATUS.get(dev)
             if status is None:
-                status = _STATUS[dev] = torch.zeros(1, dtype=_I32, device=dev)
+                status = torch.zeros(1, dtype=_I32, device=dev)
+                if dev.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+                    _STATUS[dev] = status
         else:
             _vector("status", status, 1, dev)
         self = cls.__new__(cls)
@@ -294,9 +299,10 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
     ``block_frames`` frames is not after ``p``'s (``block_frames=0``: always, as
     in a cross-attention) and, with a ``window``, when it is less than
     ``window`` frames back: ``cached_frame_mask`` over token positions.
-    Rows that see nothing are 0.  Rows behind the last request are zeros, or
-    left as they were in a given ``out``.  ``max_rows``: the most rows any
-    request has, where the caller knows it; it chooses kernels, not results.
+    Rows that see nothing are 0.  Rows of no request (before the first, behind
+    the last) are zeros, or left as they were in a given ``out``, which may be
+    ``q`` itself.  ``max_rows``: the most rows any request has, where the caller
+    knows it; it chooses kernels, not results.
     Returns ``[T, num_heads * 128]`` bf16, with ``return_lse`` also the float32
     ``[T, num_heads]`` log2-sum-exp of the scaled scores."""
     if num_heads < 1 or num_heads % cache.num_heads:

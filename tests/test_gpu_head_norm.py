@@ -326,3 +326,24 @@ def test_paged_forward_steps(head_norm, cam):
     with pytest.raises(ValueError, match="rows"):
         layer.paged_forward(x[:, 1:], freqs, cache, table, st)
     del layer.o.forward
+
+
+@pytest.mark.parametrize("H,Hk,D", [(5, 1, 64), (3, 1, 128)])
+def test_gradients_without_eps(H, Hk, D):
+    """Lanes that no head fills add nothing to the weights' gradients."""
+    x = _inputs(9, H, Hk, D, 13, 3)
+    ref, leaf = {}, {}
+    for n in ("q", "k", "wq", "wk"):
+        ref[n] = x[n].double().requires_grad_()
+        leaf[n] = x[n].cuda().requires_grad_()
+    q, k = head_norm_rope_grad(leaf["q"], leaf["k"], x["table"].cuda(), H, Hk, q_weight=leaf["wq"],
+                               k_weight=leaf["wk"], positions=x["pos"].cuda(), eps=0.0)
+    torch.autograd.backward((q, k), (x["gq"].cuda(), x["gk"].cuda()))
+    torch.autograd.backward((P.head_norm(ref["q"], ref["wq"], x["table"], x["pos"], H, eps=0.0),
+                             P.head_norm(ref["k"], ref["wk"], x["table"], x["pos"], Hk, eps=0.0)),
+                            (x["gq"].double(), x["gk"].double()))
+    for n in leaf:
+        # one bf16 rounding, and fp32 sums of terms no larger than the largest gradient times their number
+        top = ref[n].grad.abs().max()
+        err = (leaf[n].grad.cpu().double() - ref[n].grad).abs()
+        assert (err <= ref[n].grad.abs() * 2.0 ** -8 + top * 2.0 ** -14).all(), n

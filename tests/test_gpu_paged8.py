@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import paged8_oracle as P
+from multics_b200 import paged8
 from multics_b200.attention import device_error
 from multics_b200.paged8 import Paged8Cache, page_step, paged8_append, paged8_attention
 
@@ -445,6 +446,71 @@ def test_attention_query_not_finite_stays_in_its_row(counts):
     assert torch.equal(out[1:-1], clean[1:-1])
 
 
+@pytest.mark.parametrize("counts", [[1], [40], [300]])
+def test_attention_query_not_finite_has_no_log_sum(counts):
+    lengths = [400]
+    c, table, g = _filled(lengths, 1, torch.int8)
+    q = torch.randn(counts[0], 256, generator=g).to(BF)
+    args = (c, _i32(table), _i32(lengths), _i32([0] + counts), 2)
+    _, clean = paged8_attention(q.cuda(), *args, return_lse=True)
+    q[0, 3] = float("nan")
+    _, lse = paged8_attention(q.cuda(), *args, return_lse=True)
+    assert lse[0, 0].isnan()
+    assert torch.equal(lse.flatten()[1:], clean.flatten()[1:])
+
+
+@pytest.mark.parametrize("counts", [[3, 2], [9, 300], [200, 5, 300], [300, 5], [1, 1, 1]])
+@pytest.mark.parametrize("width", [9, 40])
+def test_attention_rows_before_the_first_request(counts, width):
+    """The last requests of a batch by themselves, in its rows: those of the
+    others are zeros, or left."""
+    lengths = [300, 520, 400][:len(counts)]
+    c, table, g = _filled(lengths, 2, torch.int8, width=width)
+    ends = [0]
+    for n in counts:
+        ends.append(ends[-1] + n)
+    T, first = ends[-1] + 3, counts[0]
+    q = torch.randn(T, 512, generator=g).to(BF).cuda()
+    args = (c, _i32(table[1:]), _i32(lengths[1:]), _i32(ends[1:]), 4)
+    out, lse = paged8_attention(q, *args, return_lse=True)
+    want, want_lse = paged8_attention(q[first:].contiguous(), c, _i32(table[1:]), _i32(lengths[1:]),
+                                      _i32([e - first for e in ends[1:]]), 4, return_lse=True)
+    # (which parts are joined may differ: a rounding of the output)
+    tol = 2.0 ** -7 * want.float().abs() + 2.0 ** -9 * want.float().abs().max()
+    assert ((out[first:].float() - want.float()).abs() <= tol).all()
+    assert torch.allclose(lse[first:-3], want_lse[:-3], rtol=0, atol=2.0 ** -9)
+    for rows in (slice(0, first), slice(T - 3, T)):
+        assert (out[rows] == 0).all() and (lse[rows] == float("-inf")).all()
+    given = torch.full_like(q, 7.0)
+    paged8_attention(q, *args, out=given)
+    assert torch.equal(given[first:-3], out[first:-3])
+    assert (given[:first] == 7).all() and (given[-3:] == 7).all()
+    c.check()
+
+
+@pytest.mark.parametrize("lengths,counts", [([100], [1]), ([3000], [1]), ([3000, 900], [5, 2]),
+                                            ([2500] * 30, [1] * 30), ([300], [300]), ([900, 500], [100, 3])])
+def test_attention_over_its_queries(lengths, counts):
+    c, table, g = _filled(lengths, 2, torch.float8_e4m3fn)
+    q = torch.randn(sum(counts) + 2, 512, generator=g).to(BF).cuda()
+    starts = torch.cumsum(torch.tensor([0] + counts), 0)
+    args = (c, _i32(table), _i32(lengths), _i32(starts.tolist()), 4)
+    want, tail = paged8_attention(q, *args), q[-2:].clone()
+    assert paged8_attention(q, *args, out=q) is q
+    assert torch.equal(q[:-2], want[:-2]) and torch.equal(q[-2:], tail)
+
+
+def test_attention_few_requests_with_rows_among_many():
+    """Requests without rows, before, between and behind those with some."""
+    lengths, counts = [0] * 3000, [0] * 3000
+    for b, held, n in ((7, 2400, 1), (8, 2300, 3), (1500, 700, 40), (2990, 90, 2)):
+        lengths[b], counts[b] = held, n
+    lengths[1501] = 130
+    for heads in (2, 16):
+        c, table, g = _filled(lengths, 1, torch.int8)
+        _check(c, table, lengths, counts, heads, g, spare=4)
+
+
 def test_attention_strided_rows_given_out_and_tail():
     lengths, counts = [90, 200], [2, 100]
     c, table, g = _filled(lengths, 2, torch.int8)
@@ -623,3 +689,33 @@ def test_captured_step_replays():
     st.check()
     assert s.lengths.tolist() == ref.lengths.tolist()
     assert torch.equal(s.cache.k, ref.cache.k) and torch.equal(s.cache.v, ref.cache.v)
+
+
+def test_cache_made_while_a_graph_is_captured():
+    """Its status word is the graph's own: later caches keep theirs."""
+    lengths = [70]
+    c, table, g = _filled(lengths, 1, torch.int8)
+    q = torch.randn(1, 128, generator=g).to(BF).cuda()
+    t, n, s = _i32(table), _i32(lengths), _i32([0, 1])
+    want = paged8_attention(q, c, t, n, s, 1)
+    made, words = [], dict(paged8._STATUS)
+    paged8._STATUS.clear()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            inner = Paged8Cache.from_tensors(c.k, c.v, c.k_scale, c.v_scale)
+            made.append(paged8_attention(q, inner, t, n, s, 1))
+        outer = Paged8Cache.from_tensors(c.k, c.v, c.k_scale, c.v_scale)
+        assert outer.status.data_ptr() != inner.status.data_ptr()
+        t[0, 0] = -1
+        graph.replay()
+        torch.cuda.synchronize()
+        outer.check()
+        with pytest.raises(ValueError, match="page pool"):
+            inner.check()
+        t.copy_(_i32(table))
+        graph.replay()
+        assert torch.equal(made[0], want)
+        inner.check()
+    finally:
+        paged8._STATUS.update(words)

@@ -136,6 +136,35 @@ def test_entry_points_refuse_before_any_device_work():
         _lib.check(L.hier_head_norm_rope_bwd_partials(1, 1, 1, 96, ctypes.byref(n)))
 
 
+def test_a_pool_has_pages_and_heads():
+    """An entry of no page is read as page 0's scales: there must be one."""
+    for pages, heads in ((0, 2), (2, 0)):
+        z = torch.zeros(pages, heads)
+        with pytest.raises(ValueError, match="no pages or no heads"):
+            Paged8Cache.from_tensors(torch.zeros(pages, heads, 2, 64, 64, dtype=torch.int8),
+                                     torch.zeros(pages, heads, 128, 64, dtype=torch.int8), z, z)
+    L = _lib.lib()
+    with pytest.raises(ValueError):
+        _lib.check(L.hier_paged8_attn(None, 256, 1, 2, 2, 128, 0, None, None, None, None, 0, None, 1, 1,
+                                      None, None, 1, 1, 1, -1, 0.1, 0, None, 256, None, 1, None, None,
+                                      None, None))
+    with pytest.raises(ValueError):
+        _lib.check(L.hier_paged8_append(None, 256, None, 256, 1, 2, 0, None, None, None, None, 0, None,
+                                        1, 1, None, None, 1, None, None))
+
+
+@pytest.mark.parametrize("requests", [1, 30, 3000, 200000])
+def test_workspace_follows_the_rows_not_the_requests(requests):
+    """At most 300 large tiles of 256 rows or 2^14 small ones of 8, of 130 floats."""
+    for rows in (1, 10, 5000):
+        for heads, kv in ((1, 1), (24, 4), (64, 8)):
+            for width in (4, 150, 5000):
+                floats = ctypes.c_int64(-1)
+                _lib.check(_lib.lib().hier_paged8_attn_workspace(rows, heads, kv, requests, width, 0,
+                                                                 ctypes.byref(floats)))
+                assert 0 <= floats.value <= 130 * (300 * 256 + (1 << 14) * 8)
+
+
 @pytest.mark.parametrize("dtype", list(P.TOP))
 def test_scale_is_the_least_power_of_two(dtype):
     for amax in (1e-38, 2.0 ** -20, 0.1, 1.0, 126.9, 127.0, 127.5, 448.0, 449.0, 3e38):
