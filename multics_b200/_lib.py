@@ -247,6 +247,26 @@ def lib():
     return _LIB
 
 
+_CALLS = None
+
+
+def calls():
+    """The module that calls the library's small entry points without ctypes'
+    cost per argument (``csrc/calls.c``), bound to the loaded library."""
+    global _CALLS
+    if _CALLS is None:
+        try:
+            from . import _calls
+        except ImportError as e:
+            raise RuntimeError("the calls module is not built; run `python -m multics_b200.build`") from e
+        h = lib()
+        for name in dir(_calls):
+            if name in _SIGS:
+                _calls.bind(name, ctypes.cast(getattr(h, name), c_void_p).value)
+        _CALLS = _calls
+    return _CALLS
+
+
 def declared_symbols():
     """Function names declared in include/hier_b200.h."""
     text = HEADER.read_text()

@@ -202,8 +202,7 @@ def head_norm_launch(args, num_heads, num_kv_heads, eps, out=None, q_rows=None, 
         with torch.cuda.device(dev):
             return head_norm_launch(args, num_heads, num_kv_heads, eps, out, q_rows, k_rows)
     if out is None:
-        q_out = torch.empty((T, num_heads * D), dtype=torch.bfloat16, device=dev)
-        k_out = torch.empty((T, num_kv_heads * D), dtype=torch.bfloat16, device=dev)
+        q_out, k_out = q2.new_empty((T, num_heads * D)), k2.new_empty((T, num_kv_heads * D))
     else:
         q_out, k_out = out
         for name, t, w, m in (("q_out", q_out, num_heads * D, q_rows),
@@ -212,7 +211,7 @@ def head_norm_launch(args, num_heads, num_kv_heads, eps, out=None, q_rows=None, 
                     or t.stride(1) != 1 or (m is None and t.shape[0] < T):
                 raise ValueError(f"{name} must be bf16 [{T}, {w}] rows on {dev}, got {t.dtype} "
                                  f"{tuple(t.shape)}")
-    rc = _lib.lib().hier_head_norm_rope(
+    rc = _lib.calls().hier_head_norm_rope(
         q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, num_heads, num_kv_heads, D,
         wq.data_ptr(), wk.data_ptr(), wq.dtype is torch.float32, ft.data_ptr(), ft.shape[0],
         None if pos is None else pos.data_ptr(), eps, q_out.data_ptr(), q_out.stride(0),

@@ -1,4 +1,5 @@
-"""Build libhier_b200.so (all CUDA sources of the package) for sm_100a.
+"""Build libhier_b200.so (all CUDA sources of the package) for sm_100a, and the
+module that calls its small entry points from Python.
 
 The library is built in-tree next to this file so that it travels with the
 repository to the GPU machine.  ``python -m multics_b200.build`` rebuilds it;
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -20,6 +22,7 @@ LIB = PKG / "libhier_b200.so"
 SOURCES = ["hier_capi.cu", "hier_meta.cu", "hier_prep.cu", "hier_attn.cu", "hier_selftest.cu",
            "hier_cached.cu", "hier_tiled.cu", "hier_shard.cu", "hier_bwd.cu", "hier_head_norm.cu",
            "hier_paged8.cu", "hier_paged8_attn.cu", "hier_paged8_mma.cu"]
+CALLS = PKG / "_calls.abi3.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -28,7 +31,25 @@ def nvcc() -> str:
     return cand
 
 
+def build_calls(force: bool = False) -> Path:
+    """The Python module of csrc/calls.c (plain C, stable ABI)."""
+    src, header = CSRC / "calls.c", ROOT / "include" / "hier_b200.h"
+    if CALLS.exists() and not force:
+        if CALLS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+            return CALLS
+    tmp = CALLS.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CC") or "gcc", "-O2", "-Wall", "-shared", "-fPIC", "-I", str(ROOT / "include"),
+           "-I", sysconfig.get_paths()["include"], "-o", str(tmp), str(src)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"{cmd[0]} failed building {CALLS.name}")
+    os.replace(tmp, CALLS)
+    return CALLS
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
+    build_calls(force)
     srcs = [CSRC / s for s in SOURCES if (CSRC / s).exists()]
     deps = srcs + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + [ROOT / "include" / "hier_b200.h"]
     if LIB.exists() and not force:

@@ -303,6 +303,9 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Until the kernel before this one is done, where it was launched beside it.
+__device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <int FMT>
 __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args a) {
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
@@ -314,6 +317,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
   const int unit = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - unit * a.splits.d;
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const int b = tile / a.direct, first = tile % a.direct * kRows;
+  if (b >= a.n) return wait_for_prior();
   if (a.zero_rest && split == 0)
     zero_rest(a, kvh, (int64_t)tile * kWarps + w, (int64_t)a.n * a.direct * kWarps, lane);
   // Tiles beyond those the launch counted on (a request of more rows than
@@ -532,6 +536,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
   __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  if ((int)blockIdx.x * kWarps >= units) return wait_for_prior();
   const int unit = blockIdx.x * kWarps + w;
   if (unit >= units) return;
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
@@ -572,7 +577,9 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args
 
 // The parts of a tile's keys joined in split order; one warp per (row, head)
 // pair.  The large kernel numbers its tiles from the last and counts its parts
-// in 128-key tiles.  Launched to overlap the end of the attention kernel.
+// in 128-key tiles.  Launched to overlap the end of the kernel before it (an
+// attention kernel, or the other merge), which is done after every kernel
+// before it is.
 template <int kTileRows>
 __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t tiles) {
   constexpr bool kLarge = kTileRows == kPaged8LargeRows;
@@ -583,8 +590,7 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const Paged8Tile tl = kLarge ? paged8_tile<kTileRows>(a, tiles - 1 - tile, false)
                                : small_tile(a, tile / a.direct, tile % a.direct * kRows, false);
-  // every block waits: what follows this kernel on the stream needs the attention done
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_prior();
   if (!tl.live || (kLarge && tl.pairs <= a.row_limit)) return;
   const int parts = kLarge ? parts_of<kPaged8LargeMin>((tl.np + 1) / 2, a.splits)
                            : parts_of<kMinPages>(tl.np, a.splits);
@@ -704,29 +710,40 @@ int launch_merge(const Paged8Args& a, int64_t tiles, cudaStream_t st) {
   return HIER_OK;
 }
 
-int launch_small(const Paged8Args& a, int format, int64_t tiles, cudaStream_t st) {
+// beside: on the stream after the large kernel, without waiting for it (its
+// requests are others, and its blocks leave SMs idle: few of them, or the last
+// wave's).  The blocks of one unit more do wait for it, so that what follows on
+// the stream finds both done.
+int launch_small(const Paged8Args& a, int format, int64_t tiles, bool beside, cudaStream_t st) {
   const int64_t units = tiles * a.kv_heads * a.splits;
-  if (units > INT32_MAX - kWarps) {
+  if (units > INT32_MAX - 2 * kWarps * a.splits) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
   }
+  cudaLaunchAttribute attrs[2] = {};
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = st;
+  cfg.attrs = attrs;
+  if (beside) {
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
   if (a.width <= kShortPages) {
     auto* kernel = format == P8_INT8 ? paged8_short_kernel<P8_INT8> : paged8_short_kernel<P8_E4M3>;
-    kernel<<<(unsigned)((units + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(a, (int)units);
-    HIER_CHECK_CUDA(cudaGetLastError(), "paged8_short_kernel launch");
+    cfg.gridDim = dim3((unsigned)((units + kWarps - 1) / kWarps + beside));
+    HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, (int)units), "paged8_short_kernel launch");
     return HIER_OK;
   }
   auto* kernel = format == P8_INT8 ? paged8_long_kernel<P8_INT8> : paged8_long_kernel<P8_E4M3>;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = a.splits.d;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)units);
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = a.cluster ? 1 : 0;
+  if (a.cluster) {
+    cudaLaunchAttribute& dim = attrs[cfg.numAttrs++];
+    dim.id = cudaLaunchAttributeClusterDimension;
+    dim.val.clusterDim.x = a.splits.d;
+    dim.val.clusterDim.y = dim.val.clusterDim.z = 1;
+  }
+  cfg.gridDim = dim3((unsigned)(units + (beside ? a.splits.d : 0)));
   HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a), "paged8_long_kernel launch");
   return a.splits > 1 && !a.cluster ? launch_merge<kPaged8SmallRows>(a, tiles, st) : HIER_OK;
 }
@@ -835,13 +852,13 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
   // both kernels: one rule for whose a request is; the rows of no request are the
   // small one's where it runs
   a.row_limit = !s.large ? INT32_MAX : s.small ? s.limit : 0;
+  Paged8Args large = a;
   if (s.large) {
-    a.zero_rest = zero_rest && !s.small;
-    a.splits = divisor(s.large_splits);
-    a.part_o = workspace + s.small_floats;
-    a.part_ml = a.part_o + (s.floats - s.small_floats) / 130 * 128;
-    rc = paged8_launch_large(a, format, s.large_tiles, st);
-    if (!rc && a.splits > 1) rc = launch_merge<kPaged8LargeRows>(a, s.large_tiles, st);
+    large.zero_rest = zero_rest && !s.small;
+    large.splits = divisor(s.large_splits);
+    large.part_o = workspace + s.small_floats;
+    large.part_ml = large.part_o + (s.floats - s.small_floats) / 130 * 128;
+    rc = paged8_launch_large(large, format, s.large_tiles, st);
     if (rc) return rc;
   }
   if (s.small) {
@@ -851,7 +868,9 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
     a.cluster = s.cluster;
     a.part_o = workspace;
     a.part_ml = workspace + s.small_floats / 130 * 128;
-    rc = launch_small(a, format, s.small_tiles, st);
+    rc = launch_small(a, format, s.small_tiles, s.large, st);
+    if (rc) return rc;
   }
+  if (s.large && s.large_splits > 1) rc = launch_merge<kPaged8LargeRows>(large, s.large_tiles, st);
   return rc;
 }

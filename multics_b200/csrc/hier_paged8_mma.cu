@@ -140,58 +140,56 @@ __device__ __forceinline__ bool in_pool(const Paged8Args& a, int page) {
   return page >= 0 && page < a.n_pages;
 }
 
-__device__ __forceinline__ void load_role(const Paged8Args& a, const Job& J, uint8_t* smem,
+// Returns how many tiles of keys and of values, in turn, it has asked for.
+__device__ __forceinline__ int load_role(const Paged8Args& a, const Job& J, uint8_t* smem,
                                           const Bars& B) {
-  int pg[2] = {entry(J, J.page0), entry(J, J.page0 + 1)};
-  int issued[2] = {0, 0};  // tiles of keys, of values
+  const int64_t page_bytes = (int64_t)a.kv_heads * kPageHeadBytes;
+  const uint8_t* k = a.k + (int64_t)J.kvh * kPageHeadBytes;
+  const uint8_t* v = a.v + (int64_t)J.kvh * kPageHeadBytes;
+  int pg0 = entry(J, J.page0), pg1 = entry(J, J.page0 + 1);
   for (int j = 0; j < J.n_kv; ++j) {
     const int p = J.page0 + 2 * j;
     const int raw = j % J.raw_stages, raw_phase = ((j / J.raw_stages) - 1) & 1;
-    const int now0 = pg[0], now1 = pg[1];
-    pg[0] = entry(J, p + 2), pg[1] = entry(J, p + 3);
-    const bool have0 = in_pool(a, now0), have1 = in_pool(a, now1);
+    const bool have0 = in_pool(a, pg0), have1 = in_pool(a, pg1);
+    const int64_t at0 = pg0 * page_bytes, at1 = pg1 * page_bytes;
+    pg0 = entry(J, p + 2), pg1 = entry(J, p + 3);
     if (!have0 || (!have1 && p + 1 < J.page_end)) atomicOr(a.status, P8_BAD_PAGE);
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
       uint64_t* full = B.raw_full + 2 * raw + kind;
       if (j >= J.raw_stages && !mbar_wait(B.raw_empty + 2 * raw + kind, raw_phase, a.err, 40 + kind))
-        break;
-      const uint32_t bytes = (have0 + have1) * kPageHeadBytes;
-      if (bytes)
-        mbar_arrive_expect_tx(full, bytes);
-      else
-        mbar_arrive(full);
-      const uint8_t* src = (kind ? a.v : a.k) + (int64_t)J.kvh * kPageHeadBytes;
-      const int64_t page_bytes = (int64_t)a.kv_heads * kPageHeadBytes;
+        return 2 * j + kind;
+      mbar_arrive_expect_tx(full, (have0 + have1) * kPageHeadBytes);
       uint8_t* dst = raw_stage(smem, raw, kind);
-      if (have0) bulk_load(dst, src + now0 * page_bytes, kPageHeadBytes, full);
-      if (have1) bulk_load(dst + kPageHeadBytes, src + now1 * page_bytes, kPageHeadBytes, full);
-      ++issued[kind];
+      if (have0) bulk_load(dst, (kind ? v : k) + at0, kPageHeadBytes, full);
+      if (have1) bulk_load(dst + kPageHeadBytes, (kind ? v : k) + at1, kPageHeadBytes, full);
     }
-    if (issued[1] <= j) break;
   }
-  // no copy outlives the block, whoever else gave up
-#pragma unroll
-  for (int kind = 0; kind < 2; ++kind)
-    for (int j = max(0, issued[kind] - J.raw_stages); j < issued[kind]; ++j)
-      mbar_wait(B.raw_full + 2 * (j % J.raw_stages) + kind, (j / J.raw_stages) & 1, a.err, 52);
+  return 2 * J.n_kv;
 }
 
-// False: a wait ran out, with products perhaps still running.
-__device__ __forceinline__ bool mma_role(const Paged8Args& a, const Job& J, uint32_t tbase,
+// No copy outlives the block, whoever else gave up.
+__device__ __forceinline__ void load_drain(const Paged8Args& a, const Job& J, const Bars& B, int issued) {
+  for (int i = max(0, issued - 2 * J.raw_stages); i < issued; ++i) {
+    const int j = i >> 1;
+    mbar_wait(B.raw_full + 2 * (j % J.raw_stages) + (i & 1), (j / J.raw_stages) & 1, a.err, 52);
+  }
+}
+
+__device__ __forceinline__ void mma_role(const Paged8Args& a, const Job& J, uint32_t tbase,
                                          uint8_t* smem, const Bars& B) {
   const uint32_t q_lo[2] = {sdesc_lo_kmajor(smem_u32(smem + kSmemQ)),
                             sdesc_lo_kmajor(smem_u32(smem + kSmemQ + (J.dual ? 0 : kTile)))};
   const uint32_t k_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemK));
   const uint32_t v_lo0 = sdesc_lo_kmajor(smem_u32(smem + kSmemV));
   int cp[2] = {0, 0};  // PVs issued per half
-  if (!mbar_wait(B.q_full, 0, a.err, 42)) return false;
+  if (!mbar_wait(B.q_full, 0, a.err, 42)) return;
   if (J.dual) {
     // tile j is half j % 2's, and so are the stages it passes through
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (j >= J.n_kv) break;
-      if (!mbar_wait(B.k_full + j, 0, a.err, 43)) return false;
+      if (!mbar_wait(B.k_full + j, 0, a.err, 43)) return;
       tc_fence_after();
       issue_s_f16(tbase + j * kBN, q_lo[j], k_lo0 + ((j * kTile) >> 4));
       umma_commit(B.s_full + j);
@@ -201,16 +199,16 @@ __device__ __forceinline__ bool mma_role(const Paged8Args& a, const Job& J, uint
       const int h = j & 1, phase = (j >> 1) & 1;
       const uint32_t o_t = tbase + kColO + h * kBN, p_t = tbase + h * kBN;
       const uint32_t v_lo = v_lo0 + ((h * kTile) >> 4);
-      if (!mbar_wait(B.v_full + h, phase, a.err, 44)) return false;
-      if (!mbar_wait(B.p_lo + h, phase, a.err, 45)) return false;
+      if (!mbar_wait(B.v_full + h, phase, a.err, 44)) return;
+      if (!mbar_wait(B.p_lo + h, phase, a.err, 45)) return;
       tc_fence_after();
       issue_pv_f16<0>(o_t, p_t, v_lo, j > 1);
-      if (!mbar_wait(B.p_full + h, phase, a.err, 46)) return false;
+      if (!mbar_wait(B.p_full + h, phase, a.err, 46)) return;
       tc_fence_after();
       issue_pv_f16<1>(o_t, p_t, v_lo, true);
       umma_commit(B.v_empty + h);
       if (j + 2 < J.n_kv) {
-        if (!mbar_wait(B.k_full + h, ((j + 2) / kStages) & 1, a.err, 43)) return false;
+        if (!mbar_wait(B.k_full + h, ((j + 2) / kStages) & 1, a.err, 43)) return;
         tc_fence_after();
         issue_s_f16(p_t, q_lo[h], k_lo0 + ((h * kTile) >> 4));
         umma_commit(B.s_full + h);
@@ -219,10 +217,10 @@ __device__ __forceinline__ bool mma_role(const Paged8Args& a, const Job& J, uint
     }
     umma_commit(B.o_final);
     umma_commit(B.o_final + 1);
-    return true;
+    return;
   }
   // every phase of the stage barriers is waited for, used or not
-  if (!mbar_wait(B.k_full, 0, a.err, 43)) return false;
+  if (!mbar_wait(B.k_full, 0, a.err, 43)) return;
   tc_fence_after();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -235,22 +233,22 @@ __device__ __forceinline__ bool mma_role(const Paged8Args& a, const Job& J, uint
     const bool more = j + 1 < J.n_kv;
     const int p = J.page0 + 2 * j;
     const int stv = j % kStages, stk = (j + 1) % kStages;
-    if (!mbar_wait(B.v_full + stv, (j / kStages) & 1, a.err, 44)) return false;
+    if (!mbar_wait(B.v_full + stv, (j / kStages) & 1, a.err, 44)) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (uses(J, h, p)) {
         const uint32_t o_t = tbase + kColO + h * kBN, p_t = tbase + h * kBN;
         const uint32_t v_lo = v_lo0 + ((stv * kTile) >> 4);
-        if (!mbar_wait(B.p_lo + h, cp[h] & 1, a.err, 45)) return false;
+        if (!mbar_wait(B.p_lo + h, cp[h] & 1, a.err, 45)) return;
         tc_fence_after();
         issue_pv_f16<0>(o_t, p_t, v_lo, cp[h] > 0);
-        if (!mbar_wait(B.p_full + h, cp[h] & 1, a.err, 46)) return false;
+        if (!mbar_wait(B.p_full + h, cp[h] & 1, a.err, 46)) return;
         tc_fence_after();
         issue_pv_f16<1>(o_t, p_t, v_lo, true);
         ++cp[h];
       }
       if (!more) continue;
-      if (h == 0 && !mbar_wait(B.k_full + stk, ((j + 1) / kStages) & 1, a.err, 43)) return false;
+      if (h == 0 && !mbar_wait(B.k_full + stk, ((j + 1) / kStages) & 1, a.err, 43)) return;
       if (uses(J, h, p + 2)) {
         tc_fence_after();
         issue_s_f16(tbase + h * kBN, q_lo[h], k_lo0 + ((stk * kTile) >> 4));
@@ -263,7 +261,6 @@ __device__ __forceinline__ bool mma_role(const Paged8Args& a, const Job& J, uint
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (cp[h] > 0) umma_commit(B.o_final + h);
-  return true;
 }
 
 // A page's 128 lines of 64 codes (keys: 64 of each dimension half; values: one
@@ -271,18 +268,20 @@ __device__ __forceinline__ bool mma_role(const Paged8Args& a, const Job& J, uint
 // read two lines of codes (128 bytes) and write two lines of eight different
 // 16-byte columns: no bank conflicts either way.  A thread takes 16 bytes of
 // lines line0, line0 + 32, .. of both pages; pages that are not there are zeros.
-template <int FMT, bool kValues>
-__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, bool have0, bool have1,
-                                             int tid) {
+template <int FMT>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, bool kValues, bool have0,
+                                             bool have1, int tid) {
   const int t = tid & 3, line0 = tid >> 2;
   const uint8_t* src = raw + tid * 16;
   // (the line's swizzle is that of line0: the others are multiples of 8 away)
   uint8_t* lo = dst + line0 * 128 + (((2 * t) ^ (line0 & 7)) << 4);
   uint8_t* hi = dst + line0 * 128 + (((2 * t + 1) ^ (line0 & 7)) << 4);
+  // offsets of the second page's lines and, of a page, of its second 64 lines
+  const int next_page = kValues ? kHalf : 64 * 128, next_half = kValues ? 64 * 128 : kHalf;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int page = i >> 2, line = 32 * (i & 3);  // + line0
-    const int off = kValues ? page * kHalf + line * 128 : (line >> 6) * kHalf + (64 * page + (line & 63)) * 128;
+    const int off = page * next_page + (line >> 6) * next_half + (line & 63) * 128;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (page ? have1 : have0)
       v = *reinterpret_cast<const uint4*>(src + page * kPageHeadBytes + line * 64);
@@ -306,19 +305,17 @@ __device__ __forceinline__ void convert_role(const Paged8Args& a, const Job& J, 
     const int st = j % kStages, raw = j % J.raw_stages, raw_phase = (j / J.raw_stages) & 1;
     const bool have0 = in_pool(a, pg0), have1 = in_pool(a, pg1);
     pg0 = entry(J, J.page0 + 2 * j + 2), pg1 = entry(J, J.page0 + 2 * j + 3);
-    const auto one = [&](auto values) -> bool {
-      constexpr bool kValues = decltype(values)::value;
-      uint64_t* empty = (kValues ? B.v_empty : B.k_empty) + st;
-      if (j >= kStages && !mbar_wait(empty, ((j / kStages) - 1) & 1, a.err, 47)) return false;
-      if (!mbar_wait(B.raw_full + 2 * raw + kValues, raw_phase, a.err, 48)) return false;
-      convert_tile<FMT, kValues>(raw_stage(smem, raw, kValues),
-                                 smem + (kValues ? kSmemV : kSmemK) + st * kTile, have0, have1, tid);
+#pragma unroll 1
+    for (int kind = 0; kind < 2; ++kind) {
+      uint64_t* empty = (kind ? B.v_empty : B.k_empty) + st;
+      if (j >= kStages && !mbar_wait(empty, ((j / kStages) - 1) & 1, a.err, 47)) return;
+      if (!mbar_wait(B.raw_full + 2 * raw + kind, raw_phase, a.err, 48)) return;
+      convert_tile<FMT>(raw_stage(smem, raw, kind), smem + (kind ? kSmemV : kSmemK) + st * kTile, kind,
+                        have0, have1, tid);
       fence_proxy_async_smem();
-      mbar_arrive((kValues ? B.v_full : B.k_full) + st);
-      mbar_arrive(B.raw_empty + 2 * raw + kValues);
-      return true;
-    };
-    if (!one(std::false_type{}) || !one(std::true_type{})) return;
+      mbar_arrive((kind ? B.v_full : B.k_full) + st);
+      mbar_arrive(B.raw_empty + 2 * raw + kind);
+    }
   }
 }
 
@@ -571,7 +568,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
     named_barrier(1, 256);
     if (h == 1) {
       if (!lost) {
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           uint32_t r[32];
           if (c > 0) {
@@ -608,7 +605,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
       *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_run, l_run);
     }
   }
-#pragma unroll
+#pragma unroll 1
   for (int q = 0; q < 4; ++q) {
     uint32_t r[32];
     if (c > 0) {
@@ -738,8 +735,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     if (J.n_kv > 0 && lane == 0) {
-      if (warp == 0) load_role(a, J, smem, B);
-      if (warp == 1 && !mma_role(a, J, tbase, smem, B)) {
+      if (warp == 0) load_drain(a, J, B, load_role(a, J, smem, B));
+      if (warp == 1) {
+        mma_role(a, J, tbase, smem, B);
         umma_commit(B.drained);
         mbar_wait(B.drained, 0, a.err, 51);
       }

@@ -40,6 +40,7 @@ HEAD_DIM = 128
 _I32, _BF16 = torch.int32, torch.bfloat16
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _STATUS = {}
+_SPLIT = torch.unsafe_split_with_sizes  # (integers: no versions to share)
 
 _CACHE_BITS = ((1, "row starts leave the rows or descend"),
                (2, "a length leaves the block table"),
@@ -133,11 +134,12 @@ class Paged8Cache:
         graph is captured has a word of that graph."""
         if k.dtype not in _FORMATS or v.dtype != k.dtype:
             raise ValueError(f"codes must both be int8 or float8_e4m3fn, got {k.dtype}, {v.dtype}")
-        pool = k.shape[:2]
-        if k.dim() == 5 and 0 in pool:
-            raise ValueError(f"k {tuple(k.shape)} has no pages or no heads")
-        if k.dim() != 5 or k.shape[2:] != (2, PAGE_TOKENS, 64):
-            raise ValueError(f"k must be [pages, heads, 2, 64, 64], got {tuple(k.shape)}")
+        shape = k.shape
+        if len(shape) != 5 or shape[2:] != (2, PAGE_TOKENS, 64):
+            raise ValueError(f"k must be [pages, heads, 2, 64, 64], got {tuple(shape)}")
+        pool = shape[:2]
+        if 0 in pool:
+            raise ValueError(f"k {tuple(shape)} has no pages or no heads")
         if v.shape != (*pool, HEAD_DIM, PAGE_TOKENS):
             raise ValueError(f"v must be [pages, heads, 128, 64] like k {tuple(k.shape)}, got "
                              f"{tuple(v.shape)}")
@@ -227,13 +229,13 @@ def page_step(lengths, add, table, free_pages, free_count, rows: int, *,
             return page_step(lengths, add, table, free_pages, free_count, rows, most_new=most_new,
                              in_place=in_place)
     if in_place:
-        q_start, status, slots, positions = torch.empty(
-            n + 2 + 2 * rows, dtype=_I32, device=dev).split((n + 1, 1, rows, rows))
+        q_start, status, slots, positions = _SPLIT(
+            lengths.new_empty(n + 2 + 2 * rows), (n + 1, 1, rows, rows))
         new_len, new_count = lengths, free_count
     else:
-        new_len, new_count, q_start, status, slots, positions = torch.empty(
-            2 * n + 3 + 2 * rows, dtype=_I32, device=dev).split((n, 1, n + 1, 1, rows, rows))
-    rc = _lib.lib().hier_page_step(
+        new_len, new_count, q_start, status, slots, positions = _SPLIT(
+            lengths.new_empty(2 * n + 3 + 2 * rows), (n, 1, n + 1, 1, rows, rows))
+    rc = _lib.calls().hier_page_step(
         lengths.data_ptr(), add.data_ptr(), n, table.data_ptr(), stride, width,
         free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), rows,
         -1 if most_new is None else int(most_new), new_len.data_ptr(), new_count.data_ptr(),
@@ -276,7 +278,7 @@ def paged8_append(cache: Paged8Cache, k, v, table, lengths, q_start):
     if not is_current(dev):
         with torch.cuda.device(dev):
             return paged8_append(cache, k, v, table, lengths, q_start)
-    rc = _lib.lib().hier_paged8_append(
+    rc = _lib.calls().hier_paged8_append(
         k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), k.shape[0], cache.num_heads,
         cache.format, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
         cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
@@ -337,17 +339,17 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
     most = 0 if max_rows is None else int(max_rows)
     lse = ws = None
     if out is None:
-        o = torch.empty((T, dim), dtype=_BF16, device=dev)
+        o = q.new_empty((T, dim))
     elif out.data_ptr() % 16 or out.stride(0) % 8:  # rows the kernels cannot store to
         o = out.clone(memory_format=torch.contiguous_format)
     else:
         o = out
     if return_lse:
-        lse = torch.empty((T, num_heads), dtype=torch.float32, device=dev)
+        lse = cache.k_scale.new_empty((T, num_heads))
     floats = _workspace_floats(T, num_heads, cache.num_heads, n, width, most)
     if floats:
-        ws = torch.empty(floats, dtype=torch.float32, device=dev)
-    rc = _lib.lib().hier_paged8_attn(
+        ws = cache.k_scale.new_empty(floats)
+    rc = _lib.calls().hier_paged8_attn(
         q.data_ptr(), q.stride(0), T, num_heads, cache.num_heads, HEAD_DIM, cache.format,
         cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
         cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,

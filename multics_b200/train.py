@@ -260,12 +260,11 @@ class _HeadNormFn(torch.autograd.Function):
                   else token_rows("gradient of q", gq if gq.dtype is bf else gq.to(bf), H * D))
             gk = (torch.zeros((T, Hk * D), dtype=bf, device=dev) if gk is None
                   else token_rows("gradient of k", gk if gk.dtype is bf else gk.to(bf), Hk * D))
-            dq = torch.empty(q_shape, dtype=bf, device=dev)
-            dk = torch.empty(k_shape, dtype=bf, device=dev)
+            dq, dk = q2.new_empty(q_shape), k2.new_empty(k_shape)
             dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
             blocks = _head_norm_blocks(T, H, Hk, D)
-            part = torch.empty((blocks, D), dtype=torch.float32, device=dev)
-            rc = _lib.lib().hier_head_norm_rope_bwd(
+            part = ft.new_empty((blocks, D))
+            rc = _lib.calls().hier_head_norm_rope_bwd(
                 q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), T, H, Hk, D,
                 wq.data_ptr(), wk.data_ptr(), wq.dtype is torch.float32, ft.data_ptr(),
                 ft.shape[0], None if pos is None else pos.data_ptr(), eps, gq.data_ptr(),

@@ -165,6 +165,27 @@ def test_workspace_follows_the_rows_not_the_requests(requests):
                 assert 0 <= floats.value <= 130 * (300 * 256 + (1 << 14) * 8)
 
 
+def test_calls_module_reads_the_declared_signatures():
+    letters = {ctypes.c_void_p: "p", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+    C = _lib.calls()
+    names = [n for n in dir(C) if n.startswith("hier_")]
+    assert len(names) == 5
+    for n in names:
+        assert getattr(C, n).__doc__ == "".join(letters[t] for t in _lib._SIGS[n][1])
+    args = [None, 256, None, 256, 0, 2, 0, None, None, None, None, 1, None, 1, 1, None, None, 1, None, None]
+    assert C.hier_paged8_append(*args) == 0  # no rows
+    with pytest.raises(ValueError):
+        _lib.check(C.hier_paged8_append(*args[:6], 2, *args[7:]))
+    with pytest.raises(TypeError, match="takes 20 arguments, got 19"):
+        C.hier_paged8_append(*args[1:])
+    with pytest.raises(ValueError, match="32 bits"):
+        C.hier_paged8_append(*args[:4], 1 << 31, *args[5:])
+    with pytest.raises(TypeError):
+        C.hier_paged8_append(1.5, *args[1:])
+    with pytest.raises(ValueError, match="no entry"):
+        C.bind("hier_none", 0)
+
+
 @pytest.mark.parametrize("dtype", list(P.TOP))
 def test_scale_is_the_least_power_of_two(dtype):
     for amax in (1e-38, 2.0 ** -20, 0.1, 1.0, 126.9, 127.0, 127.5, 448.0, 449.0, 3e38):
