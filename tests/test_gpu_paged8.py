@@ -90,6 +90,35 @@ def test_page_step_maps_many_rows():
     assert d[2].tolist() == table
 
 
+@pytest.mark.parametrize("n", [1, 33, 1200, 5000])
+@pytest.mark.parametrize("most", [1, 300])
+def test_page_step_maps_rows_between_requests_without_any(n, most):
+    """Rows of requests that lie far apart, few or hundreds each, mapped by the
+    step itself or by a grid of their own."""
+    r, width = random.Random(n + most), 8
+    lengths = [r.randint(0, 90) for _ in range(n)]
+    add = [0] * n
+    for b in [0, n - 1] + [r.randrange(n) for _ in range(min(n, 60))]:
+        add[b] = r.randint(1, most)
+    if n > 1:
+        add[n // 2] = -lengths[n // 2]
+    table, at = [], 0
+    for x in lengths:
+        p = -(-x // 64)
+        table.append(list(range(at, at + p)) + [-1] * (width - p))
+        at += p
+    free = list(range(at, at + 7 * n))
+    rows = sum(max(x, 0) for x in add) + 70
+    d = [_i32(lengths), _i32(add), _i32(table), _i32(free + [-1] * at), _i32([len(free)])]
+    st = page_step(*d, rows)
+    st.check()
+    after, count, q_start, slots, positions = P.step(lengths, add, table, free + [-1] * at, len(free))
+    assert st.lengths.tolist() == after and st.q_start.tolist() == q_start
+    assert st.slots.tolist() == slots + [-1] * 70
+    assert st.positions.tolist() == positions + [-1] * 70
+    assert d[2].tolist() == table
+
+
 @pytest.mark.parametrize("change,match", [
     (dict(add=[60, 64]), "free pages"), (dict(rows=5), "rows"), (dict(add=[4, 300]), "block table"),
     (dict(add=[-11, 0]), "below -length"), (dict(most=3), "above the step"),
@@ -604,6 +633,29 @@ def test_attention_of_new_data_is_that_of_old(dtype):
         kw = dict(tokens_per_frame=1 + seed % 7, block_frames=seed % 3)
         first, second = (paged8_attention(*args, **kw) for _ in range(2))
         assert torch.equal(first, second), seed
+
+
+@pytest.mark.parametrize("lengths", [[1500] * 20 + [2000, 2600], [100] * 200 + [240, 200, 130],
+                                     [9000, 2000]])
+def test_attention_of_short_and_long_requests_is_done_when_it_returns_to_the_stream(lengths):
+    """Both kernels (and their merges) run beside one another: what follows on
+    the stream changes the cache under neither."""
+    counts = [1 if n in (100, 1500, 9000) else min(n, 500) for n in lengths]
+    c, table, g = _filled(lengths, 2, torch.int8)
+    q = torch.randn(sum(counts), 12 * 128, generator=g).to(BF).cuda()
+    starts = torch.cumsum(torch.tensor([0] + counts), 0).tolist()
+    args = (_i32(table), _i32(lengths), _i32(starts), 12)
+    kept = c.k.clone(), c.v.clone()
+    torch.cuda.synchronize()
+    want = paged8_attention(q, c, *args)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        outs.append(paged8_attention(q, c, *args))
+        c.k.zero_(), c.v.zero_()
+        c.k.copy_(kept[0]), c.v.copy_(kept[1])
+    for out in outs:
+        assert torch.equal(out, want)
 
 
 def test_attention_on_two_streams_at_once():
