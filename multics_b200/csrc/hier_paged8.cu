@@ -301,16 +301,38 @@ __device__ __forceinline__ int scale_exponent(float amax) {
   return max(e, kScaleMin);
 }
 
-// codes of four values already divided by the scale; NaN becomes 0
+// Codes of four numbers within the codes' range after their scale (inv: its
+// inverse, exact), or infinite where `odd`.  int8: 1.5 * 2^23 added to |v| <= 127
+// rounds v to nearest even and leaves it, in two's complement, in the low byte.
 template <int FMT>
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float inv, bool odd) {
   if (FMT == P8_INT8) {
-    const auto q = [](float v) { return (uint32_t)min(127, max(-127, __float2int_rn(v))); };
-    return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410);
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = fmaf(x[i], inv, 12582912.f);
+    if (odd)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = fminf(12582912.f + 127.f, fmaxf(12582912.f - 127.f, f[i]));
+    const auto q = [](float v) { return __float_as_uint(v); };
+    return __byte_perm(__byte_perm(q(f[0]), q(f[1]), 0x0040), __byte_perm(q(f[2]), q(f[3]), 0x0040),
+                       0x5410);
   }
-  const auto z = [](float v) { return v == v ? v : 0.f; };
-  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(z(a), z(b)), __NV_SATFINITE, __NV_E4M3) |
-         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(z(c), z(d)), __NV_SATFINITE, __NV_E4M3) << 16;
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3) |
+         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3)
+             << 16;
+}
+
+// 4 bytes of each of 4 words, transposed
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&c)[4], uint32_t (&w)[4]) {
+  const uint32_t a = __byte_perm(c[0], c[1], 0x5140), b = __byte_perm(c[2], c[3], 0x5140);
+  const uint32_t d = __byte_perm(c[0], c[1], 0x7362), e = __byte_perm(c[2], c[3], 0x7362);
+  w[0] = __byte_perm(a, b, 0x5410), w[1] = __byte_perm(a, b, 0x7632);
+  w[2] = __byte_perm(d, e, 0x5410), w[3] = __byte_perm(d, e, 0x7632);
+}
+
+// the bytes [0, n) of a word
+__device__ __forceinline__ uint32_t low_bytes(int n) {
+  return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
 }
 
 template <int FMT>
@@ -321,8 +343,13 @@ __device__ __forceinline__ float decode1(uint32_t byte) {
 
 template <int FMT>
 __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
-  const auto d = [=](int i) { return decode1<FMT>((w >> (8 * i)) & 0xffu) * ratio; };
-  return encode4<FMT>(d(0), d(1), d(2), d(3));
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // (codes that were never written may be anything)
+    const float v = decode1<FMT>((w >> (8 * i)) & 0xffu);
+    f[i] = v == v ? fmaxf(v, -top_code<FMT>()) : 0.f;
+  }
+  return encode4<FMT>(f, ratio, false);
 }
 
 template <int FMT>
@@ -357,6 +384,14 @@ __device__ __forceinline__ void load_tokens(const AppendItem& it, int t0, uint2 
 // largest finite magnitude; odd: something was not finite
 template <int N>
 __device__ __forceinline__ float largest(const uint2 (&x)[N], bool& odd) {
+  // bf16 magnitudes order like their bits, pairs of them at a time
+  uint32_t big = 0u;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    big = __vmaxu2(big, __vmaxu2(x[j].x & 0x7fff7fffu, x[j].y & 0x7fff7fffu));
+  big = max(big << 16, big & 0xffff0000u);
+  if (big < 0x7f800000u) return __uint_as_float(big);
+  odd = true;
   float amax = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -365,12 +400,21 @@ __device__ __forceinline__ float largest(const uint2 (&x)[N], bool& odd) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float m = fabsf(f[i]);
-      const bool fin = m < INFINITY;
-      odd |= !fin;
-      amax = fmaxf(amax, fin ? m : 0.f);
+      amax = fmaxf(amax, m < INFINITY ? m : 0.f);
     }
   }
   return amax;
+}
+
+// A NaN becomes 0.
+template <int N>
+__device__ __forceinline__ void drop_nan(uint2 (&x)[N]) {
+  const auto word = [](uint32_t w) {
+    return ((w & 0x7fffu) > 0x7f80u ? 0u : w & 0xffffu) |
+           ((w & 0x7fff0000u) > 0x7f800000u ? 0u : w & 0xffff0000u);
+  };
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j].x = word(x[j].x), x[j].y = word(x[j].y);
 }
 
 // the bytes of 16 tokens of the lane's 4 value dimensions
@@ -384,49 +428,40 @@ __device__ __forceinline__ void load_old(const AppendItem& it, int t0, int lane,
 
 template <int FMT, int N>
 __device__ __forceinline__ void store_keys(const AppendItem& it, int t0, int lane, const uint2 (&x)[N],
-                                           float inv, float ratio, bool grown) {
+                                           float inv, bool odd) {
   uint8_t* dst = it.codes + (lane >> 4) * (kPage * 64) + (lane & 15) * 4;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int t = t0 + j;
-    uint32_t* at = reinterpret_cast<uint32_t*>(dst + t * 64);
     if (t >= it.o && t < it.e) {  // uniform over the warp
       float f[4];
       unpack4(x[j], f);
-      *at = encode4<FMT>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-    } else if (grown && t < it.o) {
-      *at = recode4<FMT>(*at, ratio);
+      *reinterpret_cast<uint32_t*>(dst + t * 64) = encode4<FMT>(f, inv, odd);
     }
   }
 }
 
 template <int FMT>
 __device__ __forceinline__ void store_values(const AppendItem& it, int t0, int lane, const uint2 (&x)[16],
-                                             const uint4 (&old)[4], float inv, float ratio, bool grown) {
+                                             const uint4 (&old)[4], float inv, bool odd) {
   uint32_t w[4][4];  // [dimension][4 tokens]
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    // the tokens of the four that were held before take the new scale
-    const int held = min(4, max(0, it.o - (t0 + 4 * q)));
-    const uint32_t hm = held >= 4 ? 0xffffffffu : (1u << (8 * held)) - 1u;
+    uint32_t c[4], t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float f[4];
+      unpack4(x[4 * q + j], f);
+      c[j] = encode4<FMT>(f, inv, odd);
+    }
+    transpose_bytes(c, t);
+    const int at = t0 + 4 * q;
+    const uint32_t fresh = low_bytes(it.e - at) & ~low_bytes(it.o - at);  // the new ones of the four
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint4 v = old[i];
-      uint32_t c = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
-      if (grown && held > 0) c = (recode4<FMT>(c, ratio) & hm) | (c & ~hm);
-      w[i][q] = c;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + 4 * q + j;
-      if (t < it.o || t >= it.e) continue;  // uniform over the warp
-      float f[4];
-      unpack4(x[4 * q + j], f);
-      const uint32_t c = encode4<FMT>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-      // byte i of c to byte j of dimension i
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i][q] = __byte_perm(w[i][q], c, (0x3210 & ~(0xf << (4 * j))) | ((4 + i) << (4 * j)));
+      const uint32_t b = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
+      w[i][q] = (t[i] & fresh) | (b & ~fresh);
     }
   }
 #pragma unroll
@@ -447,9 +482,8 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// page pg of request b, or -1 (reported) when it leaves the pool
-__device__ __forceinline__ int append_page(const AppendArgs& a, int b, int pg, int lane) {
-  const int page = a.table[b * a.table_stride + pg];
+// the page of a table entry, or -1 (reported) when it leaves the pool
+__device__ __forceinline__ int append_page(const AppendArgs& a, int page, int lane) {
   if (page >= 0 && page < a.n_pages) return page;
   if (lane == 0) atomicOr(a.status, P8_BAD_PAGE);
   return -1;
@@ -466,8 +500,38 @@ __device__ __forceinline__ AppendItem append_item(const AppendArgs& a, const Pag
   return it;
 }
 
+// The held codes of an item, of tokens [from, to) (multiples of 16), under a
+// scale that has grown.
 template <int FMT>
-__global__ void __launch_bounds__(128) paged8_append_pages_kernel(AppendArgs a) {
+__device__ __forceinline__ void regrow(const AppendItem& it, int kv, int from, int to, float ratio,
+                                       int lane) {
+  to = min(to, it.o);
+  if (kv) {  // 16 tokens of a dimension at a time; of the last few, the held ones
+    for (int t0 = from; t0 < to; t0 += 16)
+#pragma unroll 1
+      for (int d = lane; d < 128; d += 32) {
+        uint4* p = reinterpret_cast<uint4*>(it.codes + d * kPage + t0);
+        const uint4 v = *p;
+        uint4 w = recode16<FMT>(v, ratio);
+        const auto keep = [&](uint32_t& to, uint32_t from, int q) {
+          const uint32_t held = low_bytes(it.o - (t0 + 4 * q));
+          to = (to & held) | (from & ~held);
+        };
+        keep(w.x, v.x, 0), keep(w.y, v.y, 1), keep(w.z, v.z, 2), keep(w.w, v.w, 3);
+        *p = w;
+      }
+  } else {
+#pragma unroll 1
+    for (int t = from * 8 + lane; t < to * 8; t += 32) {  // 16-byte pieces of the held tokens
+      uint4* p = reinterpret_cast<uint4*>(it.codes + (t & 3) * 16 + (t & 4 ? kPage * 64 : 0) +
+                                          (t >> 3) * 64);
+      *p = recode16<FMT>(*p, ratio);
+    }
+  }
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(128, 8) paged8_append_pages_kernel(AppendArgs a) {
   __shared__ float most[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = blockIdx.x / a.heads, head = blockIdx.x - part * a.heads;
@@ -480,65 +544,41 @@ __global__ void __launch_bounds__(128) paged8_append_pages_kernel(AppendArgs a) 
   if (!rq.ok || rq.n == 0) return;
   const int64_t pg = (rq.held - rq.n) / kPage + vp - ((int64_t)(rq.row0 >> 6) + 2 * (int64_t)b);
   if (pg < 0 || pg * kPage >= rq.held) return;
-  const int page = append_page(a, b, (int)pg, threadIdx.x);
-  if (page < 0) return;
-  const AppendItem it = append_item(a, rq, (int)pg, page, head, kv, lane);
-  float* sp = a.scale[kv] + (int64_t)page * a.heads + head;
-  const float old_scale = it.o > 0 ? *sp : 0.f;
+  const int entry = a.table[b * a.table_stride + pg];
+  AppendItem it = append_item(a, rq, (int)pg, 0, head, kv, lane);
   const int t0 = 16 * warp;  // this warp's tokens
   const bool mine = t0 < it.e && t0 + 16 > it.o;
   uint2 x[16];
-  uint4 old[4];
+  if (mine) load_tokens(it, t0, x);  // in flight before the page is known
+  const int page = append_page(a, entry, threadIdx.x);
+  if (page < 0) return;
+  const int64_t at = (int64_t)page * a.heads;
+  it.codes += at * kPageHeadBytes;
+  float* sp = a.scale[kv] + at + head;
+  const float old_scale = it.o > 0 ? *sp : 0.f;
   float amax = 0.f;
   bool odd = false;
-  if (mine) {
-    load_tokens(it, t0, x);
-    if (kv) load_old(it, t0, lane, old);
-    amax = largest(x, odd);
-  }
+  if (mine) amax = largest(x, odd);
   amax = warp_max(amax);
-  if (odd) atomicOr(a.status, P8_NOT_FINITE);
+  odd = __any_sync(0xffffffffu, odd);
+  if (odd && lane == 0) atomicOr(a.status, P8_NOT_FINITE);
   if (lane == 0) most[warp] = amax;
   __syncthreads();  // every warp has read the old scale
   const float s = item_scale<FMT>(old_scale, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
   const float inv = 1.f / s;  // exact: s is a power of two
-  const bool grown = it.o > 0 && s > old_scale;
-  const float ratio = grown ? old_scale * inv : 1.f;
   if (threadIdx.x == 0) *sp = s;
-  if (!mine) {
-    if (!grown || t0 >= it.o) return;
-    load_tokens(it, t0, x);  // none of them new
-    if (kv) load_old(it, t0, lane, old);
+  if (it.o > 0 && s > old_scale) {
+    regrow<FMT>(it, kv, t0, t0 + 16, old_scale * inv, lane);
+    __syncwarp();  // the new codes go into words that other lanes re-encoded
   }
-  if (kv)
-    store_values<FMT>(it, t0, lane, x, old, inv, ratio, grown);
-  else
-    store_keys<FMT>(it, t0, lane, x, inv, ratio, grown);
-}
-
-// The held codes of an item under a scale that has grown.
-template <int FMT>
-__device__ __forceinline__ void regrow(const AppendItem& it, int kv, float ratio, int lane) {
-  if (kv) {  // 16 tokens of a dimension at a time; of the last few, the held ones
-    for (int t0 = 0; t0 < it.o; t0 += 16)
-      for (int d = lane; d < 128; d += 32) {
-        uint4* p = reinterpret_cast<uint4*>(it.codes + d * kPage + t0);
-        const uint4 v = *p;
-        uint4 w = recode16<FMT>(v, ratio);
-        const auto keep = [&](uint32_t& to, uint32_t from, int q) {
-          const int held = min(4, max(0, it.o - (t0 + 4 * q)));
-          const uint32_t hm = held >= 4 ? 0xffffffffu : (1u << (8 * held)) - 1u;
-          to = (to & hm) | (from & ~hm);
-        };
-        keep(w.x, v.x, 0), keep(w.y, v.y, 1), keep(w.z, v.z, 2), keep(w.w, v.w, 3);
-        *p = w;
-      }
+  if (!mine) return;
+  if (odd) drop_nan(x);
+  if (kv) {
+    uint4 old[4];
+    load_old(it, t0, lane, old);
+    store_values<FMT>(it, t0, lane, x, old, inv, odd);
   } else {
-    for (int t = lane; t < it.o * 8; t += 32) {  // 16-byte pieces of the held tokens
-      uint4* p = reinterpret_cast<uint4*>(it.codes + (t & 3) * 16 + (t & 4 ? kPage * 64 : 0) +
-                                          (t >> 3) * 64);
-      *p = recode16<FMT>(*p, ratio);
-    }
+    store_keys<FMT>(it, t0, lane, x, inv, odd);
   }
 }
 
@@ -555,7 +595,7 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
                                           lane == 0 && head == 0 ? a.status : nullptr);
   if (!rq.ok || rq.n == 0) return;
   for (int pg = (rq.held - rq.n) / kPage; pg * kPage < rq.held; ++pg) {
-    const int page = append_page(a, b, pg, lane);
+    const int page = append_page(a, a.table[b * a.table_stride + pg], lane);
     if (page < 0) continue;
     const AppendItem it = append_item(a, rq, pg, page, head, kv, lane);
     float* sp = a.scale[kv] + (int64_t)page * a.heads + head;
@@ -572,22 +612,24 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
       amax = fmaxf(amax, largest(x, odd));
     }
     amax = warp_max(amax);
-    if (odd) atomicOr(a.status, P8_NOT_FINITE);
+    odd = __any_sync(0xffffffffu, odd);
+    if (odd && lane == 0) atomicOr(a.status, P8_NOT_FINITE);
     const float s = item_scale<FMT>(old_scale, amax);
     const float inv = 1.f / s;  // exact: s is a power of two
     if (lane == 0) *sp = s;     // (the warp has read the old one)
     const bool grown = it.o > 0 && s > old_scale;
     if (grown) {
-      regrow<FMT>(it, kv, old_scale * inv, lane);
+      regrow<FMT>(it, kv, 0, kPage, old_scale * inv, lane);
       __syncwarp();  // the new codes go into words that other lanes re-encoded
     }
     for (int t0 = first; t0 < it.e; t0 += N) {
       if (!one) load_tokens(it, t0, x);
+      if (odd) drop_nan(x);
       if (!kv) {
-        store_keys<FMT>(it, t0, lane, x, inv, 1.f, false);
+        store_keys<FMT>(it, t0, lane, x, inv, odd);
       } else if constexpr (N == 16) {
         if (!one || grown) load_old(it, t0, lane, old);
-        store_values<FMT>(it, t0, lane, x, old, inv, 1.f, false);
+        store_values<FMT>(it, t0, lane, x, old, inv, odd);
       } else {
         uint8_t* dst = it.codes + 4 * lane * kPage + t0;
 #pragma unroll
@@ -595,7 +637,7 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
           if (t0 + j >= it.e) break;  // uniform over the warp
           float f[4];
           unpack4(x[j], f);
-          const uint32_t c = encode4<FMT>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+          const uint32_t c = encode4<FMT>(f, inv, odd);
 #pragma unroll
           for (int i = 0; i < 4; ++i) dst[i * kPage + j] = (uint8_t)(c >> (8 * i));
         }
