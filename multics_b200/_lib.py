@@ -252,18 +252,19 @@ _CALLS = None
 
 def calls():
     """The module that calls the library's small entry points without ctypes'
-    cost per argument (``csrc/calls.c``), bound to the loaded library."""
+    cost per argument (``csrc/bind.cpp``), bound to the loaded library."""
     global _CALLS
     if _CALLS is None:
+        import torch  # noqa: F401  (whose libraries the module needs)
+
         try:
-            from . import _calls
+            from . import _bind
         except ImportError as e:
-            raise RuntimeError("the calls module is not built; run `python -m multics_b200.build`") from e
+            raise RuntimeError("the bind module is not built; run `python -m multics_b200.build`") from e
         h = lib()
-        for name in dir(_calls):
-            if name in _SIGS:
-                _calls.bind(name, ctypes.cast(getattr(h, name), c_void_p).value)
-        _CALLS = _calls
+        for name in [n for n in dir(_bind) if n in _SIGS] + ["hier_paged8_attn_workspace"]:
+            _bind.bind(name, ctypes.cast(getattr(h, name), c_void_p).value)
+        _CALLS = _bind
     return _CALLS
 
 

@@ -183,6 +183,13 @@ def hier_head_norm_rope(q, k, freqs, num_heads, num_kv_heads, *, q_weight, k_wei
     themselves where no row moves), ``out_rows`` / ``k_out_rows`` (int32
     ``[T]``) the row of each token in them (``k_out_rows`` for k alone, e.g. the
     slots of a paged pool; negative: not written)."""
+    if q.is_cuda and out is None and out_rows is None and k_out_rows is None:
+        done = _lib.calls().head_norm(q, k, freqs, num_heads, num_kv_heads, q_weight, k_weight, positions,
+                                      eps, _dev_err(q.device))
+        if done is not None:
+            if done.__class__ is int:
+                check(done)
+            return done
     args = head_norm_args(q, k, freqs, num_heads, num_kv_heads, q_weight, k_weight, positions)
     if out is None and k_out_rows is not None:
         raise ValueError("k_out_rows needs out=(q_out, k_out)")

@@ -22,7 +22,7 @@ LIB = PKG / "libhier_b200.so"
 SOURCES = ["hier_capi.cu", "hier_meta.cu", "hier_prep.cu", "hier_attn.cu", "hier_selftest.cu",
            "hier_cached.cu", "hier_tiled.cu", "hier_shard.cu", "hier_bwd.cu", "hier_head_norm.cu",
            "hier_paged8.cu", "hier_paged8_attn.cu", "hier_paged8_mma.cu"]
-CALLS = PKG / "_calls.abi3.so"
+BIND = PKG / "_bind.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -31,25 +31,32 @@ def nvcc() -> str:
     return cand
 
 
-def build_calls(force: bool = False) -> Path:
-    """The Python module of csrc/calls.c (plain C, stable ABI)."""
-    src, header = CSRC / "calls.c", ROOT / "include" / "hier_b200.h"
-    if CALLS.exists() and not force:
-        if CALLS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
-            return CALLS
-    tmp = CALLS.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CC") or "gcc", "-O2", "-Wall", "-shared", "-fPIC", "-I", str(ROOT / "include"),
-           "-I", sysconfig.get_paths()["include"], "-o", str(tmp), str(src)]
+def build_bind(force: bool = False) -> Path:
+    """The Python module of csrc/bind.cpp (host code, PyTorch's headers)."""
+    src, header = CSRC / "bind.cpp", ROOT / "include" / "hier_b200.h"
+    if BIND.exists() and not force:
+        if BIND.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+            return BIND
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    tmp = BIND.with_suffix(".so.tmp")
+    includes = [ROOT / "include", sysconfig.get_paths()["include"], *include_paths("cuda")]
+    libs = library_paths("cuda")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in includes), "-o", str(tmp), str(src), *(f"-L{p}" for p in libs),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-lcudart"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError(f"{cmd[0]} failed building {CALLS.name}")
-    os.replace(tmp, CALLS)
-    return CALLS
+        raise RuntimeError(f"{cmd[0]} failed building {BIND.name}")
+    os.replace(tmp, BIND)
+    return BIND
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
-    build_calls(force)
+    build_bind(force)
     srcs = [CSRC / s for s in SOURCES if (CSRC / s).exists()]
     deps = srcs + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + [ROOT / "include" / "hier_b200.h"]
     if LIB.exists() and not force:

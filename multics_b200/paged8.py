@@ -23,7 +23,6 @@ length outside the table) it skips and records in the cache's status word
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -132,6 +131,24 @@ class Paged8Cache:
         scales, in ``[2^-126, 2^126]``).  Without ``status`` (int32 ``[1]``, zero)
         the caches made this way share one word per device; one made while a
         graph is captured has a word of that graph."""
+        if _lib.calls().layout(k, v, k_scale, v_scale) is None:
+            cls._refuse(k, v, k_scale, v_scale)
+        dev = k.device
+        if status is None:
+            status = _STATUS.get(dev)
+            if status is None:
+                status = torch.zeros(1, dtype=_I32, device=dev)
+                if dev.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+                    _STATUS[dev] = status
+        else:
+            _vector("status", status, 1, dev)
+        self = cls.__new__(cls)
+        self._set(k, v, k_scale, v_scale, status)
+        return self
+
+    @staticmethod
+    def _refuse(k, v, k_scale, v_scale):
+        """Raise ValueError for what is wrong with a cache's tensors."""
         if k.dtype not in _FORMATS or v.dtype != k.dtype:
             raise ValueError(f"codes must both be int8 or float8_e4m3fn, got {k.dtype}, {v.dtype}")
         shape = k.shape
@@ -148,21 +165,7 @@ class Paged8Cache:
             raise ValueError(f"k_scale and v_scale must be float32 {tuple(pool)}, got "
                              f"{k_scale.dtype} {tuple(k_scale.shape)}, {v_scale.dtype} "
                              f"{tuple(v_scale.shape)}")
-        dev = k.device
-        for t in (k, v, k_scale, v_scale):
-            if not t.is_contiguous() or t.device != dev:
-                raise ValueError(f"codes and scales must be contiguous on {dev}")
-        if status is None:
-            status = _STATUS.get(dev)
-            if status is None:
-                status = torch.zeros(1, dtype=_I32, device=dev)
-                if dev.type != "cuda" or not torch.cuda.is_current_stream_capturing():
-                    _STATUS[dev] = status
-        else:
-            _vector("status", status, 1, dev)
-        self = cls.__new__(cls)
-        self._set(k, v, k_scale, v_scale, status)
-        return self
+        raise ValueError(f"codes and scales must be contiguous on {k.device}")
 
     def check(self):
         """Raise ValueError for what the kernels recorded since the last check
@@ -212,6 +215,12 @@ def page_step(lengths, add, table, free_pages, free_count, rows: int, *,
     table, an addition above ``most_new``) changes nothing and maps no row;
     :meth:`PageStep.check` reports it.  ``in_place`` writes the new lengths and
     count over the old ones (a captured step)."""
+    done = _lib.calls().page_step(lengths, add, table, free_pages, free_count, rows, most_new, in_place)
+    if done is not None:
+        if done.__class__ is int:
+            check(done)
+        new_len, new_count, q_start, status, slots, positions = done
+        return PageStep(new_len, new_count, q_start, slots, positions, status)
     dev = table.device
     n, width, stride = _table(table, dev)
     _vector("lengths", lengths, n, dev)
@@ -253,7 +262,6 @@ def _requests(cache, table, lengths, q_start):
     return n, width, stride
 
 
-@functools.lru_cache(maxsize=256)
 def _workspace_floats(*sizes):
     floats = ctypes.c_int64()
     check(_lib.lib().hier_paged8_attn_workspace(*sizes, ctypes.byref(floats)))
@@ -266,6 +274,12 @@ def paged8_append(cache: Paged8Cache, k, v, table, lengths, q_start):
     last of request ``b``'s ``lengths[b]`` tokens.  A page written to must
     belong to one request (pages that several requests list are for reading).
     When a page's scale grows, the codes it held are re-encoded."""
+    rc = _lib.calls().append(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.status, cache.format,
+                             k, v, table, lengths, q_start)
+    if rc is not None:
+        if rc:
+            check(rc)
+        return
     width_k = cache.num_heads * HEAD_DIM
     k, v = token_rows("k", k, width_k), token_rows("v", v, width_k)
     if k.shape != v.shape:
@@ -307,6 +321,15 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
     knows it; it chooses kernels, not results.
     Returns ``[T, num_heads * 128]`` bf16, with ``return_lse`` also the float32
     ``[T, num_heads]`` log2-sum-exp of the scaled scores."""
+    if cache.device.type == "cuda":
+        done = _lib.calls().attention(
+            cache.k, cache.v, cache.k_scale, cache.v_scale, cache.status, cache.format, q, table, lengths,
+            q_start, num_heads, tokens_per_frame, block_frames, window, softmax_scale, max_rows, out,
+            return_lse, dev_err(cache.device))
+        if done is not None:
+            if done.__class__ is int:
+                check(done)
+            return done
     if num_heads < 1 or num_heads % cache.num_heads:
         raise ValueError(f"{num_heads} query heads are not a multiple of the cache's "
                          f"{cache.num_heads}")

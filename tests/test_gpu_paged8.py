@@ -771,3 +771,72 @@ def test_cache_made_while_a_graph_is_captured():
         inner.check()
     finally:
         paged8._STATUS.update(words)
+
+
+class _Apart:
+    """The bind module without its whole calls: Python checks, allocates and
+    calls the entry points."""
+
+    def __init__(self, module):
+        self.module = module
+
+    def __getattr__(self, name):
+        if name in ("append", "attention", "page_step", "head_norm", "layout"):
+            return lambda *args: 0 if name == "layout" else None
+        return getattr(self.module, name)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+def test_whole_calls_are_those_of_the_checked_path(dtype, monkeypatch):
+    """The same results and the same refusals either way."""
+    from multics_b200 import _lib
+    from multics_b200.attention import hier_head_norm_rope
+
+    lengths, add, width = [70, 0, 500], [30, 1, 64], 9
+    counts = [100, 1, 564]
+    g = _gen(4)
+    k, v = (torch.randn(95, 256, generator=g).to(BF).cuda() for _ in range(2))
+    q = torch.randn(97, 512, generator=g).to(BF).cuda()
+    f, w = torch.randn(97, 64, 2, generator=g).cuda(), torch.rand(128, generator=g).to(BF).cuda()
+
+    def run():
+        table = torch.full((3, width), -1, dtype=torch.int32)
+        table[0, :2], table[2, :8] = _i32([4, 2]).cpu(), torch.arange(10, 18)
+        table, free = table.cuda(), _i32([0, 1, 3, 5, 6, 7])
+        st = page_step(_i32(lengths), _i32(add), table, free, _i32([6]), 97, most_new=64)
+        st.check()
+        c = Paged8Cache(18, 2, dtype=dtype)
+        c = Paged8Cache.from_tensors(c.k, c.v, c.k_scale, c.v_scale, c.status)
+        paged8_append(c, k, v, table, st.lengths, st.q_start)
+        out, lse = paged8_attention(q, c, table, st.lengths, st.q_start, 4, tokens_per_frame=3, window=9,
+                                    softmax_scale=0.1, max_rows=64, return_lse=True)
+        given = paged8_attention(q, c, table, st.lengths, st.q_start, 4, out=torch.ones_like(q))
+        qn, kn = hier_head_norm_rope(q, q[:, :256], f, 4, 2, q_weight=w, k_weight=w, eps=1e-5)
+        again = page_step(st.lengths, _i32([-100, 0, 1]), table, free, st.free_count, 4, in_place=True)
+        assert again.lengths is st.lengths and again.free_count is st.free_count
+        assert st.lengths.tolist() == [0, 1, counts[2] + 1]
+        return [*st, *again, table, free, c.k.view(torch.int8), c.v.view(torch.int8), c.k_scale, c.v_scale,
+                out, lse, given, qn, kn]
+
+    whole = run()
+    module = _lib.calls()
+    c, t, n, s = Paged8Cache(2, 2, dtype=dtype), _i32([[0, 1]]), _i32([3]), _i32([0, 3])
+
+    def refuse():
+        seen = []
+        for fn, a in ((paged8_append, (c, k[:3], v[:2], t, n, s)), (paged8_append, (c, k[:3], v[:3], t, n, n)),
+                      (paged8_append, (c, k[:3].float(), v[:3], t, n, s)),
+                      (paged8_append, (c, k[:3].cpu(), v[:3], t, n, s)),
+                      (paged8_attention, (q[:3], c, t, n, s, 3)), (paged8_attention, (q[:3], c, t, n.long(), s, 4)),
+                      (paged8_attention, (q[:3], c, t, n, s, 2)), (page_step, (n, n, t, n, n, -1)),
+                      (page_step, (n, s, t, n, n, 1))):
+            with pytest.raises((ValueError, NotImplementedError)) as e:
+                fn(*a)
+            seen.append((e.type, str(e.value)))
+        return seen
+
+    refused = refuse()
+    monkeypatch.setattr(_lib, "calls", lambda: _Apart(module))
+    for a, b in zip(whole, run()):
+        assert torch.equal(a, b)
+    assert refused == refuse()
