@@ -248,6 +248,7 @@ def lib():
 
 
 _CALLS = None
+_UNSEEN = ["hier_paged8_attn_workspace", "hier_head_norm_rope_bwd_partials", "hier_last_error"]
 
 
 def calls():
@@ -262,7 +263,7 @@ def calls():
         except ImportError as e:
             raise RuntimeError("the bind module is not built; run `python -m multics_b200.build`") from e
         h = lib()
-        for name in [n for n in dir(_bind) if n in _SIGS] + ["hier_paged8_attn_workspace"]:
+        for name in [n for n in dir(_bind) if n in _SIGS] + _UNSEEN:
             _bind.bind(name, ctypes.cast(getattr(h, name), c_void_p).value)
         _CALLS = _bind
     return _CALLS

@@ -17,9 +17,12 @@
 // The module holds no code of the library: bind() gives it the addresses of
 // the one that is loaded.
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
 #include <ATen/ops/unsafe_split_with_sizes.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -110,6 +113,8 @@ ENTRY(hier_paged8_attn, "pqiiiiippppipqippiiiifipqpipppp", P(0), Q(1), I(2), I(3
       I(20), x.f, I(22), P(23), Q(24), P(25), I(26), P(27), P(28), P(29), P(30))
 
 decltype(&hier_paged8_attn_workspace) at_hier_paged8_attn_workspace;
+decltype(&hier_head_norm_rope_bwd_partials) at_hier_head_norm_rope_bwd_partials;
+decltype(&hier_last_error) at_hier_last_error;
 
 // ---- whole calls -------------------------------------------------------------
 
@@ -376,59 +381,148 @@ PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// head_norm(q, k, freqs, heads, key_heads, q_weight, k_weight, positions, eps, dev_err) -> (q, k), or a
-// status
+// The arguments of the per-head norm: q, k, freqs, heads, key heads, weights, positions (or None), eps
+// and the device's error word.
+struct HeadNorm {
+  const at::Tensor *q, *k, *freqs, *wq, *wk, *pos, *err;
+  int64_t rows, heads, kv_heads, D;
+  float eps;
+  bool f32;  // the weights
+};
+
+bool head_norm_of(PyObject* const* a, Py_ssize_t n, HeadNorm* h) {
+  if (n != 10 || !at_hier_head_norm_rope || !int_of(a[3], 1, 4096, &h->heads) ||
+      !int_of(a[4], 1, 4096, &h->kv_heads))
+    return false;
+  h->q = tensor_of(a[0]), h->k = tensor_of(a[1]), h->freqs = tensor_of(a[2]);
+  h->wq = tensor_of(a[5]), h->wk = tensor_of(a[6]), h->err = tensor_of(a[9]);
+  if (!h->q || !h->k || !h->freqs || !h->wq || !h->wk || !h->err || h->q->dim() != 2 ||
+      !on_current(h->q->device()))
+    return false;
+  const at::Device dev = h->q->device();
+  h->D = h->q->size(1) / h->heads, h->rows = h->q->size(0);
+  if (h->D * h->heads != h->q->size(1) || (h->D != 64 && h->D != 128 && h->D != 256) ||
+      !is_rows(h->q, h->heads * h->D, dev) || !is_rows(h->k, h->kv_heads * h->D, dev) ||
+      h->k->size(0) != h->rows)
+    return false;
+  for (const at::Tensor* w : {h->wq, h->wk})
+    if (w->dim() != 1 || w->size(0) != h->D || w->device() != dev || !w->is_contiguous() ||
+        w->scalar_type() != h->wq->scalar_type())
+      return false;
+  h->f32 = h->wq->scalar_type() == at::kFloat;
+  if (!h->f32 && h->wq->scalar_type() != at::kBFloat16) return false;
+  const at::Tensor& f = *h->freqs;
+  if (f.scalar_type() != at::kFloat || f.device() != dev || f.dim() != 3 || f.size(0) < 1 ||
+      f.size(1) * 2 != h->D || f.size(2) != 2 || !f.is_contiguous() || !aligned(f))
+    return false;
+  h->pos = nullptr;
+  if (a[7] != Py_None) {
+    h->pos = tensor_of(a[7]);
+    if (!is_vector(h->pos, h->rows, dev)) return false;
+  } else if (h->rows % f.size(0)) {
+    return false;
+  }
+  h->eps = (float)PyFloat_AsDouble(a[8]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+
+int head_norm_forward(const HeadNorm& h, at::Tensor* q, at::Tensor* k) {
+  *q = at::empty({h.rows, h.heads * h.D}, h.q->options());
+  *k = at::empty({h.rows, h.kv_heads * h.D}, h.k->options());
+  return at_hier_head_norm_rope(
+      h.q->data_ptr(), h.q->stride(0), h.k->data_ptr(), h.k->stride(0), h.rows, (int32_t)h.heads,
+      (int32_t)h.kv_heads, (int32_t)h.D, h.wq->data_ptr(), h.wk->data_ptr(), h.f32, data<float>(*h.freqs),
+      h.freqs->size(0), h.pos ? data<int32_t>(*h.pos) : nullptr, h.eps, q->data_ptr(), q->stride(0),
+      nullptr, h.rows, k->data_ptr(), k->stride(0), nullptr, h.rows, 1, data<int32_t>(*h.err),
+      stream_of(h.q->device()));
+}
+
+PyObject* pair_of(at::Tensor a, at::Tensor b) {
+  PyObject *first = THPVariable_Wrap(std::move(a)), *second = THPVariable_Wrap(std::move(b));
+  PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+  Py_XDECREF(first);
+  Py_XDECREF(second);
+  return both;
+}
+
+// head_norm(*arguments) -> (q, k), or a status
 PyObject* head_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return attempt([&]() -> PyObject* {
-    int64_t heads, kv_heads;
-    if (n != 10 || !at_hier_head_norm_rope || !int_of(a[3], 1, 4096, &heads) ||
-        !int_of(a[4], 1, 4096, &kv_heads))
-      return nullptr;
-    const at::Tensor *q = tensor_of(a[0]), *k = tensor_of(a[1]), *f = tensor_of(a[2]);
-    const at::Tensor *wq = tensor_of(a[5]), *wk = tensor_of(a[6]), *err = tensor_of(a[9]);
-    if (!q || !k || !f || !wq || !wk || !err || q->dim() != 2 || !on_current(q->device())) return nullptr;
-    const at::Device dev = q->device();
-    const int64_t D = q->size(1) / heads, rows = q->size(0);
-    if (D * heads != q->size(1) || (D != 64 && D != 128 && D != 256) || !is_rows(q, heads * D, dev) ||
-        !is_rows(k, kv_heads * D, dev) || k->size(0) != rows)
-      return nullptr;
-    const auto is_weight = [&](const at::Tensor* w) {
-      return w->dim() == 1 && w->size(0) == D && w->device() == dev && w->is_contiguous() &&
-             w->scalar_type() == wq->scalar_type();
-    };
-    const bool f32 = wq->scalar_type() == at::kFloat;
-    if (!is_weight(wq) || !is_weight(wk) || (!f32 && wq->scalar_type() != at::kBFloat16)) return nullptr;
-    if (f->scalar_type() != at::kFloat || f->device() != dev || f->dim() != 3 || f->size(0) < 1 ||
-        f->size(1) * 2 != D || f->size(2) != 2 || !f->is_contiguous() || !aligned(*f))
-      return nullptr;
-    const at::Tensor* pos = nullptr;
-    if (a[7] != Py_None) {
-      pos = tensor_of(a[7]);
-      if (!is_vector(pos, rows, dev)) return nullptr;
-    } else if (rows % f->size(0)) {
-      return nullptr;
+    HeadNorm h;
+    if (!head_norm_of(a, n, &h)) return nullptr;
+    at::Tensor q, k;
+    const int rc = unlocked([&] { return head_norm_forward(h, &q, &k); });
+    return rc ? PyLong_FromLong(rc) : pair_of(std::move(q), std::move(k));
+  });
+}
+
+// The same with gradients for q, k and the weights.  The engine calls back
+// without Python; differentiating twice is an error, as of any kernel.
+struct HeadNormFn : torch::autograd::Function<HeadNormFn> {
+  using Context = torch::autograd::AutogradContext;
+  using Tensors = torch::autograd::variable_list;
+
+  static Tensors forward(Context* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq,
+                         const at::Tensor& wk, const HeadNorm* h, int* rc) {
+    at::Tensor qo, ko;
+    *rc = head_norm_forward(*h, &qo, &ko);
+    ctx->save_for_backward({q, k, wq, wk, *h->freqs, h->pos ? *h->pos : at::Tensor(), *h->err});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{h->heads, h->kv_heads, h->D};
+    ctx->saved_data["eps"] = (double)h->eps;
+    return {qo, ko};
+  }
+
+  static Tensors backward(Context* ctx, Tensors g) {
+    const Tensors s = ctx->get_saved_variables();
+    const at::Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3], &freqs = s[4], &pos = s[5], &err = s[6];
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const float eps = (float)ctx->saved_data["eps"].toDouble();
+    const int64_t rows = q.size(0), D = sizes[2];
+    const int32_t heads = (int32_t)sizes[0], kv_heads = (int32_t)sizes[1];
+    const at::Device dev = q.device();
+    for (int i = 0; i < 2; ++i)  // (already of the outputs' type and shape)
+      if (!is_rows(&g[i], sizes[i] * D, dev)) g[i] = g[i].clone(at::MemoryFormat::Contiguous);
+    Tensors d;
+    {
+      const at::NoGradGuard none;
+      d = {at::empty({rows, heads * D}, q.options()), at::empty({rows, kv_heads * D}, k.options()),
+           at::empty_like(wq), at::empty_like(wk)};
     }
-    const double eps = PyFloat_AsDouble(a[8]);
-    if (PyErr_Occurred()) {
-      PyErr_Clear();
-      return nullptr;
+    int32_t blocks = 0;
+    int rc = at_hier_head_norm_rope_bwd_partials(rows, heads, kv_heads, (int32_t)D, &blocks);
+    const at::Tensor part = at::empty({blocks, D}, freqs.options());
+    if (!rc)
+      rc = at_hier_head_norm_rope_bwd(
+          q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), rows, heads, kv_heads, (int32_t)D,
+          wq.data_ptr(), wk.data_ptr(), wq.scalar_type() == at::kFloat, data<float>(freqs), freqs.size(0),
+          pos.defined() ? data<int32_t>(pos) : nullptr, eps, g[0].data_ptr(), g[0].stride(0),
+          g[1].data_ptr(), g[1].stride(0), d[0].data_ptr(), heads * D, d[1].data_ptr(), kv_heads * D,
+          data<float>(part), blocks, d[2].data_ptr(), d[3].data_ptr(), data<int32_t>(err), stream_of(dev));
+    TORCH_CHECK(!rc, at_hier_last_error());
+    if (at::GradMode::is_enabled()) {
+      for (at::Tensor& t : d) t.set_requires_grad(true);
+      const auto twice = std::make_shared<torch::autograd::DelayedError>(
+          "the per-head norm's gradients cannot be differentiated again", (int64_t)d.size());
+      d = (*twice)(std::move(d));
     }
-    at::Tensor qo = at::empty({rows, heads * D}, q->options());
-    at::Tensor ko = at::empty({rows, kv_heads * D}, k->options());
-    void* stream = stream_of(dev);
-    const int rc = unlocked([&] {
-      return at_hier_head_norm_rope(
-          q->data_ptr(), q->stride(0), k->data_ptr(), k->stride(0), rows, (int32_t)heads,
-          (int32_t)kv_heads, (int32_t)D, wq->data_ptr(), wk->data_ptr(), f32, data<float>(*f), f->size(0),
-          pos ? data<int32_t>(*pos) : nullptr, (float)eps, qo.data_ptr(), qo.stride(0), nullptr, rows,
-          ko.data_ptr(), ko.stride(0), nullptr, rows, 1, data<int32_t>(*err), stream);
-    });
-    if (rc) return PyLong_FromLong(rc);
-    PyObject *first = THPVariable_Wrap(std::move(qo)), *second = THPVariable_Wrap(std::move(ko));
-    PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
-    Py_XDECREF(first);
-    Py_XDECREF(second);
-    return both;
+    return {d[0], d[1], d[2], d[3], at::Tensor(), at::Tensor()};
+  }
+};
+
+// head_norm_grad(*arguments) -> (q, k) with their graph, or a status
+PyObject* head_norm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return attempt([&]() -> PyObject* {
+    HeadNorm h;
+    if (!at_hier_head_norm_rope_bwd || !at_hier_head_norm_rope_bwd_partials || !at_hier_last_error ||
+        !head_norm_of(a, n, &h))
+      return nullptr;
+    int rc = 0;
+    const auto out = HeadNormFn::apply(*h.q, *h.k, *h.wq, *h.wk, &h, &rc);
+    return rc ? PyLong_FromLong(rc) : pair_of(out[0], out[1]);
   });
 }
 
@@ -441,7 +535,9 @@ const struct {
   void** at;
 } entries[] = {BOUND(hier_head_norm_rope), BOUND(hier_head_norm_rope_bwd), BOUND(hier_page_step),
                BOUND(hier_paged8_append),  BOUND(hier_paged8_attn),
-               BOUND(hier_paged8_attn_workspace)};
+               BOUND(hier_paged8_attn_workspace),
+               BOUND(hier_head_norm_rope_bwd_partials),
+               BOUND(hier_last_error)};
 
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) {
@@ -471,6 +567,7 @@ PyMethodDef methods[] = {
     METHOD("attention", attention, "paged8_attention of well-formed tensors"),
     METHOD("page_step", page_step, "page_step of well-formed tensors"),
     METHOD("head_norm", head_norm, "hier_head_norm_rope of well-formed tensors"),
+    METHOD("head_norm_grad", head_norm_grad, "head_norm_rope_grad of well-formed tensors"),
     RAW(hier_head_norm_rope),
     RAW(hier_head_norm_rope_bwd),
     RAW(hier_page_step),

@@ -294,6 +294,13 @@ def head_norm_rope_grad(q, k, freqs, num_heads: int, num_kv_heads: int, *, q_wei
 
     ft = freqs if (freqs.dtype == torch.float32 and freqs.dim() == 3
                    and freqs.shape[-1] == 2) else freqs_table(freqs)
+    if q.is_cuda:
+        done = _lib.calls().head_norm_grad(q, k, ft, num_heads, num_kv_heads, q_weight, k_weight, positions,
+                                           eps, _dev_err(q.device))
+        if done is not None:
+            if done.__class__ is int:
+                check(done)
+            return done
     return _HeadNormFn.apply(q, k, q_weight, k_weight, ft, positions, num_heads, num_kv_heads, eps)
 
 

@@ -347,3 +347,40 @@ def test_gradients_without_eps(H, Hk, D):
         top = ref[n].grad.abs().max()
         err = (leaf[n].grad.cpu().double() - ref[n].grad).abs()
         assert (err <= ref[n].grad.abs() * 2.0 ** -8 + top * 2.0 ** -14).all(), n
+
+
+@pytest.mark.parametrize("wdtype", [BF, torch.float32])
+@pytest.mark.parametrize("positions", [True, False])
+def test_gradients_by_either_way_are_the_same(wdtype, positions, monkeypatch):
+    """Through the bind module's function and through Python's; gradients that
+    are broadcast, strided or missing too."""
+    from multics_b200 import _lib
+
+    x = _inputs(26, 6, 3, 128, 13, 1, wdtype)
+    pos = x["pos"].cuda() if positions else None
+
+    def run():
+        leaf = {n: x[n].cuda().requires_grad_() for n in ("q", "k", "wq", "wk")}
+        got = []
+        wide = torch.cat([x["gk"], x["gk"]], 1).cuda()
+        for grads in ((x["gq"].cuda(), x["gk"].cuda()), (x["gq"].cuda(), None), (None, wide[:, 384:]),
+                      (torch.ones(1, 1, dtype=BF, device="cuda").expand(26, 768), wide[:, 1:385])):
+            q, k = head_norm_rope_grad(leaf["q"], leaf["k"], x["table"].cuda(), 6, 3, q_weight=leaf["wq"],
+                                       k_weight=leaf["wk"], positions=pos, eps=1e-5)
+            pairs = [(o, g) for o, g in zip((q, k), grads) if g is not None]
+            got += [q, k, *torch.autograd.grad([o for o, _ in pairs], list(leaf.values()),
+                                               [g for _, g in pairs], create_graph=grads[1] is not None)]
+        with pytest.raises(RuntimeError):  # (no gradient of a gradient)
+            got[2].sum().backward()
+        return [t.detach() for t in got]
+
+    fast = run()
+    module = _lib.calls()
+
+    class Apart:
+        def __getattr__(self, name):
+            return (lambda *args: None) if name.startswith("head_norm") else getattr(module, name)
+
+    monkeypatch.setattr(_lib, "calls", lambda: Apart())
+    for a, b in zip(fast, run()):
+        assert torch.equal(a, b)
