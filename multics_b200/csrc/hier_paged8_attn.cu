@@ -14,13 +14,16 @@
 //
 // Two kernels.  paged8_long_kernel, for block tables of more than kShortPages
 // pages: four warps of a block share a tile's pages (joined in shared memory),
-// and with few tiles the keys are also split over blocks.  Up to one wave of
-// blocks they are a cluster, which joins its parts over distributed shared
-// memory: no workspace and no second launch (one row over 9 240 tokens of 24
-// heads: 20.6 us of the device, 20 of the host; with a second kernel 18.6 and
-// 25.5).  Beyond it clusters wait for places (37 rows of 4 key heads: 103 us),
-// so the parts go to a workspace and a second kernel joins them (91 us).  Parts
-// are always joined in their order.
+// and with few tiles the keys are also split over blocks.  Few parts are the
+// blocks of a cluster, which joins them over distributed shared memory: no
+// workspace and no second launch (a row of each of 4 requests over 3 000 tokens,
+// 24 heads to 8: 11.8 us, with a second kernel 14.0; 3.3 us less of the host).
+// Where twice the portable cluster's 8 blocks could share the keys, the parts go
+// to a workspace and a second kernel joins them (one row over 9 240 tokens of 24
+// heads: 19.2 us against 20.6; over 100 000 tokens, 8 heads to one: 31.7 against
+// 94), and so they do beyond one wave of blocks, where clusters wait for places
+// (37 rows of 4 key heads: 91 us against 103).  Parts are always joined in their
+// order.
 // While a page's scores are computed its values are in flight, and while its
 // values are consumed the next page's keys are: the loads of one take the
 // registers that the other's products have just used.  paged8_short_kernel: a
@@ -667,7 +670,8 @@ Shape shape_of(int64_t rows, int group, int kv_heads, int n, int width, int max_
       // (requests without rows have places in the workspace too: 68 MB of it at most)
       s.small_splits =
           clamp_int(std::max(one, four), 1, clamp_int((1 << 14) / (s.small_tiles * kv_heads), 1, 32));
-      if (s.small_splits > 1 && work * std::min(s.small_splits, kMaxCluster) <= kWave) {
+      if (s.small_splits > 1 && s.small_splits < 2 * kMaxCluster &&
+          work * std::min(s.small_splits, kMaxCluster) <= kWave) {
         s.cluster = true;
         while (s.small_splits > kMaxCluster || (s.small_splits & (s.small_splits - 1)))
           --s.small_splits;  // the power of two below, up to the portable cluster size
