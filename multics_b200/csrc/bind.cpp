@@ -1,7 +1,7 @@
 // The calls of a decoding step from Python.
 //
 // A step's kernels take a few microseconds each, and Python's checks of their
-// arguments, the allocations and a ctypes call of 20 to 36 arguments (0.15 us
+// arguments, the allocations and a ctypes call of 20 to 36 arguments (0.1 us
 // each) took 12 to 19.  Two layers take their place:
 //
 //   hier_*     an entry point of hier_b200.h as it is, called with ints

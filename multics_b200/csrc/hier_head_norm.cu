@@ -16,8 +16,8 @@
 // of its heads.  Results are stored past the caches' reuse (written once, 165
 // against 183 us).  38 556 rows of 24 + 24 heads of 128: 150 us = 6.3 TB/s, 0.97
 // of the measured copy bandwidth (8 groups per warp: 165 us, 4: 162, 2: 200).
-// Backward on 9 241 rows of 24 + 8 heads: about 50 us = 4.5 TB/s, bound by its
-// arithmetic and two reductions per head.
+// Backward on 9 241 rows of 24 + 8 heads: 46 us = 4.9 TB/s, bound by its
+// arithmetic and two reductions per head, and 4 us for the weights' sums.
 
 #include "common.cuh"
 

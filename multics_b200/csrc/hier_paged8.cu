@@ -258,11 +258,16 @@ __global__ void page_rows_kernel(StepArgs a) {
 // division is exact).  When the scale grows the held codes are re-encoded
 // under the new one.  Bytes of tokens from e on stay as they are.
 //
+// Reads 2 bytes a value and writes one, but is bound by the instructions of its
+// conversions and the chain of lookups of a short block: 4
+// requests of 660 tokens, 24 heads, e4m3 (48 MB): 15.7 us.
+//
 // A lane has 4 dimensions of a token (8 bytes), a warp its 128.  Keys are
 // written 4 bytes per token; values are stored with the tokens along the row.
 //
 // Long runs of tokens (paged8_append_pages_kernel): a block per item, 16 tokens
-// per warp kept in registers between the maximum and the codes, values written
+// per warp kept in registers between the maximum and the codes (64 registers, 8
+// blocks per SM; the rows are loaded before the page is known), values written
 // 16 bytes to each of the lane's 4 rows, merged with the bytes already there
 // (nobody else writes the page and head).  Fewer tokens per request
 // (paged8_append_rows_kernel): a warp per request, head and key or value, which
@@ -727,14 +732,16 @@ extern "C" int hier_paged8_append(const void* k, int64_t k_stride, const void* v
   a.lengths = lengths, a.q_start = q_start, a.n = n;
   a.status = status;
   cudaStream_t st = (cudaStream_t)stream;
-  // A block per page and head where requests bring more than 32 tokens each, or
-  // more than 4 and the machine has room (10 x 9 tokens, 6 heads: 4.9 us against
-  // 7.0; 201 x 8 tokens, 29 heads: 68 us against 38 by a warp each).  n rows
-  // touch at most ceil(n / 64) + 1 pages, so request b's pages fit between
-  // q_start[b] / 64 + 2 b and the next request's: the grid needs no count from
-  // the device.
-  const bool many = rows > 32 * (int64_t)n ||
-                    (rows > 4 * (int64_t)n && (int64_t)n * heads * 2 <= 148 * 8);
+  // A block per page and head where requests bring more than 48 tokens each, or
+  // fewer and the machine has room, else a warp per request and head (in us, warps
+  // and blocks, of requests x tokens x heads: 100 x 34 x 24 27.7 and 34.0, 200 x
+  // 64 x 8 33.2 and 30.5; 30 x 40 x 8 8.1 and 6.4, 100 x 30 x 8 11.4 and 13.4; 20 x
+  // 16 x 8 6.5 and 4.8, 12 x 12 x 24 4.2 and 4.9).  n rows touch at most
+  // ceil(n / 64) + 1 pages, so request b's pages fit between q_start[b] / 64 + 2 b
+  // and the next request's: the grid needs no count from the device.
+  const int64_t items = (int64_t)n * heads * 2;
+  const bool many = rows > 48 * (int64_t)n || (rows > 16 * (int64_t)n && items <= 148 * 8) ||
+                    (rows > 4 * (int64_t)n && items <= 148 * 3);
   const int64_t units = (many ? rows / kPage + 2 * (int64_t)n : (int64_t)n) * heads * 2;
   const int64_t blocks = many ? units : (units + 3) / 4;
   if (units > INT32_MAX - 4) {
