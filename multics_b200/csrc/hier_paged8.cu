@@ -22,9 +22,9 @@ namespace {
 // Bound by the launch, the chain of loads (length, list or table cell) and, for
 // a kernel that runs once, the fetch of its instructions: four requests of a
 // thread at a time, all their cells in flight, took 8.0 us for 4 requests
-// against 6.1, and 12.2 for 3 520 against 12.4.
+// against 6.1 (in 32 warps), and 12.2 for 3 520 against 12.4.
 
-constexpr int kStepThreads = 1024;
+constexpr int kStepThreads = 1024;  // at most
 
 struct StepArgs {
   const int32_t* lengths;
@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
   if (tid == 0) bad_all = 0;
   asm volatile("griddepcontrol.launch_dependents;");  // page_rows_kernel
   const int count = *a.free_count;
-  const int per = (a.n + kStepThreads - 1) / kStepThreads;
+  const int threads = blockDim.x;
+  const int per = (a.n + threads - 1) / threads;
   const int b0 = min(a.n, tid * per), b1 = min(a.n, b0 + per);
   int bad = 0;
   Sum3 mine = {0, 0, 0};
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
   __syncthreads();
   if (bad) atomicOr(&bad_all, bad);
   Sum3 base = {0, 0, 0}, total = {0, 0, 0};
-  for (int w = 0; w < kStepThreads / 32; ++w) {
+  for (int w = 0; w < threads / 32; ++w) {
     if (w == warp) base = total;
     total = total + warp_sum[w];
   }
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
       a.lengths_out[b] = a.lengths[b];
     }
     if (map_here)
-      for (int r = tid; r < a.rows; r += kStepThreads) a.slots[r] = a.positions[r] = -1;
+      for (int r = tid; r < a.rows; r += threads) a.slots[r] = a.positions[r] = -1;
     return;
   }
   // given pages first: a page may change hands within the step.  A request
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
   }
   if (!map_here) return;
   __syncthreads();
-  for (int r = tid; r < a.rows; r += kStepThreads) {
+  for (int r = tid; r < a.rows; r += threads) {
     const int b = r < total.rows ? request_of(a.q_start, 0, a.n, r) : -1;
     map_row(a, r, b, b < 0 ? 0 : a.q_start[b + 1]);
   }
@@ -600,19 +601,23 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
                                           lane == 0 && head == 0 ? a.status : nullptr);
   if (!rq.ok || rq.n == 0) return;
   for (int pg = (rq.held - rq.n) / kPage; pg * kPage < rq.held; ++pg) {
-    const int page = append_page(a, a.table[b * a.table_stride + pg], lane);
-    if (page < 0) continue;
-    const AppendItem it = append_item(a, rq, pg, page, head, kv, lane);
-    float* sp = a.scale[kv] + (int64_t)page * a.heads + head;
-    const float old_scale = it.o > 0 ? *sp : 0.f;
+    const int entry = a.table[b * a.table_stride + pg];
+    AppendItem it = append_item(a, rq, pg, 0, head, kv, lane);
     const int first = N == 4 ? it.o : it.o & ~15;
     const bool one = it.e - first <= N;  // the tokens stay in registers
     uint2 x[N];
+    if (one) load_tokens(it, first, x);  // in flight before the page is known
+    const int page = append_page(a, entry, lane);
+    if (page < 0) continue;
+    const int64_t at = (int64_t)page * a.heads;
+    it.codes += at * kPageHeadBytes;
+    float* sp = a.scale[kv] + at + head;
+    const float old_scale = it.o > 0 ? *sp : 0.f;
     uint4 old[4];
     float amax = 0.f;
     bool odd = false;
     for (int t0 = first; t0 < it.e; t0 += N) {
-      load_tokens(it, t0, x);
+      if (!one) load_tokens(it, t0, x);
       if (N == 16 && kv && one) load_old(it, t0, lane, old);
       amax = fmaxf(amax, largest(x, odd));
     }
@@ -676,11 +681,15 @@ extern "C" int hier_page_step(const int32_t* lengths, const int32_t* add, int32_
                 free_count, rows, max_add, lengths_out, free_count_out, q_start, slots,      positions,
                 status};
   cudaStream_t st = (cudaStream_t)stream;
-  // the rows are mapped by the same block up to 8 per thread (a thread's searches
-  // hit its L1 cache: 4 rows 6.1 us, 32 at a time by a warp 7.7), beyond that by a
-  // grid of their own
-  const int inside = rows <= 8 * kStepThreads;
-  page_step_kernel<<<1, kStepThreads, 0, st>>>(a, inside);
+  // Up to 1 024 rows are mapped by the same block (a thread's searches hit its L1
+  // cache: 4 rows 6.1 us, 32 at a time by a warp 7.7), more by a grid of their own
+  // (1 000 requests of 8 rows: 8.2 us against 15.9).  Warps cost their barriers:
+  // 4 requests take 2.8 us in 4 warps and 6.1 in 32, 500 5.2 in 16, 2 139 10.6 in
+  // 16 and 11.9 in 32, 5 000 24.8 and 20.0.
+  const int inside = rows <= 1024;
+  const int most = inside && rows / 2 > n ? rows / 2 : n;
+  const int threads = most <= 128 ? 128 : most <= 256 ? 256 : most <= 2560 ? 512 : kStepThreads;
+  page_step_kernel<<<1, threads, 0, st>>>(a, inside);
   HIER_CHECK_CUDA(cudaGetLastError(), "page_step_kernel launch");
   if (!inside) {
     cudaLaunchAttribute attr = {};
