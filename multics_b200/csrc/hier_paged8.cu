@@ -14,17 +14,17 @@ namespace {
 // its last tokens; -lengths[b] ends it).  Pages it no longer needs go to the
 // end of the free list in request order, pages it now needs come off the
 // list's end in request order, and its max(add, 0) new tokens become the next
-// rows of the call.  One block: a few thousand requests are a few loads per
-// thread and one scan, and the list is a single stack anyway.  A step that
-// cannot be taken whole (too few free pages or rows, a length outside the
-// table) changes nothing and maps no row.
+// rows of the call.  One block, or one cluster: the list is a single stack, and
+// the requests' places in it and in the rows are one scan.  A step that cannot
+// be taken whole (too few free pages or rows, a length outside the table)
+// changes nothing and maps no row.
 //
 // Bound by the launch, the chain of loads (length, list or table cell) and, for
 // a kernel that runs once, the fetch of its instructions: four requests of a
 // thread at a time, all their cells in flight, took 8.0 us for 4 requests
-// against 6.1 (in 32 warps), and 12.2 for 3 520 against 12.4.
+// against 6.1 (in 32 warps), and 12.2 for 3 520 against 12.4 (in one block).
 
-constexpr int kStepThreads = 1024;  // at most
+constexpr int kStepThreads = 512;  // at most, of a block
 
 struct StepArgs {
   const int32_t* lengths;
@@ -133,15 +133,16 @@ __device__ __forceinline__ void map_rows(const StepArgs& a, int64_t r0, int tota
 }
 
 __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int map_here) {
-  __shared__ Sum3 warp_sum[32];
+  __shared__ Sum3 warp_sum[kStepThreads / 32];
+  __shared__ Sum3 block_sum, sum_before, sum_all;  // this block's, those of the blocks before it, all
   __shared__ int bad_all;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) bad_all = 0;
   asm volatile("griddepcontrol.launch_dependents;");  // page_rows_kernel
   const int count = *a.free_count;
-  const int threads = blockDim.x;
+  const int threads = blockDim.x * gridDim.x, me = blockIdx.x * blockDim.x + tid;
   const int per = (a.n + threads - 1) / threads;
-  const int b0 = min(a.n, tid * per), b1 = min(a.n, b0 + per);
+  const int b0 = min(a.n, me * per), b1 = min(a.n, b0 + per);
   int bad = 0;
   Sum3 mine = {0, 0, 0};
   for (int b = b0; b < b1; ++b) mine = mine + step_of(a, b, bad);
@@ -155,18 +156,39 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
   __syncthreads();
   if (bad) atomicOr(&bad_all, bad);
   Sum3 base = {0, 0, 0}, total = {0, 0, 0};
-  for (int w = 0; w < threads / 32; ++w) {
+  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
     if (w == warp) base = total;
     total = total + warp_sum[w];
   }
-  __syncthreads();
-  bad = bad_all;
+  if (gridDim.x == 1) {
+    __syncthreads();
+    bad = bad_all;
+  } else {
+    if (tid == 0) block_sum = total;
+    cluster_sync();
+    if (tid == 0) {
+      Sum3 all = {0, 0, 0};
+      int bits = 0;
+      for (int r = 0; r < (int)gridDim.x; ++r) {
+        if (r == (int)blockIdx.x) sum_before = all;
+        const uint32_t at = peer_smem(&block_sum, r);
+        all = all + Sum3{ld_peer64(at), ld_peer64(at + 8), ld_peer64(at + 16)};
+        bits |= (int)ld_peer32(peer_smem(&bad_all, r));
+      }
+      sum_all = all;
+      warp_sum[0].rows = bits;
+    }
+    cluster_sync();  // nobody leaves, or changes it, while its sum is read
+    total = sum_all;
+    base = base + sum_before;
+    bad = (int)warp_sum[0].rows;
+  }
   if (count < 0 || count > a.capacity || count + total.given > a.capacity) bad |= STEP_BAD_LIST;
   if (total.need > count + total.given) bad |= STEP_NO_PAGES;
   if (total.rows > a.rows) bad |= STEP_NO_ROWS;
   const Sum3 before = {base.rows + incl.rows - mine.rows, base.need + incl.need - mine.need,
                        base.given + incl.given - mine.given};
-  if (tid == 0) {
+  if (me == 0) {
     *a.status = bad;
     *a.free_count_out = bad ? count : (int)(count + total.given - total.need);
     a.q_start[a.n] = bad ? 0 : (int)total.rows;
@@ -177,9 +199,15 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
       a.lengths_out[b] = a.lengths[b];
     }
     if (map_here)
-      for (int r = tid; r < a.rows; r += threads) a.slots[r] = a.positions[r] = -1;
+      for (int r = me; r < a.rows; r += threads) a.slots[r] = a.positions[r] = -1;
     return;
   }
+  const auto sync = [] {
+    if (gridDim.x == 1)
+      __syncthreads();
+    else
+      cluster_sync();
+  };
   // given pages first: a page may change hands within the step.  A request
   // with many pages is handled by its whole warp.
 #pragma unroll
@@ -223,7 +251,7 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
         }
       at = at + s;
     }
-    __syncthreads();
+    sync();
   }
   // lengths_out may be lengths itself: each thread reads its own before it writes
   Sum3 at = before;
@@ -235,8 +263,8 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(StepArgs a, int
     at = at + s;
   }
   if (!map_here) return;
-  __syncthreads();
-  for (int r = tid; r < a.rows; r += threads) {
+  sync();
+  for (int r = me; r < a.rows; r += threads) {
     const int b = r < total.rows ? request_of(a.q_start, 0, a.n, r) : -1;
     map_row(a, r, b, b < 0 ? 0 : a.q_start[b + 1]);
   }
@@ -681,25 +709,32 @@ extern "C" int hier_page_step(const int32_t* lengths, const int32_t* add, int32_
                 free_count, rows, max_add, lengths_out, free_count_out, q_start, slots,      positions,
                 status};
   cudaStream_t st = (cudaStream_t)stream;
-  // Up to 1 024 rows are mapped by the same block (a thread's searches hit its L1
+  // Up to 1 024 rows are mapped by the same kernel (a thread's searches hit its L1
   // cache: 4 rows 6.1 us, 32 at a time by a warp 7.7), more by a grid of their own
-  // (1 000 requests of 8 rows: 8.2 us against 15.9).  Warps cost their barriers:
-  // 4 requests take 2.8 us in 4 warps and 6.1 in 32, 500 5.2 in 16, 2 139 10.6 in
-  // 16 and 11.9 in 32, 5 000 24.8 and 20.0.
+  // (1 000 requests of 8 rows: 8.2 us against 15.9).  Warps cost their barriers: 4
+  // requests take 2.8 us in 4 warps and 6.1 in 32, 500 5.2 in 16.  A cluster shares
+  // out the requests of a long list (3 000: 9.7 us, one block 12.8; 1 000: 8.6 and
+  // 6.9).
   const int inside = rows <= 1024;
   const int most = inside && rows / 2 > n ? rows / 2 : n;
-  const int threads = most <= 128 ? 128 : most <= 256 ? 256 : most <= 2560 ? 512 : kStepThreads;
-  page_step_kernel<<<1, threads, 0, st>>>(a, inside);
-  HIER_CHECK_CUDA(cudaGetLastError(), "page_step_kernel launch");
+  const int blocks = n > 1024 ? 8 : 1;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(most <= 128 ? 128 : most <= 256 || blocks > 1 ? 256 : kStepThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = blocks > 1;
+  HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, page_step_kernel, a, inside), "page_step_kernel launch");
   if (!inside) {
-    cudaLaunchAttribute attr = {};
+    attr = {};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((rows + 255) / 256));
+    cfg.gridDim = dim3((unsigned)(((int64_t)rows + 255) / 256));
     cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cfg.attrs = &attr;
     cfg.numAttrs = 1;
     HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, page_rows_kernel, a), "page_rows_kernel launch");
   }

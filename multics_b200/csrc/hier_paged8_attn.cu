@@ -282,30 +282,6 @@ __device__ __forceinline__ void write_pair(const Paged8Args& a, const Paged8Tile
 
 constexpr int kMinPages = 2 * kWarps;  // of a part at least
 
-// shared memory of block `rank` of the cluster, at this block's address p
-__device__ __forceinline__ uint32_t peer_smem(const void* p, int rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float ld_peer(uint32_t at) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_peer4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(at)
-               : "memory");
-  return v;
-}
-// (blocks that have left count as arrived)
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // Until the kernel before this one is done, where it was launched beside it.
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -51,6 +51,40 @@ __device__ __forceinline__ int warp_find(int n, int64_t i, F base) {
   return lo;
 }
 
+// shared memory of block `rank` of the cluster, at this block's address p
+__device__ __forceinline__ uint32_t peer_smem(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_peer32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ int64_t ld_peer64(uint32_t at) {
+  int64_t v;
+  asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_peer(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_peer4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+// (blocks that have left count as arrived)
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // A divisor known to the host: n / d for 0 <= n < 2^31 in three instructions.
 struct Divisor {
   int d;

@@ -119,6 +119,41 @@ def test_page_step_maps_rows_between_requests_without_any(n, most):
     assert d[2].tolist() == table
 
 
+@pytest.mark.parametrize("n", [1025, 2048, 5003])
+def test_page_step_of_many_requests_is_taken_or_refused_whole(n):
+    """More requests than a block has threads: pages change hands between the
+    blocks' requests, and one request's fault refuses the step of all."""
+    r, width = random.Random(n), 3
+    lengths = [r.randint(0, 190) for _ in range(n)]
+    add = [-r.randint(0, x) if r.random() < 0.6 else r.randint(0, 192 - x) for x in lengths]
+    table, at = [], 0
+    for x in lengths:
+        p = -(-x // 64)
+        table.append(list(range(at, at + p)) + [-1] * (width - p))
+        at += p
+    free = list(range(at, at + n // 4)) + [-1] * at
+    rows = sum(max(x, 0) for x in add)
+    for change in (None, 0, n // 2, n - 1):
+        d = [_i32(lengths), _i32(add), _i32(table), _i32(free), _i32([n // 4])]
+        if change is not None:
+            d[1][change] = 193
+        st = page_step(*d, rows)
+        if change is None:
+            st.check()
+            t, f = [x[:] for x in table], free[:]
+            after, count, q_start, slots, positions = P.step(lengths, add, t, f, n // 4)
+            assert st.lengths.tolist() == after and st.free_count.tolist() == [count]
+            assert st.q_start.tolist() == q_start and st.slots.tolist() == slots
+            assert st.positions.tolist() == positions
+            assert d[2].tolist() == t and d[3].tolist()[:count] == f[:count]
+        else:
+            with pytest.raises(ValueError, match="block table"):
+                st.check()
+            assert torch.equal(st.lengths, d[0]) and st.free_count.tolist() == [n // 4]
+            assert not st.q_start.any() and (st.slots == -1).all() and (st.positions == -1).all()
+            assert d[2].tolist() == table and d[3].tolist() == free
+
+
 @pytest.mark.parametrize("change,match", [
     (dict(add=[60, 64]), "free pages"), (dict(rows=5), "rows"), (dict(add=[4, 300]), "block table"),
     (dict(add=[-11, 0]), "below -length"), (dict(most=3), "above the step"),
