@@ -23,7 +23,6 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
-#include <ATen/ops/unsafe_split_with_sizes.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -321,6 +320,14 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// n elements of a vector from `at` on, as a tensor over the same memory
+at::Tensor part_of(const at::Tensor& t, int64_t at, int64_t n) {
+  auto r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+  r.unsafeGetTensorImpl()->set_storage_offset(at);
+  r.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return r;
+}
+
 // page_step(lengths, add, table, free_pages, free_count, rows, most_new, in_place) -> (lengths,
 // free_count, q_start, status, slots, positions), or a status
 PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -340,36 +347,33 @@ PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     const int in_place = PyObject_IsTrue(a[7]);
     if (in_place < 0) return nullptr;
-    std::vector<at::Tensor> t;  // [lengths, free_count,] q_start, status, slots, positions
-    const auto options = lengths->options();
-    if (in_place)
-      t = at::unsafe_split_with_sizes(at::empty({requests + 2 + 2 * rows}, options),
-                                      {requests + 1, 1, rows, rows});
-    else
-      t = at::unsafe_split_with_sizes(at::empty({2 * requests + 3 + 2 * rows}, options),
-                                      {requests, 1, requests + 1, 1, rows, rows});
-    const int at = in_place ? 0 : 2;
-    int32_t* new_lengths = data<int32_t>(in_place ? *lengths : t[0]);
-    int32_t* new_count = data<int32_t>(in_place ? *count : t[1]);
+    // [lengths, free_count,] q_start, status, slots, positions
+    const int64_t sizes[6] = {requests, 1, requests + 1, 1, rows, rows};
+    const int first = in_place ? 2 : 0;
+    int64_t starts[7] = {};
+    for (int i = first; i < 6; ++i) starts[i + 1] = starts[i] + sizes[i];
+    const at::Tensor all = at::empty({starts[6]}, lengths->options());
+    int32_t* base = data<int32_t>(all);
+    int32_t* new_lengths = in_place ? data<int32_t>(*lengths) : base;
+    int32_t* new_count = in_place ? data<int32_t>(*count) : base + starts[1];
     void* stream = stream_of(dev);
     const int rc = unlocked([&] {
       return at_hier_page_step(
           data<int32_t>(*lengths), data<int32_t>(*add), (int32_t)requests, data<int32_t>(*table),
           table->stride(0), (int32_t)table->size(1), data<int32_t>(*list), (int32_t)list->size(0),
           data<int32_t>(*count), (int32_t)rows, (int32_t)most, new_lengths, new_count,
-          data<int32_t>(t[at]), data<int32_t>(t[at + 2]), data<int32_t>(t[at + 3]),
-          data<int32_t>(t[at + 1]), stream);
+          base + starts[2], base + starts[4], base + starts[5], base + starts[3], stream);
     });
     if (rc) return PyLong_FromLong(rc);
     PyObject* result = PyTuple_New(6);
     if (!result) return nullptr;
     for (int i = 0; i < 6; ++i) {
       PyObject* one;
-      if (in_place && i < 2) {
+      if (i < first) {
         one = a[i ? 4 : 0];
         Py_INCREF(one);
       } else {
-        one = THPVariable_Wrap(std::move(t[in_place ? i - 2 : i]));
+        one = THPVariable_Wrap(part_of(all, starts[i], sizes[i]));
       }
       if (!one) {
         Py_DECREF(result);
