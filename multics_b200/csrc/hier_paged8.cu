@@ -797,7 +797,9 @@ extern "C" int hier_paged8_append(const void* k, int64_t k_stride, const void* v
                                      : paged8_append_pages_kernel<P8_E4M3>;
     kernel<<<(unsigned)blocks, 128, 0, st>>>(a);
   } else {
-    const bool few = rows <= 4 * (int64_t)n;
+    // (115 requests, 27 heads: of one token 8.3 us by 4 and 10.8 by 16, of four 21.1
+    // and 11.1)
+    const bool few = rows <= (int64_t)n;
     auto* kernel = format == P8_INT8 ? (few ? paged8_append_rows_kernel<P8_INT8, 4>
                                             : paged8_append_rows_kernel<P8_INT8, 16>)
                                      : (few ? paged8_append_rows_kernel<P8_E4M3, 4>
