@@ -637,12 +637,21 @@ Shape shape_of(int64_t rows, int group, int kv_heads, int n, int width, int max_
   const int64_t some = n < rows ? n : rows;  // requests that can have rows
   s.large_splits = 1;
   s.limit = small_pairs(width);
+  // all of it on the small kernels where that takes no longer than one CTA of the
+  // large one, its keys in parts of 16 pages (15 requests of 19 rows over two pages,
+  // 24 heads to 3: 6.8 us against 12.9; 3 of 24 over 2 000 tokens, 16 heads to 2:
+  // 16.4 against 42.6)
+  const int64_t all = ((rows * group + kRows - 1) / kRows + some) * kv_heads;  // tiles at most
+  if (n > 0 && all * (30 + 25 * (int64_t)width) <= 148 * (1200 + 67 * (int64_t)std::min(width, 16)))
+    s.limit = INT32_MAX;
   s.small = n > 0 && (most * group <= s.limit || n > 1);
   s.large = n == 0 || most * group > s.limit;
   if (s.small) {
     // (beside the large kernel most requests may be its own: two tiles each, the
-    // others in turn)
-    s.direct = s.large ? 2 : (int)((most * group + kRows - 1) / kRows);
+    // others in turn; and where max_rows says little, four waves of blocks' worth)
+    s.direct = s.large ? 2
+                       : (int)std::min<int64_t>((most * group + kRows - 1) / kRows,
+                                                std::max<int64_t>(4 * 148 * 3 / ((int64_t)n * kv_heads), 2));
     s.small_tiles = (int64_t)n * s.direct;
     s.small_splits = 1;
     s.few_pages = width <= kShortPages;
