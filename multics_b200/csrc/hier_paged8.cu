@@ -451,13 +451,21 @@ __device__ __forceinline__ void drop_nan(uint2 (&x)[N]) {
   for (int j = 0; j < N; ++j) x[j].x = word(x[j].x), x[j].y = word(x[j].y);
 }
 
-// the bytes of 16 tokens of the lane's 4 value dimensions
-__device__ __forceinline__ void load_old(const AppendItem& it, int t0, int lane, uint4 (&old)[4]) {
-  const bool whole = t0 >= it.o && t0 + 16 <= it.e;
+// the bytes of N tokens of the lane's 4 value dimensions, 4 or 16 at a time
+template <int N>
+__device__ __forceinline__ void load_old(const AppendItem& it, int t0, int lane, uint32_t (&old)[4][N / 4]) {
+  static_assert(N == 4 || N == 16, "one access to each dimension");
+  const bool whole = t0 >= it.o && t0 + N <= it.e;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    old[i] = whole ? make_uint4(0u, 0u, 0u, 0u)
-                   : *reinterpret_cast<const uint4*>(it.codes + (4 * lane + i) * kPage + t0);
+  for (int i = 0; i < 4; ++i) {
+    const uint8_t* p = it.codes + (4 * lane + i) * kPage + t0;
+    if constexpr (N == 16) {
+      const uint4 v = whole ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4*>(p);
+      old[i][0] = v.x, old[i][1] = v.y, old[i][2] = v.z, old[i][3] = v.w;
+    } else {
+      old[i][0] = whole ? 0u : *reinterpret_cast<const uint32_t*>(p);
+    }
+  }
 }
 
 template <int FMT, int N>
@@ -475,12 +483,12 @@ __device__ __forceinline__ void store_keys(const AppendItem& it, int t0, int lan
   }
 }
 
-template <int FMT>
-__device__ __forceinline__ void store_values(const AppendItem& it, int t0, int lane, const uint2 (&x)[16],
-                                             const uint4 (&old)[4], float inv, bool odd) {
-  uint32_t w[4][4];  // [dimension][4 tokens]
+template <int FMT, int N>
+__device__ __forceinline__ void store_values(const AppendItem& it, int t0, int lane, const uint2 (&x)[N],
+                                             const uint32_t (&old)[4][N / 4], float inv, bool odd) {
+  uint32_t w[4][N / 4];  // [dimension][4 tokens]
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < N / 4; ++q) {
     uint32_t c[4], t[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -492,16 +500,16 @@ __device__ __forceinline__ void store_values(const AppendItem& it, int t0, int l
     const int at = t0 + 4 * q;
     const uint32_t fresh = low_bytes(it.e - at) & ~low_bytes(it.o - at);  // the new ones of the four
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 v = old[i];
-      const uint32_t b = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
-      w[i][q] = (t[i] & fresh) | (b & ~fresh);
-    }
+    for (int i = 0; i < 4; ++i) w[i][q] = (t[i] & fresh) | (old[i][q] & ~fresh);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint4*>(it.codes + (4 * lane + i) * kPage + t0) =
-        make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+  for (int i = 0; i < 4; ++i) {
+    uint8_t* p = it.codes + (4 * lane + i) * kPage + t0;
+    if constexpr (N == 16)
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+    else
+      *reinterpret_cast<uint32_t*>(p) = w[i][0];
+  }
 }
 
 // The scale of an item: `amax` over the new tokens of the whole item.
@@ -608,16 +616,16 @@ __global__ void __launch_bounds__(128, 8) paged8_append_pages_kernel(AppendArgs 
   if (!mine) return;
   if (odd) drop_nan(x);
   if (kv) {
-    uint4 old[4];
-    load_old(it, t0, lane, old);
-    store_values<FMT>(it, t0, lane, x, old, inv, odd);
+    uint32_t old[4][4];
+    load_old<16>(it, t0, lane, old);
+    store_values<FMT, 16>(it, t0, lane, x, old, inv, odd);
   } else {
     store_keys<FMT>(it, t0, lane, x, inv, odd);
   }
 }
 
-// N tokens at a time: 4, values written byte by byte, or 16, values merged 16
-// bytes at a time.
+// N tokens of a page at a time, from a multiple of N on: 1, values written byte
+// by byte, or 4 or 16, merged with the bytes that are there.
 template <int FMT, int N>
 __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, int units) {
   const int lane = threadIdx.x & 31;
@@ -631,7 +639,7 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
   for (int pg = (rq.held - rq.n) / kPage; pg * kPage < rq.held; ++pg) {
     const int entry = a.table[b * a.table_stride + pg];
     AppendItem it = append_item(a, rq, pg, 0, head, kv, lane);
-    const int first = N == 4 ? it.o : it.o & ~15;
+    const int first = it.o & -N;
     const bool one = it.e - first <= N;  // the tokens stay in registers
     uint2 x[N];
     if (one) load_tokens(it, first, x);  // in flight before the page is known
@@ -641,12 +649,14 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
     it.codes += at * kPageHeadBytes;
     float* sp = a.scale[kv] + at + head;
     const float old_scale = it.o > 0 ? *sp : 0.f;
-    uint4 old[4];
+    uint32_t old[4][(N + 3) / 4];
     float amax = 0.f;
     bool odd = false;
     for (int t0 = first; t0 < it.e; t0 += N) {
       if (!one) load_tokens(it, t0, x);
-      if (N == 16 && kv && one) load_old(it, t0, lane, old);
+      if constexpr (N > 1) {
+        if (kv && one) load_old<N>(it, t0, lane, old);
+      }
       amax = fmaxf(amax, largest(x, odd));
     }
     amax = warp_max(amax);
@@ -665,20 +675,15 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
       if (odd) drop_nan(x);
       if (!kv) {
         store_keys<FMT>(it, t0, lane, x, inv, odd);
-      } else if constexpr (N == 16) {
-        if (!one || grown) load_old(it, t0, lane, old);
-        store_values<FMT>(it, t0, lane, x, old, inv, odd);
+      } else if constexpr (N > 1) {
+        if (!one || grown) load_old<N>(it, t0, lane, old);
+        store_values<FMT, N>(it, t0, lane, x, old, inv, odd);
       } else {
-        uint8_t* dst = it.codes + 4 * lane * kPage + t0;
+        float f[4];
+        unpack4(x[0], f);
+        const uint32_t c = encode4<FMT>(f, inv, odd);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          if (t0 + j >= it.e) break;  // uniform over the warp
-          float f[4];
-          unpack4(x[j], f);
-          const uint32_t c = encode4<FMT>(f, inv, odd);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i * kPage + j] = (uint8_t)(c >> (8 * i));
-        }
+        for (int i = 0; i < 4; ++i) it.codes[(4 * lane + i) * kPage + t0] = (uint8_t)(c >> (8 * i));
       }
     }
   }
@@ -797,13 +802,16 @@ extern "C" int hier_paged8_append(const void* k, int64_t k_stride, const void* v
                                      : paged8_append_pages_kernel<P8_E4M3>;
     kernel<<<(unsigned)blocks, 128, 0, st>>>(a);
   } else {
-    // (115 requests, 27 heads: of one token 8.3 us by 4 and 10.8 by 16, of four 21.1
-    // and 11.1)
-    const bool few = rows <= (int64_t)n;
-    auto* kernel = format == P8_INT8 ? (few ? paged8_append_rows_kernel<P8_INT8, 4>
-                                            : paged8_append_rows_kernel<P8_INT8, 16>)
-                                     : (few ? paged8_append_rows_kernel<P8_E4M3, 4>
-                                            : paged8_append_rows_kernel<P8_E4M3, 16>);
+    // (67 requests of one token, 24 heads: 5.5 us by 1 and 6.1 by 4; 115 of 4, 27
+    // heads: 7.1 by 4 and 11.4 by 16; of 6 13.3 and 11.6)
+    const auto of = [&](auto* one, auto* four, auto* sixteen) {
+      return rows <= (int64_t)n ? one : rows <= 4 * (int64_t)n ? four : sixteen;
+    };
+    auto* kernel = format == P8_INT8
+                       ? of(paged8_append_rows_kernel<P8_INT8, 1>, paged8_append_rows_kernel<P8_INT8, 4>,
+                            paged8_append_rows_kernel<P8_INT8, 16>)
+                       : of(paged8_append_rows_kernel<P8_E4M3, 1>, paged8_append_rows_kernel<P8_E4M3, 4>,
+                            paged8_append_rows_kernel<P8_E4M3, 16>);
     kernel<<<(unsigned)blocks, 128, 0, st>>>(a, (int)units);
   }
   HIER_CHECK_CUDA(cudaGetLastError(), "paged8_append launch");

@@ -321,6 +321,41 @@ def test_append_zeros_huge_tiny_and_not_finite(dtype):
     assert float(hv[4, 0, 100]) == -top * sv and float(hv[0, 0, 0]) == 0.0
 
 
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("heads", [2, 30])
+@pytest.mark.parametrize("adds", [[3, 0, 0, 1, 0, 5, 0, 0, 0], [2, 3, 4, 1, 0, 0, 4, 3, 2],
+                                  [7, 0, 1, 9, 2, 12, 0, 17, 1], [1] * 9, [4] * 9, [0] * 8 + [2]])
+def test_append_a_few_tokens_at_a_time(dtype, heads, adds):
+    """Every token has the code of its value whatever it comes with, at every
+    place of a page; what is not finite too."""
+    s = _Session(9, heads, dtype, width=3, seed=heads)
+    top = P.TOP[dtype]
+    for i in range(-1, 10):
+        add = [1 + b for b in range(9)] if i < 0 else adds
+        total = sum(add)
+        k, v = (torch.randn(total, heads * 128, generator=s.g).clamp(-4, 4).to(BF) for _ in range(2))
+        at = 0
+        for b, n in enumerate(add):  # every page's first token has the largest value: scales stay
+            held = s.k[b].shape[0]
+            for t in range(n):
+                if (held + t) % 64 == 0:
+                    k[at + t], v[at + t] = 4.0, -4.0
+            at += n
+        if i == 3 and total > 1:
+            k[1, 5], v[total - 1, 7], k[total - 1, 130], v[1, 131] = (float(x) for x in ("nan", "nan", "inf", "-inf"))
+        s.append(add, k=k, v=v)
+    for b, (k, v) in enumerate(s.held()):
+        for got, x in ((k, s.k[b].double()), (v, s.v[b].double())):
+            sc = P.scale_for(4.0, dtype)
+            want = P.encode(torch.where(x.isfinite(), x, torch.zeros_like(x)) / sc, dtype) * sc
+            want = torch.where(x.isinf(), x.sign() * top * sc, want)
+            assert torch.equal(got, want)
+    if sum(adds) > 1:
+        with pytest.raises(ValueError, match="NaN"):
+            s.cache.check()
+    s.cache.check()
+
+
 def test_append_rows_with_strides_and_another_stream():
     s, ref = _Session(2, 3, torch.int8, seed=5), _Session(2, 3, torch.int8, seed=5)
     k = torch.randn(90, 3 * 128, generator=_gen(1)).to(BF)
