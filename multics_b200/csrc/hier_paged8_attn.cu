@@ -26,8 +26,13 @@
 // order.
 // While a page's scores are computed its values are in flight, and while its
 // values are consumed the next page's keys are: the loads of one take the
-// registers that the other's products have just used.  paged8_short_kernel: a
-// warp per tile, and products over 16 or 32 keys at a time.
+// registers that the other's products have just used.  37 rows over up to 19 001
+// tokens, 32 heads to 4, e4m3: 92 us, 5.7 TB/s, 0.88 of the measured copy rate.
+// paged8_short_kernel: a warp per tile, and products over 16 or 32 keys at a
+// time, its loads issued together.  880 requests of 3 rows over 27 tokens, 24
+// heads, int8: 55 us, 4.4 TB/s (a value's 64-byte row is read whole, which makes
+// 249 MB of 126) with half of the issue slots used; more warps than the 16 of 128
+// registers spill (5 blocks per SM: 70 us).
 
 #include <math.h>
 
