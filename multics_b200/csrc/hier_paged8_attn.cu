@@ -30,7 +30,7 @@
 // tokens, 32 heads to 4, e4m3: 92 us, 5.7 TB/s, 0.88 of the measured copy rate.
 // paged8_short_kernel: a warp per tile, and products over 16 or 32 keys at a
 // time, its loads issued together.  880 requests of 3 rows over 27 tokens, 24
-// heads, int8: 55 us, 4.4 TB/s (a value's 64-byte row is read whole, which makes
+// heads, int8: 50 us, 5.0 TB/s (a value's 64-byte row is read whole, which makes
 // 249 MB of 126) with half of the issue slots used; more warps than the 16 of 128
 // registers spill (5 blocks per SM: 70 us).
 
@@ -280,8 +280,9 @@ __device__ __forceinline__ void write_pair(const Paged8Args& a, const Paged8Tile
   const float inv = L > 0.f ? 1.f / L : 0.f;
   const int64_t r = tl.rq.row0 + (int64_t)row;
   const int h = kvh * a.group + g;
-  *reinterpret_cast<uint2*>(a.out + r * a.out_stride + h * 128 + 4 * lane) = make_uint2(
-      pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  // (written past the caches' reuse: 50.1 us for 880 requests of 3 rows, else 51.6)
+  __stcs(reinterpret_cast<uint2*>(a.out + r * a.out_stride + h * 128 + 4 * lane),
+         make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)));
   if (a.lse && lane == 0) a.lse[r * a.heads + h] = row_lse(M, L);
 }
 
@@ -450,15 +451,20 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
   }
 }
 
-template <int MB>
-__device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t (&w)[MB]) {
-  static_assert(MB == 1 || MB == 2, "4 or 8 bytes");
-  if (MB == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = v.x, w[MB - 1] = v.y;
-  } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
+// Codes that no other warp reads: past the L1 cache (880 requests of 3 rows: 51.7
+// us, with it 55.0).
+__device__ __forceinline__ uint4 ld_once(const uint8_t* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+      : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t (&w)[2]) {
+  asm("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+}
+__device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t (&w)[1]) {
+  asm("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
 }
 
 // 16 * MB of a page's keys from token `base` of it.  Keys outside [from, to] of
@@ -478,14 +484,14 @@ __device__ __forceinline__ void short_keys(const Paged8Args& a, const Columns& c
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int key = min(max(key0 + 4 * m + 2 * e, from), to);
-      kr[m][e][0] = __ldg(reinterpret_cast<const uint4*>(kp + key * 64));
-      kr[m][e][1] = __ldg(reinterpret_cast<const uint4*>(kp + kPage * 64 + key * 64));
+      kr[m][e][0] = ld_once(kp + key * 64);
+      kr[m][e][1] = ld_once(kp + kPage * 64 + key * 64);
     }
   uint32_t vw[8][2][MB];
 #pragma unroll
   for (int d = 0; d < 8; ++d)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) ld_words<MB>(vp + (16 * d + 8 * e) * kPage, vw[d][e]);
+    for (int e = 0; e < 2; ++e) ld_words(vp + (16 * d + 8 * e) * kPage, vw[d][e]);
   float s[MB][4];
 #pragma unroll
   for (int m = 0; m < MB; ++m) s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
