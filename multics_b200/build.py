@@ -33,9 +33,10 @@ def nvcc() -> str:
 
 def build_bind(force: bool = False) -> Path:
     """The Python module of csrc/bind.cpp (host code, PyTorch's headers)."""
-    src, header = CSRC / "bind.cpp", ROOT / "include" / "hier_b200.h"
+    src = CSRC / "bind.cpp"
+    deps = [src, CSRC / "pycall.h", ROOT / "include" / "hier_b200.h"]
     if BIND.exists() and not force:
-        if BIND.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+        if BIND.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
             return BIND
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths

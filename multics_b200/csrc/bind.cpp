@@ -30,8 +30,12 @@
 #include <cstring>
 
 #include "hier_b200.h"
+#include "pycall.h"
 
 namespace {
+
+using pycall::attempt;
+using pycall::unlocked;
 
 // ---- entry points as they are ----------------------------------------------
 
@@ -91,10 +95,7 @@ struct Pointer {  // any data pointer
       PyErr_SetString(PyExc_RuntimeError, #NAME " is not bound");               \
       return nullptr;                                                           \
     }                                                                           \
-    PyThreadState* state = PyEval_SaveThread();                                 \
-    const int rc = at_##NAME(__VA_ARGS__);                                      \
-    PyEval_RestoreThread(state);                                                \
-    return PyLong_FromLong(rc);                                                 \
+    return PyLong_FromLong(unlocked([&] { return at_##NAME(__VA_ARGS__); }));   \
   }
 
 ENTRY(hier_head_norm_rope, "pqpqqiiippipqpfpqpqpqpqipp", P(0), Q(1), P(2), Q(3), Q(4), I(5), I(6),
@@ -182,25 +183,6 @@ bool requests_of(PyObject* const* a, at::Device dev, Requests* r) {
   r->table = tensor_of(a[0]), r->lengths = tensor_of(a[1]), r->q_start = tensor_of(a[2]);
   return is_table(r->table, dev) && is_vector(r->lengths, r->table->size(0), dev) &&
          is_vector(r->q_start, r->table->size(0) + 1, dev);
-}
-
-// None: not a call for this path
-template <class F>
-PyObject* attempt(F f) {
-  try {
-    if (PyObject* r = f()) return r;
-  } catch (const std::exception&) {  // (a tensor without data, memory run out): Python's to report
-  }
-  if (PyErr_Occurred()) return nullptr;
-  Py_RETURN_NONE;
-}
-
-template <class F>
-int unlocked(F f) {
-  PyThreadState* state = PyEval_SaveThread();
-  const int rc = f();
-  PyEval_RestoreThread(state);
-  return rc;
 }
 
 // layout(k, v, k_scale, v_scale) -> format of a cache over them
@@ -353,6 +335,21 @@ PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t starts[7] = {};
     for (int i = first; i < 6; ++i) starts[i + 1] = starts[i] + sizes[i];
     const at::Tensor all = at::empty({starts[6]}, lengths->options());
+    // (made before the launch: nothing may fail once the step has been taken)
+    PyObject* result = PyTuple_New(6);
+    if (!result) return nullptr;
+    const pycall::Owned owned{result};
+    for (int i = 0; i < 6; ++i) {
+      PyObject* one;
+      if (i < first) {
+        one = a[i ? 4 : 0];
+        Py_INCREF(one);
+      } else {
+        one = THPVariable_Wrap(part_of(all, starts[i], sizes[i]));
+      }
+      if (!one) return nullptr;
+      PyTuple_SET_ITEM(result, i, one);
+    }
     int32_t* base = data<int32_t>(all);
     int32_t* new_lengths = in_place ? data<int32_t>(*lengths) : base;
     int32_t* new_count = in_place ? data<int32_t>(*count) : base + starts[1];
@@ -365,22 +362,7 @@ PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
           base + starts[2], base + starts[4], base + starts[5], base + starts[3], stream);
     });
     if (rc) return PyLong_FromLong(rc);
-    PyObject* result = PyTuple_New(6);
-    if (!result) return nullptr;
-    for (int i = 0; i < 6; ++i) {
-      PyObject* one;
-      if (i < first) {
-        one = a[i ? 4 : 0];
-        Py_INCREF(one);
-      } else {
-        one = THPVariable_Wrap(part_of(all, starts[i], sizes[i]));
-      }
-      if (!one) {
-        Py_DECREF(result);
-        return nullptr;
-      }
-      PyTuple_SET_ITEM(result, i, one);
-    }
+    Py_INCREF(result);
     return result;
   });
 }
