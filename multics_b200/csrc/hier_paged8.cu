@@ -585,8 +585,10 @@ __global__ void __launch_bounds__(128, 8) paged8_append_pages_kernel(AppendArgs 
   const Paged8Request rq = paged8_request(a.q_start, a.lengths, b, a.rows, a.width, true,
                                           threadIdx.x == 0 && head == 0 ? a.status : nullptr);
   if (!rq.ok || rq.n == 0) return;
-  const int64_t pg = (rq.held - rq.n) / kPage + vp - ((int64_t)(rq.row0 >> 6) + 2 * (int64_t)b);
-  if (pg < 0 || pg * kPage >= rq.held) return;
+  // (rows in front of the first request have virtual pages too: nobody's)
+  const int64_t nth = vp - ((int64_t)(rq.row0 >> 6) + 2 * (int64_t)b);
+  const int64_t pg = (rq.held - rq.n) / kPage + nth;
+  if (nth < 0 || pg * kPage >= rq.held) return;
   const int entry = a.table[b * a.table_stride + pg];
   AppendItem it = append_item(a, rq, (int)pg, 0, head, kv, lane);
   const int t0 = 16 * warp;  // this warp's tokens
