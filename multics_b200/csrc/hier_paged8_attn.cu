@@ -106,8 +106,10 @@ __device__ __forceinline__ Paged8Tile small_tile(const Paged8Args& a, int b, int
   t.b = b;
   t.rho0 = rho0;
   t.lo = t.hi = t.p0 = t.np = t.pairs = 0;
-  t.rq = paged8_request(a.q_start, a.lengths, b, a.rows, a.width, false, report ? a.status : nullptr);
-  t.live = t.rq.row0 >= 0 && t.rq.n > 0 && t.rq.row0 + (int64_t)t.rq.n <= a.rows;
+  const RowSpan span = row_span(a);
+  const int row0 = a.q_start[b], row1 = a.q_start[b + 1];
+  t.rq = paged8_request(row0, row1, a.lengths[b], a.rows, a.width, false, report ? a.status : nullptr);
+  t.live = row1 > row0 && span.holds(row0, row1);
   if (!t.live) return t;
   t.pairs = t.rq.n * a.group;
   t.live = rho0 < t.pairs && t.pairs <= a.row_limit;
@@ -291,6 +293,54 @@ constexpr int kMinPages = 2 * kWarps;  // of a part at least
 // Until the kernel before this one is done, where it was launched beside it.
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// What the blocks behind the last unit do: the first of them writes zeros to the
+// rows between q_start's ends that no kernel writes, and all wait for the kernel
+// before.  There are such rows only where row starts descend or leave the row
+// tensor: those of refused requests alone, and of requests whose tiles the large
+// kernel cannot find.  (A block of its own: a tile's warps that did this for their
+// request took 5.7 us more of 51 for the registers it cost them.)
+constexpr int kKeptWords = 128;  // 4 096 rows at a time
+__device__ __forceinline__ void keep_rows(const Paged8Args& a, bool first, uint32_t* covered) {
+  const int32_t* qs = a.q_start;
+  int bad = qs[0] < 0 || qs[a.n] > a.rows;
+  if (first && a.zero_rest)
+    for (int i = threadIdx.x; i < a.n; i += blockDim.x) bad |= qs[i + 1] < qs[i];
+  bad = __syncthreads_or(bad);
+  wait_for_prior();
+  if (!bad || !first || !a.zero_rest) return;
+  const RowSpan s = row_span(a);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  for (int64_t at = s.first; at < s.end; at += 32 * kKeptWords) {
+    for (int i = threadIdx.x; i < kKeptWords; i += blockDim.x) covered[i] = 0u;
+    __syncthreads();
+    for (int b0 = 32 * warp; b0 < a.n; b0 += 32 * warps) {
+      const int b = b0 + lane, row0 = b < a.n ? qs[b] : 0, row1 = b < a.n ? qs[b + 1] : 0;
+      bool live = row1 > row0 && s.holds(row0, row1);
+      const int pairs = live ? (row1 - row0) * a.group : 0;
+      for (unsigned large = __ballot_sync(0xffffffffu, pairs > a.row_limit); large; large &= large - 1) {
+        const int of = __ffs(large) - 1;
+        const bool found = tiles_found<kPaged8LargeRows>(a, b0 + of, __shfl_sync(0xffffffffu, row0, of),
+                                                         __shfl_sync(0xffffffffu, pairs, of));
+        if (lane == of) live = found;
+      }
+      const int64_t from = max((int64_t)row0 - at, (int64_t)0);
+      const int64_t to = min((int64_t)row1 - at, (int64_t)32 * kKeptWords);
+      for (int64_t w = from / 32; live && w * 32 < to; ++w) {
+        const uint32_t below = to >= w * 32 + 32 ? ~0u : (1u << (to - w * 32)) - 1u;
+        atomicOr(covered + w, below & (from > w * 32 ? ~0u << (from - w * 32) : ~0u));
+      }
+    }
+    __syncthreads();
+    for (int64_t w = warp; w < kKeptWords; w += warps)
+      for (uint32_t rest = ~covered[w]; rest; rest &= rest - 1) {
+        const int64_t r = at + 32 * w + __ffs(rest) - 1;
+        if (r < s.end)
+          for (int kvh = 0; kvh < a.kv_heads; ++kvh) zero_row(a, r, kvh, lane);
+      }
+    __syncthreads();
+  }
+}
+
 template <int FMT>
 __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args a) {
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
@@ -302,7 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
   const int unit = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - unit * a.splits.d;
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const int b = tile / a.direct, first = tile % a.direct * kRows;
-  if (b >= a.n) return wait_for_prior();
+  if (b >= a.n) return keep_rows(a, split == 0, reinterpret_cast<uint32_t*>(so));
   if (a.zero_rest && split == 0)
     zero_rest(a, kvh, (int64_t)tile * kWarps + w, (int64_t)a.n * a.direct * kWarps, lane);
   // Tiles beyond those the launch counted on (a request of more rows than
@@ -526,7 +576,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
   __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if ((int)blockIdx.x * kWarps >= units) return wait_for_prior();
+  if ((int)blockIdx.x * kWarps >= units) return keep_rows(a, true, reinterpret_cast<uint32_t*>(so));
   const int unit = blockIdx.x * kWarps + w;
   if (unit >= units) return;
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
@@ -722,11 +772,12 @@ int launch_merge(const Paged8Args& a, int64_t tiles, cudaStream_t st) {
 
 // beside: on the stream after the large kernel, without waiting for it (its
 // requests are others, and its blocks leave SMs idle: few of them, or the last
-// wave's).  The blocks of one unit more do wait for it, so that what follows on
-// the stream finds both done.
+// wave's).  The blocks of one unit more (keep_rows) do wait for it, so that what
+// follows on the stream finds both done.
 int launch_small(const Paged8Args& a, int format, int64_t tiles, bool few_pages, bool beside,
                  cudaStream_t st) {
   const int64_t units = tiles * a.kv_heads * a.splits;
+  const int keep = beside || a.zero_rest;
   if (units > INT32_MAX - 2 * kWarps * a.splits) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
@@ -743,7 +794,7 @@ int launch_small(const Paged8Args& a, int format, int64_t tiles, bool few_pages,
   }
   if (few_pages) {
     auto* kernel = format == P8_INT8 ? paged8_short_kernel<P8_INT8> : paged8_short_kernel<P8_E4M3>;
-    cfg.gridDim = dim3((unsigned)((units + kWarps - 1) / kWarps + beside));
+    cfg.gridDim = dim3((unsigned)((units + kWarps - 1) / kWarps + keep));
     HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, (int)units), "paged8_short_kernel launch");
     return HIER_OK;
   }
@@ -754,7 +805,7 @@ int launch_small(const Paged8Args& a, int format, int64_t tiles, bool few_pages,
     dim.val.clusterDim.x = a.splits.d;
     dim.val.clusterDim.y = dim.val.clusterDim.z = 1;
   }
-  cfg.gridDim = dim3((unsigned)(units + (beside ? a.splits.d : 0)));
+  cfg.gridDim = dim3((unsigned)(units + (keep ? a.splits.d : 0)));
   HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a), "paged8_long_kernel launch");
   return a.splits > 1 && !a.cluster ? launch_merge<kPaged8SmallRows>(a, tiles, st) : HIER_OK;
 }

@@ -706,6 +706,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_mma_kernel(Paged8Args a, i
   const bool rest = a.zero_rest && split == 0 && (warp & ~1) == 2;  // warps 2 and 3
   const int64_t rest0 = 2 * (int64_t)(unit / a.kv_heads) + (warp & 1);
   if (!J.tl.live || J.tl.pairs <= a.row_limit) {
+    // (this kernel is by itself for one request at most, whose row starts may lie
+    // behind every tile; block 0's is behind those of all requests)
+    if (a.n == 1 && blockIdx.x == 0 && threadIdx.x == 0)
+      paged8_request(a.q_start, a.lengths, 0, a.rows, a.width, false, a.status);
     if (rest) zero_rest(a, J.kvh, rest0, 2 * tiles, lane);
     return;
   }

@@ -63,6 +63,21 @@ __host__ __device__ inline int64_t paged8_tiles(int64_t rows, int group, int n) 
   return rows * group / kRows + (n < rows ? n : rows) + 1;
 }
 
+// The rows that requests can have: q_start's ends, within the row tensor.  A
+// request whose rows leave them is refused, so that the rows outside are
+// nobody's whatever stands between the ends.
+struct RowSpan {
+  int first, end;
+  __device__ __forceinline__ bool holds(int row0, int row1) const { return row0 >= first && row1 <= end; }
+};
+__device__ __forceinline__ RowSpan row_span(int first, int end, int rows) {
+  first = max(0, min(first, rows));
+  return {first, max(first, min(end, rows))};
+}
+__device__ __forceinline__ RowSpan row_span(const Paged8Args& a) {
+  return row_span(a.q_start[0], a.q_start[a.n], a.rows);
+}
+
 struct Paged8Tile {
   int b;
   Paged8Request rq;
@@ -99,6 +114,34 @@ __device__ __forceinline__ void paged8_span(const Paged8Args& a, Paged8Tile& t, 
   }
 }
 
+// Number of a request's first tile, b and q_start[b] given.
+template <int kRows>
+__device__ __forceinline__ int64_t first_tile(const Paged8Args& a, int b, int row0) {
+  return row0 * (int64_t)a.group.d / kRows + min(b, row0);
+}
+
+// The request (n: none) that tile `tile` is of, if row starts ascend; q: the
+// lane's row start where n < 32.
+template <int kRows>
+__device__ __forceinline__ int tile_request(const Paged8Args& a, int64_t tile, int q) {
+  const int32_t* qs = a.q_start;
+  if (a.n < 32) {
+    const int lane = threadIdx.x & 31;
+    return 31 - __clz(__ballot_sync(0xffffffffu, lane <= a.n && first_tile<kRows>(a, lane, q) <= tile) | 1u);
+  }
+  return warp_find(a.n + 1, tile, [&](int i) { return first_tile<kRows>(a, i, qs[i]); });
+}
+
+// Whether every tile of request b is found to be its.  (As the first and the
+// last are, so are those between: a search compares with tiles alone, and its
+// outcomes ascend with the tile.)
+template <int kRows>
+__device__ __forceinline__ bool tiles_found(const Paged8Args& a, int b, int row0, int pairs) {
+  const int q = a.q_start[min((int)(threadIdx.x & 31), a.n)];
+  const int64_t first = first_tile<kRows>(a, b, row0);
+  return tile_request<kRows>(a, first, q) == b && tile_request<kRows>(a, first + (pairs - 1) / kRows, q) == b;
+}
+
 template <int kRows>
 __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t tile, bool report) {
   Paged8Tile t;
@@ -106,28 +149,28 @@ __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t t
   const int64_t G = a.group.d;
   t.live = false;
   t.rho0 = t.pairs = t.lo = t.hi = t.p0 = t.np = 0;
-  int row0, row1, held;
+  int row0, row1, held, starts, ends;
   if (a.n < 32) {  // one read of everything
     const int lane = threadIdx.x & 31, i = min(lane, a.n);
     const int q = qs[i], len = a.n ? a.lengths[min(lane, a.n - 1)] : 0;
-    const unsigned le =
-        __ballot_sync(0xffffffffu, lane <= a.n && q * G / kRows + min(lane, q) <= tile);
-    t.b = 31 - __clz(le | 1u);
+    t.b = tile_request<kRows>(a, tile, q);
     row0 = __shfl_sync(0xffffffffu, q, t.b);
     row1 = __shfl_sync(0xffffffffu, q, min(t.b + 1, 31));
     held = __shfl_sync(0xffffffffu, len, t.b);
+    starts = __shfl_sync(0xffffffffu, q, 0);
+    ends = __shfl_sync(0xffffffffu, q, a.n);
   } else {
-    t.b = warp_find(a.n + 1, tile, [=](int i) { return qs[i] * G / kRows + min(i, qs[i]); });
+    t.b = tile_request<kRows>(a, tile, 0);
     row0 = qs[t.b];
     row1 = t.b < a.n ? qs[t.b + 1] : 0;
     held = t.b < a.n ? a.lengths[t.b] : 0;
+    starts = qs[0], ends = qs[a.n];
   }
-  const int64_t first = row0 * G / kRows + min(t.b, row0);
+  const int64_t first = first_tile<kRows>(a, t.b, row0);
   if (tile < first || t.b == a.n) return t;  // rows of no request
   const int64_t rho0 = (tile - first) * kRows;
   t.rq = paged8_request(row0, row1, held, a.rows, a.width, false, report ? a.status : nullptr);
-  if (t.rq.row0 < 0 || t.rq.n <= 0 || t.rq.row0 + (int64_t)t.rq.n > a.rows || rho0 >= t.rq.n * G)
-    return t;
+  if (row1 <= row0 || !row_span(starts, ends, a.rows).holds(row0, row1) || rho0 >= t.rq.n * G) return t;
   if (!t.rq.ok) t.rq.held = 0;  // a length outside the table: the rows see nothing
   t.live = true;
   t.rho0 = (int)rho0;
@@ -136,20 +179,21 @@ __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t t
   return t;
 }
 
-// Zeros to the rows before the first request and behind the last one, a warp's
-// heads of key head kvh; worker i of n takes every n-th row.
+// Zeros to a warp's heads, those of key head kvh, of a row.
+__device__ __forceinline__ void zero_row(const Paged8Args& a, int64_t r, int kvh, int lane) {
+  uint4* dst = reinterpret_cast<uint4*>(a.out + r * a.out_stride + kvh * a.group.d * 128);
+  for (int e = lane; e < a.group.d * 16; e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
+  if (a.lse)
+    for (int e = lane; e < a.group.d; e += 32) a.lse[r * a.heads + kvh * a.group.d + e] = -INFINITY;
+}
+
+// Zeros to the rows before the first request and behind the last one (to all
+// where the only one is refused); worker i of n takes every n-th row.
 __device__ __forceinline__ void zero_rest(const Paged8Args& a, int kvh, int64_t i, int64_t n, int lane) {
-  const int first = a.q_start[0], end = a.q_start[a.n];
-  if (first < 0 || end < first) return;
-  const int64_t rest = (int64_t)a.rows - (end - first);
-  for (int64_t j = i; j < rest; j += n) {
-    const int64_t r = j < first ? j : j + (end - first);
-    if (r >= a.rows) return;
-    uint4* dst = reinterpret_cast<uint4*>(a.out + r * a.out_stride + kvh * a.group.d * 128);
-    for (int e = lane; e < a.group.d * 16; e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
-    if (a.lse)
-      for (int e = lane; e < a.group.d; e += 32) a.lse[r * a.heads + kvh * a.group.d + e] = -INFINITY;
-  }
+  const RowSpan s = row_span(a);
+  const int64_t between = a.n == 1 && !s.holds(a.q_start[0], a.q_start[1]) ? 0 : s.end - s.first;
+  for (int64_t j = i; j < a.rows - between; j += n)
+    zero_row(a, j < s.first ? j : j + between, kvh, lane);
 }
 
 // log2-sum-exp of a pair from its maximum and sum: -inf where nothing was seen,

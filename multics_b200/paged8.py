@@ -316,8 +316,8 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
     in a cross-attention) and, with a ``window``, when it is less than
     ``window`` frames back: ``cached_frame_mask`` over token positions.
     Rows that see nothing are 0.  Rows of no request (before the first, behind
-    the last) are zeros, or left as they were in a given ``out``, which may be
-    ``q`` itself.  ``max_rows``: the most rows any request has, where the caller
+    the last, or those of a request whose row starts are refused) are zeros, or
+    left as they were in a given ``out``, which may be ``q`` itself.  ``max_rows``: the most rows any request has, where the caller
     knows it; it chooses kernels, not results.
     Returns ``[T, num_heads * 128]`` bf16, with ``return_lse`` also the float32
     ``[T, num_heads]`` log2-sum-exp of the scaled scores."""

@@ -80,3 +80,65 @@ def test_append_behind_rows_of_no_request(dtype, first, rows):
     for name in ("k", "v", "k_scale", "v_scale"):
         assert torch.equal(getattr(c, name).view(torch.int8), getattr(alone, name).view(torch.int8)), name
     c.check(), alone.check()
+
+
+def _pool(pages, heads, dtype=torch.int8, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    c = Paged8Cache(pages, heads, dtype=dtype)
+    for t in (c.k, c.v):
+        t.copy_(torch.randint(-120, 120, t.shape, generator=g).to(dtype))
+    c.k_scale.fill_(2.0 ** -7), c.v_scale.fill_(2.0 ** -6)
+    return c, g
+
+
+def _poisoned(call):
+    """call() where the memory it gets for its results held other numbers."""
+    out, lse = call()
+    out.fill_(7.0), lse.fill_(7.0)
+    del out, lse
+    return call()
+
+
+# row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
+REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
+           ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),
+           ([1, 2, -3, 7, 2], [(0, 1)]), ([0, 0, 1, 5, 5], [(1, 2)]), ([0, 1, 7, 1, 2], []), ([0, 9, 0, 9, 2], [(0, 2)])]
+
+
+@pytest.mark.parametrize("starts,none", REFUSED)
+@pytest.mark.parametrize("rows", [1, 33, 300, 1500])
+@pytest.mark.parametrize("width", [4, 40])
+def test_rows_of_refused_requests_are_zeros(starts, none, rows, width):
+    """As those of refused lengths: nothing of a result is left as allocated."""
+    n, heads = len(starts) - 1, 4
+    c, g = _pool(n * 4, 2)
+    table = torch.full((n, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :4] = _i32([[4 * b, 4 * b + 1, 4 * b + 2, 4 * b + 3] for b in range(n)])
+    q = torch.randn(2 * rows, heads * 128, generator=g).to(BF).cuda()
+    lengths = _i32([200] * n)
+    qs = _i32([s * rows for s in starts])
+    out, lse = _poisoned(lambda: paged8_attention(q, c, table, lengths, qs, heads, block_frames=0, return_lse=True))
+    with pytest.raises(ValueError, match="row starts"):
+        c.check()
+    dead = torch.zeros(2 * rows, dtype=torch.bool, device="cuda")
+    for a, b in none:
+        dead[a * rows:b * rows] = True
+    assert (out[dead] == 0).all() and (lse[dead] == float("-inf")).all()
+    for b in range(n):
+        a, e = starts[b], starts[b + 1]
+        if 0 <= a < e <= 2 and not dead[a * rows:e * rows].any():
+            want, want_lse = paged8_attention(q[a * rows:e * rows], c, table[b:b + 1], lengths[:1],
+                                              _i32([0, (e - a) * rows]), heads, block_frames=0, return_lse=True)
+            got = out[a * rows:e * rows].float()
+            # (which kernel, and which parts are joined, may differ: a rounding of the output)
+            descend = any(x > y for x, y in zip(starts, starts[1:]))
+            if descend and (got == 0).all():  # (starts that descend may hide a long request)
+                assert (lse[a * rows:e * rows] == float("-inf")).all()
+                continue
+            assert ((got - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -9 * want.float().abs().max()).all()
+            assert torch.allclose(lse[a * rows:e * rows], want_lse, rtol=0, atol=2.0 ** -9)
+    assert torch.isfinite(out).all()
+    given = torch.full_like(q, 7.0)
+    paged8_attention(q, c, table, lengths, qs, heads, block_frames=0, out=given)
+    assert (given[dead] == 7).all()
+    assert ((given[~dead] == out[~dead]) | ((given[~dead] == 7) & (out[~dead] == 0))).all()
