@@ -817,8 +817,8 @@ int hier_paged8_append(const void* k, int64_t k_stride, const void* v, int64_t v
  * (frames of `frame` tokens, causal blocks of `block` frames, window in
  * frames).  out bf16 [rows][heads*128] (may be q) is 0 for rows that see
  * nothing; rows of no request (those that a request with refused row starts
- * alone has among them, and of other requests where starts descend) are left,
- * or zeroed with zero_rest.  lse (or
+ * alone has among them, and of other requests where starts descend) are left
+ * (zero_rest 0), zeroed (1; their lse -inf) or only their lse is -inf (2).  lse (or
  * NULL): float [rows][heads], log2-sum-exp of the scaled scores.  max_rows: the most
  * rows a request has, as far as the caller knows (it chooses kernels, not
  * results); <= 0: unknown.  softmax_scale is positive and finite.  workspace:

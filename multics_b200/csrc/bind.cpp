@@ -281,7 +281,8 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
           data<float>(*c.v_scale), (int32_t)c.pages, data<int32_t>(*r.table), r.table->stride(0),
           (int32_t)r.table->size(1), data<int32_t>(*r.lengths), data<int32_t>(*r.q_start),
           (int32_t)r.table->size(0), (int32_t)frame, (int32_t)block, (int32_t)window, scale,
-          (int32_t)most, o.data_ptr(), o.stride(0), with_lse ? data<float>(lse) : nullptr, !given,
+          (int32_t)most, o.data_ptr(), o.stride(0), with_lse ? data<float>(lse) : nullptr,
+          !given ? 1 : with_lse ? 2 : 0,
           floats ? data<float>(workspace) : nullptr, data<int32_t>(*c.status), data<int32_t>(*err),
           stream);
     });

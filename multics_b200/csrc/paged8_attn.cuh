@@ -42,7 +42,7 @@ struct Paged8Args {
   __nv_bfloat16* out;
   int64_t out_stride;
   float* lse;       // [rows][heads] log2-sum-exp, or NULL
-  int zero_rest;    // write zeros to the rows of no request
+  int zero_rest;    // rows of no request: 1 zeros, 2 their log-sum-exp alone, 0 left
   Divisor splits;   // most parts a tile's keys are cut into
   float* part_o;    // [tile][kv head][split][kRows][128]
   float* part_ml;   // [tile][kv head][split][kRows][2]
@@ -179,10 +179,11 @@ __device__ __forceinline__ Paged8Tile paged8_tile(const Paged8Args& a, int64_t t
   return t;
 }
 
-// Zeros to a warp's heads, those of key head kvh, of a row.
+// Zeros to a warp's heads, those of key head kvh, of a row, as zero_rest says.
 __device__ __forceinline__ void zero_row(const Paged8Args& a, int64_t r, int kvh, int lane) {
   uint4* dst = reinterpret_cast<uint4*>(a.out + r * a.out_stride + kvh * a.group.d * 128);
-  for (int e = lane; e < a.group.d * 16; e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
+  if (a.zero_rest == 1)
+    for (int e = lane; e < a.group.d * 16; e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
   if (a.lse)
     for (int e = lane; e < a.group.d; e += 32) a.lse[r * a.heads + kvh * a.group.d + e] = -INFINITY;
 }

@@ -320,7 +320,8 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
     left as they were in a given ``out``, which may be ``q`` itself.  ``max_rows``: the most rows any request has, where the caller
     knows it; it chooses kernels, not results.
     Returns ``[T, num_heads * 128]`` bf16, with ``return_lse`` also the float32
-    ``[T, num_heads]`` log2-sum-exp of the scaled scores."""
+    ``[T, num_heads]`` log2-sum-exp of the scaled scores (-inf for rows that see
+    nothing and rows of no request)."""
     if cache.device.type == "cuda":
         done = _lib.calls().attention(
             cache.k, cache.v, cache.k_scale, cache.v_scale, cache.status, cache.format, q, table, lengths,
@@ -378,7 +379,7 @@ def paged8_attention(q, cache: Paged8Cache, table, lengths, q_start, num_heads: 
         cache.v_scale.data_ptr(), cache.num_pages, table.data_ptr(), stride, width,
         lengths.data_ptr(), q_start.data_ptr(), n, int(tokens_per_frame), int(block_frames),
         int(window), scale, most, o.data_ptr(), o.stride(0),
-        None if lse is None else lse.data_ptr(), out is None,
+        None if lse is None else lse.data_ptr(), 1 if out is None else 2 if return_lse else 0,
         None if ws is None else ws.data_ptr(), cache.status.data_ptr(),
         dev_err(dev).data_ptr(), raw_stream(dev.index))
     if rc:

@@ -99,6 +99,34 @@ def _poisoned(call):
     return call()
 
 
+@pytest.mark.parametrize("first,rows,tail", [(0, 1, 3), (2, 40, 0), (64, 300, 5), (3, 3000, 7)])
+@pytest.mark.parametrize("width", [4, 40])
+@pytest.mark.parametrize("requests", [1, 2])
+def test_log_sum_of_rows_of_no_request_beside_a_given_out(first, rows, tail, width, requests):
+    """The log-sum-exp is always a new tensor: -inf where no request is."""
+    heads, starts = 4, [first + b * rows for b in range(requests + 1)]
+    T = starts[-1] + tail
+    c, g = _pool(4, 2)
+    table = torch.full((requests, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :4] = _i32([0, 1, 2, 3])
+    q = torch.randn(T, heads * 128, generator=g).to(BF).cuda()
+    args = (q, c, table, _i32([200] * requests), _i32(starts), heads)
+    out, lse = _poisoned(lambda: paged8_attention(*args, block_frames=0, return_lse=True))
+    given = torch.empty_like(q)
+
+    def call():
+        given.fill_(7.0)
+        return paged8_attention(*args, block_frames=0, out=given, return_lse=True)[0].clone(), \
+            paged8_attention(*args, block_frames=0, out=given, return_lse=True)[1]
+
+    for i in range(2):
+        kept, other = _poisoned(call)
+        assert torch.equal(other, lse) and (lse[:first] == float("-inf")).all()
+        assert (lse[starts[-1]:] == float("-inf")).all() and torch.isfinite(lse[first:starts[-1]]).all()
+        assert torch.equal(kept[first:starts[-1]], out[first:starts[-1]])
+        assert (kept[:first] == 7).all() and (kept[starts[-1]:] == 7).all()
+
+
 # row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
 REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
            ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),
