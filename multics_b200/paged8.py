@@ -38,7 +38,7 @@ PAGE_TOKENS = 64
 HEAD_DIM = 128
 _I32, _BF16 = torch.int32, torch.bfloat16
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
-_STATUS = {}
+_STATUS = {}  # (device, stream): words that no cache has yet
 _SPLIT = torch.unsafe_split_with_sizes  # (integers: no versions to share)
 
 _CACHE_BITS = ((1, "row starts leave the rows or descend"),
@@ -49,6 +49,28 @@ _STEP_BITS = ((1, "too few free pages"), (2, "more new tokens than rows"),
               (4, "a length leaves the block table"),
               (8, "an addition is below -length or above the step's most"),
               (16, "the free count leaves the free list"))
+
+
+def _status_word(dev):
+    """A zero status word of its own for a cache: one of 256 zeroed together on
+    the current stream, or one of the graph that is being captured (whose memory
+    lasts as long as the graph)."""
+    if dev.type != "cuda":
+        key = dev, 0
+    elif not is_current(dev):
+        with torch.cuda.device(dev):
+            return _status_word(dev)
+    elif torch.cuda.is_current_stream_capturing():
+        return torch.zeros(1, dtype=_I32, device=dev)
+    else:
+        key = dev, raw_stream(dev.index)
+    try:
+        return _STATUS[key].pop()
+    except (KeyError, IndexError):
+        words = list(_SPLIT(torch.zeros(256, dtype=_I32, device=dev), (1,) * 256))
+        word = words.pop()
+        _STATUS[key] = words
+        return word
 
 
 def _vector(name, t, n, dev):
@@ -128,18 +150,14 @@ class Paged8Cache:
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale, status=None) -> "Paged8Cache":
         """A cache over tensors in the layout above (finite codes, power-of-two
-        scales, in ``[2^-126, 2^126]``).  Without ``status`` (int32 ``[1]``, zero)
-        the caches made this way share one word per device; one made while a
+        scales, in ``[2^-126, 2^126]``).  ``status`` (int32 ``[1]``, zero): a word
+        to record faults in, where caches are to share one.  A cache made while a
         graph is captured has a word of that graph."""
         if _lib.calls().layout(k, v, k_scale, v_scale) is None:
             cls._refuse(k, v, k_scale, v_scale)
         dev = k.device
         if status is None:
-            status = _STATUS.get(dev)
-            if status is None:
-                status = torch.zeros(1, dtype=_I32, device=dev)
-                if dev.type != "cuda" or not torch.cuda.is_current_stream_capturing():
-                    _STATUS[dev] = status
+            status = _status_word(dev)
         else:
             _vector("status", status, 1, dev)
         self = cls.__new__(cls)

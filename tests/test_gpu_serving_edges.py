@@ -127,6 +127,25 @@ def test_log_sum_of_rows_of_no_request_beside_a_given_out(first, rows, tail, wid
         assert (kept[:first] == 7).all() and (kept[starts[-1]:] == 7).all()
 
 
+def test_every_cache_has_its_status_word():
+    """A fault in one layer's cache is that cache's: no other reports or clears it."""
+    pools = [_pool(2, 1)[0] for _ in range(3)]
+    layers = [Paged8Cache.from_tensors(c.k, c.v, c.k_scale, c.v_scale) for c in pools for _ in range(200)]
+    assert len({c.status.data_ptr() for c in layers}) == len(layers)
+    q, bad = torch.ones(1, 128, dtype=BF, device="cuda"), _i32([[-1]])
+    for c in (layers[0], layers[450]):
+        paged8_attention(q, c, bad, _i32([5]), _i32([0, 1]), 1)
+    for i, c in enumerate(layers):
+        if i in (0, 450):
+            with pytest.raises(ValueError, match="page pool"):
+                c.check()
+        c.check()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        c = Paged8Cache.from_tensors(pools[0].k, pools[0].v, pools[0].k_scale, pools[0].v_scale)
+        c.check()
+
+
 # row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
 REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
            ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),

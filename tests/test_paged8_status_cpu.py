@@ -1,0 +1,42 @@
+"""Status words of 8-bit caches (no GPU work)."""
+
+import threading
+
+import pytest
+import torch
+
+from multics_b200 import paged8
+from multics_b200.paged8 import Paged8Cache
+
+
+def _layers(n):
+    c = Paged8Cache(2, 1, device="cpu")
+    return [Paged8Cache.from_tensors(c.k, c.v, c.k_scale, c.v_scale) for _ in range(n)]
+
+
+def test_every_cache_has_its_word():
+    a, *rest = layers = _layers(600)
+    assert len({c.status.data_ptr() for c in layers}) == 600
+    a.status.fill_(4)
+    for c in rest:
+        c.check()
+    with pytest.raises(ValueError, match="page pool"):
+        a.check()
+    a.check()
+
+
+def test_a_given_word_is_shared():
+    a = Paged8Cache(2, 1, device="cpu")
+    b = Paged8Cache.from_tensors(a.k, a.v, a.k_scale, a.v_scale, a.status)
+    assert b.status is a.status
+
+
+def test_words_are_handed_out_once_to_threads():
+    paged8._STATUS.clear()
+    seen = []
+    threads = [threading.Thread(target=lambda: seen.extend(_layers(300))) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len({c.status.data_ptr() for c in seen}) == 2400
