@@ -809,6 +809,10 @@ int hier_paged8_append(const void* k, int64_t k_stride, const void* v, int64_t v
                        int64_t table_stride, int32_t width, const int32_t* lengths,
                        const int32_t* q_start, int32_t n, int32_t* status, void* stream);
 
+/* *bits = what *status holds, which is 0 from then on: one atomic exchange, so
+ * that no kernel's record made meanwhile is lost. */
+int hier_status_take(int32_t* status, int32_t* bits, void* stream);
+
 /* Attention of q (bf16 [rows][heads*128], 16-byte aligned) over the cache:
  * query head h reads key head h / (heads / kv_heads).  Row i of request b is
  * at position p = lengths[b] - (its rows) + i and sees token j when

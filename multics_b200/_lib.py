@@ -210,6 +210,7 @@ _SIGS = {
                                c_int32, _P, _P, _P, _P, _P, _P, _P]),
     "hier_paged8_append": (c_int, [_P, c_int64, _P, c_int64, c_int32, c_int32, c_int32, _P, _P, _P,
                                    _P, c_int32, _P, c_int64, c_int32, _P, _P, c_int32, _P, _P]),
+    "hier_status_take": (c_int, [_P, _P, _P]),
     "hier_paged8_attn_workspace": (c_int, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                            _P]),
     "hier_paged8_attn": (c_int, [_P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P,
@@ -223,7 +224,7 @@ _SIGS = {
 _LIB = None
 
 # hier_abi_version() of the library these signatures describe
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 
 def lib():

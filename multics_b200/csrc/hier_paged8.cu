@@ -692,10 +692,23 @@ __global__ void __launch_bounds__(128) paged8_append_rows_kernel(AppendArgs a, i
   }
 }
 
+__global__ void status_take_kernel(int32_t* status, int32_t* bits) { *bits = atomicExch(status, 0); }
+
 }  // namespace
 }  // namespace hier
 
 using namespace hier;
+
+extern "C" int hier_status_take(int32_t* status, int32_t* bits, void* stream) {
+  clear_error();
+  if (!status || !bits) {
+    set_error(HIER_EVALUE, "no status word, or no place for its bits");
+    return HIER_EVALUE;
+  }
+  status_take_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(status, bits);
+  HIER_CHECK_CUDA(cudaGetLastError(), "status_take_kernel launch");
+  return HIER_OK;
+}
 
 extern "C" int hier_page_step(const int32_t* lengths, const int32_t* add, int32_t n, int32_t* table,
                               int64_t table_stride, int32_t width, int32_t* free_pages,

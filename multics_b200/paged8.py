@@ -22,6 +22,7 @@ length outside the table) it skips and records in the cache's status word
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import NamedTuple, Optional
@@ -188,8 +189,15 @@ class Paged8Cache:
     def check(self):
         """Raise ValueError for what the kernels recorded since the last check
         (one host read)."""
-        bits = int(self.status.item())
-        self.status.zero_()
+        if self.device.type == "cuda":  # (read and cleared at once: nothing recorded meanwhile is lost)
+            with contextlib.nullcontext() if is_current(self.device) else torch.cuda.device(self.device):
+                taken = torch.empty_like(self.status)
+                check(_lib.lib().hier_status_take(self.status.data_ptr(), taken.data_ptr(),
+                                                  raw_stream(self.device.index)))
+            bits = int(taken.item())
+        else:
+            bits = int(self.status.item())
+            self.status &= ~bits
         _raise_bits("8-bit cache", bits, _CACHE_BITS)
 
     def dequantized(self):

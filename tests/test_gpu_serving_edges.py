@@ -146,6 +146,12 @@ def test_every_cache_has_its_status_word():
         c.check()
 
 
+def test_what_is_recorded_during_a_check_is_kept(monkeypatch):
+    from test_paged8_status_cpu import late_record
+
+    late_record(_pool(2, 1)[0], monkeypatch)
+
+
 # row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
 REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
            ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),

@@ -25,6 +25,31 @@ def test_every_cache_has_its_word():
     a.check()
 
 
+def test_what_is_recorded_during_a_check_is_kept(monkeypatch):
+    c, = _layers(1)
+    late_record(c, monkeypatch)
+
+
+def late_record(c, monkeypatch):
+    """A kernel on another stream records a length while check() reads."""
+    item, late = torch.Tensor.item, [2]
+
+    def read(t):
+        v = item(t)
+        if late:
+            c.status.bitwise_or_(late.pop())
+        return v
+
+    c.status.fill_(4)
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, "item", read)
+        with pytest.raises(ValueError, match="page pool"):
+            c.check()
+    with pytest.raises(ValueError, match="block table"):
+        c.check()
+    c.check()
+
+
 def test_a_given_word_is_shared():
     a = Paged8Cache(2, 1, device="cpu")
     b = Paged8Cache.from_tensors(a.k, a.v, a.k_scale, a.v_scale, a.status)
