@@ -52,6 +52,11 @@ _STEP_BITS = ((1, "too few free pages"), (2, "more new tokens than rows"),
               (16, "the free count leaves the free list"))
 
 
+def _zeros(n, dev):
+    with torch.inference_mode(False):  # (a word may be made in that mode and cleared outside)
+        return torch.zeros(n, dtype=_I32, device=dev)
+
+
 def _status_word(dev):
     """A zero status word of its own for a cache: one of 256 zeroed together on
     the current stream, or one of the graph that is being captured (whose memory
@@ -62,13 +67,13 @@ def _status_word(dev):
         with torch.cuda.device(dev):
             return _status_word(dev)
     elif torch.cuda.is_current_stream_capturing():
-        return torch.zeros(1, dtype=_I32, device=dev)
+        return _zeros(1, dev)
     else:
         key = dev, raw_stream(dev.index)
     try:
         return _STATUS[key].pop()
     except (KeyError, IndexError):
-        words = list(_SPLIT(torch.zeros(256, dtype=_I32, device=dev), (1,) * 256))
+        words = list(_zeros(256, dev).unsafe_split_with_sizes((1,) * 256))
         word = words.pop()
         _STATUS[key] = words
         return word
@@ -138,10 +143,9 @@ class Paged8Cache:
             raise ValueError(f"invalid num_pages={num_pages} or num_heads={num_heads}")
         dev = torch.device(device)
         shape = (num_pages, num_heads)
-        self._set(torch.zeros(*shape, 2, PAGE_TOKENS, 64, dtype=torch.int8, device=dev).view(dtype),
-                  torch.zeros(*shape, HEAD_DIM, PAGE_TOKENS, dtype=torch.int8, device=dev).view(dtype),
-                  torch.ones(shape, device=dev), torch.ones(shape, device=dev),
-                  torch.zeros(1, dtype=torch.int32, device=dev))
+        k = torch.zeros(*shape, 2, PAGE_TOKENS, 64, dtype=torch.int8, device=dev).view(dtype)
+        self._set(k, torch.zeros(*shape, HEAD_DIM, PAGE_TOKENS, dtype=torch.int8, device=dev).view(dtype),
+                  torch.ones(shape, device=dev), torch.ones(shape, device=dev), _status_word(k.device))
 
     def _set(self, k, v, k_scale, v_scale, status):
         self.k, self.v, self.k_scale, self.v_scale, self.status = k, v, k_scale, v_scale, status

@@ -25,6 +25,20 @@ def test_every_cache_has_its_word():
     a.check()
 
 
+def test_caches_of_inference_mode_are_checked_outside():
+    paged8._STATUS.clear()
+    with torch.inference_mode():
+        made = [*_layers(2), Paged8Cache(2, 1, device="cpu")]
+    later, = _layers(1)
+    for c in (*made, later):
+        c.status.fill_(4)
+        with pytest.raises(ValueError, match="page pool"):
+            c.check()
+        c.check()
+        with torch.inference_mode():
+            c.check()
+
+
 def test_what_is_recorded_during_a_check_is_kept(monkeypatch):
     c, = _layers(1)
     late_record(c, monkeypatch)
