@@ -457,7 +457,8 @@ struct HeadNormFn : torch::autograd::Function<HeadNormFn> {
                          const at::Tensor& wk, const HeadNorm* h, int* rc) {
     at::Tensor qo, ko;
     *rc = head_norm_forward(*h, &qo, &ko);
-    ctx->save_for_backward({q, k, wq, wk, *h->freqs, h->pos ? *h->pos : at::Tensor(), *h->err});
+    ctx->save_for_backward({q, k, wq, wk, *h->freqs, h->pos ? *h->pos : at::Tensor()});
+    ctx->saved_data["err"] = *h->err;  // (no input: cleared when a caller likes)
     ctx->saved_data["sizes"] = std::vector<int64_t>{h->heads, h->kv_heads, h->D};
     ctx->saved_data["eps"] = (double)h->eps;
     return {qo, ko};
@@ -465,7 +466,8 @@ struct HeadNormFn : torch::autograd::Function<HeadNormFn> {
 
   static Tensors backward(Context* ctx, Tensors g) {
     const Tensors s = ctx->get_saved_variables();
-    const at::Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3], &freqs = s[4], &pos = s[5], &err = s[6];
+    const at::Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3], &freqs = s[4], &pos = s[5];
+    const at::Tensor err = ctx->saved_data["err"].toTensor();
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
     const float eps = (float)ctx->saved_data["eps"].toDouble();
     const int64_t rows = q.size(0), D = sizes[2];

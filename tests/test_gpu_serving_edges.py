@@ -152,6 +152,26 @@ def test_what_is_recorded_during_a_check_is_kept(monkeypatch):
     late_record(_pool(2, 1)[0], monkeypatch)
 
 
+def _norm_leaves(T=64):
+    g = torch.Generator().manual_seed(T)
+    q, k = (torch.randn(T, n, generator=g).to(BF).cuda().requires_grad_() for n in (256, 128))
+    return q, k, torch.randn(T, 64, 2, generator=g).cuda(), torch.ones(128, device="cuda", requires_grad=True)
+
+
+def test_error_word_cleared_between_forward_and_backward():
+    """The device's error word is no input of the gradients."""
+    from multics_b200._lib import dev_err
+    from multics_b200.train import head_norm_rope_grad
+
+    q, k, f, w = _norm_leaves()
+    want = torch.autograd.grad(sum(t.float().sum() for t in head_norm_rope_grad(
+        q, k, f, 2, 1, q_weight=w, k_weight=w)), (q, k, w))
+    out = head_norm_rope_grad(q, k, f, 2, 1, q_weight=w, k_weight=w)
+    dev_err(q.device).zero_()
+    got = torch.autograd.grad(sum(t.float().sum() for t in out), (q, k, w))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
 REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
            ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),
