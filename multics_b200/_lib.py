@@ -298,7 +298,9 @@ _DEV_ERR = {}
 
 
 def dev_err(device):
-    """The device's sticky error word of the kernels' bounded waits."""
+    """The device's sticky error word of the kernels' bounded waits.  A word that
+    a graph's capture asks for first is made beside the capture: as a part of the
+    graph every replay would clear it."""
     import torch
 
     key = device.index if isinstance(device, torch.device) else torch.device(device).index
@@ -306,7 +308,10 @@ def dev_err(device):
         key = torch.cuda.current_device()
     t = _DEV_ERR.get(key)
     if t is None:
-        t = _DEV_ERR[key] = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False), torch.cuda.device(key):
+            t = (calls().word_beside_capture(key) if torch.cuda.is_current_stream_capturing()
+                 else torch.zeros(1, dtype=torch.int32, device="cuda"))
+        _DEV_ERR[key] = t
     return t
 
 

@@ -14,6 +14,8 @@
 //              current one, rows that need a copy, arguments to refuse), which
 //              the Python functions then do or refuse; an int is a status.
 //
+// and word_beside_capture, what a capture must not make by itself.
+//
 // The module holds no code of the library: bind() gives it the addresses of
 // the one that is loaded.
 
@@ -23,7 +25,11 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <ATen/ops/zeros.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
@@ -183,6 +189,27 @@ bool requests_of(PyObject* const* a, at::Device dev, Requests* r) {
   r->table = tensor_of(a[0]), r->lengths = tensor_of(a[1]), r->q_start = tensor_of(a[2]);
   return is_table(r->table, dev) && is_vector(r->lengths, r->table->size(0), dev) &&
          is_vector(r->q_start, r->table->size(0) + 1, dev);
+}
+
+// word_beside_capture(device) -> int32 [1], zero: allocated and zeroed on a stream of its own, so
+// that neither is a part of the graph that this thread captures.
+PyObject* word_beside_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t dev;
+  if (n != 1 || !int_of(a[0], 0, 127, &dev)) {
+    PyErr_SetString(PyExc_TypeError, "word_beside_capture(device)");
+    return nullptr;
+  }
+  try {
+    const c10::InferenceMode mode(false);
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};
+    const c10::cuda::CUDAStreamGuard stream(c10::cuda::getStreamFromPool(false, (c10::DeviceIndex)dev));
+    at::Tensor word = at::zeros({1}, at::device(stream.current_stream().device()).dtype(at::kInt));
+    stream.current_stream().synchronize();
+    return THPVariable_Wrap(std::move(word));
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
 }
 
 // layout(k, v, k_scale, v_scale) -> format of a cache over them
@@ -551,6 +578,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     METHOD("bind", bind, "bind(name, address): where an entry point is"),
+    METHOD("word_beside_capture", word_beside_capture, "a zero word that no graph owns"),
     METHOD("layout", layout, "format of a cache over tensors of its layout"),
     METHOD("append", append, "paged8_append of well-formed tensors"),
     METHOD("attention", attention, "paged8_attention of well-formed tensors"),

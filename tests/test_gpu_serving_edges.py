@@ -172,6 +172,61 @@ def test_error_word_cleared_between_forward_and_backward():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.fixture
+def no_error_word():
+    """As in a process that has called nothing yet."""
+    from multics_b200 import _lib
+
+    words = dict(_lib._DEV_ERR)
+    _lib._DEV_ERR.clear()
+    yield _lib
+    _lib._DEV_ERR.clear()
+    _lib._DEV_ERR.update(words)
+
+
+def test_error_word_first_used_in_a_graph(no_error_word):
+    """It is zero before the first replay, and no replay clears it."""
+    from multics_b200.attention import device_error
+
+    T, H = 9, 2
+    g = torch.Generator().manual_seed(0)
+    q, k = (torch.randn(T, H * 128, generator=g).to(BF).cuda() for _ in range(2))
+    f, w, pos = torch.randn(4, 64, 2, generator=g).cuda(), torch.ones(128, device="cuda"), _i32([1] * T)
+    warm = [torch.randn(64, 64, device="cuda") for _ in range(8)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hier_head_norm_rope(q, k, f, H, H, q_weight=w, k_weight=w, positions=pos)
+    del warm
+    word = no_error_word.dev_err(q.device)
+    assert device_error() == 0
+    graph.replay()
+    assert device_error() == 0 and (out[0] != 0).any()
+    pos.fill_(4)
+    graph.replay()
+    assert device_error() == 2
+    pos.fill_(1)
+    graph.replay()
+    assert device_error() == 2 and no_error_word.dev_err(q.device) is word
+    word.zero_()
+    graph.replay()
+    assert device_error() == 0
+    del graph
+    torch.cuda.empty_cache()
+    filled = [torch.full((1024,), 5, dtype=torch.int32, device="cuda") for _ in range(64)]
+    assert device_error() == 0 and len(filled) == 64
+
+
+def test_error_word_of_inference_mode_is_cleared_outside(no_error_word):
+    with torch.inference_mode():
+        word = no_error_word.dev_err(torch.device("cuda", 0))
+    word.zero_()
+    q, k, f, w = _norm_leaves()
+    from multics_b200.train import head_norm_rope_grad
+
+    out = head_norm_rope_grad(q, k, f, 2, 1, q_weight=w, k_weight=w)
+    assert torch.isfinite(torch.autograd.grad(out[0].float().sum(), q)[0]).all()
+
+
 # row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
 REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
            ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),
