@@ -710,10 +710,11 @@ class SelfAttention(nn.Module):
         values first.  ``x`` ``[T, dim]`` (or ``[1, T, dim]``) holds the tokens
         request by request, ``step`` is the :func:`~multics_b200.paged8.page_step`
         that placed them, ``table`` its block table; ``freqs`` is indexed by a
-        token's position in its request.  Rows behind the last request give the
-        output projection's bias.  Masks as in
+        token's position in its request; a row past it is NaN, which the cache
+        reports (:meth:`~multics_b200.paged8.Paged8Cache.check`).  Rows behind the
+        last request give the output projection's bias.  Masks as in
         :func:`~multics_b200.paged8.paged8_attention`."""
-        from .paged8 import paged8_append, paged8_attention
+        from .paged8 import PAGE_TOKENS, paged8_append, paged8_attention
 
         if cam_tokens is not None and (self.cam_q is None or self.cam_k is None):
             raise RuntimeError("camera_pose was provided but enable_camera_pose_qk() was not called")
@@ -734,9 +735,11 @@ class SelfAttention(nn.Module):
             q, k = hier_head_norm_rope(qx, kx, ft, self.num_heads, self.num_heads,
                                        q_weight=self.norm_q.weight, k_weight=self.norm_k.weight,
                                        positions=step.positions, eps=self.norm_q.eps)
+            if table.shape[1] * PAGE_TOKENS > ft.shape[0]:  # requests may outgrow the table
+                past = (step.positions >= ft.shape[0])[:, None]
+                q.masked_fill_(past, float("nan")), k.masked_fill_(past, float("nan"))
         else:
             ft, pos = ft.to(x.device), step.positions
-            # a position past the table reads NaN, which the cache reports
             rows = ft[pos.clamp(0, ft.shape[0] - 1).long()].masked_fill(
                 (pos >= ft.shape[0])[:, None, None], float("nan"))
             q, k = self._prologue(qx, kx, rows, cam) if T else (qx, kx)

@@ -227,6 +227,41 @@ def test_error_word_of_inference_mode_is_cleared_outside(no_error_word):
     assert torch.isfinite(torch.autograd.grad(out[0].float().sum(), q)[0]).all()
 
 
+@pytest.mark.parametrize("head_norm", [True, False])
+def test_paged_forward_past_the_rotation_table(head_norm):
+    """A request that outgrows the table: its new rows are NaN and the cache
+    reports them, whichever norm the module has; the others are as ever."""
+    from multics_b200._lib import dev_err
+    from multics_b200.attention import SelfAttention
+
+    torch.manual_seed(3)
+    layer = SelfAttention(256, 2, head_norm=head_norm).to("cuda", BF)
+    freqs = torch.randn(70, 64, 2, device="cuda")
+    x = torch.randn(1, 70, 256, device="cuda").to(BF)
+
+    def run(adds, rows):
+        cache = Paged8Cache(6, 2)
+        table, free, count = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), _i32(list(range(6))), _i32([6])
+        lengths, outs = _i32([0, 0]), []
+        for add in adds:
+            st = page_step(lengths, _i32(add), table, free, count, rows)
+            st.check()
+            outs.append(layer.paged_forward(x[:, :rows], freqs, cache, table, st))
+            lengths, count = st.lengths, st.free_count
+        return outs, cache, st
+
+    outs, cache, st = run([[66, 2], [3, 4]], 68)
+    cache.check()  # 69 tokens
+    assert torch.isfinite(outs[0]).all() and torch.isfinite(outs[1]).all()
+    outs, cache, st = run([[66, 2], [3, 4], [4, 1]], 68)  # positions 69 to 72: three past the table
+    with pytest.raises(ValueError, match="NaN"):
+        cache.check()
+    assert outs[2][0, 1:4].isnan().all()
+    keep = [0, *range(4, 68)]
+    assert torch.isfinite(outs[2][0, keep]).all()
+    dev_err(x.device).zero_()
+
+
 # row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
 REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
            ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),
