@@ -188,13 +188,13 @@ __device__ __forceinline__ void load_queries(const Paged8Args& a, const Columns&
 
 // Running softmax of a lane's two columns and their output.
 struct Running {
-  float m[2], l[2], o[8][4];
+  float m[2], n[2], l[2], o[8][4];
 };
 
 __device__ __forceinline__ void start(Running& R) {
 #pragma unroll
   for (int d = 0; d < 8; ++d) R.o[d][0] = R.o[d][1] = R.o[d][2] = R.o[d][3] = 0.f;
-  R.m[0] = R.m[1] = -INFINITY;
+  R.m[0] = R.m[1] = R.n[0] = R.n[1] = -INFINITY;
   R.l[0] = R.l[1] = 0.f;
 }
 
@@ -225,23 +225,44 @@ __device__ __forceinline__ void weigh(Running& R, float (&s)[MB][4], const Colum
     mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], i));
     mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], i));
   }
-  float ref[2], alpha[2];
+  float ref[2], factor[2];
+  bool grown = false, far[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const float m_new = fmaxf(R.m[k], mx[k]);
-    ref[k] = m_new == -INFINITY ? 0.f : m_new;
-    alpha[k] = ex2_approx(R.m[k] - ref[k]);
-    R.m[k] = m_new;
+    const float top = mx[k] - vef;
+    far[k] = far_page(fmaxf(R.m[k], mx[k]), mx[k], fmaxf(R.n[k], top), top);
+    grown = grown || far[k] || mx[k] > R.m[k] || top > R.n[k];
   }
-  if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+  const bool any = __any_sync(0xffffffffu, grown);
+  if (any) {
+    float alpha[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float m_new = fmaxf(R.m[k], mx[k]), n_new = fmaxf(R.n[k], mx[k] - vef);
+      alpha[k] = ex2_approx(R.m[k] - finite_or_0(m_new));
+      R.l[k] *= ex2_approx(R.n[k] - finite_or_0(n_new));
+      R.m[k] = m_new, R.n[k] = n_new;
+    }
 #pragma unroll
     for (int d = 0; d < 8; ++d)
 #pragma unroll
       for (int r = 0; r < 4; ++r) R.o[d][r] *= alpha[r & 1];
-    R.l[0] *= alpha[0];
-    R.l[1] *= alpha[1];
   }
-  const float unscale = exp2_int(max(-126, min(126, -ve)));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    ref[k] = finite_or_0(R.m[k]);
+    factor[k] = sum_factor(ref[k], vef, finite_or_0(R.n[k]));
+  }
+  if (any && __any_sync(0xffffffffu, far[0] || far[1])) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (far[k]) {
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+          R.l[k] += ex2_approx(s[m][k] - vef - R.n[k]) + ex2_approx(s[m][k + 2] - vef - R.n[k]);
+        factor[k] = 0.f;
+      }
+  }
   float sum[2] = {0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < MB; ++m)
@@ -252,41 +273,62 @@ __device__ __forceinline__ void weigh(Running& R, float (&s)[MB][4], const Colum
       sum[1] += p1;
       pb[m][e] = transpose8x8(pack_f16x2(p0, p1));
     }
-  R.l[0] = fmaf(sum[0], unscale, R.l[0]);
-  R.l[1] = fmaf(sum[1], unscale, R.l[1]);
+  R.l[0] = fmaf(sum[0], factor[0], R.l[0]);
+  R.l[1] = fmaf(sum[1], factor[1], R.l[1]);
 }
 
-// The lanes' results as rows of 128 floats in shared memory.
-__device__ __forceinline__ void spill(Running& R, float (*so)[kPitch], float* sm, float* sl, int lane) {
+// The lanes' results as rows of 128 floats in shared memory, with n and l.
+__device__ __forceinline__ void spill(Running& R, float (*so)[kPitch], float* sn, float* sl, int lane) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int i = 4; i < 32; i <<= 1) {
     R.l[0] += __shfl_xor_sync(0xffffffffu, R.l[0], i);
     R.l[1] += __shfl_xor_sync(0xffffffffu, R.l[1], i);
   }
+  const OutFactor f[2] = {{R.m[0], R.n[0], R.l[0]}, {R.m[1], R.n[1], R.l[1]}};
+  if (__any_sync(0xffffffffu, f[0].b != 1.f || f[1].b != 1.f)) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) R.o[d][r] *= f[r & 1].b;
+  }
 #pragma unroll
   for (int d = 0; d < 8; ++d)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) so[2 * t + (r & 1)][16 * d + 8 * (r >> 1) + g] = R.o[d][r];
+    for (int r = 0; r < 4; ++r) so[2 * t + (r & 1)][16 * d + 8 * (r >> 1) + g] = R.o[d][r] * f[r & 1].a;
   if (g == 0) {
-    sm[2 * t] = R.m[0], sm[2 * t + 1] = R.m[1];
+    sn[2 * t] = R.n[0], sn[2 * t + 1] = R.n[1];
     sl[2 * t] = R.l[0], sl[2 * t + 1] = R.l[1];
   }
 }
 
-// one pair's output row: 4 dimensions per lane, M and L its maximum and sum
+// one pair's output row: 4 dimensions per lane, and its denominator
 __device__ __forceinline__ void write_pair(const Paged8Args& a, const Paged8Tile& tl, int rho, int kvh,
-                                           int lane, const float (&acc)[4], float M, float L) {
+                                           int lane, const float (&o)[4], float N, float L) {
   int row, g;
   split_pair(a, rho, row, g);
-  const float inv = L > 0.f ? 1.f / L : 0.f;
   const int64_t r = tl.rq.row0 + (int64_t)row;
   const int h = kvh * a.group + g;
   // (written past the caches' reuse: 50.1 us for 880 requests of 3 rows, else 51.6)
   __stcs(reinterpret_cast<uint2*>(a.out + r * a.out_stride + h * 128 + 4 * lane),
-         make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)));
-  if (a.lse && lane == 0) a.lse[r * a.heads + h] = row_lse(M, L);
+         make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])));
+  if (a.lse && lane == 0) a.lse[r * a.heads + h] = row_lse(N, L);
 }
+
+// The shares of up to 32 parts of a pair's keys in its output, lane s's of part s,
+// from the parts' n and l; N and L those of all.
+struct Shares {
+  float N, L, mine;
+  __device__ __forceinline__ Shares(float n, float l) : N(n) {
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) N = fmaxf(N, __shfl_xor_sync(0xffffffffu, N, i));
+    mine = l * ex2_approx(n - finite_or_0(N));
+    L = mine;
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) L += __shfl_xor_sync(0xffffffffu, L, i);
+    mine *= inverse_or_0(L);
+  }
+};
 
 constexpr int kMinPages = 2 * kWarps;  // of a part at least
 
@@ -345,7 +387,7 @@ template <int FMT>
 __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args a) {
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
   __shared__ __align__(16) uint32_t sq[kWarps][8][32][2];
-  __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+  __shared__ float sn[kWarps][kRows], sl[kWarps][kRows];
   asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -448,33 +490,37 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
         }
       }
     }
-    spill(R, so[w], sm[w], sl[w], lane);
+    spill(R, so[w], sn[w], sl[w], lane);
     __syncthreads();
     for (int r = w; r < kRows && tl.rho0 + r < tl.pairs; r += kWarps) {
-      float M = -INFINITY;
+      float N = -INFINITY;
 #pragma unroll
-      for (int q = 0; q < kWarps; ++q) M = fmaxf(M, sm[q][r]);
-      const float ref = M == -INFINITY ? 0.f : M;
-      float L = 0.f, acc[4] = {};
+      for (int q = 0; q < kWarps; ++q) N = fmaxf(N, sn[q][r]);
+      float L = 0.f, acc[4] = {}, share[kWarps];
 #pragma unroll
       for (int q = 0; q < kWarps; ++q) {
-        const float f = ex2_approx(sm[q][r] - ref);
-        L = fmaf(sl[q][r], f, L);
+        share[q] = sl[q][r] * ex2_approx(sn[q][r] - finite_or_0(N));
+        L += share[q];
+      }
+      const float inv = inverse_or_0(L);
+#pragma unroll
+      for (int q = 0; q < kWarps; ++q) {
+        const float f = share[q] * inv;
         const float4 v = *reinterpret_cast<const float4*>(&so[q][r][4 * lane]);
         acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
         acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
       }
       if (parts == 1) {
-        write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, M, L);
+        write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, N, L);
       } else if (!a.cluster) {
         const int64_t at = (int64_t)blockIdx.x * kRows + r;
         *reinterpret_cast<float4*>(a.part_o + at * 128 + 4 * lane) =
             make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+        if (lane == 0) *reinterpret_cast<float2*>(a.part_nl + at * 2) = make_float2(N, L);
       } else {  // the block's result takes the place of its first warp's
         *reinterpret_cast<float4*>(&so[0][r][4 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         __syncwarp();
-        if (lane == 0) sm[0][r] = M, sl[0][r] = L;
+        if (lane == 0) sn[0][r] = N, sl[0][r] = L;
       }
     }
     if (parts == 1 || !a.cluster) {
@@ -484,18 +530,16 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
     // blocks of the cluster: each joins some of the rows, part by part
     cluster_sync();
     for (int r = split + w * parts; r < kRows && tl.rho0 + r < tl.pairs; r += kWarps * parts) {
-      float M = -INFINITY;
-      for (int s = 0; s < parts; ++s) M = fmaxf(M, ld_peer(peer_smem(&sm[0][r], s)));
-      const float ref = M == -INFINITY ? 0.f : M;
-      float L = 0.f, acc[4] = {};
+      Shares sh(lane < parts ? ld_peer(peer_smem(&sn[0][r], lane)) : -INFINITY,
+                lane < parts ? ld_peer(peer_smem(&sl[0][r], lane)) : 0.f);
+      float acc[4] = {};
       for (int s = 0; s < parts; ++s) {
-        const float f = ex2_approx(ld_peer(peer_smem(&sm[0][r], s)) - ref);
-        L = fmaf(ld_peer(peer_smem(&sl[0][r], s)), f, L);
+        const float f = __shfl_sync(0xffffffffu, sh.mine, s);
         const float4 v = ld_peer4(peer_smem(&so[0][r][4 * lane], s));
         acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
         acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
       }
-      write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, M, L);
+      write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, sh.N, sh.L);
     }
     cluster_sync();  // nobody leaves while its rows are read
   }
@@ -574,7 +618,7 @@ __device__ __forceinline__ void short_keys(const Paged8Args& a, const Columns& c
 template <int FMT>
 __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args a, int units) {
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
-  __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+  __shared__ float sn[kWarps][kRows], sl[kWarps][kRows];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   if ((int)blockIdx.x * kWarps >= units) return keep_rows(a, true, reinterpret_cast<uint32_t*>(so));
   const int unit = blockIdx.x * kWarps + w;
@@ -604,12 +648,12 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args
           short_keys<FMT, 2>(a, c, R, qf, sc, at, p * kPage, base, from, to, lane);
       }
     }
-    spill(R, so[w], sm[w], sl[w], lane);
+    spill(R, so[w], sn[w], sl[w], lane);
     __syncwarp();
     for (int r = 0; r < kRows && tl.rho0 + r < tl.pairs; ++r) {
       const float4 v = *reinterpret_cast<const float4*>(&so[w][r][4 * lane]);
       const float acc[4] = {v.x, v.y, v.z, v.w};
-      write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, sm[w][r], sl[w][r]);
+      write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, sn[w][r], sl[w][r]);
     }
     __syncwarp();
   }
@@ -637,25 +681,18 @@ __global__ void __launch_bounds__(256) paged8_merge_kernel(Paged8Args a, int64_t
   const int pr = tl.rho0 + r;
   if (parts == 1 || pr >= tl.pairs) return;
   const int64_t at = (int64_t)unit * a.splits * kTileRows + r;
-  // lane s holds part s's maximum and sum (at most 32 parts)
-  float2 ml = make_float2(-INFINITY, 0.f);
-  if (lane < parts) ml = *reinterpret_cast<const float2*>(a.part_ml + (at + (int64_t)lane * kTileRows) * 2);
-  float M = ml.x;
-#pragma unroll
-  for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
-  const float mine = ex2_approx(ml.x - (M == -INFINITY ? 0.f : M));
-  float L = ml.y * mine;
-#pragma unroll
-  for (int i = 16; i > 0; i >>= 1) L += __shfl_xor_sync(0xffffffffu, L, i);
+  float2 nl = make_float2(-INFINITY, 0.f);
+  if (lane < parts) nl = *reinterpret_cast<const float2*>(a.part_nl + (at + (int64_t)lane * kTileRows) * 2);
+  const Shares sh(nl.x, nl.y);
   float acc[4] = {};
 #pragma unroll 8
   for (int s = 0; s < parts; ++s) {
     const float4 v = *reinterpret_cast<const float4*>(a.part_o + (at + (int64_t)s * kTileRows) * 128 + 4 * lane);
-    const float f = __shfl_sync(0xffffffffu, mine, s);
+    const float f = __shfl_sync(0xffffffffu, sh.mine, s);
     acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
     acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
   }
-  write_pair(a, tl, pr, kvh, lane, acc, M, L);
+  write_pair(a, tl, pr, kvh, lane, acc, sh.N, sh.L);
 }
 
 // How a call is cut, from the sizes the host knows (the same for every content
@@ -925,7 +962,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
     large.zero_rest = s.small ? 0 : zero_rest;
     large.splits = divisor(s.large_splits);
     large.part_o = workspace + s.small_floats;
-    large.part_ml = large.part_o + (s.floats - s.small_floats) / 130 * 128;
+    large.part_nl = large.part_o + (s.floats - s.small_floats) / 130 * 128;
     rc = paged8_launch_large(large, format, s.large_tiles, st);
     if (rc) return rc;
   }
@@ -935,7 +972,7 @@ extern "C" int hier_paged8_attn(const void* q, int64_t q_stride, int32_t rows, i
     a.splits = divisor(s.small_splits);
     a.cluster = s.cluster;
     a.part_o = workspace;
-    a.part_ml = workspace + s.small_floats / 130 * 128;
+    a.part_nl = workspace + s.small_floats / 130 * 128;
     rc = launch_small(a, format, s.small_tiles, s.few_pages, s.large, st);
     if (rc) return rc;
   }

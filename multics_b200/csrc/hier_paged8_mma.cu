@@ -342,6 +342,34 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t* w) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t col, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(col));
+  tmem_wait_ld();
+}
+
+// The denominator's terms of a tile's pages that are far_page, from the scores
+// where they lie (factors c0, c1; the row sees keys lo to hi of the tile).  One
+// at a time: eight took 1.5 % more of calls without such a page, for its code.
+__device__ __forceinline__ float far_sum(uint32_t s_col, float c0, float c1, float n, int lo, int hi,
+                                         bool far0, bool far1) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int q = 0; q < 128; ++q) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(s_col + q));
+    tmem_wait_ld();
+    const float p = ex2_approx(fmaf(__uint_as_float(r), q < 64 ? c0 : c1, -n));
+    sum += (q < 64 ? far0 : far1) && q >= lo && q < hi ? p : 0.f;
+  }
+  return sum;
+}
+
 __device__ __forceinline__ void rescale_o(uint32_t o_col, float alpha) {
 #pragma unroll 1
   for (int q = 0; q < 16; ++q) {
@@ -453,7 +481,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
   const int qi = (in_row ? rho : 0) / a.group;
   const int head = J.kvh * a.group.d + (in_row ? rho - qi * a.group.d : 0);
   const int64_t grow = J.tl.rq.row0 + (int64_t)qi;
-  float m_run = -INFINITY, l_run = 0.f;
+  float m_run = -INFINITY, n_run = -INFINITY, l_run = 0.f;
   int c = 0;
   bool lost = false;  // a wait ran out: nothing more is waited for or written
   if (J.n_kv > 0) {
@@ -522,20 +550,27 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
         m8[i & 3] = fmaxf(m8[i & 3], sv[i]);
         m8[4 + (i & 3)] = fmaxf(m8[4 + (i & 3)], sv[64 + i]);
       }
-      const float mx = fmaxf(fmaf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), c0, (float)ve0),
-                             fmaf(fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])), c1, (float)ve1));
+      const float x0 = fmaf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), c0, (float)ve0);
+      const float x1 = fmaf(fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])), c1, (float)ve1);
+      const float mx = fmaxf(x0, x1);
       const bool grow_max = mx > m_run + kRescaleThreshold;
       const bool need_rescale = grow_max && m_run != -INFINITY;
-      if (__any_sync(0xffffffffu, need_rescale)) {
-        const float alpha = need_rescale ? ex2_approx(m_run - mx) : 1.f;
-        rescale_o(o_col, alpha);
-        l_run *= alpha;
+      const float m_new = grow_max ? mx : m_run, ref = finite_or_0(m_new);
+      bool far0 = false, far1 = false;
+      float own = 0.f;
+      if (__any_sync(0xffffffffu, need_rescale || ref - fminf(x0, x1) > kFarWeights)) {
+        if (__any_sync(0xffffffffu, need_rescale))
+          rescale_o(o_col, need_rescale ? ex2_approx(m_run - ref) : 1.f);
+        const float nref = finite_or_0(fmaxf(n_run, fmaxf(x0 - (float)ve0, x1 - (float)ve1)));
+        far0 = far_page(ref, x0, nref, x0 - (float)ve0), far1 = far_page(ref, x1, nref, x1 - (float)ve1);
+        if (__any_sync(0xffffffffu, far0 || far1))
+          own = far_sum(s_col, c0, c1, nref, lo - k0, hi - k0, far0, far1);
       }
-      if (grow_max) m_run = mx;
-      const float nref = m_run == -INFINITY ? 0.f : -m_run;
+      m_run = m_new;
+      float sums[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float ch = half ? c1 : c0, rh = nref + (float)(half ? ve1 : ve0);
+        const float ch = half ? c1 : c0, vh = (float)(half ? ve1 : ve0), rh = vh - ref;
         const uint64_t sc2 = f2_pack(ch, ch), ref2 = f2_pack(rh, rh);
         uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
         uint32_t pk[32];
@@ -556,11 +591,17 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
         }
         float s0, s1;
         f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
-        l_run = fmaf(s0 + s1, exp2_int(max(-126, min(126, half ? -ve1 : -ve0))), l_run);
+        sums[half] = s0 + s1;
       }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(B.p_full + h);
+      const float top0 = x0 - (float)ve0, top1 = x1 - (float)ve1;
+      const float n_new = fmaxf(n_run, fmaxf(top0, top1)), nref = finite_or_0(n_new);
+      l_run = fmaf(l_run, ex2_approx(n_run - nref), own);
+      if (!far0) l_run = fmaf(sums[0], sum_factor(ref, (float)ve0, nref), l_run);
+      if (!far1) l_run = fmaf(sums[1], sum_factor(ref, (float)ve1, nref), l_run);
+      n_run = n_new;
       ++c;
     }
   }
@@ -568,87 +609,82 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
     lost = !mbar_wait(B.o_final + h, 0, a.err, 50);
     tc_fence_after();
   }
-  // The halves of a dual tile joined: the second leaves its rows, column by
+  // The halves of a dual tile joined: the second leaves its outputs, column by
   // column, where the queries were (every product is done), the first adds them.
   float* other = reinterpret_cast<float*>(smem + kSmemQ) + row;
-  float2* other_ml = reinterpret_cast<float2*>(smem + kSmemRaw) + row;
-  float keep = 1.f, add = 0.f;
+  float2* other_nl = reinterpret_cast<float2*>(smem + kSmemRaw) + row;
+  OutFactor keep(m_run, n_run, l_run);
+  float add = 0.f;
   if (J.dual && J.n_kv > 0) {
     named_barrier(1, 256);
     if (h == 1) {
       if (!lost) {
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          uint32_t r[32];
-          if (c > 0) {
-            tmem_ld32(o_col + q * 32, r);
-            tmem_wait_ld();
-          }
+        for (int q = 0; q < 8; ++q) {
+          uint32_t r[16];
+          if (c > 0) tmem_ld16(o_col + q * 16, r);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            other[(32 * q + i) * 128] = c > 0 ? __uint_as_float(r[i]) : 0.f;
+          for (int i = 0; i < 16; ++i)
+            other[(16 * q + i) * 128] = c > 0 ? __uint_as_float(r[i]) * keep.a * keep.b : 0.f;
         }
       }
-      *other_ml = make_float2(m_run, l_run);
+      *other_nl = make_float2(n_run, l_run);
     }
     named_barrier(1, 256);
     if (h == 1) return;
-    const float2 ml = *other_ml;
-    const float M = fmaxf(m_run, ml.x), ref = M == -INFINITY ? 0.f : M;
-    keep = ex2_approx(m_run - ref), add = ex2_approx(ml.x - ref);
-    l_run = fmaf(l_run, keep, ml.y * add);
-    m_run = M;
+    const float2 nl = *other_nl;
+    const float N = fmaxf(n_run, nl.x);
+    const float mine = l_run * ex2_approx(n_run - finite_or_0(N)), theirs = nl.y * ex2_approx(nl.x - finite_or_0(N));
+    n_run = N, l_run = mine + theirs;
+    const float inv = inverse_or_0(l_run);
+    keep.a *= mine * inv, add = theirs * inv;
   } else if (J.dual && h == 1) {
     return;
   }
   if (lost) return;
   const bool whole = parts == 1;
-  const float inv = whole ? (l_run > 0.f ? 1.f / l_run : l_run == 0.f ? 0.f : l_run) : 1.f;
-  keep *= inv, add *= inv;
   __nv_bfloat16* orow = a.out + grow * a.out_stride + head * 128;
   const int64_t at = whole ? 0 : ((int64_t)blockIdx.x * kRows + (rho - J.tl.rho0));
   if (in_row) {
     if (whole) {
-      if (a.lse) a.lse[grow * a.heads + head] = row_lse(m_run, l_run);
+      if (a.lse) a.lse[grow * a.heads + head] = row_lse(n_run, l_run);
     } else {
-      *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_run, l_run);
+      *reinterpret_cast<float2*>(a.part_nl + at * 2) = make_float2(n_run, l_run);
     }
   }
 #pragma unroll 1
-  for (int q = 0; q < 4; ++q) {
-    uint32_t r[32];
+  for (int q = 0; q < 8; ++q) {
+    uint32_t r[16];
     if (c > 0) {
-      tmem_ld32(o_col + q * 32, r);
-      tmem_wait_ld();
+      tmem_ld16(o_col + q * 16, r);
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = 0u;
+      for (int i = 0; i < 16; ++i) r[i] = 0u;
     }
     if (!in_row) continue;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float v = __uint_as_float(r[i]) * keep;
-      if (J.dual && J.n_kv > 0) v = fmaf(other[(32 * q + i) * 128], add, v);
+    for (int i = 0; i < 16; ++i) {
+      float v = __uint_as_float(r[i]) * keep.a * keep.b;
+      if (J.dual && J.n_kv > 0) v = fmaf(other[(16 * q + i) * 128], add, v);
       r[i] = __float_as_uint(v);
     }
     if (whole) {
-      uint32_t w[16];
+      uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
+      for (int i = 0; i < 8; ++i)
         w[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
       if ((reinterpret_cast<uintptr_t>(orow) & 31) == 0) {
-        st_global_v8(orow + q * 32, w);
-        st_global_v8(orow + q * 32 + 16, w + 8);
+        st_global_v8(orow + q * 16, w);
       } else {
-        uint4* dst = reinterpret_cast<uint4*>(orow + q * 32);
+        uint4* dst = reinterpret_cast<uint4*>(orow + q * 16);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 2; ++k)
           dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
       }
     } else {
-      uint4* dst = reinterpret_cast<uint4*>(a.part_o + at * 128 + q * 32);
+      uint4* dst = reinterpret_cast<uint4*>(a.part_o + at * 128 + q * 16);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < 4; ++k)
         dst[k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
     }
   }

@@ -10,11 +10,17 @@
 // requests without any take no numbers.)
 //
 // The page scales never touch the codes: a page's key scale multiplies its
-// scores, and its value scale 2^ve is added to their exponents, so that with
-//   x_j = scale log2(e) sk q.k_j + ve,   m = max x_j,   p_j = 2^(x_j - m)
-// the product sum p_j V8[j] is the output times 2^-m, p_j is at most 1 (fp16
-// keeps 11 bits of it whatever the pages' scales are), and the softmax's
-// denominator is sum p_j 2^-ve.
+// scores s_j, and its value scale 2^ve is added to their exponents, so that with
+//   s_j = scale log2(e) sk q.k_j,   m = max (s_j + ve),   p_j = 2^(s_j + ve - m)
+// the product sum p_j V8[j] is the output's numerator times 2^-m and p_j is at
+// most 1 (fp16 keeps 11 bits of it whatever the pages' scales are).  The
+// denominator has a maximum of its own, n = max s_j:
+//   l = sum 2^(s_j - n) = sum over pages 2^(m - ve - n) sum p_j,
+// from the same exponentials.  Only a page whose p_j are below 2^-60 and whose
+// s_j are not far below n (far_page: value scales far apart, such as those of a
+// page of zeros) is summed by exponentials of its own: its p_j may be flushed
+// though it weighs.  Results of parts of the keys are joined as outputs with the
+// weights l 2^n.
 #pragma once
 
 #include "paged8.cuh"
@@ -45,7 +51,7 @@ struct Paged8Args {
   int zero_rest;    // rows of no request: 1 zeros, 2 their log-sum-exp alone, 0 left
   Divisor splits;   // most parts a tile's keys are cut into
   float* part_o;    // [tile][kv head][split][kRows][128]
-  float* part_ml;   // [tile][kv head][split][kRows][2]
+  float* part_nl;   // [tile][kv head][split][kRows][2]: n and l
   int cluster;      // the parts of a small tile are the blocks of a cluster
   int row_limit;    // requests of up to row_limit pairs are the small kernel's, the others the
                     // large one's (INT_MAX: all the small one's, 0: all the large one's)
@@ -196,6 +202,32 @@ __device__ __forceinline__ void zero_rest(const Paged8Args& a, int kvh, int64_t 
   for (int64_t j = i; j < a.rows - between; j += n)
     zero_row(a, j < s.first ? j : j + between, kvh, lane);
 }
+
+__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Whether a page's weights p, of maximum x and of scores up to s, are too small
+// for the denominator's terms to be taken from them.
+constexpr float kFarWeights = 60.f;
+__device__ __forceinline__ bool far_page(float m, float x, float n, float s) {
+  return m - x > kFarWeights && n - s < 48.f;
+}
+// 2^(m - ve - n): the denominator's terms from p.  (Beyond 2^126 only for pages
+// whose terms are below 2^-48.)
+__device__ __forceinline__ float sum_factor(float m, float ve, float n) {
+  return ex2_approx(fminf(m - ve - n, 126.f));
+}
+// What brings the numerator to the output, 2^(m - n) / l: 0 where nothing was seen,
+// NaN where the sum is.  In two factors, the second 1 but for outputs below 2^-90,
+// so that none leaves fp32's normal numbers.
+struct OutFactor {
+  float a, b;
+  __device__ __forceinline__ OutFactor(float m, float n, float l) : a(l), b(1.f) {
+    if (!(l > 0.f)) return;
+    a = ex2_approx(fmaxf(m - n, -96.f)) / l;
+    b = ex2_approx(fminf(m - n + 96.f, 0.f));
+  }
+};
+__device__ __forceinline__ float inverse_or_0(float l) { return l > 0.f ? 1.f / l : l; }
 
 // log2-sum-exp of a pair from its maximum and sum: -inf where nothing was seen,
 // NaN where the sum is

@@ -262,6 +262,68 @@ def test_paged_forward_past_the_rotation_table(head_norm):
     dev_err(x.device).zero_()
 
 
+SCALES = [[-126] * 6, [-126, 0, -126, 0, -126, 0], [0, -126, 0, -126, 0, -126], [-100, 27, 27, 27, 27, 27],
+          [27, -100, 27, -100, 60, 60], [-126, 126, -126, 126, -126, 126], [126, -126] * 3, [-126, -63, 0, 63, 119, 126],
+          [126, 119, 63, 0, -63, -126], [126] * 6, [-90, 0, 90, -90, 0, 90]]
+
+
+@pytest.mark.parametrize("scales", SCALES)
+@pytest.mark.parametrize("rows", [1, 40, 1200])
+@pytest.mark.parametrize("shape", ["short", "long", "split"])
+@pytest.mark.parametrize("spread", [0.0, 0.3, 6.0])
+def test_value_scales_at_the_ends_of_their_range(scales, rows, shape, spread):
+    """The weights of a page count in the denominator whatever its values are:
+    outputs and log-sum-exps of value scales from 2^-126 to 2^126, even scores
+    (spread 0), near ones and ones that leave pages far behind."""
+    import paged8_oracle as P
+
+    pages, width = (3, 4) if shape == "short" else (6, 40) if shape == "long" else (66, 66)
+    heads, kv, n = 2, 1, 1 if shape == "split" else 3
+    c, g = _pool(pages * n, kv, seed=rows)
+    order = torch.randperm(pages * n, generator=g).view(n, pages)
+    table = torch.full((n, width), -1, dtype=torch.int32)
+    table[:, :pages] = order
+    e = torch.tensor([scales[p % 6] for p in range(pages)])
+    vs, v = c.v_scale.cpu(), c.v.cpu()
+    for b in range(n):
+        vs[order[b]] = (2.0 ** e.double()).float()[:, None]
+        big = order[b][e >= 119]
+        v[big] = v[big].sign()  # values within bf16
+        if -100 in scales:
+            v[order[b][e == -100]] = 0
+    c.v_scale.copy_(vs), c.v.copy_(v)
+    held, starts = [pages * 64 - 5] * n, [b * rows for b in range(n + 1)]
+    q = (torch.randn(n * rows, heads * 128, generator=g) * spread).to(BF)
+    out, lse = paged8_attention(q.cuda(), c, table.cuda(), _i32(held), _i32(starts), heads, block_frames=0, return_lse=True)
+    kk, vv = P.values(c)
+    want, want_lse, mag = P.attention(q, kk, vv, table.tolist(), held, starts, heads, block=0)
+    vmax = float(vv.abs().max())
+    tol = P.attention_bound(want, mag, held[0], vmax) + 2.0 ** -126  # (and fp32's least normal number)
+    err = (out.cpu().double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    # the bound of the other tests: sums off by 2^-11, and fp32's own step
+    assert ((lse.cpu().double() - want_lse).abs() <= 2.0 ** -10 + want_lse.abs() * 2.0 ** -20).all()
+    c.check()
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_values_of_zeros_beside_large_ones_weigh(first):
+    """By appends alone: a page of zero values and one of 1e10, all scores equal:
+    half the weight is on the zeros."""
+    c, table = Paged8Cache(2, 1), _i32([[0, 1]])
+    k = torch.ones(128, 128, dtype=BF, device="cuda")
+    v = torch.zeros(128, 128, dtype=BF, device="cuda")
+    v[slice(64, 128) if first else slice(0, 64)] = 1e10
+    paged8_append(c, k, v, table, _i32([128]), _i32([0, 128]))
+    large = float(v.max())
+    for rows in (1, 200):
+        q = torch.zeros(rows, 128, dtype=BF, device="cuda")
+        out, lse = paged8_attention(q, c, table, _i32([128]), _i32([0, rows]), 1, block_frames=0, return_lse=True)
+        # codes within half a step of 2^-7 (large has 8 bits), weights of 2^-10
+        assert ((out.double() / (large / 2) - 1).abs() <= 2.0 ** -6).all()
+        assert ((lse - 7).abs() <= 2.0 ** -10).all()
+
+
 # row starts in units of R rows, of 2 R; the rows (in R) that only refused requests or none have
 REFUSED = [([0, 1, 3], [(1, 2)]), ([-1, 1, 2], [(0, 1)]), ([0, 5, 2], [(0, 2)]), ([1, 0, 2], [(0, 2)]),
            ([0, 3], [(0, 2)]), ([-1, 2], [(0, 2)]), ([3, 4], [(0, 2)]), ([1, 3], [(0, 2)]), ([2, 0], [(0, 2)]),
