@@ -206,13 +206,14 @@ __device__ __forceinline__ void weigh(Running& R, float (&s)[MB][4], const Colum
                                       int key0, uint32_t (&pb)[MB][2]) {
   const int ve = scale_log2_of(vs);
   const float vef = (float)ve;
+  const float c_ks[2] = {score_factor(sc[0], ks), score_factor(sc[1], ks)};
   float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
   for (int m = 0; m < MB; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int k = r & 1;
-      float x = fmaf(s[m][r], sc[k] * ks, vef);
+      float x = fmaf(s[m][r], c_ks[k], vef);
       if (!whole) {
         const int key = key0 + 4 * m + (r & 2);
         x = have && key >= c.lo[k] && key < c.hi[k] ? x : -INFINITY;

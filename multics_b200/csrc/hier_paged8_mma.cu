@@ -42,8 +42,6 @@
 // runs the faster the smaller it is: one converter for keys and values 206 us
 // against 222 (4 requests' chunks of 660 rows over 4 620 keys, int8).
 
-#include <float.h>
-
 #include <type_traits>
 
 #include "paged8_attn.cuh"
@@ -515,7 +513,7 @@ __device__ __forceinline__ void softmax_role(const Paged8Args& a, const Job& J, 
       pg0 = entry(J, p + 4), pg1 = entry(J, p + 5);
       if (!uses(J, h, p)) continue;
       const bool b0 = e0.have, b1 = e1.have;
-      const float c0 = fmaxf(sc * e0.ks, FLT_MIN), c1 = fmaxf(sc * e1.ks, FLT_MIN);
+      const float c0 = score_factor(sc, e0.ks), c1 = score_factor(sc, e1.ks);
       const int ve0 = scale_log2_of(e0.vs), ve1 = scale_log2_of(e1.vs);
       const int k0 = p * kPage;
       const bool partial = !(k0 >= all_lo && k0 + 2 * kPage <= all_hi && b0 && b1);

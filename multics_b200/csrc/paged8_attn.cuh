@@ -23,6 +23,8 @@
 // weights l 2^n.
 #pragma once
 
+#include <float.h>
+
 #include "paged8.cuh"
 
 namespace hier {
@@ -228,6 +230,11 @@ struct OutFactor {
   }
 };
 __device__ __forceinline__ float inverse_or_0(float l) { return l > 0.f ? 1.f / l : l; }
+
+// factor of a page's scores: finite and not 0, since a score may be 0 or -infinity
+__device__ __forceinline__ float score_factor(float sc, float ks) {
+  return fminf(fmaxf(sc * ks, FLT_MIN), FLT_MAX);
+}
 
 // log2-sum-exp of a pair from its maximum and sum: -inf where nothing was seen,
 // NaN where the sum is

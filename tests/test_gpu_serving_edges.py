@@ -306,6 +306,25 @@ def test_value_scales_at_the_ends_of_their_range(scales, rows, shape, spread):
     c.check()
 
 
+@pytest.mark.parametrize("rows", [1, 40, 1500])
+def test_scores_of_nothing_between_huge_numbers(rows):
+    """Queries and keys so large that their factor passes fp32's range, and no
+    dimension in common: the scores are 0, and every key weighs the same."""
+    c, g = _pool(8, 1)
+    c.k.view(8, 1, 2, 64, 64)[:, :, 1] = 0
+    c.k_scale.fill_(2.0 ** 100)
+    q = torch.zeros(rows, 256, dtype=BF)
+    q[:, 64:128], q[:, 192:] = 2.0 ** 90, -2.0 ** 60
+    table = torch.full((1, 40), -1, dtype=torch.int32, device="cuda")
+    table[0, :8] = torch.arange(8)
+    out, lse = paged8_attention(q.cuda(), c, table, _i32([500]), _i32([0, rows]), 2, block_frames=0, return_lse=True)
+    v = (c.v.double() * c.v_scale.double()[..., None, None]).transpose(2, 3).reshape(512, 128)[:500]
+    want = v.mean(0).repeat(2)
+    # bf16's half step of the value, and fp16's of the weights (all 1) and of their fp32 sum
+    assert ((out.double() - want).abs() <= want.abs() * 2.0 ** -8 + v.abs().mean() * 2.0 ** -10).all()
+    assert ((lse.double() - torch.tensor(500.0, device="cuda").log2()).abs() <= 2.0 ** -10).all()
+
+
 @pytest.mark.parametrize("first", [True, False])
 def test_values_of_zeros_beside_large_ones_weigh(first):
     """By appends alone: a page of zero values and one of 1e10, all scores equal:
