@@ -82,6 +82,33 @@ def test_append_behind_rows_of_no_request(dtype, first, rows):
     c.check(), alone.check()
 
 
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("prompt", [100, 3000])
+@pytest.mark.parametrize("at", [0, 31, 63])
+def test_append_of_a_prompt_beside_single_tokens(dtype, prompt, at):
+    """A step of continuous batching: every request's pages are those of an append
+    of its own."""
+    n, heads = 64, 2
+    counts = [prompt if b == at else 1 for b in range(n)]
+    held = [prompt if b == at else 1 + 7 * b % 90 for b in range(n)]
+    pages = [-(-h // 64) for h in held]
+    g = torch.Generator().manual_seed(at)
+    order = torch.randperm(sum(pages), generator=g).to(torch.int32)
+    table, used = torch.full((n, max(pages)), -1, dtype=torch.int32), 0
+    for b, p in enumerate(pages):
+        table[b, :p], used = order[used:used + p], used + p
+    starts = torch.tensor([0] + counts).cumsum(0).tolist()
+    k, v = (torch.randn(starts[-1], heads * 128, generator=g).to(BF).cuda() for _ in range(2))
+    c, alone = (Paged8Cache(sum(pages), heads, dtype=dtype) for _ in range(2))
+    paged8_append(c, k, v, table.cuda(), _i32(held), _i32(starts))
+    for b in range(n):
+        part = slice(starts[b], starts[b + 1])
+        paged8_append(alone, k[part], v[part], table[b:b + 1].cuda(), _i32(held[b:b + 1]), _i32([0, counts[b]]))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(c, name).view(torch.int8), getattr(alone, name).view(torch.int8)), name
+    c.check(), alone.check()
+
+
 def _pool(pages, heads, dtype=torch.int8, seed=0):
     g = torch.Generator().manual_seed(seed)
     c = Paged8Cache(pages, heads, dtype=dtype)
