@@ -278,8 +278,10 @@ __device__ __forceinline__ void weigh(Running& R, float (&s)[MB][4], const Colum
   R.l[1] = fmaf(sum[1], factor[1], R.l[1]);
 }
 
-// The lanes' results as rows of 128 floats in shared memory, with n and l.
-__device__ __forceinline__ void spill(Running& R, float (*so)[kPitch], float* sn, float* sl, int lane) {
+// The lanes' numerators as rows of 128 floats in shared memory, with n, l and the
+// factor to the outputs.
+__device__ __forceinline__ void spill(Running& R, float (*so)[kPitch], float* sn, float* sl, float* sf,
+                                      int lane) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int i = 4; i < 32; i <<= 1) {
@@ -296,10 +298,11 @@ __device__ __forceinline__ void spill(Running& R, float (*so)[kPitch], float* sn
 #pragma unroll
   for (int d = 0; d < 8; ++d)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) so[2 * t + (r & 1)][16 * d + 8 * (r >> 1) + g] = R.o[d][r] * f[r & 1].a;
+    for (int r = 0; r < 4; ++r) so[2 * t + (r & 1)][16 * d + 8 * (r >> 1) + g] = R.o[d][r];
   if (g == 0) {
     sn[2 * t] = R.n[0], sn[2 * t + 1] = R.n[1];
     sl[2 * t] = R.l[0], sl[2 * t + 1] = R.l[1];
+    sf[2 * t] = f[0].a, sf[2 * t + 1] = f[1].a;
   }
 }
 
@@ -336,18 +339,22 @@ constexpr int kMinPages = 2 * kWarps;  // of a part at least
 // Until the kernel before this one is done, where it was launched beside it.
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// What the blocks behind the last unit do: the first of them writes zeros to the
-// rows between q_start's ends that no kernel writes, and all wait for the kernel
+// What the blocks of no unit do (in front of the short kernel's units, behind the
+// long one's): the first of them writes zeros to the rows between q_start's ends that no kernel writes, and all wait for the kernel
 // before.  There are such rows only where row starts descend or leave the row
 // tensor: those of refused requests alone, and of requests whose tiles the large
 // kernel cannot find.  (A block of its own: 0.5 us of 51 for 880 requests of 3
-// rows; done by the tiles' warps for their own request it took 5.7.)
+// rows, where the tiles' warps took 5.7 to do it for their own request; in front,
+// since it took 30 us of 168 as the last block of 20 000 requests; and a function of
+// its own for the registers of the kernels.)
 constexpr int kKeptWords = 128;  // 4 096 rows at a time
-__device__ __forceinline__ void keep_rows(const Paged8Args& a, bool first, uint32_t* covered) {
+__device__ __noinline__ void keep_rows(const Paged8Args& a, bool first, uint32_t* covered) {
   const int32_t* qs = a.q_start;
   int bad = qs[0] < 0 || qs[a.n] > a.rows;
-  if (first && a.zero_rest)
-    for (int i = threadIdx.x; i < a.n; i += blockDim.x) bad |= qs[i + 1] < qs[i];
+  if (first && a.zero_rest) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < a.n; i += kWarps * 32) bad |= qs[i + 1] < qs[i];
+  }
   bad = __syncthreads_or(bad);
   wait_for_prior();
   if (!bad || !first || !a.zero_rest) return;
@@ -385,10 +392,10 @@ __device__ __forceinline__ void keep_rows(const Paged8Args& a, bool first, uint3
 }
 
 template <int FMT>
-__global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args a) {
+__global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(const __grid_constant__ Paged8Args a) {
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
   __shared__ __align__(16) uint32_t sq[kWarps][8][32][2];
-  __shared__ float sn[kWarps][kRows], sl[kWarps][kRows];
+  __shared__ float sn[kWarps][kRows], sl[kWarps][kRows], sf[kWarps][kRows];
   asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -491,7 +498,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
         }
       }
     }
-    spill(R, so[w], sn[w], sl[w], lane);
+    spill(R, so[w], sn[w], sl[w], sf[w], lane);
     __syncthreads();
     for (int r = w; r < kRows && tl.rho0 + r < tl.pairs; r += kWarps) {
       float N = -INFINITY;
@@ -506,7 +513,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) paged8_long_kernel(Paged8Args 
       const float inv = inverse_or_0(L);
 #pragma unroll
       for (int q = 0; q < kWarps; ++q) {
-        const float f = share[q] * inv;
+        const float f = share[q] * inv * sf[q][r];
         const float4 v = *reinterpret_cast<const float4*>(&so[q][r][4 * lane]);
         acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
         acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
@@ -617,12 +624,12 @@ __device__ __forceinline__ void short_keys(const Paged8Args& a, const Columns& c
 }
 
 template <int FMT>
-__global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args a, int units) {
+__global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(const __grid_constant__ Paged8Args a, int units) {
   __shared__ __align__(16) float so[kWarps][kRows][kPitch];
-  __shared__ float sn[kWarps][kRows], sl[kWarps][kRows];
+  __shared__ float sn[kWarps][kRows], sl[kWarps][kRows], sf[kWarps][kRows];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if ((int)blockIdx.x * kWarps >= units) return keep_rows(a, true, reinterpret_cast<uint32_t*>(so));
-  const int unit = blockIdx.x * kWarps + w;
+  if ((int)blockIdx.x < a.keep) return keep_rows(a, true, reinterpret_cast<uint32_t*>(so));
+  const int unit = ((int)blockIdx.x - a.keep) * kWarps + w;
   if (unit >= units) return;
   const int tile = unit / a.kv_heads, kvh = unit - tile * a.kv_heads.d;
   const int b = tile / a.direct;
@@ -649,11 +656,11 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged8_short_kernel(Paged8Args
           short_keys<FMT, 2>(a, c, R, qf, sc, at, p * kPage, base, from, to, lane);
       }
     }
-    spill(R, so[w], sn[w], sl[w], lane);
+    spill(R, so[w], sn[w], sl[w], sf[w], lane);
     __syncwarp();
     for (int r = 0; r < kRows && tl.rho0 + r < tl.pairs; ++r) {
       const float4 v = *reinterpret_cast<const float4*>(&so[w][r][4 * lane]);
-      const float acc[4] = {v.x, v.y, v.z, v.w};
+      const float f = sf[w][r], acc[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
       write_pair(a, tl, tl.rho0 + r, kvh, lane, acc, sn[w][r], sl[w][r]);
     }
     __syncwarp();
@@ -812,10 +819,10 @@ int launch_merge(const Paged8Args& a, int64_t tiles, cudaStream_t st) {
 // requests are others, and its blocks leave SMs idle: few of them, or the last
 // wave's).  The blocks of one unit more (keep_rows) do wait for it, so that what
 // follows on the stream finds both done.
-int launch_small(const Paged8Args& a, int format, int64_t tiles, bool few_pages, bool beside,
+int launch_small(Paged8Args a, int format, int64_t tiles, bool few_pages, bool beside,
                  cudaStream_t st) {
   const int64_t units = tiles * a.kv_heads * a.splits;
-  const int keep = beside || a.zero_rest;
+  a.keep = beside || a.zero_rest;
   if (units > INT32_MAX - 2 * kWarps * a.splits) {
     set_error(HIER_EVALUE, "too many rows, requests and heads");
     return HIER_EVALUE;
@@ -832,7 +839,7 @@ int launch_small(const Paged8Args& a, int format, int64_t tiles, bool few_pages,
   }
   if (few_pages) {
     auto* kernel = format == P8_INT8 ? paged8_short_kernel<P8_INT8> : paged8_short_kernel<P8_E4M3>;
-    cfg.gridDim = dim3((unsigned)((units + kWarps - 1) / kWarps + keep));
+    cfg.gridDim = dim3((unsigned)((units + kWarps - 1) / kWarps + a.keep));
     HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, (int)units), "paged8_short_kernel launch");
     return HIER_OK;
   }
@@ -843,7 +850,7 @@ int launch_small(const Paged8Args& a, int format, int64_t tiles, bool few_pages,
     dim.val.clusterDim.x = a.splits.d;
     dim.val.clusterDim.y = dim.val.clusterDim.z = 1;
   }
-  cfg.gridDim = dim3((unsigned)(units + (keep ? a.splits.d : 0)));
+  cfg.gridDim = dim3((unsigned)(units + a.keep * a.splits.d));
   HIER_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a), "paged8_long_kernel launch");
   return a.splits > 1 && !a.cluster ? launch_merge<kPaged8SmallRows>(a, tiles, st) : HIER_OK;
 }

@@ -57,6 +57,7 @@ struct Paged8Args {
   int cluster;      // the parts of a small tile are the blocks of a cluster
   int row_limit;    // requests of up to row_limit pairs are the small kernel's, the others the
                     // large one's (INT_MAX: all the small one's, 0: all the large one's)
+  int keep;         // small kernels: whether there are blocks of no unit (keep_rows)
   Divisor direct;   // small kernel: its tile t is tile t % direct of request t / direct
   int32_t* status;
   int* err;         // bounded waits
@@ -225,11 +226,11 @@ struct OutFactor {
   float a, b;
   __device__ __forceinline__ OutFactor(float m, float n, float l) : a(l), b(1.f) {
     if (!(l > 0.f)) return;
-    a = ex2_approx(fmaxf(m - n, -96.f)) / l;
+    a = __fdividef(ex2_approx(fmaxf(m - n, -96.f)), l);
     b = ex2_approx(fminf(m - n + 96.f, 0.f));
   }
 };
-__device__ __forceinline__ float inverse_or_0(float l) { return l > 0.f ? 1.f / l : l; }
+__device__ __forceinline__ float inverse_or_0(float l) { return l > 0.f ? __fdividef(1.f, l) : l; }
 
 // factor of a page's scores: finite and not 0, since a score may be 0 or -infinity
 __device__ __forceinline__ float score_factor(float sc, float ks) {

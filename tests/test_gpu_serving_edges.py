@@ -154,6 +154,40 @@ def test_log_sum_of_rows_of_no_request_beside_a_given_out(first, rows, tail, wid
         assert (kept[:first] == 7).all() and (kept[starts[-1]:] == 7).all()
 
 
+@pytest.mark.parametrize("n,T", [(3, 40), (31, 700), (200, 9000), (1500, 5000)])
+@pytest.mark.parametrize("width", [4, 40])
+@pytest.mark.parametrize("seed", range(4))
+def test_row_starts_that_are_anything(n, T, width, seed):
+    """Whatever the row starts are, every row of a fresh result is some request's
+    or zeros, and rows that no request can have are zeros."""
+    heads, g = 2, torch.Generator().manual_seed(seed)
+    c, _ = _pool(4, 1)
+    qs = torch.randint(-20, T + 20, (n + 1,), generator=g)
+    if seed % 2:  # ascending but for a few
+        qs = qs.sort().values
+        qs[torch.randint(0, n + 1, (2,), generator=g)] = torch.tensor([T + 7, -3])
+    table = torch.full((n, width), -1, dtype=torch.int32)
+    table[:, :2] = torch.randint(0, 4, (n, 2), generator=g)
+    q = torch.randn(T, heads * 128, generator=g).to(BF).cuda()
+    args = (q, c, table.cuda(), _i32([100] * n), qs.to(torch.int32).cuda(), heads)
+    out, lse = _poisoned(lambda: paged8_attention(*args, block_frames=0, return_lse=True))
+    with pytest.raises(ValueError, match="row starts"):
+        c.check()
+    first = min(max(int(qs[0]), 0), T)
+    end = max(first, min(int(qs[-1]), T))
+    had = torch.zeros(T, dtype=torch.bool)
+    for a, e in zip(qs.tolist(), qs.tolist()[1:]):
+        if first <= a < e <= end:
+            had[a:e] = True
+    o, s = out.view(T, heads, 128).cpu(), lse.cpu()
+    assert (o[~had] == 0).all() and (s[~had] == float("-inf")).all()
+    zero = (o == 0).all(2)
+    assert torch.equal(zero, s == float("-inf"))
+    assert torch.isfinite(s[~zero]).all() and not (o == 7).all(2).any()
+    # values of up to 120 * 2^-6: nothing but averages of them
+    assert (o.abs() <= 2).all() and (s[~zero] != 7).all()
+
+
 def test_every_cache_has_its_status_word():
     """A fault in one layer's cache is that cache's: no other reports or clears it."""
     pools = [_pool(2, 1)[0] for _ in range(3)]
