@@ -309,7 +309,7 @@ def dev_err(device):
     t = _DEV_ERR.get(key)
     if t is None:
         with torch.inference_mode(False), torch.cuda.device(key):
-            t = (calls().word_beside_capture(key) if torch.cuda.is_current_stream_capturing()
+            t = (calls().words_beside_capture(key, 1) if torch.cuda.is_current_stream_capturing()
                  else torch.zeros(1, dtype=torch.int32, device="cuda"))
         _DEV_ERR[key] = t
     return t

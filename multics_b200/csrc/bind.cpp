@@ -14,7 +14,7 @@
 //              current one, rows that need a copy, arguments to refuse), which
 //              the Python functions then do or refuse; an int is a status.
 //
-// and word_beside_capture, what a capture must not make by itself.
+// and words_beside_capture, what a capture must not make by itself.
 //
 // The module holds no code of the library: bind() gives it the addresses of
 // the one that is loaded.
@@ -191,21 +191,21 @@ bool requests_of(PyObject* const* a, at::Device dev, Requests* r) {
          is_vector(r->q_start, r->table->size(0) + 1, dev);
 }
 
-// word_beside_capture(device) -> int32 [1], zero: allocated and zeroed on a stream of its own, so
-// that neither is a part of the graph that this thread captures.
-PyObject* word_beside_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  int64_t dev;
-  if (n != 1 || !int_of(a[0], 0, 127, &dev)) {
-    PyErr_SetString(PyExc_TypeError, "word_beside_capture(device)");
+// words_beside_capture(device, count) -> int32 [count], zeros: allocated and zeroed on a stream of
+// its own, so that neither is a part of the graph that this thread captures.
+PyObject* words_beside_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t dev, count;
+  if (n != 2 || !int_of(a[0], 0, 127, &dev) || !int_of(a[1], 1, INT32_MAX, &count)) {
+    PyErr_SetString(PyExc_TypeError, "words_beside_capture(device, count)");
     return nullptr;
   }
   try {
     const c10::InferenceMode mode(false);
     const c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};
     const c10::cuda::CUDAStreamGuard stream(c10::cuda::getStreamFromPool(false, (c10::DeviceIndex)dev));
-    at::Tensor word = at::zeros({1}, at::device(stream.current_stream().device()).dtype(at::kInt));
+    at::Tensor words = at::zeros({count}, at::device(stream.current_stream().device()).dtype(at::kInt));
     stream.current_stream().synchronize();
-    return THPVariable_Wrap(std::move(word));
+    return THPVariable_Wrap(std::move(words));
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
@@ -578,7 +578,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     METHOD("bind", bind, "bind(name, address): where an entry point is"),
-    METHOD("word_beside_capture", word_beside_capture, "a zero word that no graph owns"),
+    METHOD("words_beside_capture", words_beside_capture, "zeros that no graph owns"),
     METHOD("layout", layout, "format of a cache over tensors of its layout"),
     METHOD("append", append, "paged8_append of well-formed tensors"),
     METHOD("attention", attention, "paged8_attention of well-formed tensors"),

@@ -15,7 +15,7 @@ tables are built on the GPU:
   (``multics/models/blocks.py:300-305,366-371``).
 
 None of them reads back from the device, so a step can be captured into a CUDA
-graph.  What a kernel finds wrong in device tables (a page outside the pool, a
+graph (whose caches, like its tensors, the caller keeps).  What a kernel finds wrong in device tables (a page outside the pool, a
 length outside the table) it skips and records in the cache's status word
 (:meth:`Paged8Cache.check`).
 """
@@ -40,6 +40,7 @@ HEAD_DIM = 128
 _I32, _BF16 = torch.int32, torch.bfloat16
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _STATUS = {}  # (device, stream): words that no cache has yet
+_KEPT = []  # words that captured graphs write to
 _SPLIT = torch.unsafe_split_with_sizes  # (integers: no versions to share)
 
 _CACHE_BITS = ((1, "row starts leave the rows or descend"),
@@ -52,28 +53,29 @@ _STEP_BITS = ((1, "too few free pages"), (2, "more new tokens than rows"),
               (16, "the free count leaves the free list"))
 
 
-def _zeros(n, dev):
-    with torch.inference_mode(False):  # (a word may be made in that mode and cleared outside)
-        return torch.zeros(n, dtype=_I32, device=dev)
-
-
 def _status_word(dev):
     """A zero status word of its own for a cache: one of 256 zeroed together on
-    the current stream, or one of the graph that is being captured (whose memory
-    lasts as long as the graph)."""
+    the current stream, or beside the graph that is being captured (no replay
+    clears it, and it is kept for replays after the cache is gone)."""
     if dev.type != "cuda":
         key = dev, 0
     elif not is_current(dev):
         with torch.cuda.device(dev):
             return _status_word(dev)
     elif torch.cuda.is_current_stream_capturing():
-        return _zeros(1, dev)
+        key = dev, "captured"
     else:
         key = dev, raw_stream(dev.index)
     try:
         return _STATUS[key].pop()
     except (KeyError, IndexError):
-        words = list(_zeros(256, dev).unsafe_split_with_sizes((1,) * 256))
+        if key[1] == "captured":
+            zeros = _lib.calls().words_beside_capture(dev.index, 256)
+            _KEPT.append(zeros)
+        else:
+            with torch.inference_mode(False):  # (made in that mode, cleared outside)
+                zeros = torch.zeros(256, dtype=_I32, device=dev)
+        words = list(zeros.unsafe_split_with_sizes((1,) * 256))
         word = words.pop()
         _STATUS[key] = words
         return word
@@ -156,8 +158,7 @@ class Paged8Cache:
     def from_tensors(cls, k, v, k_scale, v_scale, status=None) -> "Paged8Cache":
         """A cache over tensors in the layout above (finite codes, power-of-two
         scales, in ``[2^-126, 2^126]``).  ``status`` (int32 ``[1]``, zero): a word
-        to record faults in, where caches are to share one.  A cache made while a
-        graph is captured has a word of that graph."""
+        to record faults in, where caches are to share one."""
         if _lib.calls().layout(k, v, k_scale, v_scale) is None:
             cls._refuse(k, v, k_scale, v_scale)
         dev = k.device

@@ -207,6 +207,34 @@ def test_every_cache_has_its_status_word():
         c.check()
 
 
+def test_faults_of_replays_are_kept_until_checked():
+    """A cache made in a capture: no replay clears what an earlier one recorded,
+    and nothing else gets its word when the cache object is gone."""
+    c, _ = _pool(2, 1)
+    q, table, lengths, starts = torch.ones(1, 128, dtype=BF, device="cuda"), _i32([[0]]), _i32([5]), _i32([0, 1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inner = [Paged8Cache.from_tensors(c.k, c.v, c.k_scale, c.v_scale) for _ in range(2)]
+        paged8_attention(q, inner[0], table, lengths, starts, 1)
+        paged8_attention(q, inner[1], table, lengths, starts, 1)
+    graph.replay()
+    inner[0].check(), inner[1].check()
+    table.fill_(-1)
+    graph.replay()
+    table.fill_(0)
+    graph.replay()
+    for layer in inner:
+        with pytest.raises(ValueError, match="page pool"):
+            layer.check()
+        layer.check()
+    del layer, inner
+    table.fill_(-1)
+    others = [Paged8Cache.from_tensors(c.k, c.v, c.k_scale, c.v_scale) for _ in range(600)]
+    graph.replay()
+    for other in others:
+        other.check()
+
+
 def test_what_is_recorded_during_a_check_is_kept(monkeypatch):
     from test_paged8_status_cpu import late_record
 
