@@ -16,8 +16,10 @@
 // of its heads.  Results are stored past the caches' reuse (written once, 165
 // against 183 us).  38 556 rows of 24 + 24 heads of 128: 150 us = 6.3 TB/s, 0.97
 // of the measured copy bandwidth (8 groups per warp: 165 us, 4: 162, 2: 200).
-// Backward on 9 241 rows of 24 + 8 heads: 46 us = 4.9 TB/s, bound by its
-// arithmetic and two reductions per head, and 4 us for the weights' sums.
+// Backward on 9 241 rows of 24 + 8 heads: 46 us = 4.9 TB/s, and 4 us for the
+// weights' sums.  DRAM is half busy and so are the issue slots: its 16 warps per SM
+// wait for their loads, and then for two sums per head one after the other with no
+// load in flight.
 
 #include "common.cuh"
 

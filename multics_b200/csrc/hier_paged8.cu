@@ -797,6 +797,8 @@ extern "C" int hier_paged8_append(const void* k, int64_t k_stride, const void* v
   a.lengths = lengths, a.q_start = q_start, a.n = n;
   a.status = status;
   cudaStream_t st = (cudaStream_t)stream;
+  // (The mean decides: a prompt beside many single tokens may be walked by a warp
+  // per head, its pages one after the other.)
   // A block per page and head where requests bring more than 48 tokens each, or
   // fewer and the machine has room, else a warp per request and head (in us, warps
   // and blocks, of requests x tokens x heads: 100 x 34 x 24 27.7 and 34.0, 200 x

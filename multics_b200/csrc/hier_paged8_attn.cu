@@ -17,22 +17,27 @@
 // and with few tiles the keys are also split over blocks.  Few parts are the
 // blocks of a cluster, which joins them over distributed shared memory: no
 // workspace and no second launch (a row of each of 4 requests over 3 000 tokens,
-// 24 heads to 8: 11.8 us, with a second kernel 14.0; 3.3 us less of the host).
+// 24 heads to 8: 11.9 us, with a second kernel 2.2 more; 3.3 us less of the host).
 // Where twice the portable cluster's 8 blocks could share the keys, the parts go
 // to a workspace and a second kernel joins them (one row over 9 240 tokens of 24
-// heads: 19.2 us against 20.6; over 100 000 tokens, 8 heads to one: 31.7 against
-// 94), and so they do beyond one wave of blocks, where clusters wait for places
+// heads: 20.0 us, as a cluster 1.4 more; over 100 000 tokens, 8 heads to one: 32.5
+// against 94), and so they do beyond one wave of blocks, where clusters wait for places
 // (37 rows of 4 key heads: 91 us against 103).  Parts are always joined in their
 // order.
 // While a page's scores are computed its values are in flight, and while its
 // values are consumed the next page's keys are: the loads of one take the
 // registers that the other's products have just used.  37 rows over up to 19 001
-// tokens, 32 heads to 4, e4m3: 92 us, 5.7 TB/s, 0.88 of the measured copy rate.
+// tokens, 32 heads to 4, e4m3: 92.5 us, 5.7 TB/s, 0.87 of the measured copy rate.
+// One row over 9 240 tokens: DRAM 39 % and issue slots 42 % busy, its warps with two
+// pages each wait for loads.  Beyond 888 (request, key head) tiles the keys are not
+// split whatever the lengths are: one long request among hundreds of short ones is
+// read by a block per key head.
 // paged8_short_kernel: a warp per tile, and products over 16 or 32 keys at a
-// time, its loads issued together.  880 requests of 3 rows over 27 tokens, 24
-// heads, int8: 50 us, 5.0 TB/s (a value's 64-byte row is read whole, which makes
+// time, its loads issued together.  880 requests of 3 rows over 12 to 24 tokens, 24
+// heads, int8: 51 us, 4.9 TB/s (a value's 64-byte row is read whole, which makes
 // 249 MB of 126) with half of the issue slots used; more warps than the 16 of 128
-// registers spill (5 blocks per SM: 70 us).
+// registers spill much (5 blocks per SM: 70 us; as built 4 bytes, 16 for e4m3, and 44
+// in the other kernel).
 
 #include <math.h>
 

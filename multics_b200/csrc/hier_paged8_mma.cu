@@ -33,14 +33,17 @@
 // Tensor memory: S0 | S1 | O0 | O1, P over the first half of its S.
 // Every mbarrier wait is bounded and records a timeout in dev_err.
 //
-// Bound by shared memory: a 128-key tile of two halves takes 3 830 cycles from
-// e4m3 codes and about 4 000 from int8, against 3 216 for its four products, the
-// rest being the converter's 96 KiB; a tile of one half 2 500 to 2 750.  A CTA
-// adds 11 us (finding its tile 2.4, queries 3.2, first scores 1, last products
-// and output 3.4).  One sequence of 9 240 rows, causal by 220, 24 heads, e4m3:
-// 551 us = 975 TFLOP/s of the pairs seen.  The code of all roles is 95 KB, and
-// runs the faster the smaller it is: one converter for keys and values 206 us
-// against 222 (4 requests' chunks of 660 rows over 4 620 keys, int8).
+// Bound by the chain of each half, scores to weights to products: no unit is busy
+// for more than 53 % of the time (tensor pipe 46, tensor memory 53, issue slots
+// 48), and one instruction more per pair of weights costs 5 %.  A 128-key tile of
+// two halves takes about 3 870 cycles from e4m3 codes, against 3 216 for its four
+// products; a tile of one half 2 500 to 2 750.  A CTA adds 11 us (finding its tile
+// 2.4, queries 3.2, first scores 1, last products and output 3.4).  One sequence of
+// 9 240 rows, causal by 220, 24 heads, e4m3: 556 us = 966 TFLOP/s of the pairs seen
+// at 1 965 MHz, 590 us in calls for seconds, at 1 845 MHz under the power cap.  The
+// code of all roles is large and runs the faster the smaller it is: one converter
+// for keys and values 206 us against 222 (4 requests' chunks of 660 rows over 4 620
+// keys, int8), 210 now.
 
 #include <type_traits>
 

@@ -240,7 +240,8 @@ def page_step(lengths, add, table, free_pages, free_count, rows: int, *,
     ``table`` int32 ``[n, width]`` (row-major, updated) lists each request's
     pages; ``free_pages`` int32 (updated) is a stack of ``free_count`` (int32
     ``[1]``) free pages: pages given up are put on its end, pages needed are
-    taken from there, both in request order.  ``rows`` is the number of rows of
+    taken from there, both in request order (as they are listed: entries below a
+    request's length are its pages until it gives them up here).  ``rows`` is the number of rows of
     the step's token tensors; the new tokens fill them request by request.  A
     step that cannot be taken whole (too few pages or rows, a length outside the
     table, an addition above ``most_new``) changes nothing and maps no row;
