@@ -28,7 +28,7 @@
 // values are consumed the next page's keys are: the loads of one take the
 // registers that the other's products have just used.  37 rows over up to 19 001
 // tokens, 32 heads to 4, e4m3: 92.5 us, 5.7 TB/s, 0.87 of the measured copy rate.
-// One row over 9 240 tokens: DRAM 39 % and issue slots 42 % busy, its warps with two
+// One row over 9 240 tokens: DRAM 37 % and issue slots 41 % busy, its warps with two
 // pages each wait for loads.  Beyond 888 (request, key head) tiles the keys are not
 // split whatever the lengths are: one long request among hundreds of short ones is
 // read by a block per key head.
@@ -345,13 +345,13 @@ constexpr int kMinPages = 2 * kWarps;  // of a part at least
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // What the blocks of no unit do (in front of the short kernel's units, behind the
-// long one's): the first of them writes zeros to the rows between q_start's ends that no kernel writes, and all wait for the kernel
-// before.  There are such rows only where row starts descend or leave the row
-// tensor: those of refused requests alone, and of requests whose tiles the large
-// kernel cannot find.  (A block of its own: 0.5 us of 51 for 880 requests of 3
-// rows, where the tiles' warps took 5.7 to do it for their own request; in front,
-// since it took 30 us of 168 as the last block of 20 000 requests; and a function of
-// its own for the registers of the kernels.)
+// long one's): the first of them writes zeros to the rows between q_start's ends
+// that no kernel writes, and all wait for the kernel before.  There are such rows
+// only where row starts descend or leave the row tensor: those of refused requests
+// alone, and of requests whose tiles the large kernel cannot find.  (A block of its
+// own: 0.5 us of 51 for 880 requests of 3 rows, where the tiles' warps took 5.7 to do
+// it for their own request; in front, since it took 30 us of 168 as the last block of
+// 20 000 requests; a function of its own for the registers of the kernels.)
 constexpr int kKeptWords = 128;  // 4 096 rows at a time
 __device__ __noinline__ void keep_rows(const Paged8Args& a, bool first, uint32_t* covered) {
   const int32_t* qs = a.q_start;
